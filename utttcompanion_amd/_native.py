@@ -1,4 +1,4 @@
-"""ctypes binding of libuttt_amd.so (the C ABI declared in include/uttt_amd.h).
+"""ctypes binding of libuttt_amd.so (the C ABI declared in include/uttt_amd.h and include/uttt_serve.h).
 
 The library is loaded lazily on first use and there is no fallback: a missing or
 stale library raises ``RuntimeError`` naming the build command.
@@ -12,22 +12,26 @@ import threading
 from .build import HEADER_PATH, LIB_PATH
 
 
-def _header_abi_version(path: str = HEADER_PATH) -> int:
+def _header_abi_version(path: str = HEADER_PATH, name: str = "UTTT_ABI_VERSION") -> int:
     """UTTT_ABI_VERSION as include/uttt_amd.h defines it (the library is built from that header)."""
     import re
     with open(path, "r", encoding="utf-8") as fh:
-        m = re.search(r"^#define UTTT_ABI_VERSION (\d+)$", fh.read(), re.M)
+        m = re.search(rf"^#define {name} (\d+)$", fh.read(), re.M)
     if m is None:
-        raise RuntimeError(f"{path} defines no UTTT_ABI_VERSION")
+        raise RuntimeError(f"{path} defines no {name}")
     return int(m.group(1))
 
 
 ABI_VERSION = _header_abi_version()
+SERVE_HEADER_PATH = os.path.join(os.path.dirname(HEADER_PATH), "uttt_serve.h")
+SERVE_ABI_VERSION = _header_abi_version(SERVE_HEADER_PATH, "UTTT_SERVE_ABI_VERSION")
 MAX_CHAIN = 64
 MAX_UPDATE_TOKENS = 512  # UTTT_MAX_UPDATE_TOKENS: longest chunk one uttt_chunk_update writes
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
 UPDATE_PHASES = 5
+MAX_TREE_NODES = 64  # of one request's draft (uttt_swa_tree)
+MAX_FORK_REQUESTS = 128  # of one uttt_kv_fork
 
 _P = C.c_void_p
 _I64 = C.c_int64
@@ -275,6 +279,69 @@ SIGNATURES = {
     "uttt_greedy_select": (C.c_int, [C.POINTER(GreedyArgs), _P]),
 }
 
+# include/uttt_serve.h: the serving operators, with a version of their own
+
+
+class SampleArgs(C.Structure):
+    _fields_ = [
+        ("rows", _I64), ("vocab", _I64), ("dtype", _I32), ("n_banned", _I32),
+        ("banned", _I32 * 8), ("active_limit", _I64),
+        ("logits", _P), ("row_stride", _I64),
+        ("uniforms", _P), ("temperature", _P), ("top_k", _P), ("top_p", _P), ("min_p", _P),
+        ("out", _P), ("logprob", _P), ("advance", _P),
+    ]
+
+
+class SwaTreeArgs(C.Structure):
+    _fields_ = [
+        ("n_req", _I64), ("n_heads", _I64), ("n_kv_heads", _I64), ("nodes", _I64), ("head_dim", _I64),
+        ("window", _I64), ("sinks", _I64),
+        ("act_dtype", _I32), ("write_ring", _I32), ("scale", _F),
+        ("positions", _P), ("parents", _P), ("counts", _P),
+        ("cos_table", _P), ("sin_table", _P), ("table_len", _I64),
+        ("q", _P), ("q_stride_n", _I64), ("q_stride_t", _I64), ("q_stride_h", _I64),
+        ("k_new", _P), ("k_stride_n", _I64), ("k_stride_t", _I64), ("k_stride_h", _I64),
+        ("v_new", _P), ("v_stride_n", _I64), ("v_stride_t", _I64), ("v_stride_h", _I64),
+        ("k_ring", _P), ("v_ring", _P), ("ring_stride_n", _I64),
+        ("out", _P), ("o_stride_n", _I64), ("o_stride_t", _I64), ("o_stride_h", _I64),
+        ("k_nodes", _P), ("v_nodes", _P),
+        ("workspace", _P), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class KvCommitArgs(C.Structure):
+    _fields_ = [
+        ("layers", _I64), ("n_req", _I64), ("n_kv_heads", _I64), ("n_nodes", _I64), ("path", _I64),
+        ("head_dim", _I64), ("window", _I64), ("sinks", _I64),
+        ("act_dtype", _I32), ("advance", _I32),
+        ("k_nodes", _P), ("v_nodes", _P), ("nodes_stride_l", _I64), ("nodes_stride_n", _I64),
+        ("nodes", _P), ("path_stride", _I64), ("counts", _P),
+        ("k_ring", _P), ("v_ring", _P), ("ring_stride_l", _I64), ("ring_stride_n", _I64),
+        ("positions", _P),
+    ]
+
+
+class KvForkArgs(C.Structure):
+    _fields_ = [
+        ("layers", _I64), ("n_req", _I64), ("n_kv_heads", _I64), ("slots", _I64), ("head_dim", _I64),
+        ("act_dtype", _I32),
+        ("sources", _P),
+        ("k_ring", _P), ("v_ring", _P), ("ring_stride_l", _I64), ("ring_stride_n", _I64),
+        ("positions", _P),
+    ]
+
+
+SERVE_SIGNATURES = {
+    "uttt_serve_abi_version": (C.c_int, []),
+    "uttt_sample_select": (C.c_int, [C.POINTER(SampleArgs), _P]),
+    "uttt_swa_prefill_sinks_workspace": (C.c_size_t, [_I64, _I64, _I64, _I64, _I64, _I64, _I64]),
+    "uttt_swa_prefill_sinks": (C.c_int, [C.POINTER(SwaPrefillArgs), _I64, _P]),
+    "uttt_swa_tree_workspace": (C.c_size_t, [_I64, _I64, _I64, _I64, _I64, _I64, _I32]),
+    "uttt_swa_tree": (C.c_int, [C.POINTER(SwaTreeArgs), _P]),
+    "uttt_kv_commit": (C.c_int, [C.POINTER(KvCommitArgs), _P]),
+    "uttt_kv_fork": (C.c_int, [C.POINTER(KvForkArgs), _P]),
+}
+
 _lib = None
 _lock = threading.Lock()
 
@@ -295,7 +362,10 @@ def load_library(path: str = LIB_PATH) -> C.CDLL:
         version = lib.uttt_abi_version()  # before the symbols: another version may lack some
         if version != ABI_VERSION:
             raise RuntimeError(f"{path} has ABI version {version}, expected {ABI_VERSION}: rebuild it")
-        for name, (res, argt) in SIGNATURES.items():
+        serve = lib.uttt_serve_abi_version() if hasattr(lib, "uttt_serve_abi_version") else 0
+        if serve != SERVE_ABI_VERSION:
+            raise RuntimeError(f"{path} has serving ABI version {serve}, expected {SERVE_ABI_VERSION}: rebuild it")
+        for name, (res, argt) in {**SIGNATURES, **SERVE_SIGNATURES}.items():
             fn = getattr(lib, name)
             fn.restype = res
             fn.argtypes = argt

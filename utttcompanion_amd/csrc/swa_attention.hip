@@ -10,6 +10,7 @@
 
 #include <algorithm>
 
+#include "../../include/uttt_serve.h"
 #include "swa_prefill.h"
 #include "uttt_device.h"
 #include "uttt_host.h"
@@ -270,12 +271,13 @@ __host__ __device__ __forceinline__ int prefill_max_tiles(int64_t kv_len, int64_
   return (int)((span + 63) / 64) + 1;
 }
 
-static PrefillPlan prefill_plan(int64_t batch, int64_t heads, int64_t q_len, int64_t kv_len, int64_t window) {
+static PrefillPlan prefill_plan(int64_t batch, int64_t heads, int64_t q_len, int64_t kv_len, int64_t window,
+                                int64_t sinks) {
   PrefillPlan p;
   p.nqt = (int)((q_len + 63) / 64);
   p.q_pad = p.nqt * 64;
   const int64_t base = (int64_t)p.nqt * heads * batch;
-  const int max_tiles = prefill_max_tiles(kv_len, window);
+  const int max_tiles = prefill_max_tiles(kv_len, window) + (int)((std::min(sinks, kv_len) + 63) / 64);
   // about 256 workgroups (one per CU): in the chunk-first prefill the attention shares the GPU
   // with the layer chain, and at config 3 (64 workgroups before the split) 256 measured faster
   // than 128, 192, 320 or 512 workgroups (prefill 552-556 against 554-561 ms on one box)
@@ -314,9 +316,10 @@ __device__ __forceinline__ float row16_sum(float v) {
 // fp32 and bf16 tolerances of the attention output
 __device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
 
-template <int HD>
+// SINK: the first `sinks` keys stay visible; those ahead of the window are tiles of their own in front of its tiles
+template <int HD, bool SINK>
 __global__ void __launch_bounds__(kThreads) k_swa_prefill(const uttt_swa_prefill_args a, float* part, int nsplit,
-                                                          int tiles_per_split, int q_pad, int nqt) {
+                                                          int tiles_per_split, int q_pad, int nqt, int64_t sinks) {
   constexpr int PAD = 4;         // rows stay 16-byte aligned
   constexpr int LQ = HD + PAD;   // q/k rows [token][e]
   constexpr int LV = 64 + PAD;   // v^T rows [e][key], p rows [query][key]
@@ -337,8 +340,15 @@ __global__ void __launch_bounds__(kThreads) k_swa_prefill(const uttt_swa_prefill
   const int64_t p_first = a.q_offset + q0, p_last = a.q_offset + q0 + qn - 1;
   const int64_t lo = max((int64_t)0, p_first - a.window + 1);
   const int64_t hi = min(a.kv_len, p_last + 1);  // exclusive
-  const int ntiles = (int)((hi - lo + 63) / 64);
+  const int64_t sink_hi = SINK ? min(lo, sinks) : 0;
+  const int nsink = SINK ? (int)((sink_hi + 63) / 64) : 0;
+  const int ntiles = nsink + (int)((hi - lo + 63) / 64);
   const int t_begin = sp * tiles_per_split, t_end = min(ntiles, t_begin + tiles_per_split);
+  auto first_key = [&](int t) {  // of tile t
+    if constexpr (SINK) return t < nsink ? (int64_t)t * 64 : lo + (int64_t)(t - nsink) * 64;
+    return lo + (int64_t)t * 64;
+  };
+  auto last_key = [&](int t) { return SINK && t < nsink ? sink_hi : hi; };  // exclusive
 
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int g = lane >> 4, c = lane & 15;
@@ -375,19 +385,19 @@ __global__ void __launch_bounds__(kThreads) k_swa_prefill(const uttt_swa_prefill
 
   AttnStage<HD> stg;
   {
-    const int64_t kt0 = lo + (int64_t)t_begin * 64;
+    const int64_t kt0 = first_key(t_begin);
     stg.load(kg + kt0 * a.k_stride_t, vg + kt0 * a.v_stride_t, a.k_stride_t, a.v_stride_t,
-             (int)min((int64_t)64, hi - kt0));
+             (int)min((int64_t)64, last_key(t_begin) - kt0));
   }
   for (int kt = t_begin; kt < t_end; ++kt) {
-    const int64_t kt0 = lo + (int64_t)kt * 64;
+    const int64_t kt0 = first_key(kt), kt1 = last_key(kt);
     __syncthreads();  // previous tile fully consumed
     stg.template store<LQ, LV>(ks, vt);
     __syncthreads();
     if (kt + 1 < t_end) {
-      const int64_t nx = kt0 + 64;
+      const int64_t nx = first_key(kt + 1);
       stg.load(kg + nx * a.k_stride_t, vg + nx * a.v_stride_t, a.k_stride_t, a.v_stride_t,
-               (int)min((int64_t)64, hi - nx));
+               (int)min((int64_t)64, last_key(kt + 1) - nx));
     }
 
     // S = Q K^T for this wave's 16 queries x 64 keys (4 tiles of 16 keys)
@@ -405,7 +415,7 @@ __global__ void __launch_bounds__(kThreads) k_swa_prefill(const uttt_swa_prefill
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
         const int64_t key = kt0 + 16 * n + c;
-        const bool vis = qi < a.q_len && key < hi && p - key >= 0 && p - key < a.window;
+        const bool vis = qi < a.q_len && key < kt1 && p - key >= 0 && (p - key < a.window || (SINK && key < sinks));
         const float val = vis ? s[n][i] * a.scale : -INFINITY;
         s[n][i] = val;
         mx = fmaxf(mx, val);
@@ -1043,14 +1053,18 @@ __global__ void __launch_bounds__(kThreads) k_swa_decode_combine(const uttt_swa_
 }
 
 template <typename T, int HD>
-static void launch_prefill(const uttt_swa_prefill_args& a, const PrefillPlan& p, hipStream_t st) {
+static void launch_prefill(const uttt_swa_prefill_args& a, int64_t sinks, const PrefillPlan& p, hipStream_t st) {
   float* part = static_cast<float*>(a.workspace);
   if constexpr (sizeof(T) == 2) {
-    launch_swa_prefill_mm(a, part, p.q_pad, st);
+    launch_swa_prefill_mm(a, sinks, part, p.q_pad, st);
   } else {
     const dim3 grid((unsigned)row_tile_blocks((int)(a.batch * a.n_kv_heads), p.nqt * (int)(a.n_heads / a.n_kv_heads) * p.nsplit));
-    hipLaunchKernelGGL(k_swa_prefill<HD>, grid, dim3(kThreads), 0, st, a, part, p.nsplit, p.tiles_per_split,
-                       p.q_pad, p.nqt);
+    if (sinks > 0)
+      hipLaunchKernelGGL((k_swa_prefill<HD, true>), grid, dim3(kThreads), 0, st, a, part, p.nsplit, p.tiles_per_split,
+                         p.q_pad, p.nqt, sinks);
+    else
+      hipLaunchKernelGGL((k_swa_prefill<HD, false>), grid, dim3(kThreads), 0, st, a, part, p.nsplit, p.tiles_per_split,
+                         p.q_pad, p.nqt, sinks);
   }
   if (p.nsplit > 1)
     hipLaunchKernelGGL((k_swa_prefill_combine<T, HD>),
@@ -1170,17 +1184,22 @@ extern "C" int uttt_rope_kv_roll(const uttt_rope_append_args* a, const uttt_kv_r
   return launch_status("uttt_rope_kv_roll");
 }
 
-extern "C" size_t uttt_swa_prefill_workspace(int64_t batch, int64_t n_heads, int64_t q_len, int64_t kv_len,
-                                             int64_t head_dim, int64_t window) {
-  if (batch < 1 || n_heads < 1 || q_len < 1 || kv_len < 1 || window < 1 || head_dim < 1) return 0;
+extern "C" size_t uttt_swa_prefill_sinks_workspace(int64_t batch, int64_t n_heads, int64_t q_len, int64_t kv_len,
+                                                   int64_t head_dim, int64_t window, int64_t sinks) {
+  if (batch < 1 || n_heads < 1 || q_len < 1 || kv_len < 1 || window < 1 || head_dim < 1 || sinks < 0) return 0;
   // the query does not name the type or the kv heads: room for either type's splits
-  const PrefillPlan p = prefill_plan(batch, n_heads, q_len, kv_len, window);
-  const int nsplit = std::max(p.nsplit, swa_prefill_mm_max_splits(batch, n_heads, q_len, kv_len, window));
+  const PrefillPlan p = prefill_plan(batch, n_heads, q_len, kv_len, window, sinks);
+  const int nsplit = std::max(p.nsplit, swa_prefill_mm_max_splits(batch, n_heads, q_len, kv_len, window, sinks));
   if (nsplit == 1) return 16;
   return sizeof(float) * (size_t)nsplit * (size_t)batch * (size_t)n_heads * (size_t)p.q_pad * (size_t)(head_dim + 2);
 }
 
-extern "C" int uttt_swa_prefill(const uttt_swa_prefill_args* a, uttt_stream_t stream) {
+extern "C" size_t uttt_swa_prefill_workspace(int64_t batch, int64_t n_heads, int64_t q_len, int64_t kv_len,
+                                             int64_t head_dim, int64_t window) {
+  return uttt_swa_prefill_sinks_workspace(batch, n_heads, q_len, kv_len, head_dim, window, 0);
+}
+
+static int swa_prefill(const uttt_swa_prefill_args* a, int64_t sinks, hipStream_t st, const char* name) {
   UTTT_REQUIRE(a != nullptr, "args is NULL");
   UTTT_REQUIRE(a->head_dim == 64 || a->head_dim == 128, "head_dim must be 64 or 128 (got %lld)", (long long)a->head_dim);
   UTTT_REQUIRE(a->batch >= 1 && a->n_heads >= 1 && a->n_heads <= 65535, "batch / n_heads out of range");
@@ -1200,22 +1219,32 @@ extern "C" int uttt_swa_prefill(const uttt_swa_prefill_args* a, uttt_stream_t st
   UTTT_REQUIRE(a->k_stride_t >= a->head_dim && a->v_stride_t >= a->head_dim &&
                    a->k_stride_t * 64 * 4 <= 0x7fffffffLL && a->v_stride_t * 64 * 4 <= 0x7fffffffLL,
                "k/v token strides must cover a row and fit a 64-row buffer range");
-  PrefillPlan p = prefill_plan(a->batch, a->n_heads, a->q_len, a->kv_len, a->window);
-  if (a->act_dtype == UTTT_DTYPE_BF16) p.nsplit = swa_prefill_mm_splits(*a);
+  PrefillPlan p = prefill_plan(a->batch, a->n_heads, a->q_len, a->kv_len, a->window, sinks);
+  if (a->act_dtype == UTTT_DTYPE_BF16) p.nsplit = swa_prefill_mm_splits(*a, sinks);
   UTTT_REQUIRE(a->batch * p.nsplit <= 65535 && a->batch * a->n_heads * p.nqt * p.nsplit + 8LL * a->n_heads <= 0x7fffffffLL,
                "batch too large for the attention grid");
   UTTT_REQUIRE(p.nsplit == 1 || (a->workspace != nullptr &&
-                                 a->workspace_bytes >= uttt_swa_prefill_workspace(a->batch, a->n_heads, a->q_len,
-                                                                                  a->kv_len, a->head_dim, a->window)),
+                                 a->workspace_bytes >= uttt_swa_prefill_sinks_workspace(a->batch, a->n_heads,
+                                                                                        a->q_len, a->kv_len, a->head_dim,
+                                                                                        a->window, sinks)),
                "attention workspace too small");
-  hipStream_t st = static_cast<hipStream_t>(stream);
   const bool b16 = a->act_dtype == UTTT_DTYPE_BF16;
   if (a->head_dim == 64) {
-    if (b16) launch_prefill<bf16, 64>(*a, p, st); else launch_prefill<float, 64>(*a, p, st);
+    if (b16) launch_prefill<bf16, 64>(*a, sinks, p, st); else launch_prefill<float, 64>(*a, sinks, p, st);
   } else {
-    if (b16) launch_prefill<bf16, 128>(*a, p, st); else launch_prefill<float, 128>(*a, p, st);
+    if (b16) launch_prefill<bf16, 128>(*a, sinks, p, st); else launch_prefill<float, 128>(*a, sinks, p, st);
   }
-  return launch_status("uttt_swa_prefill");
+  return launch_status(name);
+}
+
+extern "C" int uttt_swa_prefill(const uttt_swa_prefill_args* a, uttt_stream_t stream) {
+  return swa_prefill(a, 0, static_cast<hipStream_t>(stream), "uttt_swa_prefill");
+}
+
+extern "C" int uttt_swa_prefill_sinks(const uttt_swa_prefill_args* a, int64_t sinks, uttt_stream_t stream) {
+  UTTT_REQUIRE(a != nullptr, "args is NULL");
+  UTTT_REQUIRE(sinks >= 0 && a->kv_len < (1LL << 31), "sinks must be >= 0 and kv_len below 2^31");
+  return swa_prefill(a, sinks, static_cast<hipStream_t>(stream), "uttt_swa_prefill_sinks");
 }
 
 extern "C" size_t uttt_swa_decode_workspace(int64_t n_req, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,

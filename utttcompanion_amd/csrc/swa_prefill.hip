@@ -45,7 +45,7 @@ struct SwaMmArgs {
   int n_kv_heads, rep, heads;
   int q_len, nqb, wgs;  // 32-query blocks, workgroups per (row, kv head) and split
   int nsplit, tiles_per_split, q_pad, groups;
-  int64_t q_offset, kv_len, window;
+  int64_t q_offset, kv_len, window, sinks;
   float scale, q_sign;  // scale > 0; Q enters times q_sign
   const bf16 *q, *k, *v;
   int64_t q_sb, q_sh, q_st, k_sb, k_sh, k_st, v_sb, v_sh, v_st;
@@ -102,7 +102,9 @@ __device__ __forceinline__ void pv_mfma(f32x16 (&o)[NB], const i16x4 (&f)[2 * NB
   }
 }
 
-template <int HD, int NW>
+// SINK: the first a.sinks keys stay visible.  Those ahead of the workgroup's window come first, as tiles of their own
+// (whose last may be partly empty), then the window's tiles as without them.
+template <int HD, int NW, bool SINK>
 __global__ void __launch_bounds__(NW * 64, NW >= 6 ? 1 : 2) k_swa_prefill_mm(const SwaMmArgs a) {
   constexpr int NT = HD / 64;          // 64-dim tiles of K and of V per 64 keys
   constexpr int NB = HD / 32;          // 32-dim output blocks
@@ -125,8 +127,14 @@ __global__ void __launch_bounds__(NW * 64, NW >= 6 ? 1 : 2) k_swa_prefill_mm(con
   const int qb_first = u0 / a.rep, qb_last = min(u0 + NW - 1, units - 1) / a.rep;
   const int64_t lo = max((int64_t)0, a.q_offset + qb_first * kQB - a.window + 1);
   const int64_t hi = a.q_offset + min((int64_t)a.q_len, (int64_t)(qb_last + 1) * kQB);  // <= kv_len
-  const int ntiles = (int)((hi - lo + 63) / 64);
+  const int64_t sink_hi = SINK ? min(lo, a.sinks) : 0;
+  const int nsink = SINK ? (int)((sink_hi + 63) / 64) : 0;
+  const int ntiles = nsink + (int)((hi - lo + 63) / 64);
   const int t_begin = sp * a.tiles_per_split, t_end = min(ntiles, t_begin + a.tiles_per_split);
+  auto first_key = [&](int t) {  // of tile t
+    if constexpr (SINK) return t < nsink ? (int64_t)t * 64 : lo + (int64_t)(t - nsink) * 64;
+    return lo + (int64_t)t * 64;
+  };
 
   const int qi = qb * kQB + r;  // this lane's query
   const bool q_ok = unit_ok && qi < a.q_len;
@@ -179,8 +187,8 @@ __global__ void __launch_bounds__(NW * 64, NW >= 6 ? 1 : 2) k_swa_prefill_mm(con
     dst[i] = ring0 + (uint32_t)(g * 1024);
   }
   auto issue = [&](int t) {
-    const int64_t kt0 = lo + (int64_t)t * 64;
-    const int n = (int)min((int64_t)64, hi - kt0);  // keys past hi read as zeros
+    const int64_t kt0 = first_key(t);
+    const int n = (int)min((int64_t)64, (SINK && t < nsink ? sink_hi : hi) - kt0);  // keys past them read as zeros
     const uint32_t so = (uint32_t)((t & 1) * SLOT);
 #pragma unroll
     for (int i = 0; i < PER; ++i)
@@ -215,8 +223,9 @@ __global__ void __launch_bounds__(NW * 64, NW >= 6 ? 1 : 2) k_swa_prefill_mm(con
     wait_vmcnt<0>();
     __builtin_amdgcn_s_barrier();  // the tile is in LDS; every wave is done with the other slot
     if (t + 1 < t_end) issue(t + 1);
-    const int64_t kt0 = lo + (int64_t)t * 64;
-    if (!unit_ok || kt0 > p_last || kt0 + 63 <= p_first - a.window) continue;  // wave-uniform
+    const int64_t kt0 = first_key(t);
+    if (!unit_ok || kt0 > p_last) continue;  // wave-uniform
+    if ((!SINK || kt0 >= a.sinks) && kt0 + 63 <= p_first - a.window) continue;
     const uint32_t so = (uint32_t)((t & 1) * SLOT);
 
     f32x16 s[2];
@@ -258,7 +267,13 @@ __global__ void __launch_bounds__(NW * 64, NW >= 6 ? 1 : 2) k_swa_prefill_mm(con
         mm(f1, qf[7]);
       }
     }
-    if (kt0 + 63 > p_first || p_last - kt0 >= a.window) {  // an edge of the window crosses the tile
+    if (SINK && kt0 < a.sinks) {  // sinks, and what of the window shares their tile
+      const int rel = (int)(p_first - kt0) + r, end = t < nsink ? (int)(sink_hi - kt0) : 64;
+      const uint64_t seen = bit_range(rel - win + 1, min(rel + 1, end)) |
+                            bit_range(0, min(rel + 1, min(end, (int)(a.sinks - kt0))));
+      mask_keys(s[0], (uint32_t)seen);
+      mask_keys(s[1], (uint32_t)(seen >> 32));
+    } else if (kt0 + 63 > p_first || p_last - kt0 >= a.window) {  // an edge of the window crosses the tile
       const int rel = (int)(p_first - kt0) + r;
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
@@ -362,7 +377,7 @@ struct SwaPlan {
   int nw, wgs, nsplit, tiles_per_split;
 };
 
-SwaPlan plan_swa(const uttt_swa_prefill_args& a) {
+SwaPlan plan_swa(const uttt_swa_prefill_args& a, int64_t sinks) {
   SwaPlan p;
   const int64_t rep = a.n_heads / a.n_kv_heads, nqb = (a.q_len + kQB - 1) / kQB, groups = a.batch * a.n_kv_heads;
   const int big = rep % 3 == 0 ? 6 : 8;
@@ -373,42 +388,43 @@ SwaPlan plan_swa(const uttt_swa_prefill_args& a) {
   // query blocks a workgroup's units can touch, and the key tiles they can see
   const int64_t blocks = std::min<int64_t>(nqb, (p.nw - 1 + rep - 1) / rep + 1);
   const int64_t span = std::min<int64_t>(a.kv_len, std::min<int64_t>(a.window, a.kv_len) + blocks * kQB - 1);
-  const int tiles = (int)((span + 63) / 64);
+  const int tiles = (int)((span + 63) / 64 + (std::min(sinks, a.kv_len) + 63) / 64);
   const int ns = use_big ? 1 : std::min(tiles, wanted_splits(a.batch, a.n_heads, a.q_len));
   p.tiles_per_split = (tiles + ns - 1) / ns;
   p.nsplit = (tiles + p.tiles_per_split - 1) / p.tiles_per_split;
   return p;
 }
 
-template <int HD>
+template <int HD, bool SINK>
 void launch(const SwaMmArgs& m, int nw, dim3 grid, hipStream_t st) {
   if (nw == 3)
-    hipLaunchKernelGGL((k_swa_prefill_mm<HD, 3>), grid, dim3(192), 0, st, m);
+    hipLaunchKernelGGL((k_swa_prefill_mm<HD, 3, SINK>), grid, dim3(192), 0, st, m);
   else if (nw == 4)
-    hipLaunchKernelGGL((k_swa_prefill_mm<HD, 4>), grid, dim3(256), 0, st, m);
+    hipLaunchKernelGGL((k_swa_prefill_mm<HD, 4, SINK>), grid, dim3(256), 0, st, m);
   else if (nw == 6)
-    hipLaunchKernelGGL((k_swa_prefill_mm<HD, 6>), grid, dim3(384), 0, st, m);
+    hipLaunchKernelGGL((k_swa_prefill_mm<HD, 6, SINK>), grid, dim3(384), 0, st, m);
   else
-    hipLaunchKernelGGL((k_swa_prefill_mm<HD, 8>), grid, dim3(512), 0, st, m);
+    hipLaunchKernelGGL((k_swa_prefill_mm<HD, 8, SINK>), grid, dim3(512), 0, st, m);
 }
 
 }  // namespace
 
-int swa_prefill_mm_max_splits(int64_t batch, int64_t n_heads, int64_t q_len, int64_t kv_len, int64_t window) {
-  const int64_t tiles = (std::min<int64_t>(kv_len, window) + 8 * kQB + 63) / 64;
+int swa_prefill_mm_max_splits(int64_t batch, int64_t n_heads, int64_t q_len, int64_t kv_len, int64_t window,
+                              int64_t sinks) {
+  const int64_t tiles = (std::min<int64_t>(kv_len, window) + 8 * kQB + 63) / 64 + (std::min(sinks, kv_len) + 63) / 64;
   return (int)std::min<int64_t>(tiles, wanted_splits(batch, n_heads, q_len));
 }
 
-int swa_prefill_mm_splits(const uttt_swa_prefill_args& a) { return plan_swa(a).nsplit; }
+int swa_prefill_mm_splits(const uttt_swa_prefill_args& a, int64_t sinks) { return plan_swa(a, sinks).nsplit; }
 
-void launch_swa_prefill_mm(const uttt_swa_prefill_args& a, float* part, int q_pad, hipStream_t st) {
-  const SwaPlan p = plan_swa(a);
+void launch_swa_prefill_mm(const uttt_swa_prefill_args& a, int64_t sinks, float* part, int q_pad, hipStream_t st) {
+  const SwaPlan p = plan_swa(a, sinks);
   SwaMmArgs m{};
   m.n_kv_heads = (int)a.n_kv_heads; m.heads = (int)a.n_heads; m.rep = (int)(a.n_heads / a.n_kv_heads);
   m.q_len = (int)a.q_len; m.nqb = (int)((a.q_len + kQB - 1) / kQB); m.wgs = p.wgs;
   m.nsplit = p.nsplit; m.tiles_per_split = p.tiles_per_split; m.q_pad = q_pad;
   m.groups = (int)(a.batch * a.n_kv_heads);
-  m.q_offset = a.q_offset; m.kv_len = a.kv_len; m.window = a.window;
+  m.q_offset = a.q_offset; m.kv_len = a.kv_len; m.window = a.window; m.sinks = sinks;
   // the kernel takes maxima of, and masks, the raw scores, which holds for a positive scale: Q carries
   // the sign of another one (exact in bf16), and for 0 the scores are 0 whatever their scale
   m.scale = a.scale != 0.f ? fabsf(a.scale) : 1.f;
@@ -421,10 +437,11 @@ void launch_swa_prefill_mm(const uttt_swa_prefill_args& a, float* part, int q_pa
   m.o_sb = a.o_stride_b; m.o_sh = a.o_stride_h; m.o_st = a.o_stride_t;
   m.part = part;
   const dim3 grid((unsigned)row_tile_blocks(m.groups, p.wgs * p.nsplit));
-  if (a.head_dim == 64)
-    launch<64>(m, p.nw, grid, st);
-  else
-    launch<128>(m, p.nw, grid, st);
+  if (a.head_dim == 64) {
+    if (sinks > 0) launch<64, true>(m, p.nw, grid, st); else launch<64, false>(m, p.nw, grid, st);
+  } else {
+    if (sinks > 0) launch<128, true>(m, p.nw, grid, st); else launch<128, false>(m, p.nw, grid, st);
+  }
 }
 
 }  // namespace uttt

@@ -109,6 +109,20 @@ __device__ __forceinline__ void zero(f32x16& acc) {
 __device__ __forceinline__ int acc_row(int i) { return 8 * (i >> 2) + 4 * ((threadIdx.x & 63) >> 5) + (i & 3); }
 __device__ __forceinline__ int acc_col() { return threadIdx.x & 31; }
 
+// Bits [lo, hi) of a 64-bit mask, where either end may lie outside.
+__device__ __forceinline__ uint64_t bit_range(int lo, int hi) {
+  lo = max(lo, 0);
+  const uint64_t below = hi >= 64 ? ~0ull : hi <= 0 ? 0 : (1ull << hi) - 1;
+  return lo >= 64 ? 0 : below >> lo << lo;
+}
+
+// Scores of 32 keys (the rows of a wave tile) whose bit is not set become -inf.
+__device__ __forceinline__ void mask_keys(f32x16& s, uint32_t seen) {
+  seen >>= 4 * ((threadIdx.x & 63) >> 5);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s[i] = seen & (1u << (8 * (i >> 2) + (i & 3))) ? s[i] : -INFINITY;
+}
+
 // ---------------------------------------------------------------------------
 // LDS staging of 64 x KT operand tiles (256 threads cooperate)
 // ---------------------------------------------------------------------------

@@ -959,6 +959,66 @@ def greedy_select(logits: Tensor, banned: Sequence[int] = (), active_limit: Opti
     return out
 
 
+def _row_setting(t: Optional[Tensor], rows: int, dtype: torch.dtype, name: str) -> Optional[Tensor]:
+    if t is not None and (t.shape != (rows,) or t.dtype != dtype or not t.is_contiguous()):
+        raise ValueError(f"{name} must be {rows} contiguous {dtype} entries")
+    return t
+
+
+def sample_select(logits: Tensor, uniforms: Tensor, temperature: Tensor, top_k: Optional[Tensor] = None,
+                  top_p: Optional[Tensor] = None, min_p: Optional[Tensor] = None, banned: Sequence[int] = (),
+                  active_limit: Optional[int] = None, out: Optional[Tensor] = None,
+                  logprobs: Optional[Tensor] = None, advance: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
+    """Sampled next tokens (rows,) int64 and the logarithms (rows,) fp32 of their probabilities from
+    logits (rows, vocab) bf16 / fp32 (``uttt_sample_select``), each row with its own settings, all on the
+    device: ``temperature``, ``top_p``, ``min_p`` (rows,) fp32 and ``top_k`` (rows,) int32.  The ``banned``
+    ids and those at or past ``active_limit`` are left out first, then, in the order (logit descending, id
+    ascending) with weights exp((x - max x) / temperature), the first ``top_k`` ids stay (<= 0: all),
+    those of at least ``min_p`` times the largest weight, and those whose mass ahead is at most
+    ``top_p`` of the mass that is left (the rule of reference sample_next_token,
+    model/uttt_model.py:1203-1235).  ``uniforms`` (rows,) fp32 in [0, 1) choose: the first id, in id
+    order, whose cumulative mass exceeds uniform * total.  A row with temperature <= 1e-5 takes the
+    greedy choice (``greedy_select``'s), log-probability 0; a row whose largest logit is not finite
+    takes it too, log-probability NaN.  ``advance`` as in ``greedy_select``."""
+    if logits.dim() != 2 or logits.stride(1) != 1:
+        raise ValueError("logits must be (rows, vocab) with unit column stride")
+    if len(banned) > 8:
+        raise ValueError("at most 8 excluded ids")
+    rows, vocab = logits.shape
+    if not 1 <= vocab <= 1 << 20:
+        raise ValueError("sampling takes vocabularies of 1 to 2^20 ids")
+    dev = logits.device
+    code = _act_code(logits.dtype)
+    _row_setting(uniforms, rows, torch.float32, "uniforms")
+    _row_setting(temperature, rows, torch.float32, "temperature")
+    _row_setting(top_k, rows, torch.int32, "top_k")
+    _row_setting(top_p, rows, torch.float32, "top_p")
+    _row_setting(min_p, rows, torch.float32, "min_p")
+    _row_setting(advance, rows, torch.int64, "advance")
+    _row_setting(out, rows, torch.int64, "out")
+    _row_setting(logprobs, rows, torch.float32, "logprobs")
+    _require_device(dev, uniforms, temperature, top_k, top_p, min_p, advance, out, logprobs)
+    if out is None:
+        out = torch.empty(rows, dtype=torch.int64, device=dev)
+    if logprobs is None:
+        logprobs = torch.empty(rows, dtype=torch.float32, device=dev)
+    if rows == 0:
+        return out, logprobs
+    a = N.SampleArgs()
+    a.rows, a.vocab, a.dtype, a.n_banned = rows, vocab, code, len(banned)
+    for i, t in enumerate(banned):
+        a.banned[i] = int(t)
+    a.active_limit = -1 if active_limit is None else int(active_limit)
+    a.logits, a.row_stride = _p(logits), max(logits.stride(0), vocab) if rows == 1 else logits.stride(0)
+    a.uniforms, a.temperature = _p(uniforms), _p(temperature)
+    a.top_k, a.top_p, a.min_p = _p(top_k), _p(top_p), _p(min_p)
+    a.out, a.logprob, a.advance = _p(out), _p(logprobs), _p(advance)
+    lib = N.load_library()
+    with torch.cuda.device(dev):
+        N.check(lib.uttt_sample_select(C.byref(a), _stream(dev)), "uttt_sample_select")
+    return out, logprobs
+
+
 def readout_workspace(x: Tensor, w_up: Tensor) -> Tensor:
     """A workspace for ``swiglu_readout`` of x (B, T, D) through weights shaped like ``w_up``,
     reused by every later call that it is large enough for.  A call of fewer rows or tokens can need
@@ -1214,9 +1274,11 @@ def _attention_workspace(dev: torch.device, nbytes: int) -> Tensor:
 
 def swa_prefill(q: Tensor, k: Tensor, v: Tensor, window: int, q_offset: int,
                 out: Optional[Tensor] = None, kv_len: Optional[int] = None,
-                workspace: Optional[Tensor] = None, build_only: bool = False):
+                workspace: Optional[Tensor] = None, build_only: bool = False, sinks: int = 0):
     """q (B, H, Tq, hd), k/v (B, Hkv, Tkv, hd) (any strides with hd contiguous).  Query i sits
-    at key index q_offset + i and sees key j iff 0 <= q_offset + i - j < window.  ``out``
+    at key index q_offset + i and sees key j iff 0 <= q_offset + i - j < window.  With ``sinks``
+    the first keys stay visible (0 <= q_offset + i - j and j < sinks) beside the window
+    (``uttt_swa_prefill_sinks``; not with ``build_only``, whose arguments carry no sinks).  ``out``
     (B, H, Tq, hd) may be a strided view, e.g. of a (B, Tq, H, hd) buffer.  Without a
     ``workspace`` the call uses one zero-filled buffer per device, shared by every call: calls on
     concurrent streams must each pass their own.  ``build_only``
@@ -1232,6 +1294,8 @@ def swa_prefill(q: Tensor, k: Tensor, v: Tensor, window: int, q_offset: int,
         raise ValueError("queries must index keys inside the kv range")
     if window < 1:
         raise ValueError("window must be >= 1")
+    if sinks < 0 or (sinks and build_only):
+        raise ValueError("sinks must be >= 0, and a prepared call takes none")
     if k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError("q/k/v must share one dtype")
     vec = 16 // q.element_size()
@@ -1260,7 +1324,7 @@ def swa_prefill(q: Tensor, k: Tensor, v: Tensor, window: int, q_offset: int,
     a.v, a.v_stride_b, a.v_stride_h, a.v_stride_t = _p(v), v.stride(0), v.stride(1), v.stride(2)
     a.out, a.o_stride_b, a.o_stride_h, a.o_stride_t = _p(out), out.stride(0), out.stride(1), out.stride(2)
     lib = N.load_library()
-    nbytes = lib.uttt_swa_prefill_workspace(bsz, heads, tq, tkv, hd, window)
+    nbytes = lib.uttt_swa_prefill_sinks_workspace(bsz, heads, tq, tkv, hd, window, sinks)
     if workspace is None:
         workspace = _attention_workspace(dev, nbytes)
     elif workspace.numel() < nbytes or workspace.device != dev:
@@ -1269,16 +1333,31 @@ def swa_prefill(q: Tensor, k: Tensor, v: Tensor, window: int, q_offset: int,
     if build_only:
         return a
     with torch.cuda.device(dev):
-        N.check(lib.uttt_swa_prefill(C.byref(a), _stream(dev)), "uttt_swa_prefill")
+        if sinks:
+            N.check(lib.uttt_swa_prefill_sinks(C.byref(a), int(sinks), _stream(dev)), "uttt_swa_prefill_sinks")
+        else:
+            N.check(lib.uttt_swa_prefill(C.byref(a), _stream(dev)), "uttt_swa_prefill")
     return out
 
 
 def swa_decode(q: Tensor, k_new: Tensor, v_new: Tensor, k_ring: Tensor, v_ring: Tensor, positions: Tensor,
                cos: Optional[Tensor] = None, sin: Optional[Tensor] = None, out: Optional[Tensor] = None,
-               workspace: Optional[Tensor] = None) -> Tensor:
+               workspace: Optional[Tensor] = None, sinks: int = 0) -> Tensor:
     """One decode step for N requests.  q (N, H, hd), k_new/v_new (N, Hkv, hd) (un-rotated when
-    tables are given), rings (N, Hkv, W, hd), positions (N,) int64 on the device."""
+    tables are given), rings (N, Hkv, W, hd), positions (N,) int64 on the device.  With ``sinks``
+    the rings hold sinks + W slots: the first tokens keep the first ``sinks`` of them and stay
+    visible, the others share the last W as a ring (``uttt_swa_tree`` with one node)."""
     n, heads, hd = q.shape
+    if sinks < 0:
+        raise ValueError("sinks must be >= 0")
+    if sinks:
+        if k_new.shape != v_new.shape or k_new.dim() != 3 or positions.shape != (n,):
+            raise ValueError("k_new / v_new must be (N, Hkv, hd) and positions (N,)")
+        if out is not None and out.shape != q.shape:
+            raise ValueError("out must match q's shape")
+        res = _tree_call(q[:, None], k_new[:, None], v_new[:, None], k_ring, v_ring, positions, None, cos, sin, sinks,
+                         None, None if out is None else out[:, None], workspace, write_ring=True)[0]
+        return res[:, 0]
     hkv, window = k_ring.shape[1], k_ring.shape[2]
     if k_new.shape != (n, hkv, hd) or v_new.shape != k_new.shape:
         raise ValueError("k_new / v_new must be (N, Hkv, hd)")
@@ -1319,6 +1398,233 @@ def swa_decode(q: Tensor, k_new: Tensor, v_new: Tensor, k_ring: Tensor, v_ring: 
     with torch.cuda.device(dev):
         N.check(lib.uttt_swa_decode(C.byref(a), _stream(dev)), "uttt_swa_decode")
     return out
+
+
+def _pieces(t: Tensor) -> Tensor:
+    """``t`` with a contiguous last dimension and 16-byte aligned rows (a copy where it is not)."""
+    vec = 16 // t.element_size()
+    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % vec for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _whole(strides: Sequence[int], shape: Sequence[int]) -> Tuple[int, ...]:
+    """Strides of dimensions of one element do not matter: 0."""
+    return tuple(s if n > 1 else 0 for s, n in zip(strides, shape))
+
+
+def _rings(k_ring: Tensor, v_ring: Tensor, lead: int, name: str) -> None:
+    """k_ring / v_ring (.., Hkv, slots, hd) with ``lead`` leading dimensions: alike, each request's
+    part contiguous."""
+    if k_ring.dim() != lead + 3 or v_ring.shape != k_ring.shape or v_ring.dtype != k_ring.dtype:
+        raise ValueError(f"rings must be two {name} tensors of one dtype")
+    _act_code(k_ring.dtype)
+    for r in (k_ring, v_ring):
+        if r.numel() == 0:
+            continue
+        if not r[(0,) * lead].is_contiguous():
+            raise ValueError("each request's rings must be contiguous")
+        vec = 16 // r.element_size()
+        if r.data_ptr() % 16 or any(s % vec for s, n in zip(r.stride()[:lead], r.shape[:lead]) if n > 1):
+            raise ValueError("rings must be 16-byte aligned")
+    if _whole(k_ring.stride()[:lead], k_ring.shape) != _whole(v_ring.stride()[:lead], v_ring.shape):
+        raise ValueError("k and v rings must share their strides")
+
+
+def _tree_call(q: Tensor, k_new: Tensor, v_new: Tensor, k_ring: Tensor, v_ring: Tensor, positions: Tensor,
+               parents: Optional[Tensor], cos: Optional[Tensor], sin: Optional[Tensor], sinks: int,
+               counts: Optional[Tensor], out: Optional[Tensor], workspace: Optional[Tensor], write_ring: bool,
+               node_outputs: Optional[Tuple[Tensor, Tensor]] = None) -> Tuple[Tensor, Optional[Tensor], Optional[Tensor]]:
+    n, nodes, heads, hd = q.shape
+    if not 1 <= nodes <= N.MAX_TREE_NODES:
+        raise ValueError(f"a tree has 1 to {N.MAX_TREE_NODES} nodes, got {nodes}")
+    _rings(k_ring, v_ring, 1, "(N, Hkv, slots, hd)")
+    hkv, slots = k_ring.shape[1], k_ring.shape[2]
+    window = slots - sinks
+    if sinks < 0 or window < 1:
+        raise ValueError("rings must have sinks >= 0 slots and a window of at least one behind them")
+    if k_ring.shape != (n, hkv, slots, hd) or k_new.shape != (n, nodes, hkv, hd) or v_new.shape != k_new.shape:
+        raise ValueError("new keys / values must be (N, nodes, Hkv, hd) and rings (N, Hkv, slots, hd)")
+    if hd not in (64, 128) or heads % hkv:
+        raise ValueError("head_dim must be 64/128 and n_heads a multiple of n_kv_heads")
+    if any(t.dtype != q.dtype for t in (k_new, v_new, k_ring)):
+        raise ValueError("q, new keys / values and rings must share one dtype")
+    if positions.shape != (n,) or positions.dtype != torch.int64 or not positions.is_contiguous():
+        raise ValueError("positions must be an int64 (N,) device tensor")
+    if parents is not None and (parents.shape != (n, nodes) or parents.dtype != torch.int32
+                                or not parents.is_contiguous()):
+        raise ValueError("parents must be a contiguous int32 (N, nodes) tensor")
+    if counts is not None and (counts.shape != (n,) or counts.dtype != torch.int32 or not counts.is_contiguous()):
+        raise ValueError("counts must be an int32 (N,) device tensor")
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin must both be given or both omitted")
+    for t in (cos, sin):
+        if t is not None and (t.dim() != 2 or t.shape != cos.shape or t.shape[1] != hd or t.dtype != torch.float32
+                              or not t.is_contiguous() or t.data_ptr() % 16):
+            raise ValueError("cos / sin must be contiguous fp32 (positions, head_dim) tables")
+    dev = q.device
+    _require_device(dev, k_new, v_new, k_ring, v_ring, positions, parents, counts, cos, sin, out, workspace)
+    _forward_only(q, k_new, v_new, k_ring, v_ring)
+    given = out
+    if out is None:
+        out = torch.empty((n, nodes, heads, hd), dtype=q.dtype, device=dev)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError("out must match q's shape and dtype")
+    elif _pieces(out) is not out:
+        raise ValueError("out must have contiguous, 16-byte aligned heads")
+    k_nodes = v_nodes = None
+    if not write_ring:
+        if node_outputs is not None:
+            k_nodes, v_nodes = node_outputs
+            for t in node_outputs:
+                if (t.shape != k_new.shape or t.dtype != q.dtype or not t.is_contiguous() or t.data_ptr() % 16
+                        or t.device != dev):
+                    raise ValueError("node outputs must be contiguous (N, nodes, Hkv, hd) tensors of q's dtype")
+        elif counts is None:
+            k_nodes = torch.empty((n, nodes, hkv, hd), dtype=q.dtype, device=dev)
+            v_nodes = torch.empty_like(k_nodes)
+        else:  # rows behind a request's nodes are not written
+            k_nodes = torch.zeros((n, nodes, hkv, hd), dtype=q.dtype, device=dev)
+            v_nodes = torch.zeros_like(k_nodes)
+    if counts is not None and given is None:
+        out.zero_()
+    if n == 0:
+        return out, k_nodes, v_nodes
+    q, k_new, v_new = _pieces(q), _pieces(k_new), _pieces(v_new)
+    a = N.SwaTreeArgs()
+    a.n_req, a.n_heads, a.n_kv_heads, a.nodes, a.head_dim = n, heads, hkv, nodes, hd
+    a.window, a.sinks, a.act_dtype, a.write_ring = window, sinks, _act_code(q.dtype), int(write_ring)
+    a.scale = 1.0 / math.sqrt(hd)
+    a.positions, a.parents, a.counts = _p(positions), _p(parents), _p(counts)
+    a.cos_table, a.sin_table = _p(cos), _p(sin)
+    a.table_len = 0 if cos is None else cos.shape[0]
+    a.q, (a.q_stride_n, a.q_stride_t, a.q_stride_h) = _p(q), _whole(q.stride(), q.shape[:3])
+    a.k_new, (a.k_stride_n, a.k_stride_t, a.k_stride_h) = _p(k_new), _whole(k_new.stride(), k_new.shape[:3])
+    a.v_new, (a.v_stride_n, a.v_stride_t, a.v_stride_h) = _p(v_new), _whole(v_new.stride(), v_new.shape[:3])
+    a.k_ring, a.v_ring, a.ring_stride_n = _p(k_ring), _p(v_ring), k_ring.stride(0) if n > 1 else 0
+    a.out, (a.o_stride_n, a.o_stride_t, a.o_stride_h) = _p(out), _whole(out.stride(), out.shape[:3])
+    a.k_nodes, a.v_nodes = _p(k_nodes), _p(v_nodes)
+    lib = N.load_library()
+    nbytes = lib.uttt_swa_tree_workspace(n, heads, hkv, nodes, hd, slots, a.act_dtype)
+    if workspace is None:
+        workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+    elif workspace.numel() * workspace.element_size() < nbytes:
+        raise ValueError(f"the tree attention workspace must hold {nbytes} bytes")
+    a.workspace, a.workspace_bytes = _p(workspace), workspace.numel() * workspace.element_size()
+    with torch.cuda.device(dev):
+        N.check(lib.uttt_swa_tree(C.byref(a), _stream(dev)), "uttt_swa_tree")
+    return out, k_nodes, v_nodes
+
+
+def swa_tree(q: Tensor, k_new: Tensor, v_new: Tensor, k_ring: Tensor, v_ring: Tensor, positions: Tensor,
+             parents: Optional[Tensor] = None, cos: Optional[Tensor] = None, sin: Optional[Tensor] = None,
+             sinks: int = 0, counts: Optional[Tensor] = None, out: Optional[Tensor] = None,
+             node_outputs: Optional[Tuple[Tensor, Tensor]] = None,
+             workspace: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor]:
+    """Attention of a tree of drafted tokens per request over ring caches (``uttt_swa_tree``), up
+    to 64 nodes: q (N, T, H, hd), k_new / v_new (N, T, Hkv, hd) (un-rotated when tables are given), rings
+    (N, Hkv, sinks + W, hd) holding ``positions`` (N,) int64 tokens each, ``parents`` (N, T) int32 (-1:
+    the node follows the cache, else an earlier node; None: a chain).  A node stands at
+    positions + its depth and sees its ancestors, itself and the cached tokens, those less than W
+    back and the first ``sinks``.  Returns the output (N, T, H, hd) and the nodes' keys, rotated, and values
+    (N, T, Hkv, hd) (``node_outputs``, when given), which ``kv_commit`` takes; the rings are not written.
+    ``counts`` (N,) int32: only that many of a request's nodes exist, rows behind them are left as they
+    were (zeros in outputs made here).  A request with parents, or a position, out of range gets NaN outputs.
+    ``workspace``: calls that share one must be ordered."""
+    if q.dim() != 4:
+        raise ValueError("q must be (N, T, H, hd)")
+    return _tree_call(q, k_new, v_new, k_ring, v_ring, positions, parents, cos, sin, int(sinks), counts, out, workspace,
+                      False, node_outputs)
+
+
+def kv_commit(k_nodes: Tensor, v_nodes: Tensor, nodes: Tensor, counts: Tensor, k_ring: Tensor, v_ring: Tensor,
+              positions: Tensor, sinks: int = 0, advance: bool = False) -> None:
+    """The accepted nodes of each request's draft into its rings (``uttt_kv_commit``): node nodes[n, a], for
+    a < counts[n], becomes the token at positions[n] + a.  k_nodes / v_nodes (N, T, Hkv, hd) as ``swa_tree``
+    returns them, or (L, N, T, Hkv, hd) for L layers in one launch, with rings (N, Hkv, sinks + W, hd) or
+    (L, N, Hkv, sinks + W, hd); nodes (N, A) and counts (N,) int32, positions (N,) int64.  With ``advance`` the
+    positions grow by counts afterwards."""
+    layered = k_ring.dim() == 5
+    if not layered:
+        k_ring, v_ring, k_nodes, v_nodes = (t[None] for t in (k_ring, v_ring, k_nodes, v_nodes))
+    _rings(k_ring, v_ring, 2, "([L,] N, Hkv, slots, hd)")
+    layers, n, hkv, slots, hd = k_ring.shape
+    if k_nodes.dim() != 5 or v_nodes.shape != k_nodes.shape or k_nodes.shape[:2] != (layers, n) \
+            or k_nodes.shape[3:] != (hkv, hd):
+        raise ValueError("nodes' keys / values must be ([L,] N, T, Hkv, hd), one row per ring")
+    if k_nodes.dtype != k_ring.dtype or v_nodes.dtype != k_ring.dtype:
+        raise ValueError("nodes and rings must share one dtype")
+    if sinks < 0 or slots - sinks < 1:
+        raise ValueError("rings must have sinks >= 0 slots and a window of at least one behind them")
+    if hd % (16 // k_ring.element_size()):
+        raise ValueError("head_dim must be whole 16-byte pieces")
+    if nodes.dim() != 2 or nodes.shape[0] != n or nodes.dtype != torch.int32 or (nodes.numel() and nodes.stride(1) != 1):
+        raise ValueError("nodes must be int32 (N, A) with unit column stride")
+    if counts.shape != (n,) or counts.dtype != torch.int32 or not counts.is_contiguous():
+        raise ValueError("counts must be an int32 (N,) device tensor")
+    if positions.shape != (n,) or positions.dtype != torch.int64 or not positions.is_contiguous():
+        raise ValueError("positions must be an int64 (N,) device tensor")
+    dev = k_ring.device
+    _require_device(dev, v_ring, k_nodes, v_nodes, nodes, counts, positions)
+    _forward_only(k_nodes, v_nodes, k_ring, v_ring)
+    if layers == 0 or n == 0 or nodes.shape[1] == 0 or k_nodes.shape[2] == 0:
+        return
+    fixed = []
+    for t in (k_nodes, v_nodes):
+        vec = 16 // t.element_size()
+        if not t[0, 0].is_contiguous() or t.data_ptr() % 16 or any(
+                s % vec for s, m in zip(t.stride()[:2], t.shape[:2]) if m > 1):
+            t = t.clone(memory_format=torch.contiguous_format)
+        fixed.append(t)
+    if _whole(fixed[0].stride()[:2], (layers, n)) != _whole(fixed[1].stride()[:2], (layers, n)):
+        fixed = [t.clone(memory_format=torch.contiguous_format) for t in fixed]
+    k_nodes, v_nodes = fixed
+    a = N.KvCommitArgs()
+    a.layers, a.n_req, a.n_kv_heads, a.n_nodes, a.path, a.head_dim = layers, n, hkv, k_nodes.shape[2], nodes.shape[1], hd
+    a.window, a.sinks, a.act_dtype, a.advance = slots - sinks, sinks, _act_code(k_ring.dtype), int(bool(advance))
+    a.k_nodes, a.v_nodes = _p(k_nodes), _p(v_nodes)
+    a.nodes_stride_l, a.nodes_stride_n = _whole(k_nodes.stride()[:2], (layers, n))
+    a.nodes, a.path_stride, a.counts = _p(nodes), nodes.stride(0), _p(counts)
+    a.k_ring, a.v_ring = _p(k_ring), _p(v_ring)
+    a.ring_stride_l, a.ring_stride_n = _whole(k_ring.stride()[:2], (layers, n))
+    a.positions = _p(positions)
+    lib = N.load_library()
+    with torch.cuda.device(dev):
+        N.check(lib.uttt_kv_commit(C.byref(a), _stream(dev)), "uttt_kv_commit")
+
+
+def kv_fork(k_ring: Tensor, v_ring: Tensor, sources: Tensor, positions: Tensor) -> None:
+    """Requests' caches copied over others', in place (``uttt_kv_fork``): request n takes the used slots and the
+    position of request sources[n], as they were before the call, whatever the map (forks of one
+    prompt, beams reordered, gaps closed).  Rings (N, Hkv, slots, hd), or (L, N, Hkv, slots, hd) for L layers in
+    one launch, of at most 128 requests; sources (N,) int32 (n itself, or an id out of range: left as it
+    was), positions (N,) int64."""
+    if k_ring.dim() == 4:
+        k_ring, v_ring = k_ring[None], v_ring[None]
+    _rings(k_ring, v_ring, 2, "([L,] N, Hkv, slots, hd)")
+    layers, n, hkv, slots, hd = k_ring.shape
+    if n > N.MAX_FORK_REQUESTS:
+        raise ValueError(f"at most {N.MAX_FORK_REQUESTS} requests")
+    if hd % (16 // k_ring.element_size()):
+        raise ValueError("head_dim must be whole 16-byte pieces")
+    if sources.shape != (n,) or sources.dtype != torch.int32 or not sources.is_contiguous():
+        raise ValueError("sources must be an int32 (N,) device tensor")
+    if positions.shape != (n,) or positions.dtype != torch.int64 or not positions.is_contiguous():
+        raise ValueError("positions must be an int64 (N,) device tensor")
+    dev = k_ring.device
+    _require_device(dev, v_ring, sources, positions)
+    _forward_only(k_ring, v_ring)
+    if layers == 0 or n == 0:
+        return
+    a = N.KvForkArgs()
+    a.layers, a.n_req, a.n_kv_heads, a.slots, a.head_dim = layers, n, hkv, slots, hd
+    a.act_dtype, a.sources = _act_code(k_ring.dtype), _p(sources)
+    a.k_ring, a.v_ring = _p(k_ring), _p(v_ring)
+    a.ring_stride_l, a.ring_stride_n = _whole(k_ring.stride()[:2], (layers, n))
+    a.positions = _p(positions)
+    lib = N.load_library()
+    with torch.cuda.device(dev):
+        N.check(lib.uttt_kv_fork(C.byref(a), _stream(dev)), "uttt_kv_fork")
 
 
 # ---------------------------------------------------------------------------
