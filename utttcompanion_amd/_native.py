@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 import threading
 
 from .build import HEADER_PATH, LIB_PATH
@@ -331,15 +332,31 @@ class KvForkArgs(C.Structure):
     ]
 
 
+def _packer(args):
+    """A function of an argument block's fields, in order (pointers as integers), to its bytes: what a call costs the
+    host is mostly Python, and one pack is several times cheaper than setting forty ctypes fields."""
+    codes = {_P: "P", _I64: "q", _I32: "i", _F: "f", C.c_size_t: "N", _I32 * 8: "8i"}
+    packed = struct.Struct("@" + "".join(codes[kind] for _, kind in args._fields_) + "0q")
+    if packed.size != C.sizeof(args):
+        raise RuntimeError(f"the layout of {args.__name__} is not the platform's")
+    return packed.pack
+
+
+pack_sample = _packer(SampleArgs)
+pack_swa_tree = _packer(SwaTreeArgs)
+pack_kv_commit = _packer(KvCommitArgs)
+pack_kv_fork = _packer(KvForkArgs)
+
+# the argument blocks of these calls may come as bytes
 SERVE_SIGNATURES = {
     "uttt_serve_abi_version": (C.c_int, []),
-    "uttt_sample_select": (C.c_int, [C.POINTER(SampleArgs), _P]),
+    "uttt_sample_select": (C.c_int, [_P, _P]),
     "uttt_swa_prefill_sinks_workspace": (C.c_size_t, [_I64, _I64, _I64, _I64, _I64, _I64, _I64]),
     "uttt_swa_prefill_sinks": (C.c_int, [C.POINTER(SwaPrefillArgs), _I64, _P]),
     "uttt_swa_tree_workspace": (C.c_size_t, [_I64, _I64, _I64, _I64, _I64, _I64, _I32]),
-    "uttt_swa_tree": (C.c_int, [C.POINTER(SwaTreeArgs), _P]),
-    "uttt_kv_commit": (C.c_int, [C.POINTER(KvCommitArgs), _P]),
-    "uttt_kv_fork": (C.c_int, [C.POINTER(KvForkArgs), _P]),
+    "uttt_swa_tree": (C.c_int, [_P, _P]),
+    "uttt_kv_commit": (C.c_int, [_P, _P]),
+    "uttt_kv_fork": (C.c_int, [_P, _P]),
 }
 
 _lib = None

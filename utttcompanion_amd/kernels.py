@@ -51,6 +51,29 @@ def _stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def _serve_call(fn, packed: bytes, index: int, what: str) -> None:
+    """A serving call on the current stream of GPU ``index``: the device is only switched where it is not the current
+    one, and the stream's handle is read without making a stream object."""
+    if torch.cuda.current_device() == index:
+        rc = fn(packed, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(packed, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        N.check(rc, what)
+
+
+def _gpu_index(t: Tensor, *others: Optional[Tensor]) -> int:
+    """The GPU that all tensors lie on (``_require_device``'s rules)."""
+    index = t.get_device()
+    if index < 0:
+        raise ValueError("the uTTT HIP kernels need GPU (ROCm) tensors; there is no CPU path")
+    for o in others:
+        if o is not None and o.get_device() != index:
+            raise ValueError(f"all tensors must be on {t.device}, found one on {o.device}")
+    return index
+
+
 def _rows(x: Tensor) -> Tensor:
     """(B, T, D) with feature stride 1, token stride D and a 16-byte aligned base and row
     stride (the kernels read activations with 16-byte vector loads)."""
@@ -959,10 +982,13 @@ def greedy_select(logits: Tensor, banned: Sequence[int] = (), active_limit: Opti
     return out
 
 
-def _row_setting(t: Optional[Tensor], rows: int, dtype: torch.dtype, name: str) -> Optional[Tensor]:
-    if t is not None and (t.shape != (rows,) or t.dtype != dtype or not t.is_contiguous()):
+def _row_setting(t: Optional[Tensor], rows: int, dtype: torch.dtype, name: str) -> int:
+    """The address of a per-row tensor, 0 for None."""
+    if t is None:
+        return 0
+    if t.dtype is not dtype or t.shape != (rows,) or not t.is_contiguous():
         raise ValueError(f"{name} must be {rows} contiguous {dtype} entries")
-    return t
+    return t.data_ptr()
 
 
 def sample_select(logits: Tensor, uniforms: Tensor, temperature: Tensor, top_k: Optional[Tensor] = None,
@@ -987,35 +1013,28 @@ def sample_select(logits: Tensor, uniforms: Tensor, temperature: Tensor, top_k: 
     rows, vocab = logits.shape
     if not 1 <= vocab <= 1 << 20:
         raise ValueError("sampling takes vocabularies of 1 to 2^20 ids")
-    dev = logits.device
     code = _act_code(logits.dtype)
-    _row_setting(uniforms, rows, torch.float32, "uniforms")
-    _row_setting(temperature, rows, torch.float32, "temperature")
-    _row_setting(top_k, rows, torch.int32, "top_k")
-    _row_setting(top_p, rows, torch.float32, "top_p")
-    _row_setting(min_p, rows, torch.float32, "min_p")
-    _row_setting(advance, rows, torch.int64, "advance")
-    _row_setting(out, rows, torch.int64, "out")
-    _row_setting(logprobs, rows, torch.float32, "logprobs")
-    _require_device(dev, uniforms, temperature, top_k, top_p, min_p, advance, out, logprobs)
+    f32, i64 = torch.float32, torch.int64
+    p_u = _row_setting(uniforms, rows, f32, "uniforms")
+    p_t = _row_setting(temperature, rows, f32, "temperature")
+    p_k = _row_setting(top_k, rows, torch.int32, "top_k")
+    p_p = _row_setting(top_p, rows, f32, "top_p")
+    p_m = _row_setting(min_p, rows, f32, "min_p")
+    p_a = _row_setting(advance, rows, i64, "advance")
+    index = _gpu_index(logits, uniforms, temperature, top_k, top_p, min_p, advance, out, logprobs)
     if out is None:
-        out = torch.empty(rows, dtype=torch.int64, device=dev)
+        out = logits.new_empty(rows, dtype=i64)
     if logprobs is None:
-        logprobs = torch.empty(rows, dtype=torch.float32, device=dev)
+        logprobs = logits.new_empty(rows, dtype=f32)
+    p_o, p_l = _row_setting(out, rows, i64, "out"), _row_setting(logprobs, rows, f32, "logprobs")
     if rows == 0:
         return out, logprobs
-    a = N.SampleArgs()
-    a.rows, a.vocab, a.dtype, a.n_banned = rows, vocab, code, len(banned)
-    for i, t in enumerate(banned):
-        a.banned[i] = int(t)
-    a.active_limit = -1 if active_limit is None else int(active_limit)
-    a.logits, a.row_stride = _p(logits), max(logits.stride(0), vocab) if rows == 1 else logits.stride(0)
-    a.uniforms, a.temperature = _p(uniforms), _p(temperature)
-    a.top_k, a.top_p, a.min_p = _p(top_k), _p(top_p), _p(min_p)
-    a.out, a.logprob, a.advance = _p(out), _p(logprobs), _p(advance)
-    lib = N.load_library()
-    with torch.cuda.device(dev):
-        N.check(lib.uttt_sample_select(C.byref(a), _stream(dev)), "uttt_sample_select")
+    ids = [int(b) for b in banned]
+    stride = logits.stride(0) if rows > 1 else vocab
+    packed = N.pack_sample(rows, vocab, code, len(ids), *ids, *([0] * (8 - len(ids))),
+                           -1 if active_limit is None else int(active_limit), logits.data_ptr(), stride,
+                           p_u, p_t, p_k, p_p, p_m, p_o, p_l, p_a)
+    _serve_call(N.load_library().uttt_sample_select, packed, index, "uttt_sample_select")
     return out, logprobs
 
 
@@ -1351,13 +1370,8 @@ def swa_decode(q: Tensor, k_new: Tensor, v_new: Tensor, k_ring: Tensor, v_ring: 
     if sinks < 0:
         raise ValueError("sinks must be >= 0")
     if sinks:
-        if k_new.shape != v_new.shape or k_new.dim() != 3 or positions.shape != (n,):
-            raise ValueError("k_new / v_new must be (N, Hkv, hd) and positions (N,)")
-        if out is not None and out.shape != q.shape:
-            raise ValueError("out must match q's shape")
-        res = _tree_call(q[:, None], k_new[:, None], v_new[:, None], k_ring, v_ring, positions, None, cos, sin, sinks,
-                         None, None if out is None else out[:, None], workspace, write_ring=True)[0]
-        return res[:, 0]
+        return _tree_call(q, k_new, v_new, k_ring, v_ring, positions, None, cos, sin, sinks, None, out, workspace,
+                          write_ring=True)[0]
     hkv, window = k_ring.shape[1], k_ring.shape[2]
     if k_new.shape != (n, hkv, hd) or v_new.shape != k_new.shape:
         raise ValueError("k_new / v_new must be (N, Hkv, hd)")
@@ -1400,119 +1414,151 @@ def swa_decode(q: Tensor, k_new: Tensor, v_new: Tensor, k_ring: Tensor, v_ring: 
     return out
 
 
-def _pieces(t: Tensor) -> Tensor:
-    """``t`` with a contiguous last dimension and 16-byte aligned rows (a copy where it is not)."""
+def _pieces(t: Tensor, lead: int) -> Tensor:
+    """``t`` with whole 16-byte pieces behind its first ``lead`` dimensions (contiguous there, aligned, strides of
+    whole pieces): itself, or a copy where it is not."""
     vec = 16 // t.element_size()
-    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % vec for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
+    inner = 1
+    for n, s in zip(reversed(t.shape[lead:]), reversed(t.stride()[lead:])):
+        if n > 1 and s != inner:
+            return t.clone(memory_format=torch.contiguous_format)
+        inner *= n
+    if t.data_ptr() % 16 or any(s % vec for s, n in zip(t.stride()[:lead], t.shape[:lead]) if n > 1):
         return t.clone(memory_format=torch.contiguous_format)
     return t
 
 
-def _whole(strides: Sequence[int], shape: Sequence[int]) -> Tuple[int, ...]:
-    """Strides of dimensions of one element do not matter: 0."""
-    return tuple(s if n > 1 else 0 for s, n in zip(strides, shape))
+def _strides(t: Tensor, lead: int) -> Tuple[int, ...]:
+    """The first ``lead`` strides; those of dimensions of one element, which do not matter, as 0."""
+    return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:lead], t.shape[:lead]))
 
 
-def _rings(k_ring: Tensor, v_ring: Tensor, lead: int, name: str) -> None:
-    """k_ring / v_ring (.., Hkv, slots, hd) with ``lead`` leading dimensions: alike, each request's
-    part contiguous."""
-    if k_ring.dim() != lead + 3 or v_ring.shape != k_ring.shape or v_ring.dtype != k_ring.dtype:
-        raise ValueError(f"rings must be two {name} tensors of one dtype")
-    _act_code(k_ring.dtype)
-    for r in (k_ring, v_ring):
-        if r.numel() == 0:
-            continue
-        if not r[(0,) * lead].is_contiguous():
-            raise ValueError("each request's rings must be contiguous")
-        vec = 16 // r.element_size()
-        if r.data_ptr() % 16 or any(s % vec for s, n in zip(r.stride()[:lead], r.shape[:lead]) if n > 1):
-            raise ValueError("rings must be 16-byte aligned")
-    if _whole(k_ring.stride()[:lead], k_ring.shape) != _whole(v_ring.stride()[:lead], v_ring.shape):
-        raise ValueError("k and v rings must share their strides")
+def _heads(t: Tensor, mask: int) -> Tuple[Tensor, int, int, int, int]:
+    """(N, T, H, hd), or (N, H, hd) for T = 1, as ``_pieces`` has it: the tensor, its address and the strides of N, T and
+    H; ``mask``: elements of a 16-byte piece, less one."""
+    s0, *s1, s2, s3 = t.stride()
+    s1 = s1[0] if s1 else 0
+    address = t.data_ptr()
+    if s3 != 1 or (s0 | s1 | s2) & mask or address & 15:
+        t = _pieces(t, t.dim() - 1)
+        s0, *s1, s2 = _strides(t, t.dim() - 1)
+        return t, t.data_ptr(), s0, s1[0] if s1 else 0, s2
+    return t, address, s0, s1, s2
+
+
+def _rings(k_ring: Tensor, v_ring: Tensor, lead: int) -> Tuple[int, ...]:
+    """Strides of the ``lead`` leading dimensions of k_ring / v_ring (.., Hkv, slots, hd): alike, each
+    request's part contiguous and aligned."""
+    shape, ks = k_ring.shape, k_ring.stride()
+    if len(shape) != lead + 3 or v_ring.shape != shape or v_ring.dtype is not k_ring.dtype:
+        raise ValueError(f"rings must be two {'(L, N' if lead == 2 else '(N'}, Hkv, slots, hd) tensors of one dtype")
+    hd = shape[-1]
+    if (v_ring.stride() != ks or ks[lead:] != (shape[-2] * hd, hd, 1)
+            or (ks[0] | ks[lead - 1]) & (7 if k_ring.dtype is torch.bfloat16 else 3)):
+        if 0 in shape:
+            return (0,) * lead
+        for r in (k_ring, v_ring):
+            if _pieces(r, lead) is not r:
+                raise ValueError("each request's rings must be contiguous and 16-byte aligned")
+        if _strides(k_ring, lead) != _strides(v_ring, lead):
+            raise ValueError("k and v rings must share their strides")
+        return _strides(k_ring, lead)
+    if (k_ring.data_ptr() | v_ring.data_ptr()) & 15:
+        raise ValueError("each request's rings must be contiguous and 16-byte aligned")
+    return ks[:lead]
+
+
+def _per_request(t: Tensor, n: int, dtype: torch.dtype, name: str) -> int:
+    if t.dtype is not dtype or t.shape != (n,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be an {dtype} (N,) device tensor".replace("torch.", ""))
+    return t.data_ptr()
 
 
 def _tree_call(q: Tensor, k_new: Tensor, v_new: Tensor, k_ring: Tensor, v_ring: Tensor, positions: Tensor,
                parents: Optional[Tensor], cos: Optional[Tensor], sin: Optional[Tensor], sinks: int,
                counts: Optional[Tensor], out: Optional[Tensor], workspace: Optional[Tensor], write_ring: bool,
                node_outputs: Optional[Tuple[Tensor, Tensor]] = None) -> Tuple[Tensor, Optional[Tensor], Optional[Tensor]]:
-    n, nodes, heads, hd = q.shape
+    """(N, T, H, hd) operands, or (N, H, hd) ones for a node per request (a decode step, ``write_ring``)."""
+    shape = q.shape
+    if write_ring:
+        (n, heads, hd), nodes = shape, 1
+    else:
+        n, nodes, heads, hd = shape
     if not 1 <= nodes <= N.MAX_TREE_NODES:
         raise ValueError(f"a tree has 1 to {N.MAX_TREE_NODES} nodes, got {nodes}")
-    _rings(k_ring, v_ring, 1, "(N, Hkv, slots, hd)")
-    hkv, slots = k_ring.shape[1], k_ring.shape[2]
+    ring_stride = _rings(k_ring, v_ring, 1)[0]
+    _, hkv, slots, _ = ring_shape = k_ring.shape
     window = slots - sinks
     if sinks < 0 or window < 1:
         raise ValueError("rings must have sinks >= 0 slots and a window of at least one behind them")
-    if k_ring.shape != (n, hkv, slots, hd) or k_new.shape != (n, nodes, hkv, hd) or v_new.shape != k_new.shape:
-        raise ValueError("new keys / values must be (N, nodes, Hkv, hd) and rings (N, Hkv, slots, hd)")
-    if hd not in (64, 128) or heads % hkv:
+    new_shape = (n, hkv, hd) if write_ring else (n, nodes, hkv, hd)
+    if ring_shape[0] != n or ring_shape[3] != hd or k_new.shape != new_shape or v_new.shape != new_shape:
+        raise ValueError("new keys / values must be (N, [nodes,] Hkv, hd) and rings (N, Hkv, slots, hd)")
+    if (hd != 64 and hd != 128) or hkv < 1 or heads < 1 or heads % hkv:
         raise ValueError("head_dim must be 64/128 and n_heads a multiple of n_kv_heads")
-    if any(t.dtype != q.dtype for t in (k_new, v_new, k_ring)):
+    dt = q.dtype
+    code = _act_code(dt)
+    if k_new.dtype is not dt or v_new.dtype is not dt or k_ring.dtype is not dt:
         raise ValueError("q, new keys / values and rings must share one dtype")
-    if positions.shape != (n,) or positions.dtype != torch.int64 or not positions.is_contiguous():
-        raise ValueError("positions must be an int64 (N,) device tensor")
-    if parents is not None and (parents.shape != (n, nodes) or parents.dtype != torch.int32
-                                or not parents.is_contiguous()):
-        raise ValueError("parents must be a contiguous int32 (N, nodes) tensor")
-    if counts is not None and (counts.shape != (n,) or counts.dtype != torch.int32 or not counts.is_contiguous()):
-        raise ValueError("counts must be an int32 (N,) device tensor")
+    p_pos = _per_request(positions, n, torch.int64, "positions")
+    p_counts = 0 if counts is None else _per_request(counts, n, torch.int32, "counts")
+    p_up = p_cos = p_sin = positions_len = 0
+    if parents is not None:
+        if parents.dtype is not torch.int32 or parents.shape != (n, nodes) or not parents.is_contiguous():
+            raise ValueError("parents must be a contiguous int32 (N, nodes) tensor")
+        p_up = parents.data_ptr()
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin must both be given or both omitted")
-    for t in (cos, sin):
-        if t is not None and (t.dim() != 2 or t.shape != cos.shape or t.shape[1] != hd or t.dtype != torch.float32
-                              or not t.is_contiguous() or t.data_ptr() % 16):
+    if cos is not None:
+        positions_len = cos.shape[0]
+        p_cos, p_sin = cos.data_ptr(), sin.data_ptr()
+        if (cos.shape != (positions_len, hd) or sin.shape != cos.shape or cos.dtype is not torch.float32
+                or sin.dtype is not torch.float32 or not cos.is_contiguous() or not sin.is_contiguous()
+                or (p_cos | p_sin) & 15):
             raise ValueError("cos / sin must be contiguous fp32 (positions, head_dim) tables")
-    dev = q.device
-    _require_device(dev, k_new, v_new, k_ring, v_ring, positions, parents, counts, cos, sin, out, workspace)
-    _forward_only(q, k_new, v_new, k_ring, v_ring)
-    given = out
+    index = _gpu_index(q, k_new, v_new, k_ring, v_ring, positions, parents, counts, cos, sin, out, workspace)
+    if torch.is_grad_enabled():
+        _forward_only(q, k_new, v_new, k_ring, v_ring)
     if out is None:
-        out = torch.empty((n, nodes, heads, hd), dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype:
+        out = q.new_empty(shape) if counts is None else q.new_zeros(shape)
+    elif out.shape != shape or out.dtype is not dt:
         raise ValueError("out must match q's shape and dtype")
-    elif _pieces(out) is not out:
+    mask = 7 if dt is torch.bfloat16 else 3
+    given = _heads(out, mask)
+    if given[0] is not out:
         raise ValueError("out must have contiguous, 16-byte aligned heads")
     k_nodes = v_nodes = None
+    p_kn = p_vn = 0
     if not write_ring:
         if node_outputs is not None:
             k_nodes, v_nodes = node_outputs
+            _gpu_index(q, k_nodes, v_nodes)
             for t in node_outputs:
-                if (t.shape != k_new.shape or t.dtype != q.dtype or not t.is_contiguous() or t.data_ptr() % 16
-                        or t.device != dev):
+                if t.shape != new_shape or t.dtype is not dt or not t.is_contiguous() or t.data_ptr() & 15:
                     raise ValueError("node outputs must be contiguous (N, nodes, Hkv, hd) tensors of q's dtype")
-        elif counts is None:
-            k_nodes = torch.empty((n, nodes, hkv, hd), dtype=q.dtype, device=dev)
-            v_nodes = torch.empty_like(k_nodes)
         else:  # rows behind a request's nodes are not written
-            k_nodes = torch.zeros((n, nodes, hkv, hd), dtype=q.dtype, device=dev)
-            v_nodes = torch.zeros_like(k_nodes)
-    if counts is not None and given is None:
-        out.zero_()
+            made = q.new_empty if counts is None else q.new_zeros
+            k_nodes, v_nodes = made(new_shape), made(new_shape)
+        p_kn, p_vn = k_nodes.data_ptr(), v_nodes.data_ptr()
     if n == 0:
         return out, k_nodes, v_nodes
-    q, k_new, v_new = _pieces(q), _pieces(k_new), _pieces(v_new)
-    a = N.SwaTreeArgs()
-    a.n_req, a.n_heads, a.n_kv_heads, a.nodes, a.head_dim = n, heads, hkv, nodes, hd
-    a.window, a.sinks, a.act_dtype, a.write_ring = window, sinks, _act_code(q.dtype), int(write_ring)
-    a.scale = 1.0 / math.sqrt(hd)
-    a.positions, a.parents, a.counts = _p(positions), _p(parents), _p(counts)
-    a.cos_table, a.sin_table = _p(cos), _p(sin)
-    a.table_len = 0 if cos is None else cos.shape[0]
-    a.q, (a.q_stride_n, a.q_stride_t, a.q_stride_h) = _p(q), _whole(q.stride(), q.shape[:3])
-    a.k_new, (a.k_stride_n, a.k_stride_t, a.k_stride_h) = _p(k_new), _whole(k_new.stride(), k_new.shape[:3])
-    a.v_new, (a.v_stride_n, a.v_stride_t, a.v_stride_h) = _p(v_new), _whole(v_new.stride(), v_new.shape[:3])
-    a.k_ring, a.v_ring, a.ring_stride_n = _p(k_ring), _p(v_ring), k_ring.stride(0) if n > 1 else 0
-    a.out, (a.o_stride_n, a.o_stride_t, a.o_stride_h) = _p(out), _whole(out.stride(), out.shape[:3])
-    a.k_nodes, a.v_nodes = _p(k_nodes), _p(v_nodes)
+    q, *q_at = _heads(q, mask)
+    k_new, *k_at = _heads(k_new, mask)
+    v_new, *v_at = _heads(v_new, mask)
     lib = N.load_library()
-    nbytes = lib.uttt_swa_tree_workspace(n, heads, hkv, nodes, hd, slots, a.act_dtype)
-    if workspace is None:
-        workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
-    elif workspace.numel() * workspace.element_size() < nbytes:
-        raise ValueError(f"the tree attention workspace must hold {nbytes} bytes")
-    a.workspace, a.workspace_bytes = _p(workspace), workspace.numel() * workspace.element_size()
-    with torch.cuda.device(dev):
-        N.check(lib.uttt_swa_tree(C.byref(a), _stream(dev)), "uttt_swa_tree")
+    nbytes = lib.uttt_swa_tree_workspace(n, heads, hkv, nodes, hd, slots, code)
+    p_ws = 0
+    if workspace is not None:
+        if workspace.numel() * workspace.element_size() < nbytes:
+            raise ValueError(f"the tree attention workspace must hold {nbytes} bytes")
+        p_ws, nbytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    elif nbytes > 16:
+        workspace = q.new_empty(nbytes, dtype=torch.uint8)
+        p_ws = workspace.data_ptr()
+    packed = N.pack_swa_tree(n, heads, hkv, nodes, hd, window, sinks, code, write_ring, hd ** -0.5, p_pos, p_up, p_counts,
+                             p_cos, p_sin, positions_len, *q_at, *k_at, *v_at, k_ring.data_ptr(), v_ring.data_ptr(),
+                             ring_stride, *given[1:], p_kn, p_vn, p_ws, nbytes)
+    _serve_call(lib.uttt_swa_tree, packed, index, "uttt_swa_tree")
     return out, k_nodes, v_nodes
 
 
@@ -1544,53 +1590,43 @@ def kv_commit(k_nodes: Tensor, v_nodes: Tensor, nodes: Tensor, counts: Tensor, k
     returns them, or (L, N, T, Hkv, hd) for L layers in one launch, with rings (N, Hkv, sinks + W, hd) or
     (L, N, Hkv, sinks + W, hd); nodes (N, A) and counts (N,) int32, positions (N,) int64.  With ``advance`` the
     positions grow by counts afterwards."""
-    layered = k_ring.dim() == 5
-    if not layered:
-        k_ring, v_ring, k_nodes, v_nodes = (t[None] for t in (k_ring, v_ring, k_nodes, v_nodes))
-    _rings(k_ring, v_ring, 2, "([L,] N, Hkv, slots, hd)")
+    if k_ring.dim() == 4:
+        k_ring, v_ring, k_nodes, v_nodes = k_ring[None], v_ring[None], k_nodes[None], v_nodes[None]
+    ring_l, ring_n = _rings(k_ring, v_ring, 2)
     layers, n, hkv, slots, hd = k_ring.shape
-    if k_nodes.dim() != 5 or v_nodes.shape != k_nodes.shape or k_nodes.shape[:2] != (layers, n) \
-            or k_nodes.shape[3:] != (hkv, hd):
+    shape = k_nodes.shape
+    if len(shape) != 5 or v_nodes.shape != shape or shape[:2] != (layers, n) or shape[3:] != (hkv, hd):
         raise ValueError("nodes' keys / values must be ([L,] N, T, Hkv, hd), one row per ring")
-    if k_nodes.dtype != k_ring.dtype or v_nodes.dtype != k_ring.dtype:
+    dt = k_ring.dtype
+    code = _act_code(dt)
+    if k_nodes.dtype is not dt or v_nodes.dtype is not dt:
         raise ValueError("nodes and rings must share one dtype")
     if sinks < 0 or slots - sinks < 1:
         raise ValueError("rings must have sinks >= 0 slots and a window of at least one behind them")
     if hd % (16 // k_ring.element_size()):
         raise ValueError("head_dim must be whole 16-byte pieces")
-    if nodes.dim() != 2 or nodes.shape[0] != n or nodes.dtype != torch.int32 or (nodes.numel() and nodes.stride(1) != 1):
+    if nodes.dim() != 2 or nodes.shape[0] != n or nodes.dtype is not torch.int32 or (nodes.numel() and nodes.stride(1) != 1):
         raise ValueError("nodes must be int32 (N, A) with unit column stride")
-    if counts.shape != (n,) or counts.dtype != torch.int32 or not counts.is_contiguous():
-        raise ValueError("counts must be an int32 (N,) device tensor")
-    if positions.shape != (n,) or positions.dtype != torch.int64 or not positions.is_contiguous():
-        raise ValueError("positions must be an int64 (N,) device tensor")
-    dev = k_ring.device
-    _require_device(dev, v_ring, k_nodes, v_nodes, nodes, counts, positions)
-    _forward_only(k_nodes, v_nodes, k_ring, v_ring)
-    if layers == 0 or n == 0 or nodes.shape[1] == 0 or k_nodes.shape[2] == 0:
+    p_counts = _per_request(counts, n, torch.int32, "counts")
+    p_pos = _per_request(positions, n, torch.int64, "positions")
+    index = _gpu_index(k_ring, v_ring, k_nodes, v_nodes, nodes, counts, positions)
+    if torch.is_grad_enabled():
+        _forward_only(k_nodes, v_nodes, k_ring, v_ring)
+    path = nodes.shape[1]
+    if layers == 0 or n == 0 or path == 0 or shape[2] == 0:
         return
-    fixed = []
-    for t in (k_nodes, v_nodes):
-        vec = 16 // t.element_size()
-        if not t[0, 0].is_contiguous() or t.data_ptr() % 16 or any(
-                s % vec for s, m in zip(t.stride()[:2], t.shape[:2]) if m > 1):
-            t = t.clone(memory_format=torch.contiguous_format)
-        fixed.append(t)
-    if _whole(fixed[0].stride()[:2], (layers, n)) != _whole(fixed[1].stride()[:2], (layers, n)):
-        fixed = [t.clone(memory_format=torch.contiguous_format) for t in fixed]
-    k_nodes, v_nodes = fixed
-    a = N.KvCommitArgs()
-    a.layers, a.n_req, a.n_kv_heads, a.n_nodes, a.path, a.head_dim = layers, n, hkv, k_nodes.shape[2], nodes.shape[1], hd
-    a.window, a.sinks, a.act_dtype, a.advance = slots - sinks, sinks, _act_code(k_ring.dtype), int(bool(advance))
-    a.k_nodes, a.v_nodes = _p(k_nodes), _p(v_nodes)
-    a.nodes_stride_l, a.nodes_stride_n = _whole(k_nodes.stride()[:2], (layers, n))
-    a.nodes, a.path_stride, a.counts = _p(nodes), nodes.stride(0), _p(counts)
-    a.k_ring, a.v_ring = _p(k_ring), _p(v_ring)
-    a.ring_stride_l, a.ring_stride_n = _whole(k_ring.stride()[:2], (layers, n))
-    a.positions = _p(positions)
-    lib = N.load_library()
-    with torch.cuda.device(dev):
-        N.check(lib.uttt_kv_commit(C.byref(a), _stream(dev)), "uttt_kv_commit")
+    nodes_l, nodes_n, s2, s3, s4 = k_nodes.stride()
+    if (s4 != 1 or s3 != hd or s2 != hkv * hd or (nodes_l | nodes_n) & (7 if dt is torch.bfloat16 else 3)
+            or v_nodes.stride() != k_nodes.stride() or (k_nodes.data_ptr() | v_nodes.data_ptr()) & 15):
+        k_nodes, v_nodes = _pieces(k_nodes, 2), _pieces(v_nodes, 2)
+        nodes_l, nodes_n = _strides(k_nodes, 2)
+    if v_nodes.stride() != k_nodes.stride() and _strides(v_nodes, 2) != (nodes_l, nodes_n):
+        k_nodes, v_nodes = (t.clone(memory_format=torch.contiguous_format) for t in (k_nodes, v_nodes))
+        nodes_l, nodes_n = _strides(k_nodes, 2)
+    packed = N.pack_kv_commit(layers, n, hkv, shape[2], path, hd, slots - sinks, sinks, code, bool(advance),
+                              k_nodes.data_ptr(), v_nodes.data_ptr(), nodes_l, nodes_n, nodes.data_ptr(), nodes.stride(0),
+                              p_counts, k_ring.data_ptr(), v_ring.data_ptr(), ring_l, ring_n, p_pos)
+    _serve_call(N.load_library().uttt_kv_commit, packed, index, "uttt_kv_commit")
 
 
 def kv_fork(k_ring: Tensor, v_ring: Tensor, sources: Tensor, positions: Tensor) -> None:
@@ -1601,30 +1637,23 @@ def kv_fork(k_ring: Tensor, v_ring: Tensor, sources: Tensor, positions: Tensor) 
     was), positions (N,) int64."""
     if k_ring.dim() == 4:
         k_ring, v_ring = k_ring[None], v_ring[None]
-    _rings(k_ring, v_ring, 2, "([L,] N, Hkv, slots, hd)")
+    ring_l, ring_n = _rings(k_ring, v_ring, 2)
     layers, n, hkv, slots, hd = k_ring.shape
+    code = _act_code(k_ring.dtype)
     if n > N.MAX_FORK_REQUESTS:
         raise ValueError(f"at most {N.MAX_FORK_REQUESTS} requests")
     if hd % (16 // k_ring.element_size()):
         raise ValueError("head_dim must be whole 16-byte pieces")
-    if sources.shape != (n,) or sources.dtype != torch.int32 or not sources.is_contiguous():
-        raise ValueError("sources must be an int32 (N,) device tensor")
-    if positions.shape != (n,) or positions.dtype != torch.int64 or not positions.is_contiguous():
-        raise ValueError("positions must be an int64 (N,) device tensor")
-    dev = k_ring.device
-    _require_device(dev, v_ring, sources, positions)
-    _forward_only(k_ring, v_ring)
+    p_src = _per_request(sources, n, torch.int32, "sources")
+    p_pos = _per_request(positions, n, torch.int64, "positions")
+    index = _gpu_index(k_ring, v_ring, sources, positions)
+    if torch.is_grad_enabled():
+        _forward_only(k_ring, v_ring)
     if layers == 0 or n == 0:
         return
-    a = N.KvForkArgs()
-    a.layers, a.n_req, a.n_kv_heads, a.slots, a.head_dim = layers, n, hkv, slots, hd
-    a.act_dtype, a.sources = _act_code(k_ring.dtype), _p(sources)
-    a.k_ring, a.v_ring = _p(k_ring), _p(v_ring)
-    a.ring_stride_l, a.ring_stride_n = _whole(k_ring.stride()[:2], (layers, n))
-    a.positions = _p(positions)
-    lib = N.load_library()
-    with torch.cuda.device(dev):
-        N.check(lib.uttt_kv_fork(C.byref(a), _stream(dev)), "uttt_kv_fork")
+    packed = N.pack_kv_fork(layers, n, hkv, slots, hd, code, p_src, k_ring.data_ptr(), v_ring.data_ptr(), ring_l, ring_n,
+                            p_pos)
+    _serve_call(N.load_library().uttt_kv_fork, packed, index, "uttt_kv_fork")
 
 
 # ---------------------------------------------------------------------------
