@@ -3,15 +3,18 @@
 //
 // With w_i = 2^(c (x_i - max)), c = log2(e) / temperature, every rule keeps a prefix of the order (logit
 // descending, id ascending), so the kept set is a cut (key, ties): the ids whose logit lies above the key's,
-// and the first `ties` of those at it.  A cut is found from a histogram of counts and masses over x (bins of 1/48 of a
-// factor of two), then inside the one bin where the count or the mass passes its bound: its few ids are
-// ranked against each other, or, when there are many, its range of keys is divided again.  The token is
-// found by the kept mass of 16 stretches of the row, one per wave, then of 16 parts of the stretch that holds
-// it, then by a scan inside one wave.
+// and the first `ties` of those at it.  Passes over the row, one workgroup each:
+//   1. the largest logit (rows that fit are kept in LDS for the passes behind);
+//   2. a histogram of counts and masses over x, of the ids within 16 factors of two of the top (bins of 1/128
+//      of one; when the cut lies further down, a second one of 1/48 over everything), and the whole mass;
+//   3. the mass of 16 stretches of the row (one per wave) ahead of the bin in which the count or the mass
+//      passes its bound, and that bin's ids, which are few: they are ranked against each other.  When there are
+//      many (equal or nearly equal logits), the bin's range of keys is divided further first;
+//   4. the same masses of 16 parts of the stretch that holds the chosen id, and a scan inside one wave.
 //
-// The sums decide between neighbouring ids, so weights are formed in 64 bits (2^f by its Taylor series to
-// degree 10, 2^-42 off) and added as integers in units of 2^-42 of the largest weight: exact whatever the order, so
-// atomics in any order give equal bits.
+// The sums decide between neighbouring ids, so weights are formed in 64 bits and added as integers in units of
+// 2^-42 of the largest weight: exact whatever the order, so atomics in any order give equal bits.  (fp64 and
+// unpacked fp32 arithmetic issue at the same rate here.)
 #include <math.h>
 
 #include <algorithm>
@@ -42,15 +45,8 @@ struct SampleArgs {
 
 constexpr int kSmpThreads = 1024, kSmpWaves = kSmpThreads / 64;
 constexpr int kBins = 2 * kSmpThreads;  // two per thread in the scan
-constexpr float kBinsPerOctave = 48.f;  // kBins / 48 > 42: every weight that is not 0 has a bin of its own width
 constexpr int kList = 256;
-
-__device__ __forceinline__ bool excluded(const SampleArgs& a, int i) {
-  if (i < 64) return (a.low >> i) & 1;
-  bool m = false;
-  for (int k = 0; k < a.n_high; ++k) m |= i == a.high[k];
-  return m;
-}
+constexpr int kStageBytes = 96 * 1024;  // rows up to this size stay in LDS
 
 // order-preserving key of a logit that is not NaN; -0 and +0 are equal
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -61,24 +57,28 @@ __device__ __forceinline__ float of_key(uint32_t k) {
   return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-// 2^t for t <= 0 in units of 2^-42, to the nearest unit
+// 2^t for t <= 0 in units of 2^-42, to the nearest unit: 2^f, |f| <= 1/2, by its Taylor series to degree 10 (2.2e-13
+// off at the ends), the whole part of t straight into the exponent
 __device__ __forceinline__ u64 weight_units(double t) {
-  if (!(t > -44.0)) return 0;
-  const double n = __builtin_rint(t), f = (t - n) * 0.6931471805599453;
-  double p = 1.0 / 3628800;
-  p = __builtin_fma(p, f, 1.0 / 362880);
-  p = __builtin_fma(p, f, 1.0 / 40320);
-  p = __builtin_fma(p, f, 1.0 / 5040);
-  p = __builtin_fma(p, f, 1.0 / 720);
-  p = __builtin_fma(p, f, 1.0 / 120);
-  p = __builtin_fma(p, f, 1.0 / 24);
-  p = __builtin_fma(p, f, 1.0 / 6);
-  p = __builtin_fma(p, f, 0.5);
+  const double kRound = 6755399441055744.0;  // 1.5 2^52: adding it leaves the nearest integer in the low bits
+  const double shifted = t + kRound;
+  const double f = t - (shifted - kRound);
+  constexpr double kL = 0.6931471805599453, kL2 = kL * kL, kL4 = kL2 * kL2;
+  double p = kL4 * kL4 * kL2 / 3628800;
+  p = __builtin_fma(p, f, kL4 * kL4 * kL / 362880);
+  p = __builtin_fma(p, f, kL4 * kL4 / 40320);
+  p = __builtin_fma(p, f, kL4 * kL2 * kL / 5040);
+  p = __builtin_fma(p, f, kL4 * kL2 / 720);
+  p = __builtin_fma(p, f, kL4 * kL / 120);
+  p = __builtin_fma(p, f, kL4 / 24);
+  p = __builtin_fma(p, f, kL2 * kL / 6);
+  p = __builtin_fma(p, f, kL2 / 2);
+  p = __builtin_fma(p, f, kL);
   p = __builtin_fma(p, f, 1.0);
-  p = __builtin_fma(p, f, 1.0);
+  const u64 scaled = __builtin_bit_cast(u64, p) + ((u64)(uint32_t)((int)__builtin_bit_cast(u64, shifted) + 42) << 52);
   // adding 2^52 rounds to whole units, which are then the low bits
-  const double u = __builtin_ldexp(p, (int)n + 42) + 4503599627370496.0;
-  return __builtin_bit_cast(u64, u) & 0xfffffffffffffull;
+  const double u = __builtin_bit_cast(double, scaled) + 4503599627370496.0;
+  return t > -44.0 ? __builtin_bit_cast(u64, u) & 0xfffffffffffffull : 0;
 }
 
 __device__ __forceinline__ u64 shfl_up64(u64 v, int off) {
@@ -107,30 +107,40 @@ struct Shared {
   uint32_t count[kBins];
   u64 mass2[kBins];  // of a range of keys inside one bin
   uint32_t count2[kBins];
-  u64 wave_mass[kSmpWaves];
-  uint32_t wave_count[kSmpWaves];
+  u64 wave_mass[kSmpWaves], scan_mass[kSmpWaves];
+  uint32_t wave_count[kSmpWaves], scan_count[kSmpWaves];
   float wave_best[kSmpWaves];
-  int wave_id[kSmpWaves];
   uint32_t list_key[kList];
   int list_id[kList];
   u64 list_mass[kList];
   uint32_t n, kmin, kmax, before_count;
   u64 before_mass;
-  int bin;
+  int bin, best;
   u64 kept;
   uint32_t cut_key;
   int cut_ties;
-  int token;
 };
 
-// ids [lo, hi) of the row, in order, VEC at a time and 64 VEC to a wave step, kUnroll steps in flight
-template <typename T, int VEC, int kUnroll, typename F>
-__device__ __forceinline__ void scan_ids(const T* x, int lo, int hi, int lane, F&& f) {
-  typedef T vec_t __attribute__((ext_vector_type(VEC)));
-  for (int b = lo; b < hi; b += 64 * VEC * kUnroll) {
-    vec_t v[kUnroll];
+// ids that are left out read as -inf
+template <int VEC>
+__device__ __forceinline__ void leave_out(const SampleArgs& a, float (&v)[VEC], int i) {
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
+  for (int e = 0; e < VEC; ++e) {
+    bool out = i + e < 64 && ((a.low >> (i + e)) & 1);
+    for (int k = 0; k < a.n_high; ++k) out |= i + e == a.high[k];
+    v[e] = out ? -INFINITY : v[e];
+  }
+}
+
+// f(values, first id, ids) for ids [lo, hi) of the row in order, VEC to a lane; U steps of 64 VEC ids in flight
+template <typename T, int VEC, int U, bool RAW, typename F>
+__device__ __forceinline__ void scan_ids(const SampleArgs& a, const T* x, int lo, int hi, int lane, F&& f) {
+  typedef T vec_t __attribute__((ext_vector_type(VEC)));
+#pragma unroll 1
+  for (int b = lo; b < hi; b += 64 * VEC * U) {
+    vec_t v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
       const int i = b + (u * 64 + lane) * VEC;
       if (i + VEC <= hi) {
         v[u] = *reinterpret_cast<const vec_t*>(x + i);
@@ -140,55 +150,80 @@ __device__ __forceinline__ void scan_ids(const T* x, int lo, int hi, int lane, F
       }
     }
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
+    for (int u = 0; u < U; ++u) {
       const int i = b + (u * 64 + lane) * VEC;
+      float y[VEC];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e)
-        if (i + e < hi) f(to_f32(v[u][e]), i + e);
+      for (int e = 0; e < VEC; ++e) y[e] = to_f32((T)v[u][e]);
+      if (RAW && (b < 64 || a.n_high > 0)) leave_out<VEC>(a, y, i);
+      if (i < hi) f(y, i, min(VEC, hi - i));
     }
   }
 }
 
-template <typename T, int VEC>
+// STAGED: the row stays in LDS behind the first pass, without the ids that are left out.
+template <typename T, int VEC, bool STAGED>
 __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs a) {
   __shared__ Shared s;
-  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  __shared__ __align__(16) T stage[STAGED ? kStageBytes / sizeof(T) : 1];
+  constexpr int W = STAGED ? 4 : VEC;  // ids to a lane in the passes behind the first
+  constexpr float kFine = 128.f, kCoarse = 48.f;  // bins to a factor of two: kBins / 48 > 42, what weights reach
+  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const T* x = static_cast<const T*>(a.logits) + (int64_t)row * a.rs;
   // a wave's stretch of the row
-  constexpr int kStep = 64 * VEC;
+  constexpr int kStep = 64 * W;
   const int stretch = ((a.limit + kSmpWaves - 1) / kSmpWaves + kStep - 1) / kStep * kStep;
   const int lo = min(w * stretch, a.limit), hi = min(lo + stretch, a.limit);
-
-  // ---- the largest logit (NaN above all, ties to the lowest id), as a greedy choice has it
-  float bv = -INFINITY;
-  int bi = 0x7fffffff;
-  auto take = [&](float v, int i) {
-    const bool vn = v != v, bn = bv != bv;
-    const bool ahead = vn != bn ? vn : (!vn && v != bv) ? v > bv : i < bi;
-    if (ahead) {
-      bv = v;
-      bi = i;
-    }
+  auto scan = [&](int from, int to, auto&& f) __attribute__((always_inline)) {
+    if constexpr (STAGED)
+      scan_ids<T, W, 1, false>(a, stage, from, to, lane, f);
+    else
+      scan_ids<T, W, 2, true>(a, x, from, to, lane, f);
   };
-  scan_ids<T, VEC, 16 / VEC < 4 ? 16 / VEC : 4>(x, lo, hi, lane, [&](float v, int i) { take(excluded(a, i) ? -INFINITY : v, i); });
+
+  // ---- the largest logit; NaN makes it NaN
+  float top = -INFINITY;
+  bool nan = false;
+  scan_ids<T, VEC, 4, true>(a, x, lo, hi, lane, [&](const float(&v)[VEC], int i, int n) __attribute__((always_inline)) {
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) take(__shfl_xor(bv, off, 64), __shfl_xor(bi, off, 64));
-  if (lane == 0) {
-    s.wave_best[w] = bv;
-    s.wave_id[w] = bi;
-  }
+    for (int e = 0; e < VEC; ++e)
+      if (e < n) {
+        top = fmaxf(top, v[e]);
+        nan |= v[e] != v[e];
+        if constexpr (STAGED) stage[i + e] = from_f32<T>(v[e]);
+      }
+  });
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+  if (__any(nan)) top = NAN;
+  if (lane == 0) s.wave_best[w] = top;
   for (int i = tid; i < kBins; i += kSmpThreads) {
     s.mass[i] = 0;
     s.count[i] = 0;
   }
+  if (tid == 0) s.best = 0x7fffffff;
   __syncthreads();
+  top = -INFINITY;
+  nan = false;
+#pragma unroll 4
+  for (int q = 0; q < kSmpWaves; ++q) {
+    const float v = s.wave_best[q];
+    nan |= v != v;
+    top = fmaxf(top, v);
+  }
+  const float temp = a.temperature[row];
+  const bool greedy = !(temp > 1e-5f);
+  if (greedy || nan || !(fabsf(top) < INFINITY)) {  // the lowest id of the largest value (NaN above all)
+    int best = 0x7fffffff;
+    scan(lo, hi, [&](const float(&v)[W], int i, int n) __attribute__((always_inline)) {
 #pragma unroll
-  for (int q = 0; q < kSmpWaves; ++q) take(s.wave_best[q], s.wave_id[q]);
-  const float temp = a.temperature[row], top = bv;
-  const bool greedy = !(temp > 1e-5f), odd = !(fabsf(top) < INFINITY);
-  if (greedy || odd) {
+      for (int e = 0; e < W; ++e)
+        if (e < n && (nan ? v[e] != v[e] : v[e] == top)) best = min(best, i + e);
+    });
+    if (best != 0x7fffffff) atomicMin(&s.best, best);
+    __syncthreads();
     if (tid == 0) {
-      a.out[row] = bi == 0x7fffffff ? 0 : bi;
+      a.out[row] = s.best == 0x7fffffff ? 0 : s.best;
       if (a.logprob != nullptr) a.logprob[row] = greedy ? 0.f : NAN;
       if (a.advance != nullptr) a.advance[row] += 1;
     }
@@ -200,25 +235,47 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
   const float top_p = a.top_p != nullptr ? a.top_p[row] : 1.f, min_p = a.min_p != nullptr ? a.min_p[row] : 0.f;
   const bool by_count = top_k > 0 && top_k < a.limit, by_mass = top_p < 1.f;
   const u64 least = min_p > 0.f ? (u64)__builtin_ceil(fmin((double)min_p, 1.0) * 4398046511104.0) : 1;
-  auto weight = [&](float v) -> u64 {
+  auto weight = [&](float v) __attribute__((always_inline)) -> u64 {
     const u64 u = weight_units(((double)v - dtop) * c);
     return u >= least ? u : 0;
   };
-  const float per_unit = fminf((float)c * kBinsPerOctave, 3e38f);
-  auto bin_of = [&](float v) { return (int)fminf((top - v) * per_unit, (float)(kBins - 1)); };
+  float per_unit = fminf((float)c * kFine, 3e38f);  // bins to a unit of the logits
+  float last = (float)kBins;                        // ids in bins from here on are not counted, or with ...
+  bool clamp = false;                               // ... clamp put into the last bin
+  auto place = [&](float v) __attribute__((always_inline)) { return clamp && v > -INFINITY ? fminf((top - v) * per_unit, last) : (top - v) * per_unit; };
 
   Cut cut{0, 0x7fffffff, 0};  // keeps everything
+  bool masses = false;        // the stretches' masses up to the cut are known
   if (by_count || by_mass) {
-    scan_ids<T, VEC, 1>(x, lo, hi, lane, [&](float v, int i) {
-      if (excluded(a, i)) return;
-      const int b = bin_of(v);
-      const u64 u = weight(v);
-      if (u != 0) atomicAdd(&s.mass[b], u);
-      if (by_count) atomicAdd(&s.count[b], 1u);
-    });
-    __syncthreads();
-    // what lies ahead of each thread's two bins, and where the bound falls; `bound` counts or mass
-    auto find = [&](const u64* mass, const uint32_t* count, u64 mass0, uint32_t count0, bool counts, u64 bound) {
+    u64 whole = 0;
+    auto histogram = [&]() __attribute__((always_inline)) {
+      u64 sum = 0;
+      scan(lo, hi, [&](const float(&v)[W], int, int n) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          if (e >= n) continue;
+          u64 u = 0;
+          if (by_mass) {
+            u = weight(v[e]);
+            sum += u;
+          }
+          const float d = place(v[e]);
+          if (d < (float)kBins) {
+            if (u != 0) atomicAdd(&s.mass[(int)d], u);
+            if (by_count) atomicAdd(&s.count[(int)d], 1u);
+          }
+        }
+      });
+      sum = wave_sum64(sum);
+      if (lane == 0) s.wave_mass[w] = sum;
+      __syncthreads();
+      whole = 0;
+#pragma unroll 4
+      for (int q = 0; q < kSmpWaves; ++q) whole += s.wave_mass[q];
+    };
+    // the bin with the last kept id (s.bin, -1: none), and what lies ahead of it: the bound-th id, or the last one
+    // whose mass ahead is within the bound
+    auto find = [&](const u64* mass, const uint32_t* count, u64 mass0, uint32_t count0, bool counts, u64 bound) __attribute__((always_inline)) {
       const u64 m0 = mass[2 * tid], m1 = mass[2 * tid + 1];
       const uint32_t n0 = count[2 * tid], n1 = count[2 * tid + 1];
       u64 m = m0 + m1;
@@ -233,27 +290,22 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
         }
       }
       if (lane == 63) {
-        s.wave_mass[w] = m;
-        s.wave_count[w] = n;
+        s.scan_mass[w] = m;
+        s.scan_count[w] = n;
       }
       if (tid == 0) s.bin = -1;
       __syncthreads();
       m -= m0 + m1;
       n -= n0 + n1;
-      u64 total = mass0;
-#pragma unroll
+#pragma unroll 4
       for (int q = 0; q < kSmpWaves; ++q) {
-        const u64 wm = s.wave_mass[q];
-        total += wm;
         if (q < w) {
-          m += wm;
-          n += s.wave_count[q];
+          m += s.scan_mass[q];
+          n += s.scan_count[q];
         }
       }
       m += mass0;
       n += count0;
-      if (!counts && bound == ~0ull) bound = (u64)((double)fmaxf(top_p, 0.f) * (double)total);
-      // the bin with the last kept id: the bound-th, or the last whose mass ahead is within the bound
       const bool in0 = counts ? n < bound && bound <= n + n0 : m <= bound && bound < m + m0;
       const bool in1 = counts ? n + n0 < bound && bound <= n + n0 + n1 : m + m0 <= bound && bound < m + m0 + m1;
       if (in0 || in1) {
@@ -262,10 +314,13 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
         s.before_count = in0 ? n : n + n0;
       }
       __syncthreads();
-      return bound;
+      const int bin = s.bin;
+      __syncthreads();
+      return bin;
     };
-    // the ids of one bin (and range of keys): how many, the first kList, the range of their keys
-    auto gather = [&](int bin, uint32_t kmin, uint32_t kmax) {
+    // the ids of one bin with keys in [kmin, kmax]: how many, the first kList, the range of their keys; and per
+    // stretch the mass of the bins ahead
+    auto gather = [&](int bin, uint32_t kmin, uint32_t kmax, bool ahead) __attribute__((always_inline)) {
       if (tid == 0) {
         s.n = 0;
         s.kmin = 0xffffffffu;
@@ -273,32 +328,47 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
       }
       __syncthreads();
       uint32_t mn = 0xffffffffu, mx = 0;
-      scan_ids<T, VEC, 1>(x, lo, hi, lane, [&](float v, int i) {
-        if (bin_of(v) != bin || excluded(a, i)) return;
-        const uint32_t k = key_of(v);
-        if (k < kmin || k > kmax) return;
-        mn = min(mn, k);
-        mx = max(mx, k);
-        const uint32_t at = atomicAdd(&s.n, 1u);
-        if (at < kList) {
-          s.list_key[at] = k;
-          s.list_id[at] = i;
-          s.list_mass[at] = weight(v);
+      u64 sum = 0;
+      scan(lo, hi, [&](const float(&v)[W], int i, int n) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          const float d = place(v[e]);
+          if (e >= n || !(d < (float)(bin + 1))) continue;
+          if (d < (float)bin) {
+            if (ahead) sum += weight(v[e]);
+            continue;
+          }
+          const uint32_t k = key_of(v[e]);
+          if (k < kmin || k > kmax) continue;
+          mn = min(mn, k);
+          mx = max(mx, k);
+          const uint32_t at = atomicAdd(&s.n, 1u);
+          if (at < kList) {
+            s.list_key[at] = k;
+            s.list_id[at] = i + e;
+            s.list_mass[at] = weight(v[e]);
+          }
         }
       });
       if (mn <= mx) {
         atomicMin(&s.kmin, mn);
         atomicMax(&s.kmax, mx);
       }
+      if (ahead) {
+        sum = wave_sum64(sum);
+        if (lane == 0) {
+          s.wave_mass[w] = sum;
+          s.wave_count[w] = 0;
+        }
+      }
       __syncthreads();
     };
-    // the cut inside the bin that find() left
-    auto resolve = [&](bool counts, u64 bound) -> Cut {
-      const int bin = s.bin;
+    // the cut inside a bin that find() named
+    auto resolve = [&](int bin, bool counts, u64 bound, bool ahead) __attribute__((always_inline)) -> Cut {
       u64 mass0 = s.before_mass;
       uint32_t count0 = s.before_count;
-      __syncthreads();
-      gather(bin, 0, 0xffffffffu);
+      gather(bin, 0, 0xffffffffu, ahead);
+      masses = ahead && s.n <= kList;
       uint32_t kmin = s.kmin, kmax = s.kmax;
       while (s.n > kList && kmin != kmax) {
         const int shift = max(0, 32 - 11 - __builtin_clz(kmax - kmin));
@@ -307,39 +377,41 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
           s.count2[i] = 0;
         }
         __syncthreads();
-        scan_ids<T, VEC, 1>(x, lo, hi, lane, [&](float v, int i) {
-          if (bin_of(v) != bin || excluded(a, i)) return;
-          const uint32_t k = key_of(v);
-          if (k < kmin || k > kmax) return;
-          const int b = (int)((kmax - k) >> shift);
-          const u64 u = weight(v);
-          if (u != 0) atomicAdd(&s.mass2[b], u);
-          atomicAdd(&s.count2[b], 1u);
+        scan(lo, hi, [&](const float(&v)[W], int, int n) __attribute__((always_inline)) {
+#pragma unroll
+          for (int e = 0; e < W; ++e) {
+            const float d = place(v[e]);
+            if (e >= n || !(d >= (float)bin && d < (float)(bin + 1))) continue;
+            const uint32_t k = key_of(v[e]);
+            if (k < kmin || k > kmax) continue;
+            const int b = (int)((kmax - k) >> shift);
+            const u64 u = weight(v[e]);
+            if (u != 0) atomicAdd(&s.mass2[b], u);
+            atomicAdd(&s.count2[b], 1u);
+          }
         });
         __syncthreads();
-        find(s.mass2, s.count2, mass0, count0, counts, bound);
-        if (s.bin < 0) break;  // the bound lies inside the bin, so one of its parts has it
-        const uint32_t b = (uint32_t)s.bin;
+        const int part = find(s.mass2, s.count2, mass0, count0, counts, bound);
+        if (part < 0) break;  // the bound lies inside the bin, so one of its parts has it
         mass0 = s.before_mass;
         count0 = s.before_count;
-        const uint32_t hi_key = kmax - (b << shift), width = (1u << shift) - 1;
+        const uint32_t hi_key = kmax - ((uint32_t)part << shift), width = (1u << shift) - 1;
         const uint32_t lo_key = hi_key - kmin > width ? hi_key - width : kmin;
-        __syncthreads();
-        gather(bin, lo_key, hi_key);
+        gather(bin, lo_key, hi_key, false);
         kmin = s.kmin;
         kmax = s.kmax;
       }
       Cut r;
+      const int n = (int)min(s.n, (uint32_t)kList);
       if (kmin == kmax) {  // equal logits: a number of them
         const u64 u = weight(of_key(kmin));
-        const u64 n = s.n;
-        u64 t = counts ? bound - count0 : u != 0 ? (bound - mass0) / u + 1 : n;
-        t = t < n ? t : n;
+        const u64 all = s.n;
+        u64 t = counts ? bound - count0 : u != 0 ? (bound - mass0) / u + 1 : all;
+        t = t < all ? t : all;
         r.key = kmin;
         r.ties = (int)t;
         r.mass = mass0 + t * u;
       } else {
-        const int n = (int)s.n;
         if (tid == 0) {
           s.kept = 0;
           s.cut_key = 0xffffffffu;
@@ -353,6 +425,7 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
           const int id = s.list_id[tid];
           u64 m = mass0;
           uint32_t cnt = count0;
+#pragma unroll 4
           for (int j = 0; j < n; ++j) {
             const uint32_t kj = s.list_key[j];
             if (kj > k || (kj == k && s.list_id[j] < id)) {
@@ -373,38 +446,67 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
         r.ties = s.cut_ties;
         r.mass = mass0 + s.kept;
       }
+      if (masses && tid < n) {  // the bin's own part of the stretches' masses, and its ids at the cut
+        const int q = s.list_id[tid] / stretch;
+        if (s.list_key[tid] > r.key) atomicAdd(&s.wave_mass[q], s.list_mass[tid]);
+        if (s.list_key[tid] == r.key) atomicAdd(&s.wave_count[q], 1u);
+      }
       __syncthreads();
       return r;
     };
-    u64 limit_mass = ~0ull;  // top_p of the row's mass, or of what top_k keeps
-    if (by_count) {
-      find(s.mass, s.count, 0, 0, true, (u64)top_k);
-      if (s.bin >= 0) {  // else fewer ids than top_k
-        cut = resolve(true, (u64)top_k);
-        limit_mass = (u64)((double)fmaxf(top_p, 0.f) * (double)cut.mass);
+#pragma unroll 1
+    for (int round = 0; round < 2; ++round) {
+      histogram();
+      u64 bound = (u64)((double)fmaxf(top_p, 0.f) * (double)whole);  // top_p of the row's mass
+      bool found = true;
+      if (by_count) {
+        const int bin = find(s.mass, s.count, 0, 0, true, (u64)top_k);
+        if (bin >= 0) {
+          cut = resolve(bin, true, (u64)top_k, !by_mass);
+          bound = (u64)((double)fmaxf(top_p, 0.f) * (double)cut.mass);  // or of what top_k keeps
+        } else {
+          found = false;  // it lies further down, or there are fewer ids than top_k
+        }
       }
-    }
-    if (by_mass) {
-      const u64 bound = find(s.mass, s.count, 0, 0, false, limit_mass);
-      if (s.bin >= 0) {
-        const Cut p = resolve(false, bound);
-        if (p.key > cut.key || (p.key == cut.key && p.ties < cut.ties)) cut = p;
+      if (by_mass && (found || round == 1)) {
+        const int bin = find(s.mass, s.count, 0, 0, false, bound);
+        found = bin >= 0;
+        if (found) {
+          const Cut p = resolve(bin, false, bound, true);
+          if (p.key > cut.key || (p.key == cut.key && p.ties < cut.ties))
+            cut = p;
+          else
+            masses = false;
+        }
       }
+      if (found || round == 1) break;
+      per_unit = fminf((float)c * kCoarse, 3e38f);
+      last = (float)(kBins - 1);
+      clamp = true;
+      __syncthreads();
+      for (int i = tid; i < kBins; i += kSmpThreads) {
+        s.mass[i] = 0;
+        s.count[i] = 0;
+      }
+      __syncthreads();
     }
   }
 
   // ---- the kept mass of parts [lo, hi) of the row, one per wave: above the cut's key, and ids at it
-  const u64 tie_mass = cut.key != 0 ? weight(of_key(cut.key)) : 0;
-  auto part_mass = [&](int p_lo, int p_hi) {
+  const float at_cut = cut.key != 0 ? of_key(cut.key) : -INFINITY;
+  const u64 tie_mass = cut.key != 0 ? weight(at_cut) : 0;
+  auto part_mass = [&](int p_lo, int p_hi) __attribute__((always_inline)) {
     u64 m = 0;
     uint32_t t = 0;
-    scan_ids<T, VEC, 1>(x, p_lo, p_hi, lane, [&](float v, int i) {
-      const uint32_t k = key_of(v);
-      if (k < cut.key || excluded(a, i)) return;
-      if (k == cut.key)
-        ++t;
-      else
-        m += weight(v);
+    scan(p_lo, p_hi, [&](const float(&v)[W], int, int n) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        if (e >= n || !(v[e] >= at_cut)) continue;
+        if (v[e] > at_cut)
+          m += weight(v[e]);
+        else
+          ++t;
+      }
     });
     m = wave_sum64(m);
 #pragma unroll
@@ -417,13 +519,13 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
     __syncthreads();
   };
   const u64 max_ties = (u64)cut.ties;
-  auto with_ties = [&](u64 ties, u64 more) {  // mass of `more` ids at the cut's key behind `ties` of them
+  auto with_ties = [&](u64 ties, u64 more) __attribute__((always_inline)) {  // mass of `more` ids at the cut's key behind `ties` of them
     const u64 left = ties < max_ties ? max_ties - ties : 0;
     return (more < left ? more : left) * tie_mass;
   };
-  part_mass(lo, hi);
+  if (!masses) part_mass(lo, hi);
   u64 total = 0, ties = 0;
-#pragma unroll
+#pragma unroll 4
   for (int q = 0; q < kSmpWaves; ++q) {
     total += s.wave_mass[q] + with_ties(ties, s.wave_count[q]);
     ties += s.wave_count[q];
@@ -434,11 +536,11 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
   want = want < total ? want : total - 1;
   // the part whose mass first exceeds `want`, and the mass and ties ahead of it
   u64 ahead = 0, ties_ahead = 0;
-  auto pick = [&]() {
+  auto pick = [&]() __attribute__((always_inline)) {
     u64 m = ahead, t = ties_ahead;
     int found = kSmpWaves - 1;
     bool done = false;
-#pragma unroll
+#pragma unroll 4
     for (int q = 0; q < kSmpWaves; ++q) {
       if (!done) {
         const u64 next = m + s.wave_mass[q] + with_ties(t, s.wave_count[q]);
@@ -453,7 +555,7 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
     }
     ahead = m;
     ties_ahead = t;
-    return found;
+    return __builtin_amdgcn_readfirstlane(found);
   };
   const int p0 = min(pick() * stretch, a.limit), p1 = min(p0 + stretch, a.limit);
   const int part = ((p1 - p0 + kSmpWaves - 1) / kSmpWaves + kStep - 1) / kStep * kStep;
@@ -468,17 +570,19 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
   int token = -1;
   for (int b = q0; b < q1 && token < 0; b += 64) {
     const int i = b + lane;
-    u64 u = 0;
-    uint32_t tie = 0;
-    if (i < q1 && !excluded(a, i)) {
-      const float v = to_f32(x[i]);
-      const uint32_t k = key_of(v);
-      if (k > cut.key) u = weight(v);
-      tie = k == cut.key;
+    float v[1] = {-INFINITY};
+    if (i < q1) {
+      if constexpr (STAGED) {
+        v[0] = to_f32(stage[i]);
+      } else {
+        v[0] = to_f32(x[i]);
+        leave_out<1>(a, v, i);
+      }
     }
+    u64 u = v[0] > at_cut ? weight(v[0]) : 0;
+    const bool tie = v[0] == at_cut && tie_mass != 0;
     const u64 tied = __ballot(tie);
-    const u64 before = t + __popcll(tied & ((1ull << lane) - 1));
-    if (tie) u = before < max_ties ? tie_mass : 0;
+    if (tie) u = t + __popcll(tied & ((1ull << lane) - 1)) < max_ties ? tie_mass : 0;
     u64 sum = u;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
@@ -486,20 +590,32 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
       if (lane >= off) sum += p;
     }
     const u64 over = __ballot(m + sum > want);
-    if (over != 0) {
-      token = b + __builtin_ctzll(over);
-    }
+    if (over != 0) token = b + __builtin_ctzll(over);
     m += (u64)(uint32_t)__shfl((uint32_t)(sum >> 32), 63, 64) << 32 | (uint32_t)__shfl((uint32_t)sum, 63, 64);
     t += __popcll(tied);
   }
   if (lane == 0) {
-    token = token < 0 ? bi : token;
+    token = token < 0 ? q0 : token;  // integers add up the same way at every level, so one is found
     a.out[row] = token;
     // log(w / total): the weight's own exponent, not its rounded units
     if (a.logprob != nullptr)
       a.logprob[row] = (float)(((double)to_f32(x[token]) - dtop) / (double)temp - log((double)total * 0x1p-42));
     if (a.advance != nullptr) a.advance[row] += 1;
   }
+}
+
+template <typename T>
+void launch_sample(const SampleArgs& s, int64_t rows, bool vec, hipStream_t st) {
+  const dim3 grid((unsigned)rows), block(kSmpThreads);
+  const bool staged = (int64_t)s.limit * (int64_t)sizeof(T) <= kStageBytes;
+  if (vec && staged)
+    hipLaunchKernelGGL((k_sample_select<T, 4, true>), grid, block, 0, st, s);
+  else if (vec)
+    hipLaunchKernelGGL((k_sample_select<T, 4, false>), grid, block, 0, st, s);
+  else if (staged)
+    hipLaunchKernelGGL((k_sample_select<T, 1, true>), grid, block, 0, st, s);
+  else
+    hipLaunchKernelGGL((k_sample_select<T, 1, false>), grid, block, 0, st, s);
 }
 
 }  // namespace
@@ -533,16 +649,10 @@ extern "C" int uttt_sample_select(const uttt_sample_args* a, uttt_stream_t strea
   s.top_k = a->top_k; s.top_p = a->top_p; s.min_p = a->min_p;
   s.out = a->out; s.logprob = a->logprob; s.advance = a->advance;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)a->rows);
-  const bool bf = a->dtype == UTTT_DTYPE_BF16;
-  const bool vec = aligned16(a->logits) && (a->rows == 1 || a->row_stride % 4 == 0);
-  if (bf && vec)
-    hipLaunchKernelGGL((k_sample_select<bf16, 4>), grid, dim3(kSmpThreads), 0, st, s);
-  else if (bf)
-    hipLaunchKernelGGL((k_sample_select<bf16, 1>), grid, dim3(kSmpThreads), 0, st, s);
-  else if (vec)
-    hipLaunchKernelGGL((k_sample_select<float, 4>), grid, dim3(kSmpThreads), 0, st, s);
+  const bool vec = aligned16(a->logits) && (a->rows == 1 || a->row_stride % 4 == 0);  // four ids at a time
+  if (a->dtype == UTTT_DTYPE_BF16)
+    launch_sample<bf16>(s, a->rows, vec, st);
   else
-    hipLaunchKernelGGL((k_sample_select<float, 1>), grid, dim3(kSmpThreads), 0, st, s);
+    launch_sample<float>(s, a->rows, vec, st);
   return launch_status("uttt_sample_select");
 }
