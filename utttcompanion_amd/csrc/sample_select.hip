@@ -57,9 +57,10 @@ __device__ __forceinline__ float of_key(uint32_t k) {
   return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-// 2^t for t <= 0 in units of 2^-42, to the nearest unit: 2^f, |f| <= 1/2, by its Taylor series to degree 10 (2.2e-13
-// off at the ends), the whole part of t straight into the exponent
+// 2^t for t <= 0 (0 for NaN) in units of 2^-42, to the nearest unit: 2^f, |f| <= 1/2, by its Taylor series to degree 10
+// (2.2e-13 off at the ends), the whole part of t straight into the exponent
 __device__ __forceinline__ u64 weight_units(double t) {
+  t = __builtin_fmax(t, -60.0);  // far below half a unit
   const double kRound = 6755399441055744.0;  // 1.5 2^52: adding it leaves the nearest integer in the low bits
   const double shifted = t + kRound;
   const double f = t - (shifted - kRound);
@@ -78,21 +79,34 @@ __device__ __forceinline__ u64 weight_units(double t) {
   const u64 scaled = __builtin_bit_cast(u64, p) + ((u64)(uint32_t)((int)__builtin_bit_cast(u64, shifted) + 42) << 52);
   // adding 2^52 rounds to whole units, which are then the low bits
   const double u = __builtin_bit_cast(double, scaled) + 4503599627370496.0;
-  return t > -44.0 ? __builtin_bit_cast(u64, u) & 0xfffffffffffffull : 0;
+  return __builtin_bit_cast(u64, u) & 0xfffffffffffffull;
 }
 
-__device__ __forceinline__ u64 shfl_up64(u64 v, int off) {
-  const uint32_t lo = __shfl_up((uint32_t)v, off, 64), hi = __shfl_up((uint32_t)(v >> 32), off, 64);
-  return (u64)hi << 32 | lo;
+// Sums over lanes through DPP operands: within rows of 16 lanes by shifts, then the rows' last lanes to the rows behind.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp0(uint32_t v) {  // 0 where the source lane does not exist
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
 }
-__device__ __forceinline__ u64 shfl_xor64(u64 v, int off) {
-  const uint32_t lo = __shfl_xor((uint32_t)v, off, 64), hi = __shfl_xor((uint32_t)(v >> 32), off, 64);
-  return (u64)hi << 32 | lo;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 dpp0(u64 v) {
+  return (u64)dpp0<CTRL, ROWS>((uint32_t)(v >> 32)) << 32 | dpp0<CTRL, ROWS>((uint32_t)v);
 }
-__device__ __forceinline__ u64 wave_sum64(u64 v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += shfl_xor64(v, off);
-  return v;
+template <typename V>
+__device__ __forceinline__ V row_scan(V v) {  // inclusive, 16 lanes
+  v += dpp0<0x111, 0xF>(v);
+  v += dpp0<0x112, 0xF>(v);
+  v += dpp0<0x114, 0xF>(v);
+  return v + dpp0<0x118, 0xF>(v);
+}
+template <typename V>
+__device__ __forceinline__ V wave_scan(V v) {  // inclusive, 64 lanes
+  v = row_scan(v);
+  v += dpp0<0x142, 0xA>(v);
+  return v + dpp0<0x143, 0xC>(v);
+}
+__device__ __forceinline__ uint32_t of_lane(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }
+__device__ __forceinline__ u64 of_lane(u64 v, int lane) {
+  return (u64)of_lane((uint32_t)(v >> 32), lane) << 32 | of_lane((uint32_t)v, lane);
 }
 
 // A cut: ids with a larger key are kept, and the first `ties` of those with this key.
@@ -132,21 +146,23 @@ __device__ __forceinline__ void leave_out(const SampleArgs& a, float (&v)[VEC], 
   }
 }
 
-// f(values, first id, ids) for ids [lo, hi) of the row in order, VEC to a lane; U steps of 64 VEC ids in flight
+// f(values, first id) for ids [lo, hi) of the row in order, VEC to a lane; U steps of 64 VEC ids in flight.  What a step
+// has past hi reads as -inf.
 template <typename T, int VEC, int U, bool RAW, typename F>
 __device__ __forceinline__ void scan_ids(const SampleArgs& a, const T* x, int lo, int hi, int lane, F&& f) {
   typedef T vec_t __attribute__((ext_vector_type(VEC)));
 #pragma unroll 1
   for (int b = lo; b < hi; b += 64 * VEC * U) {
     vec_t v[U];
+    const bool whole = b + 64 * VEC * U <= hi;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = b + (u * 64 + lane) * VEC;
-      if (i + VEC <= hi) {
+      if (whole || i + VEC <= hi) {
         v[u] = *reinterpret_cast<const vec_t*>(x + i);
-      } else if (i < hi) {
+      } else {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[u][e] = i + e < hi ? x[i + e] : x[i];
+        for (int e = 0; e < VEC; ++e) v[u][e] = i + e < hi ? x[i + e] : from_f32<T>(-INFINITY);
       }
     }
 #pragma unroll
@@ -156,7 +172,7 @@ __device__ __forceinline__ void scan_ids(const SampleArgs& a, const T* x, int lo
 #pragma unroll
       for (int e = 0; e < VEC; ++e) y[e] = to_f32((T)v[u][e]);
       if (RAW && (b < 64 || a.n_high > 0)) leave_out<VEC>(a, y, i);
-      if (i < hi) f(y, i, min(VEC, hi - i));
+      f(y, i);
     }
   }
 }
@@ -166,14 +182,17 @@ template <typename T, int VEC, bool STAGED>
 __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs a) {
   __shared__ Shared s;
   __shared__ __align__(16) T stage[STAGED ? kStageBytes / sizeof(T) : 1];
-  constexpr int W = STAGED ? 4 : VEC;  // ids to a lane in the passes behind the first
+  constexpr int W = STAGED || VEC > 4 ? 4 : VEC;  // ids to a lane in the passes behind the first
   constexpr float kFine = 128.f, kCoarse = 48.f;  // bins to a factor of two: kBins / 48 > 42, what weights reach
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const T* x = static_cast<const T*>(a.logits) + (int64_t)row * a.rs;
   // a wave's stretch of the row
-  constexpr int kStep = 64 * W;
+  constexpr int kStep = 64 * (VEC > W ? VEC : W);
   const int stretch = ((a.limit + kSmpWaves - 1) / kSmpWaves + kStep - 1) / kStep * kStep;
   const int lo = min(w * stretch, a.limit), hi = min(lo + stretch, a.limit);
+  const float temp = a.temperature[row], uniform = a.uniforms[row];
+  const int top_k = a.top_k != nullptr ? a.top_k[row] : 0;
+  const float top_p = a.top_p != nullptr ? a.top_p[row] : 1.f, min_p = a.min_p != nullptr ? a.min_p[row] : 0.f;
   auto scan = [&](int from, int to, auto&& f) __attribute__((always_inline)) {
     if constexpr (STAGED)
       scan_ids<T, W, 1, false>(a, stage, from, to, lane, f);
@@ -184,14 +203,19 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
   // ---- the largest logit; NaN makes it NaN
   float top = -INFINITY;
   bool nan = false;
-  scan_ids<T, VEC, 4, true>(a, x, lo, hi, lane, [&](const float(&v)[VEC], int i, int n) __attribute__((always_inline)) {
+  scan_ids<T, VEC, 4, true>(a, x, lo, hi, lane, [&](const float(&v)[VEC], int i) __attribute__((always_inline)) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e)
-      if (e < n) {
-        top = fmaxf(top, v[e]);
-        nan |= v[e] != v[e];
-        if constexpr (STAGED) stage[i + e] = from_f32<T>(v[e]);
-      }
+    for (int e = 0; e < VEC; ++e) {
+      top = fmaxf(top, v[e]);
+      nan |= v[e] != v[e];
+    }
+    if constexpr (STAGED) {
+      typedef T vec_t __attribute__((ext_vector_type(VEC)));
+      vec_t y;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) y[e] = from_f32<T>(v[e]);
+      if (i < hi) *reinterpret_cast<vec_t*>(stage + i) = y;  // past the last id: -inf
+    }
   });
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
@@ -211,14 +235,13 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
     nan |= v != v;
     top = fmaxf(top, v);
   }
-  const float temp = a.temperature[row];
   const bool greedy = !(temp > 1e-5f);
   if (greedy || nan || !(fabsf(top) < INFINITY)) {  // the lowest id of the largest value (NaN above all)
     int best = 0x7fffffff;
-    scan(lo, hi, [&](const float(&v)[W], int i, int n) __attribute__((always_inline)) {
+    scan(lo, hi, [&](const float(&v)[W], int i) __attribute__((always_inline)) {
 #pragma unroll
       for (int e = 0; e < W; ++e)
-        if (e < n && (nan ? v[e] != v[e] : v[e] == top)) best = min(best, i + e);
+        if (nan ? v[e] != v[e] : v[e] == top) best = min(best, i + e);
     });
     if (best != 0x7fffffff) atomicMin(&s.best, best);
     __syncthreads();
@@ -231,13 +254,11 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
   }
 
   const double c = 1.4426950408889634 / (double)temp, dtop = (double)top;
-  const int top_k = a.top_k != nullptr ? a.top_k[row] : 0;
-  const float top_p = a.top_p != nullptr ? a.top_p[row] : 1.f, min_p = a.min_p != nullptr ? a.min_p[row] : 0.f;
   const bool by_count = top_k > 0 && top_k < a.limit, by_mass = top_p < 1.f;
   const u64 least = min_p > 0.f ? (u64)__builtin_ceil(fmin((double)min_p, 1.0) * 4398046511104.0) : 1;
   auto weight = [&](float v) __attribute__((always_inline)) -> u64 {
     const u64 u = weight_units(((double)v - dtop) * c);
-    return u >= least ? u : 0;
+    return least <= 1 || u >= least ? u : 0;
   };
   float per_unit = fminf((float)c * kFine, 3e38f);  // bins to a unit of the logits
   float last = (float)kBins;                        // ids in bins from here on are not counted, or with ...
@@ -246,49 +267,45 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
 
   Cut cut{0, 0x7fffffff, 0};  // keeps everything
   bool masses = false;        // the stretches' masses up to the cut are known
+  u64 whole = 0;              // the row's mass; at the end the kept ids'
   if (by_count || by_mass) {
-    u64 whole = 0;
     auto histogram = [&]() __attribute__((always_inline)) {
       u64 sum = 0;
-      scan(lo, hi, [&](const float(&v)[W], int, int n) __attribute__((always_inline)) {
+      scan(lo, hi, [&](const float(&v)[W], int) __attribute__((always_inline)) {
+        u64 u[W] = {};
+        if (by_mass) {
+#pragma unroll
+          for (int e = 0; e < W; ++e) u[e] = weight(v[e]);
+#pragma unroll
+          for (int e = 0; e < W; ++e) sum += u[e];
+        }
+        float d[W], nearest = INFINITY;
 #pragma unroll
         for (int e = 0; e < W; ++e) {
-          if (e >= n) continue;
-          u64 u = 0;
-          if (by_mass) {
-            u = weight(v[e]);
-            sum += u;
-          }
-          const float d = place(v[e]);
-          if (d < (float)kBins) {
-            if (u != 0) atomicAdd(&s.mass[(int)d], u);
-            if (by_count) atomicAdd(&s.count[(int)d], 1u);
-          }
+          d[e] = place(v[e]);
+          nearest = fminf(nearest, d[e]);
+        }
+        if (nearest < (float)kBins) {
+#pragma unroll
+          for (int e = 0; e < W; ++e)
+            if (d[e] < (float)kBins) {
+              if (by_mass) atomicAdd(&s.mass[(int)d[e]], u[e]);
+              if (by_count) atomicAdd(&s.count[(int)d[e]], 1u);
+            }
         }
       });
-      sum = wave_sum64(sum);
-      if (lane == 0) s.wave_mass[w] = sum;
+      sum = wave_scan(sum);
+      if (lane == 63) s.wave_mass[w] = sum;
       __syncthreads();
-      whole = 0;
-#pragma unroll 4
-      for (int q = 0; q < kSmpWaves; ++q) whole += s.wave_mass[q];
+      whole = of_lane(row_scan(s.wave_mass[lane & 15]), 15);
     };
     // the bin with the last kept id (s.bin, -1: none), and what lies ahead of it: the bound-th id, or the last one
     // whose mass ahead is within the bound
     auto find = [&](const u64* mass, const uint32_t* count, u64 mass0, uint32_t count0, bool counts, u64 bound) __attribute__((always_inline)) {
       const u64 m0 = mass[2 * tid], m1 = mass[2 * tid + 1];
       const uint32_t n0 = count[2 * tid], n1 = count[2 * tid + 1];
-      u64 m = m0 + m1;
-      uint32_t n = n0 + n1;
-#pragma unroll
-      for (int off = 1; off < 64; off <<= 1) {
-        const u64 pm = shfl_up64(m, off);
-        const uint32_t pn = __shfl_up(n, off, 64);
-        if (lane >= off) {
-          m += pm;
-          n += pn;
-        }
-      }
+      u64 m = wave_scan(m0 + m1);
+      uint32_t n = wave_scan(n0 + n1);
       if (lane == 63) {
         s.scan_mass[w] = m;
         s.scan_count[w] = n;
@@ -297,12 +314,9 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
       __syncthreads();
       m -= m0 + m1;
       n -= n0 + n1;
-#pragma unroll 4
-      for (int q = 0; q < kSmpWaves; ++q) {
-        if (q < w) {
-          m += s.scan_mass[q];
-          n += s.scan_count[q];
-        }
+      if (w > 0) {
+        m += of_lane(row_scan(s.scan_mass[lane & 15]), w - 1);
+        n += of_lane(row_scan(s.scan_count[lane & 15]), w - 1);
       }
       m += mass0;
       n += count0;
@@ -329,16 +343,25 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
       __syncthreads();
       uint32_t mn = 0xffffffffu, mx = 0;
       u64 sum = 0;
-      scan(lo, hi, [&](const float(&v)[W], int i, int n) __attribute__((always_inline)) {
+      scan(lo, hi, [&](const float(&v)[W], int i) __attribute__((always_inline)) {
+        float d[W], nearest = INFINITY;
 #pragma unroll
         for (int e = 0; e < W; ++e) {
-          const float d = place(v[e]);
-          if (e >= n || !(d < (float)(bin + 1))) continue;
-          if (d < (float)bin) {
-            if (ahead) sum += weight(v[e]);
+          d[e] = place(v[e]);
+          nearest = fminf(nearest, d[e]);
+        }
+        if (!(nearest < (float)(bin + 1))) return;
+#pragma unroll 1
+        for (int e = 0; e < W; ++e) {
+          const float de = e == 0 ? d[0] : e == 1 ? d[1 % W] : e == 2 ? d[2 % W] : d[3 % W];
+          const float ve = e == 0 ? v[0] : e == 1 ? v[1 % W] : e == 2 ? v[2 % W] : v[3 % W];
+          if (!(de < (float)(bin + 1))) continue;
+          const u64 u = weight(ve);
+          if (de < (float)bin) {
+            sum += u;
             continue;
           }
-          const uint32_t k = key_of(v[e]);
+          const uint32_t k = key_of(ve);
           if (k < kmin || k > kmax) continue;
           mn = min(mn, k);
           mx = max(mx, k);
@@ -346,7 +369,7 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
           if (at < kList) {
             s.list_key[at] = k;
             s.list_id[at] = i + e;
-            s.list_mass[at] = weight(v[e]);
+            s.list_mass[at] = u;
           }
         }
       });
@@ -355,8 +378,8 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
         atomicMax(&s.kmax, mx);
       }
       if (ahead) {
-        sum = wave_sum64(sum);
-        if (lane == 0) {
+        sum = wave_scan(sum);
+        if (lane == 63) {
           s.wave_mass[w] = sum;
           s.wave_count[w] = 0;
         }
@@ -377,16 +400,16 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
           s.count2[i] = 0;
         }
         __syncthreads();
-        scan(lo, hi, [&](const float(&v)[W], int, int n) __attribute__((always_inline)) {
-#pragma unroll
+        scan(lo, hi, [&](const float(&v)[W], int) __attribute__((always_inline)) {
+#pragma unroll 1
           for (int e = 0; e < W; ++e) {
-            const float d = place(v[e]);
-            if (e >= n || !(d >= (float)bin && d < (float)(bin + 1))) continue;
-            const uint32_t k = key_of(v[e]);
+            const float ve = e == 0 ? v[0] : e == 1 ? v[1 % W] : e == 2 ? v[2 % W] : v[3 % W];
+            const float d = place(ve);
+            if (!(d >= (float)bin && d < (float)(bin + 1))) continue;
+            const uint32_t k = key_of(ve);
             if (k < kmin || k > kmax) continue;
             const int b = (int)((kmax - k) >> shift);
-            const u64 u = weight(v[e]);
-            if (u != 0) atomicAdd(&s.mass2[b], u);
+            atomicAdd(&s.mass2[b], weight(ve));
             atomicAdd(&s.count2[b], 1u);
           }
         });
@@ -498,21 +521,24 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
   auto part_mass = [&](int p_lo, int p_hi) __attribute__((always_inline)) {
     u64 m = 0;
     uint32_t t = 0;
-    scan(p_lo, p_hi, [&](const float(&v)[W], int, int n) __attribute__((always_inline)) {
+    scan(p_lo, p_hi, [&](const float(&v)[W], int) __attribute__((always_inline)) {
+      float most = v[0];
+#pragma unroll
+      for (int e = 1; e < W; ++e) most = fmaxf(most, v[e]);
+      if (!(most >= at_cut)) return;
+      u64 u[W];
+#pragma unroll
+      for (int e = 0; e < W; ++e) u[e] = weight(v[e]);
 #pragma unroll
       for (int e = 0; e < W; ++e) {
-        if (e >= n || !(v[e] >= at_cut)) continue;
-        if (v[e] > at_cut)
-          m += weight(v[e]);
-        else
-          ++t;
+        m += v[e] > at_cut ? u[e] : 0;
+        t += v[e] == at_cut;
       }
     });
-    m = wave_sum64(m);
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) t += __shfl_xor(t, off, 64);
+    m = wave_scan(m);
+    t = wave_scan(t);
     __syncthreads();
-    if (lane == 0) {
+    if (lane == 63) {
       s.wave_mass[w] = m;
       s.wave_count[w] = t;
     }
@@ -524,46 +550,34 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
     return (more < left ? more : left) * tie_mass;
   };
   if (!masses) part_mass(lo, hi);
-  u64 total = 0, ties = 0;
-#pragma unroll 4
-  for (int q = 0; q < kSmpWaves; ++q) {
-    total += s.wave_mass[q] + with_ties(ties, s.wave_count[q]);
-    ties += s.wave_count[q];
-  }
-  float uf = a.uniforms[row];
-  uf = uf > 0.f ? fminf(uf, 0.99999994f) : 0.f;
-  u64 want = (u64)((double)uf * (double)total);
-  want = want < total ? want : total - 1;
-  // the part whose mass first exceeds `want`, and the mass and ties ahead of it
-  u64 ahead = 0, ties_ahead = 0;
-  auto pick = [&]() __attribute__((always_inline)) {
-    u64 m = ahead, t = ties_ahead;
-    int found = kSmpWaves - 1;
-    bool done = false;
-#pragma unroll 4
-    for (int q = 0; q < kSmpWaves; ++q) {
-      if (!done) {
-        const u64 next = m + s.wave_mass[q] + with_ties(t, s.wave_count[q]);
-        if (next > want) {
-          found = q;
-          done = true;
-        } else {
-          m = next;
-          t += s.wave_count[q];
-        }
-      }
+  const float uf = uniform > 0.f ? fminf(uniform, 0.99999994f) : 0.f;
+  u64 want = 0, ahead = 0, ties_ahead = 0;
+  // the part whose mass first exceeds `want`, and the mass and ties ahead of it; lane q of a row of 16 has part q
+  auto pick = [&](bool first) __attribute__((always_inline)) {
+    const u64 mine = s.wave_mass[lane & 15], t = s.wave_count[lane & 15];
+    const u64 t_end = ties_ahead + row_scan(t);
+    const u64 m_end = ahead + row_scan(mine + with_ties(t_end - t, t));
+    if (first) {
+      const u64 total = of_lane(m_end, 15);
+      want = (u64)((double)uf * (double)total);
+      want = want < total ? want : total - 1;
+      whole = total;
     }
-    ahead = m;
-    ties_ahead = t;
-    return __builtin_amdgcn_readfirstlane(found);
+    const uint32_t over = (uint32_t)__ballot(m_end > want) & 0xffffu;
+    const int found = over != 0 ? __builtin_ctz(over) : 15;
+    if (found > 0) {
+      ahead = of_lane(m_end, found - 1);
+      ties_ahead = of_lane(t_end, found - 1);
+    }
+    return found;
   };
-  const int p0 = min(pick() * stretch, a.limit), p1 = min(p0 + stretch, a.limit);
+  const int p0 = min(pick(true) * stretch, a.limit), p1 = min(p0 + stretch, a.limit);
   const int part = ((p1 - p0 + kSmpWaves - 1) / kSmpWaves + kStep - 1) / kStep * kStep;
   {
     const int q_lo = min(p0 + w * part, p1);
     part_mass(q_lo, min(q_lo + part, p1));
   }
-  const int q0 = min(p0 + pick() * part, p1), q1 = min(q0 + part, p1);
+  const int q0 = min(p0 + pick(false) * part, p1), q1 = min(q0 + part, p1);
   if (w != 0) return;
   // ---- inside one wave: 64 ids at a time
   u64 m = ahead, t = ties_ahead;
@@ -583,15 +597,10 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
     const bool tie = v[0] == at_cut && tie_mass != 0;
     const u64 tied = __ballot(tie);
     if (tie) u = t + __popcll(tied & ((1ull << lane) - 1)) < max_ties ? tie_mass : 0;
-    u64 sum = u;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const u64 p = shfl_up64(sum, off);
-      if (lane >= off) sum += p;
-    }
+    const u64 sum = wave_scan(u);
     const u64 over = __ballot(m + sum > want);
     if (over != 0) token = b + __builtin_ctzll(over);
-    m += (u64)(uint32_t)__shfl((uint32_t)(sum >> 32), 63, 64) << 32 | (uint32_t)__shfl((uint32_t)sum, 63, 64);
+    m += of_lane(sum, 63);
     t += __popcll(tied);
   }
   if (lane == 0) {
@@ -599,19 +608,21 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
     a.out[row] = token;
     // log(w / total): the weight's own exponent, not its rounded units
     if (a.logprob != nullptr)
-      a.logprob[row] = (float)(((double)to_f32(x[token]) - dtop) / (double)temp - log((double)total * 0x1p-42));
+      a.logprob[row] = (float)(((double)to_f32(x[token]) - dtop) / (double)temp - log((double)whole * 0x1p-42));
     if (a.advance != nullptr) a.advance[row] += 1;
   }
 }
 
 template <typename T>
-void launch_sample(const SampleArgs& s, int64_t rows, bool vec, hipStream_t st) {
+void launch_sample(const SampleArgs& s, int64_t rows, hipStream_t st) {
+  constexpr int VEC = 16 / (int)sizeof(T);
   const dim3 grid((unsigned)rows), block(kSmpThreads);
-  const bool staged = (int64_t)s.limit * (int64_t)sizeof(T) <= kStageBytes;
+  const bool vec = aligned16(s.logits) && (rows == 1 || s.rs % VEC == 0);
+  const bool staged = (int64_t)s.limit * (int64_t)sizeof(T) <= kStageBytes - 16;
   if (vec && staged)
-    hipLaunchKernelGGL((k_sample_select<T, 4, true>), grid, block, 0, st, s);
+    hipLaunchKernelGGL((k_sample_select<T, VEC, true>), grid, block, 0, st, s);
   else if (vec)
-    hipLaunchKernelGGL((k_sample_select<T, 4, false>), grid, block, 0, st, s);
+    hipLaunchKernelGGL((k_sample_select<T, VEC, false>), grid, block, 0, st, s);
   else if (staged)
     hipLaunchKernelGGL((k_sample_select<T, 1, true>), grid, block, 0, st, s);
   else
@@ -649,10 +660,9 @@ extern "C" int uttt_sample_select(const uttt_sample_args* a, uttt_stream_t strea
   s.top_k = a->top_k; s.top_p = a->top_p; s.min_p = a->min_p;
   s.out = a->out; s.logprob = a->logprob; s.advance = a->advance;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const bool vec = aligned16(a->logits) && (a->rows == 1 || a->row_stride % 4 == 0);  // four ids at a time
   if (a->dtype == UTTT_DTYPE_BF16)
-    launch_sample<bf16>(s, a->rows, vec, st);
+    launch_sample<bf16>(s, a->rows, st);
   else
-    launch_sample<float>(s, a->rows, vec, st);
+    launch_sample<float>(s, a->rows, st);
   return launch_status("uttt_sample_select");
 }
