@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
     if constexpr (STAGED)
       scan_ids<T, W, 1, false>(a, stage, from, to, lane, f);
     else
-      scan_ids<T, W, 2, true>(a, x, from, to, lane, f);
+      scan_ids<T, W, 4, true>(a, x, from, to, lane, f);
   };
 
   // ---- the largest logit; NaN makes it NaN
@@ -351,17 +351,20 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
           nearest = fminf(nearest, d[e]);
         }
         if (!(nearest < (float)(bin + 1))) return;
-#pragma unroll 1
+        bool here = false;
+        u64 u[W];
+#pragma unroll
+        for (int e = 0; e < W; ++e) u[e] = weight(v[e]);
+#pragma unroll
         for (int e = 0; e < W; ++e) {
-          const float de = e == 0 ? d[0] : e == 1 ? d[1 % W] : e == 2 ? d[2 % W] : d[3 % W];
-          const float ve = e == 0 ? v[0] : e == 1 ? v[1 % W] : e == 2 ? v[2 % W] : v[3 % W];
-          if (!(de < (float)(bin + 1))) continue;
-          const u64 u = weight(ve);
-          if (de < (float)bin) {
-            sum += u;
-            continue;
-          }
-          const uint32_t k = key_of(ve);
+          sum += d[e] < (float)bin ? u[e] : 0;
+          here |= d[e] >= (float)bin && d[e] < (float)(bin + 1);
+        }
+        if (!here) return;
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          if (!(d[e] >= (float)bin && d[e] < (float)(bin + 1))) continue;
+          const uint32_t k = key_of(v[e]);
           if (k < kmin || k > kmax) continue;
           mn = min(mn, k);
           mx = max(mx, k);
@@ -369,7 +372,7 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
           if (at < kList) {
             s.list_key[at] = k;
             s.list_id[at] = i + e;
-            s.list_mass[at] = u;
+            s.list_mass[at] = u[e];
           }
         }
       });
