@@ -83,6 +83,69 @@ def test_tree_matches_the_definition(n, t, heads, hkv, hd, window, sinks, positi
     check(out, kn, vn, qkv, rings, positions, None, cos, sin, heads, hkv, window, sinks)
 
 
+def wide_case(n, t, hd, seed):
+    """Enough rows per key head and requests that the rows share a workgroup's tiles."""
+    heads, hkv, window, sinks = 8, 2, 300, 4
+    g = torch.Generator().manual_seed(seed)
+    positions = torch.randint(0, 1000, (n,), generator=g).tolist()
+    return (heads, hkv, window, sinks, positions, *make(n, t, heads, hkv, hd, window, sinks, positions, torch.bfloat16, seed))
+
+
+@pytest.mark.parametrize("n,t,hd", [(43, 25, 64), (17, 64, 64), (40, 31, 128), (17, 49, 128)])
+def test_many_rows_share_tiles(n, t, hd):
+    from utttcompanion_amd import kernels as K
+    heads, hkv, window, sinks, positions, qkv, rings, pos, parents, (cos, sin) = wide_case(n, t, hd, t)
+    g = torch.Generator().manual_seed(1)
+    counts = torch.randint(0, t + 1, (n,), generator=g).tolist()
+    counts[0], counts[1] = t, 1
+    q, k, v = qkv.to(DEV).split([heads, hkv, hkv], dim=2)
+    kr, vr = (r.to(DEV) for r in rings)
+    out, kn, vn = K.swa_tree(q, k, v, kr, vr, pos.to(DEV), parents.to(DEV), cos.to(DEV), sin.to(DEV), sinks=sinks,
+                             counts=torch.tensor(counts, dtype=torch.int32, device=DEV))
+    check(out, kn, vn, qkv, rings, positions, parents, cos, sin, heads, hkv, window, sinks, counts)
+    # infinities and NaN in one branch of a request, and at the edge of another's window
+    odd = qkv.clone()
+    parents = parents.clone()
+    parents[0] = torch.arange(t) - 1
+    parents[0, 2] = 0  # node 1 is a leaf beside the chain 2, 3, ..
+    odd[0, 1] = float("nan")
+    args = (pos.to(DEV), parents.to(DEV), cos.to(DEV), sin.to(DEV))
+    want = K.swa_tree(q, k, v, kr, vr, *args, sinks=sinks)[0]
+    got = K.swa_tree(*odd.to(DEV).split([heads, hkv, hkv], dim=2), kr, vr, *args, sinks=sinks)[0]
+    tol = 2.0 ** -6  # the same sums in another order, values up to about 4
+    others = [i for i in range(t) if i != 1]
+    assert float((got[0, others].float() - want[0, others].float()).abs().max()) <= tol
+    assert bool(got[0, 1].isnan().all()) and torch.equal(got[1:], want[1:])
+    full = next(i for i, p in enumerate(positions) if p > window + sinks)
+    p = positions[full]
+    vr[full, :, sinks + (p - window + 1 - sinks) % window] = float("inf")  # the oldest in the window of depth 0
+    got = K.swa_tree(q, k, v, kr, vr, *args, sinks=sinks)[0]
+    depth = torch.tensor([len(x) - 1 for x in tree_paths(parents[full].tolist())])
+    deep = depth > 0
+    assert float((got[full].float() - want[full].float())[deep].abs().max()) <= tol
+    assert bool(got[full].float()[~deep].isinf().all())
+
+
+def test_many_rows_split_over_slots():
+    """The same with the slots of a request split over workgroups, and requests that cannot be computed."""
+    from utttcompanion_amd import kernels as K
+    n, t, heads, hkv, hd, window, sinks = 16, 64, 16, 4, 128, 2500, 4
+    positions = [0, 5000, 100, 2503, 2504, 900] + [3000 + i for i in range(10)]
+    qkv, rings, pos, parents, (cos, sin) = make(n, t, heads, hkv, hd, window, sinks, positions, torch.bfloat16, 7)
+    q, k, v = qkv.to(DEV).split([heads, hkv, hkv], dim=2)
+    kr, vr = (r.to(DEV) for r in rings)
+    out, kn, vn = K.swa_tree(q, k, v, kr, vr, pos.to(DEV), parents.to(DEV), cos.to(DEV), sin.to(DEV), sinks=sinks)
+    some = [0, 1, 3, 4]
+    check(out[some], kn[some], vn[some], qkv[some], [r[some] for r in rings], [positions[i] for i in some], parents[some], cos,
+          sin, heads, hkv, window, sinks)
+    bad = pos.clone()
+    bad[2], bad[7] = -1, len(cos)
+    got = K.swa_tree(q, k, v, kr, vr, bad.to(DEV), parents.to(DEV), cos.to(DEV), sin.to(DEV), sinks=sinks)[0]
+    assert bool(got[2].isnan().all()) and bool(got[7].isnan().all())
+    keep = [i for i in range(n) if i not in (2, 7)]
+    assert torch.equal(got[keep], out[keep])
+
+
 @pytest.mark.parametrize("dtype", BOTH)
 @pytest.mark.parametrize("hd,window", [(64, 40), (128, 40), (64, 3000)])
 def test_ragged_node_counts_leave_the_rows_behind_alone(hd, window, dtype):

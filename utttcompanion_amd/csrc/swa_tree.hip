@@ -16,8 +16,8 @@
 // in fp32 and rounded once.
 //
 // Slots that no node of the request may see (unwritten, or out of the window for all) are zeroed in LDS.
-// Where a tile's values are seen by some nodes only and hold infinities or NaN, weights of 0 must not meet
-// them: that tile's second product is formed with selections instead of MFMA.
+// Where values that some nodes see and others do not hold infinities or NaN, weights of 0 must not meet them: those
+// rows are computed again, a row per wave and only over the keys it sees (selected_row; slow, and rare).
 #include <math.h>
 
 #include <algorithm>
@@ -30,6 +30,7 @@ namespace uttt {
 namespace {
 
 constexpr int kMaxNodes = 64;
+constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kWaves = 4;
 
 struct TreeArgs {
@@ -153,14 +154,18 @@ __device__ __forceinline__ int64_t part_row(const TreeArgs& a, const Place& p, i
   return (((int64_t)p.n * a.n_kv_heads + p.kvh) * a.nsplit + p.split) * a.rows + row;
 }
 
+template <typename T>
+__device__ __forceinline__ T* out_row(const TreeArgs& a, const Place& p, int row) {
+  return static_cast<T*>(a.out) + p.n * a.o_n + row / a.rep * a.o_t + (p.kvh * a.rep + row % a.rep) * a.o_h;
+}
+
 // NaN for rows [row0, row1) of a request that cannot be computed
 template <typename T, int HD>
-__device__ __forceinline__ void refuse_rows(const TreeArgs& a, const Place& p, int row0, int row1) {
-  for (int i = threadIdx.x; i < (row1 - row0) * HD; i += kThreads) {
+__device__ __forceinline__ void refuse_rows(const TreeArgs& a, const Place& p, int row0, int row1, int threads) {
+  for (int i = threadIdx.x; i < (row1 - row0) * HD; i += threads) {
     const int row = row0 + i / HD, e = i % HD;
     if (a.nsplit == 1)
-      static_cast<T*>(a.out)[p.n * a.o_n + row / a.rep * a.o_t + (p.kvh * a.rep + row % a.rep) * a.o_h + e] =
-          from_f32<T>(NAN);
+      out_row<T>(a, p, row)[e] = from_f32<T>(NAN);
     else if (e == 0)
       a.part_ml[2 * part_row(a, p, row)] = NAN;
   }
@@ -183,86 +188,51 @@ __device__ __forceinline__ bool finite16(const uint4& v) {  // eight bf16
   return ok(v.x) && ok(v.y) && ok(v.z) && ok(v.w);
 }
 
-template <int HD, int U>
-__global__ void __launch_bounds__(kThreads, HD == 64 ? 2 : 1) k_swa_tree_mm(const TreeArgs a) {
-  constexpr int NT = HD / 64, NB = HD / 32, KS = HD / 16;
-  constexpr int TILE = NT * 8192;  // K (or V) of 64 slots
-  constexpr int LOADS = NT * 8;    // 1 KB loads of a tile
-  constexpr int RED = HD + 4;      // floats of a query's row when the waves' results meet
-  constexpr float kLog2e = 1.4426950408889634f;
-  static_assert(kWaves * 32 * RED * 4 <= kWaves * 2 * TILE, "the waves' results fit the tiles' LDS");
-  __shared__ __align__(1024) char lds[kWaves * 2 * TILE];
-  __shared__ float red_ml[kWaves][32][2];
-  __shared__ int tree_odd;  // the new values hold infinities or NaN
-  const Place p = place_of(a);
-  if (!p.valid) return;
-  const int w = uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
-  const int count = a.counts != nullptr ? min(max(uniform(a.counts[p.n]), 0), a.nodes) : a.nodes;
-  const int row0 = p.group * 32 * U, row1 = min(row0 + 32 * U, count * a.rep);
-  if (row0 >= row1) return;
-  const bool first = p.split == 0;
+// LDS bytes of 64 keys (or values): HD / 64 row tiles (slabs) of 8 KB
+template <int HD>
+constexpr int kTileBytes = HD / 64 * 8192;
 
-  // ---- this wave's tiles: 64 slots each, in LDS of its own
-  const uint32_t k_lds = lds_addr(lds) + (uint32_t)(w * 2 * TILE), v_lds = k_lds + TILE;
-  const bf16* kr = static_cast<const bf16*>(a.k_ring) + p.n * a.ring_n + (int64_t)p.kvh * a.slots * HD;
-  const bf16* vr = static_cast<const bf16*>(a.v_ring) + p.n * a.ring_n + (int64_t)p.kvh * a.slots * HD;
-  const int voff_k[2] = {row_src_off(0, lane, HD), row_src_off(1, lane, HD) - 16 * HD};
-  const int voff_v = slab_src_off(0, lane, HD);
-  auto issue = [&](const bf16* ring, uint32_t dst, int tile, bool is_k) {
-    const int n = max(min(a.slots - tile * 64, 64), 0);  // slots past the ring read as zeros
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const __amdgpu_buffer_rsrc_t rs =
-          buffer_rsrc(ring + (int64_t)tile * 64 * HD + 64 * t, (uint32_t)max(n * HD * 2 - 128 * t, 0));
-#pragma unroll
-      for (int g = 0; g < 8; ++g)
-        buffer_load_lds_raw(rs, lds_ptr(dst + (uint32_t)(t * 8192 + g * 1024)), 16,
-                            (is_k ? voff_k[g & 1] : voff_v) + g * 16 * HD, 0, 0, 0);
-    }
-  };
-  // the tile a wave starts with needs no position in the first split: ask for it at once (the last wave
-  // starts with the new tokens there)
-  const bool early = first && w < kWaves - 1;
-  if (early) {
-    issue(kr, k_lds, w, true);
-    issue(vr, v_lds, w, false);
+// The 1 KB loads g of the HD / 8 that bring a tile of 64 slots into LDS, as a row tile (K) or a slab (V).  Slots past the
+// ring read as zeros.
+template <int HD>
+struct TileLoad {
+  int voff_k[2], voff_v;
+  __device__ __forceinline__ explicit TileLoad(int lane)
+      : voff_k{row_src_off(0, lane, HD), row_src_off(1, lane, HD) - 16 * HD}, voff_v(slab_src_off(0, lane, HD)) {}
+  __device__ __forceinline__ void issue(const bf16* ring, int slots, uint32_t dst, int tile, int g, bool is_k) const {
+    const int n = max(min(slots - tile * 64, 64), 0), t = g >> 3, rg = g & 7;
+    const __amdgpu_buffer_rsrc_t rs =
+        buffer_rsrc(ring + (int64_t)tile * 64 * HD + 64 * t, (uint32_t)max(n * HD * 2 - 128 * t, 0));
+    buffer_load_lds_raw(rs, lds_ptr(dst + (uint32_t)(g * 1024)), 16, (is_k ? voff_k[rg & 1] : voff_v) + rg * 16 * HD, 0, 0, 0);
   }
-  if (threadIdx.x == 0) tree_odd = 0;
-  const int64_t pos = uniform(a.positions[p.n]);
-  const Tree tree = read_tree(a, p.n, count, pos, lane);
-  if (tree.bad) {
-    refuse_rows<bf16, HD>(a, p, row0, row1);
-    wait_vmcnt<0>();  // no LDS write of this workgroup's loads outlives it
-    return;
-  }
-  const Ring ring = read_ring(a, pos);
-  const int ntiles = (ring.used + 63) / 64;
-  const int t_begin = (int)((int64_t)ntiles * p.split / a.nsplit), t_end = (int)((int64_t)ntiles * (p.split + 1) / a.nsplit);
-  // wave w takes places w, w + kWaves, .. of the split's list; the first split's has the new tokens at place
-  // kWaves - 1, whether or not its cache reaches that far
-  auto tile_at = [&](int i) { return t_begin + (first && i >= kWaves ? i - 1 : i); };
-  auto has = [&](int i) { return (first && i == kWaves - 1) || tile_at(i) < t_end; };
+};
 
-  // ---- queries: row r of each unit, dims 16 s + 8 h .. + 7 in fragment s; rotated ones as two terms
-  const bool turned = a.cos_table != nullptr;
-  bf16x8 qf[U][KS], ql[U][KS];
-  int lim[U];
-  uint64_t sees[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int row = row0 + 32 * u + r;
+// 32 rows of a (request, kv head) in one wave: a query per lane (both halves of the wave hold it), its softmax and its
+// output, transposed (o[b][e]: dim 32 b + 8 (e / 4) + 4 h + e % 4).
+template <int HD>
+struct Unit {
+  static constexpr int NB = HD / 32, KS = HD / 16;
+  bf16x8 qf[KS], ql[KS];  // dims 16 s + 8 h .. + 7 in fragment s; rotated queries as two terms
+  int lim;                // ages below it are seen
+  uint64_t sees;          // nodes that are seen
+  float m, l;
+  f32x16 o[NB];
+
+  __device__ __forceinline__ void load(const TreeArgs& a, const Place& p, const Tree& tree, const Ring& ring, int64_t pos,
+                                       int row, int row1) {
+    const int h = (threadIdx.x & 63) >> 5;
     const bool ok = row < row1;
     const int t = ok ? row / a.rep : 0, head = p.kvh * a.rep + (ok ? row % a.rep : 0);
     const int d = __shfl(tree.depth, t, 64);
-    sees[u] = shfl64(tree.sees, t);
-    lim[u] = visible_age(a, ring, d);
+    sees = shfl64(tree.sees, t);
+    lim = visible_age(a, ring, d);
     const bf16* qr = static_cast<const bf16*>(a.q) + p.n * a.q_n + t * a.q_t + head * a.q_h + 8 * h;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      qf[u][s] = ok ? *reinterpret_cast<const bf16x8*>(qr + 16 * s) : bf16x8{};
-      ql[u][s] = bf16x8{};
+      qf[s] = ok ? *reinterpret_cast<const bf16x8*>(qr + 16 * s) : bf16x8{};
+      ql[s] = bf16x8{};
     }
-    if (turned) {
+    if (a.cos_table != nullptr) {
       const float* cr = a.cos_table + (pos + d) * HD + 8 * h;
       const float* sr = a.sin_table + (pos + d) * HD + 8 * h;
 #pragma unroll
@@ -274,95 +244,364 @@ __global__ void __launch_bounds__(kThreads, HD == 64 ? 2 : 1) k_swa_tree_mm(cons
         sn[1] = *reinterpret_cast<const f32x4*>(sr + 16 * s + 4);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float lo = to_f32((bf16)qf[u][s][e]), hi = to_f32((bf16)qf[u][s + KS / 2][e]);
+          const float lo = to_f32((bf16)qf[s][e]), hi = to_f32((bf16)qf[s + KS / 2][e]);
           const float ce = c[e >> 2][e & 3], se = sn[e >> 2][e & 3];
           const float x = lo * ce - hi * se, y = hi * ce + lo * se;
           const bf16 xh = from_f32<bf16>(x), yh = from_f32<bf16>(y);
-          qf[u][s][e] = xh;
-          qf[u][s + KS / 2][e] = yh;
-          ql[u][s][e] = from_f32<bf16>(x - to_f32(xh));
-          ql[u][s + KS / 2][e] = from_f32<bf16>(y - to_f32(yh));
+          qf[s][e] = xh;
+          qf[s + KS / 2][e] = yh;
+          ql[s][e] = from_f32<bf16>(x - to_f32(xh));
+          ql[s + KS / 2][e] = from_f32<bf16>(y - to_f32(yh));
         }
+      }
+    }
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) zero(o[b]);
+  }
+
+  // s = K Q^T of a tile of 64 keys (a row tile at LDS address k)
+  __device__ __forceinline__ void scores(f32x16 (&s)[2], uint32_t k, bool two_terms) const {
+    const int lane = threadIdx.x & 63;
+    zero(s[0]);
+    zero(s[1]);
+    bf16x8 f[2][4];
+    auto read = [&](bf16x8(&x)[4], int ks) {
+      const uint32_t at = k + (uint32_t)((ks >> 2) * 8192);
+      const uint32_t at0 = row_frag_addr(at, 0, lane, ks & 3), at1 = row_frag_addr(at, 0, lane, (ks + 1) & 3);
+      x[0] = lds_read_bf16x8<0>(at0);
+      x[1] = lds_read_bf16x8<4096>(at0);
+      x[2] = lds_read_bf16x8<0>(at1);
+      x[3] = lds_read_bf16x8<4096>(at1);
+    };
+    read(f[0], 0);
+#pragma unroll
+    for (int ks = 0; ks < KS; ks += 2) {
+      bf16x8(&x)[4] = f[(ks >> 1) & 1];
+      if (ks + 2 < KS) {
+        read(f[((ks >> 1) + 1) & 1], ks + 2);
+        asm volatile("s_waitcnt lgkmcnt(4)" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]));
+      } else {
+        asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]));
+      }
+      s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], qf[ks], s[0], 0, 0, 0);
+      s[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[1], qf[ks], s[1], 0, 0, 0);
+      s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[2], qf[ks + 1], s[0], 0, 0, 0);
+      s[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[3], qf[ks + 1], s[1], 0, 0, 0);
+      if (two_terms) {
+        s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[0], ql[ks], s[0], 0, 0, 0);
+        s[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[1], ql[ks], s[1], 0, 0, 0);
+        s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[2], ql[ks + 1], s[0], 0, 0, 0);
+        s[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[3], ql[ks + 1], s[1], 0, 0, 0);
       }
     }
   }
 
-  // ---- the new tokens' tile, by all waves into the last one's buffers (row tile for K, slab for V)
-  if (first) {
-    constexpr int HP = HD / 16;  // pairs of 16-byte pieces of a key
-    char* kt = lds + (kWaves - 1) * 2 * TILE;
-    char* vt = kt + TILE;
-    const bool keep = p.group == 0 && (a.write_ring || a.k_nodes != nullptr);
-    const bf16* kn = static_cast<const bf16*>(a.k) + p.n * a.k_n + p.kvh * a.k_h;
-    const bf16* vn = static_cast<const bf16*>(a.v) + p.n * a.v_n + p.kvh * a.v_h;
+  // the tile's weights, rounded, as the B operand of the second product
+  __device__ __forceinline__ void softmax(const f32x16 (&s)[2], bf16x8 (&p)[4], float c2) {
+    float tm = s[0][0];
 #pragma unroll
-    for (int i = 0; i < 64 * HP / kThreads; ++i) {
-      const int idx = threadIdx.x + i * kThreads, t = idx / HP, pc = idx % HP;
-      const int d = __shfl(tree.depth, t, 64);
-      bf16x8 lo{}, hi{};
-      if (t < count) {
-        lo = *reinterpret_cast<const bf16x8*>(kn + t * a.k_t + 8 * pc);
-        hi = *reinterpret_cast<const bf16x8*>(kn + t * a.k_t + HD / 2 + 8 * pc);
-        if (turned) {
-          const float* cr = a.cos_table + (pos + d) * HD + 8 * pc;
-          const float* sr = a.sin_table + (pos + d) * HD + 8 * pc;
+    for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float x = to_f32((bf16)lo[e]), y = to_f32((bf16)hi[e]);
-            lo[e] = from_f32<bf16>(x * cr[e] - y * sr[e]);
-            hi[e] = from_f32<bf16>(y * cr[e] + x * sr[e]);
-          }
-        }
-        if (keep) {
-          bf16* to = node_row<bf16, HD>(a, p, a.k_nodes, a.k_ring, t, pos);
-          *reinterpret_cast<bf16x8*>(to + 8 * pc) = lo;
-          *reinterpret_cast<bf16x8*>(to + HD / 2 + 8 * pc) = hi;
-        }
-      }
-      const int ph = pc + HP;  // piece of the second half
-      *reinterpret_cast<bf16x8*>(kt + (pc >> 3) * 8192 + t * 128 + (((pc & 7) ^ row_swz(t)) * 16)) = lo;
-      *reinterpret_cast<bf16x8*>(kt + (ph >> 3) * 8192 + t * 128 + (((ph & 7) ^ row_swz(t)) * 16)) = hi;
+      for (int e = 0; e < 16; ++e) tm = fmaxf(tm, s[kb][e]);
+    tm = fmaxf(tm, other_half(tm));
+    if (__any(tm > m)) {
+      const float m_new = fmaxf(m, tm);
+      const float corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - m_new) * c2);
+      m = m_new;
+      l *= corr;
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[b][e] *= corr;
     }
-    bool odd = false;
+    const float base = m == -INFINITY ? 0.f : m * c2;
 #pragma unroll
-    for (int i = 0; i < 64 * 2 * HP / kThreads; ++i) {
-      const int idx = threadIdx.x + i * kThreads, t = idx / (2 * HP), pc = idx % (2 * HP);
-      uint4 x = make_uint4(0u, 0u, 0u, 0u);
-      if (t < count) {
-        x = *reinterpret_cast<const uint4*>(vn + t * a.v_t + 8 * pc);
-        odd |= !finite16(x);
-        if (keep) *reinterpret_cast<uint4*>(node_row<bf16, HD>(a, p, a.v_nodes, a.v_ring, t, pos) + 8 * pc) = x;
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][e], c2, -base));
+        l += x;
+        p[2 * kb + (e >> 3)][e & 7] = from_f32<bf16>(x);
       }
-      *reinterpret_cast<uint4*>(vt + (pc >> 3) * 8192 + t * 128 + (((pc & 7) ^ slab_swz(t)) * 16)) = x;
-    }
-    __syncthreads();  // tree_odd is 0 before it is set
-    if (odd) tree_odd = 1;
-    __syncthreads();
   }
 
-  // ---- the tiles
-  uint32_t ka[4], va[NB];
+  // o += V^T P^T of a tile (a slab at LDS address v), keys in the accumulator's order: half h reads keys 4 h .. + 3, then
+  // 8 + 4 h .. of each 16
+  __device__ __forceinline__ void values(const bf16x8 (&p)[4], uint32_t v) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, j16 = lane & 15, t = 4 * (g >> 1) + (j16 >> 2);
+    uint32_t va[NB];
 #pragma unroll
-  for (int s = 0; s < 4; ++s) ka[s] = row_frag_addr(k_lds, 0, lane, s);
-  {
-    // transposing reads in the accumulator's key order: half h takes keys 4 h .. + 3, then 8 + 4 h ..
-    const int g = lane >> 4, j16 = lane & 15, t = 4 * (g >> 1) + (j16 >> 2);
+    for (int b = 0; b < NB; ++b) {
+      const int c = 32 * (b & 1) + 16 * (g & 1) + 4 * (j16 & 3);
+      va[b] = v + (uint32_t)((b / 2) * 8192 + t * 128 + (((c >> 3) ^ slab_swz(t)) * 16) + (c & 7) * 2);
+    }
+    i16x4 f[2][2 * NB];
+    auto read = [&](i16x4(&x)[2 * NB], int ks) {
 #pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      const int c = 32 * (i & 1) + 16 * (g & 1) + 4 * (j16 & 3);
-      va[i] = v_lds + (uint32_t)((i / 2) * 8192 + t * 128 + (((c >> 3) ^ slab_swz(t)) * 16) + (c & 7) * 2);
+      for (int b = 0; b < NB; ++b) {
+        x[2 * b] = lds_read_tr16<0>(va[b] + (uint32_t)(ks * 2048));
+        x[2 * b + 1] = lds_read_tr16<1024>(va[b] + (uint32_t)(ks * 2048));
+      }
+    };
+    auto wait = [&](i16x4(&x)[2 * NB], bool more) {
+      if constexpr (NB == 4) {
+        if (more)
+          asm volatile("s_waitcnt lgkmcnt(8)"
+                       : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]), "+v"(x[4]), "+v"(x[5]), "+v"(x[6]), "+v"(x[7]));
+        else
+          asm volatile("s_waitcnt lgkmcnt(0)"
+                       : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]), "+v"(x[4]), "+v"(x[5]), "+v"(x[6]), "+v"(x[7]));
+      } else {
+        if (more)
+          asm volatile("s_waitcnt lgkmcnt(4)" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]));
+        else
+          asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]));
+      }
+    };
+    read(f[0], 0);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      i16x4(&x)[2 * NB] = f[ks & 1];
+      if (ks < 3) read(f[(ks + 1) & 1], ks + 1);
+      wait(x, ks < 3);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x[2 * b], x[2 * b + 1], 0, 1, 2, 3, 4, 5, 6, 7));
+        o[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, p[ks], o[b], 0, 0, 0);
+      }
     }
   }
+};
+
+// (x of this lane's dims lane, lane + 64, ..) rotated; HD 64 has a pair's halves 32 lanes apart
+template <int HD>
+__device__ __forceinline__ void rotate_row(const TreeArgs& a, float (&x)[HD / 64], int64_t at) {
+  if (a.cos_table == nullptr) return;
+  const int e = (threadIdx.x & 63) & (HD / 2 - 1);
+  const float c = a.cos_table[at * HD + e], s = a.sin_table[at * HD + e];
+  if constexpr (HD == 64) {
+    const float y = other_half(x[0]);
+    x[0] = (threadIdx.x & 63) < 32 ? x[0] * c - y * s : x[0] * c + y * s;
+  } else {
+    const float lo = x[0], hi = x[1];
+    x[0] = lo * c - hi * s;
+    x[1] = hi * c + lo * s;
+  }
+}
+
+// One row by one wave over the keys that it sees, of tiles [t_begin, t_end) and, with `nodes`, of the new tokens: nothing
+// else is touched.  Writes what the tiled kernels write.
+template <int HD>
+__device__ __forceinline__ void selected_row(const TreeArgs& a, const Place& p, const Tree& tree, const Ring& ring, int64_t pos,
+                                             int row, int t_begin, int t_end, bool nodes) {
+  constexpr int E = HD / 64;
+  const int lane = threadIdx.x & 63, t = row / a.rep;
+  const int d = uniform(__shfl(tree.depth, t, 64));
+  const uint64_t sees = shfl64(tree.sees, t);
+  const int lim = visible_age(a, ring, d);
   const float c2 = a.scale * kLog2e;
-  float m[U], l[U];
-  f32x16 o[U][NB];
+  float q[E], o[E], m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    m[u] = -INFINITY;
-    l[u] = 0.f;
-#pragma unroll
-    for (int i = 0; i < NB; ++i) zero(o[u][i]);
+  for (int i = 0; i < E; ++i) {
+    q[i] = to_f32(static_cast<const bf16*>(a.q)[p.n * a.q_n + t * a.q_t + (p.kvh * a.rep + row % a.rep) * a.q_h + lane + 64 * i]);
+    o[i] = 0.f;
   }
+  rotate_row<HD>(a, q, pos + d);
+  auto take = [&](const float(&k)[E], const bf16* v) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) s += q[i] * k[i];
+    s = wave_sum(s) * c2;
+    const float m_new = fmaxf(m, s), corr = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
+    const float x = s == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s - m_new);
+    l = l * corr + x;
+#pragma unroll
+    for (int i = 0; i < E; ++i) o[i] = o[i] * corr + x * to_f32(v[lane + 64 * i]);
+    m = m_new;
+  };
+  const int64_t base = p.n * a.ring_n + (int64_t)p.kvh * a.slots * HD;
+  for (int tile = t_begin; tile < t_end; ++tile) {
+    uint64_t seen = seen_slots(a, ring, tile * 64, lim);
+    while (seen != 0) {
+      const int64_t at = base + ((int64_t)tile * 64 + __builtin_ctzll(seen)) * HD;
+      seen &= seen - 1;
+      float k[E];
+#pragma unroll
+      for (int i = 0; i < E; ++i) k[i] = to_f32(static_cast<const bf16*>(a.k_ring)[at + lane + 64 * i]);
+      take(k, static_cast<const bf16*>(a.v_ring) + at);
+    }
+  }
+  uint64_t seen = nodes ? sees : 0;
+  while (seen != 0) {
+    const int j = __builtin_ctzll(seen);
+    seen &= seen - 1;
+    float k[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) k[i] = to_f32(static_cast<const bf16*>(a.k)[p.n * a.k_n + j * a.k_t + p.kvh * a.k_h + lane + 64 * i]);
+    rotate_row<HD>(a, k, pos + __shfl(tree.depth, j, 64));
+#pragma unroll
+    for (int i = 0; i < E; ++i) k[i] = to_f32(from_f32<bf16>(k[i]));
+    take(k, static_cast<const bf16*>(a.v) + p.n * a.v_n + j * a.v_t + p.kvh * a.v_h);
+  }
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    if (a.nsplit == 1)
+      out_row<bf16>(a, p, row)[lane + 64 * i] = from_f32<bf16>(o[i] / l);
+    else
+      a.part_o[part_row(a, p, row) * HD + lane + 64 * i] = o[i];
+  }
+  if (a.nsplit > 1 && lane == 0) {
+    a.part_ml[2 * part_row(a, p, row)] = l == l ? m : NAN;
+    a.part_ml[2 * part_row(a, p, row) + 1] = l;
+  }
+}
+
+// The new tokens' tile (keys rotated; a row tile, then a slab) by all threads, kept for the caller by the first row
+// group.  Whether the values hold infinities or NaN comes back through `odd` (LDS, 0 before); ends with a barrier.
+template <int HD, int THREADS>
+__device__ __forceinline__ void new_tile(const TreeArgs& a, const Place& p, const Tree& tree, int count, int64_t pos,
+                                         char* kt, int* odd) {
+  constexpr int HP = HD / 16;  // pairs of 16-byte pieces of a key
+  char* vt = kt + kTileBytes<HD>;
+  const bool keep = p.group == 0 && (a.write_ring || a.k_nodes != nullptr);
+  const bf16* kn = static_cast<const bf16*>(a.k) + p.n * a.k_n + p.kvh * a.k_h;
+  const bf16* vn = static_cast<const bf16*>(a.v) + p.n * a.v_n + p.kvh * a.v_h;
+#pragma unroll 1
+  for (int idx = threadIdx.x; idx < 64 * HP; idx += THREADS) {
+    const int t = idx / HP, pc = idx % HP;
+    const int d = __shfl(tree.depth, t, 64);
+    bf16x8 lo{}, hi{};
+    if (t < count) {
+      lo = *reinterpret_cast<const bf16x8*>(kn + t * a.k_t + 8 * pc);
+      hi = *reinterpret_cast<const bf16x8*>(kn + t * a.k_t + HD / 2 + 8 * pc);
+      if (a.cos_table != nullptr) {
+        const float* cr = a.cos_table + (pos + d) * HD + 8 * pc;
+        const float* sr = a.sin_table + (pos + d) * HD + 8 * pc;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = to_f32((bf16)lo[e]), y = to_f32((bf16)hi[e]);
+          lo[e] = from_f32<bf16>(x * cr[e] - y * sr[e]);
+          hi[e] = from_f32<bf16>(y * cr[e] + x * sr[e]);
+        }
+      }
+      if (keep) {
+        bf16* to = node_row<bf16, HD>(a, p, a.k_nodes, a.k_ring, t, pos);
+        *reinterpret_cast<bf16x8*>(to + 8 * pc) = lo;
+        *reinterpret_cast<bf16x8*>(to + HD / 2 + 8 * pc) = hi;
+      }
+    }
+    const int ph = pc + HP;  // piece of the second half
+    *reinterpret_cast<bf16x8*>(kt + (pc >> 3) * 8192 + t * 128 + (((pc & 7) ^ row_swz(t)) * 16)) = lo;
+    *reinterpret_cast<bf16x8*>(kt + (ph >> 3) * 8192 + t * 128 + (((ph & 7) ^ row_swz(t)) * 16)) = hi;
+  }
+  bool bad = false;
+#pragma unroll 2
+  for (int idx = threadIdx.x; idx < 64 * 2 * HP; idx += THREADS) {
+    const int t = idx / (2 * HP), pc = idx % (2 * HP);
+    uint4 x = make_uint4(0u, 0u, 0u, 0u);
+    if (t < count) {
+      x = *reinterpret_cast<const uint4*>(vn + t * a.v_t + 8 * pc);
+      bad |= !finite16(x);
+      if (keep) *reinterpret_cast<uint4*>(node_row<bf16, HD>(a, p, a.v_nodes, a.v_ring, t, pos) + 8 * pc) = x;
+    }
+    *reinterpret_cast<uint4*>(vt + (pc >> 3) * 8192 + t * 128 + (((pc & 7) ^ slab_swz(t)) * 16)) = x;
+  }
+  if (bad) *odd = 1;
+  __syncthreads();
+}
+
+// What of a tile of slots some node sees (`any`) and all see (`all`); then the values' slab in LDS: rows that no node
+// sees are zeroed, and whether rows that only some see hold infinities or NaN comes back.
+template <int HD>
+__device__ __forceinline__ bool guard_values(char* vt, uint64_t any, uint64_t all) {
+  const int lane = threadIdx.x & 63;
+  if (any != ~0ull) {
+    for (int t = lane >> 3; t < 64; t += 8)
+      if (!((any >> t) & 1)) {
+#pragma unroll
+        for (int b = 0; b < HD / 64; ++b)
+          *reinterpret_cast<uint4*>(vt + b * 8192 + t * 128 + (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+      }
+  }
+  bool bad = false;
+  if (any != all) {
+    if (((any & ~all) >> lane) & 1) {
+#pragma unroll
+      for (int b = 0; b < HD / 64; ++b)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) bad |= !finite16(*reinterpret_cast<const uint4*>(vt + b * 8192 + lane * 128 + j * 16));
+    }
+    bad = __any(bad);
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  return bad;
+}
+
+// The keys of a tile that a unit's rows see, as a mask; -inf for the others' scores.
+__device__ __forceinline__ void mask_tile(f32x16 (&s)[2], uint64_t seen) {
+  mask_keys(s[0], (uint32_t)seen);
+  mask_keys(s[1], (uint32_t)(seen >> 32));
+}
+
+// One unit, its keys spread over the workgroup's waves.
+template <int HD>
+__global__ void __launch_bounds__(kThreads, HD == 64 ? 2 : 1) k_swa_tree_mm(const TreeArgs a) {
+  constexpr int NB = HD / 32;
+  constexpr int TILE = kTileBytes<HD>, LOADS = TILE / 1024;
+  constexpr int RED = HD + 4;  // floats of a query's row when the waves' results meet
+  static_assert(kWaves * 32 * RED * 4 <= kWaves * 2 * TILE, "the waves' results fit the tiles' LDS");
+  __shared__ __align__(1024) char lds[kWaves * 2 * TILE];  // a K tile and a V slab per wave
+  __shared__ float red_ml[kWaves][32][2];
+  __shared__ int odd_values;  // values that only some rows see hold infinities or NaN
+  const Place p = place_of(a);
+  if (!p.valid) return;
+  const int w = uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
+  const int count = a.counts != nullptr ? min(max(uniform(a.counts[p.n]), 0), a.nodes) : a.nodes;
+  const int row0 = p.group * 32, row1 = min(row0 + 32, count * a.rep);
+  if (row0 >= row1) return;
+  const bool first = p.split == 0;
+
+  char* kt = lds + w * 2 * TILE;
+  char* vt = kt + TILE;
+  const uint32_t k_lds = lds_addr(kt), v_lds = k_lds + TILE;
+  const bf16* kr = static_cast<const bf16*>(a.k_ring) + p.n * a.ring_n + (int64_t)p.kvh * a.slots * HD;
+  const bf16* vr = static_cast<const bf16*>(a.v_ring) + p.n * a.ring_n + (int64_t)p.kvh * a.slots * HD;
+  const TileLoad<HD> load(lane);
+  auto issue = [&](const bf16* src, uint32_t dst, int tile, bool is_k) {
+#pragma unroll
+    for (int g = 0; g < LOADS; ++g) load.issue(src, a.slots, dst, tile, g, is_k);
+  };
+  // the tile a wave starts with needs no position in the first split: ask for it at once (the last wave
+  // starts with the new tokens there)
+  const bool early = first && w < kWaves - 1;
+  if (early) {
+    issue(kr, k_lds, w, true);
+    issue(vr, v_lds, w, false);
+  }
+  const int64_t pos = uniform(a.positions[p.n]);
+  const Tree tree = read_tree(a, p.n, count, pos, lane);
+  if (tree.bad) {
+    refuse_rows<bf16, HD>(a, p, row0, row1, kThreads);
+    wait_vmcnt<0>();  // no LDS write of this workgroup's loads outlives it
+    return;
+  }
+  if (threadIdx.x == 0) odd_values = 0;
+  const Ring ring = read_ring(a, pos);
+  const int ntiles = (ring.used + 63) / 64;
+  const int t_begin = (int)((int64_t)ntiles * p.split / a.nsplit), t_end = (int)((int64_t)ntiles * (p.split + 1) / a.nsplit);
+  // wave w takes places w, w + kWaves, .. of the split's list; the first split's has the new tokens at place
+  // kWaves - 1, whether or not its cache reaches that far
+  auto tile_at = [&](int i) { return t_begin + (first && i >= kWaves ? i - 1 : i); };
+  auto has = [&](int i) { return (first && i == kWaves - 1) || tile_at(i) < t_end; };
+
+  const bool turned = a.cos_table != nullptr;
+  Unit<HD> u;
+  u.load(a, p, tree, ring, pos, row0 + r, row1);
+  __syncthreads();  // odd_values is 0
+  if (first) new_tile<HD, kThreads>(a, p, tree, count, pos, lds + (kWaves - 1) * 2 * TILE, &odd_values);
+  const float c2 = a.scale * kLog2e;
   const int lim_any = visible_age(a, ring, 0), lim_all = visible_age(a, ring, tree.deepest);
 
   bool loaded = early;  // this wave's next ring tile is on its way
@@ -377,223 +616,197 @@ __global__ void __launch_bounds__(kThreads, HD == 64 ? 2 : 1) k_swa_tree_mm(cons
       }
       wait_vmcnt<LOADS>();  // K has landed, V may still be on its way
     }
-    f32x16 s[U][2];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      zero(s[u][0]);
-      zero(s[u][1]);
-    }
-#pragma unroll
-    for (int ks = 0; ks < KS; ks += 2) {
-      bf16x8 f0[2], f1[2];
-      const uint32_t at0 = ka[ks & 3] + (uint32_t)((ks >> 2) * 8192), at1 = ka[(ks + 1) & 3] + (uint32_t)((ks >> 2) * 8192);
-      f0[0] = lds_read_bf16x8<0>(at0);
-      f0[1] = lds_read_bf16x8<4096>(at0);
-      f1[0] = lds_read_bf16x8<0>(at1);
-      f1[1] = lds_read_bf16x8<4096>(at1);
-      asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(f0[0]), "+v"(f0[1]), "+v"(f1[0]), "+v"(f1[1]));
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          s[u][kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f0[kb], qf[u][ks], s[u][kb], 0, 0, 0);
-          s[u][kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f1[kb], qf[u][ks + 1], s[u][kb], 0, 0, 0);
-        }
-        if (turned) {
-#pragma unroll
-          for (int kb = 0; kb < 2; ++kb) {
-            s[u][kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f0[kb], ql[u][ks], s[u][kb], 0, 0, 0);
-            s[u][kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f1[kb], ql[u][ks + 1], s[u][kb], 0, 0, 0);
-          }
-        }
-      }
-    }
+    f32x16 s[2];
+    u.scores(s, k_lds, turned);
     pin_loads();
     // every K read is back: the next tile's K on its way
     const int next = more ? tile_at(i + kWaves) : 0;
     if (more) issue(kr, k_lds, next, true);
-
-    // ---- masks
-    uint64_t any = ~0ull, all = 0;  // keys that some node sees, that all see
+    uint64_t any = ~0ull, all = 0;
     if (!is_tree) {
       any = seen_slots(a, ring, s0, lim_any);
       all = seen_slots(a, ring, s0, lim_all);
     }
-    if (all != ~0ull) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const uint64_t vis = is_tree ? sees[u] : seen_slots(a, ring, s0, lim[u]);
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) mask_keys(s[u][kb], (uint32_t)(vis >> (32 * kb)));
-      }
-    }
-    // ---- softmax of the tile
-    bf16x8 pw[U][4];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float tm = s[u][0][0];
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) tm = fmaxf(tm, s[u][kb][e]);
-      tm = fmaxf(tm, other_half(tm));
-      if (__any(tm > m[u])) {
-        const float m_new = fmaxf(m[u], tm);
-        const float corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m[u] - m_new) * c2);
-        m[u] = m_new;
-        l[u] *= corr;
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[u][b][e] *= corr;
-      }
-      const float base = m[u] == -INFINITY ? 0.f : m[u] * c2;
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][kb][e], c2, -base));
-          l[u] += x;
-          s[u][kb][e] = x;
-          pw[u][2 * kb + (e >> 3)][e & 7] = from_f32<bf16>(x);
-        }
-    }
-    // ---- values
-    bool odd = is_tree && tree_odd != 0;
+    if (all != ~0ull) mask_tile(s, is_tree ? u.sees : seen_slots(a, ring, s0, u.lim));
+    bf16x8 pw[4];
+    u.softmax(s, pw, c2);
     if (!is_tree) {
       if (more)
         wait_vmcnt<LOADS>();
       else
         wait_vmcnt<0>();
       pin_loads();
-      if (any != ~0ull) {  // rows that no node sees: zeros
-        for (int t = lane >> 3; t < 64; t += 8)
-          if (!((any >> t) & 1)) {
-#pragma unroll
-            for (int b = 0; b < NT; ++b)
-              *reinterpret_cast<uint4*>(lds + (w * 2 + 1) * TILE + b * 8192 + t * 128 + (lane & 7) * 16) =
-                  make_uint4(0u, 0u, 0u, 0u);
-          }
-      }
-      if (any != all) {  // rows that some nodes see: infinities or NaN must not meet the others' zeros
-        bool bad = false;
-        if (((any & ~all) >> lane) & 1) {
-#pragma unroll
-          for (int b = 0; b < NT; ++b)
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              bad |= !finite16(*reinterpret_cast<const uint4*>(lds + (w * 2 + 1) * TILE + b * 8192 + lane * 128 + j * 16));
-        }
-        odd = __any(bad);
-      }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (all != ~0ull && guard_values<HD>(vt, any, all)) odd_values = 1;
     }
-    if (!odd) {
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        i16x4 f[2 * NB];
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          const uint32_t at = va[b] + (uint32_t)(ks * 2048);
-          f[2 * b] = lds_read_tr16<0>(at);
-          f[2 * b + 1] = lds_read_tr16<1024>(at);
-        }
-        if constexpr (NB == 4)
-          asm volatile("s_waitcnt lgkmcnt(0)"
-                       : "+v"(f[0]), "+v"(f[1]), "+v"(f[2]), "+v"(f[3]), "+v"(f[4]), "+v"(f[5]), "+v"(f[6]), "+v"(f[7]));
-        else
-          asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(f[0]), "+v"(f[1]), "+v"(f[2]), "+v"(f[3]));
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          const bf16x8 vf =
-              __builtin_bit_cast(bf16x8, __builtin_shufflevector(f[2 * b], f[2 * b + 1], 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-          for (int u = 0; u < U; ++u) o[u][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pw[u][ks], o[u][b], 0, 0, 0);
-        }
-      }
-    } else {
-      // the weights through this wave's K buffer (whatever was on its way there lands first and is asked for
-      // again), a key at a time, selected
-      wait_vmcnt<0>();
-      pin_loads();
-      float* ps = reinterpret_cast<float*>(lds + w * 2 * TILE);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) ps[(32 * kb + acc_row(e)) * 32 + r] = s[u][kb][e];
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        for (int key = 0; key < 64; ++key) {
-          const float x = ps[key * 32 + r];
-          const char* row = lds + (w * 2 + 1) * TILE + key * 128;
-#pragma unroll
-          for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int d = 32 * (b & 1) + 8 * (e >> 2) + 4 * h + (e & 3);
-              const float y = to_f32(*reinterpret_cast<const bf16*>(row + (b >> 1) * 8192 + (((d >> 3) ^ slab_swz(key)) * 16) + (d & 7) * 2));
-              o[u][b][e] = x > 0.f ? __builtin_fmaf(x, y, o[u][b][e]) : o[u][b][e];
-            }
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      }
-      if (more) issue(kr, k_lds, next, true);
-    }
+    u.values(pw, v_lds);
     pin_loads();
     if (more) issue(vr, v_lds, next, false);
     loaded = more;
   }
   if (early && !has(w)) wait_vmcnt<0>();  // an early tile that the request does not have
 
-  // ---- the waves' results meet, unit by unit
+  // ---- the waves' results meet
   float* red = reinterpret_cast<float*>(lds);
+  __syncthreads();
+  u.l += other_half(u.l);
+  if (h == 0) {
+    red_ml[w][r][0] = u.m;
+    red_ml[w][r][1] = u.l;
+  }
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    __syncthreads();
-    l[u] += other_half(l[u]);
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4)
+      *reinterpret_cast<f32x4*>(red + (w * 32 + r) * RED + 32 * b + 2 * e + 4 * h) =
+          f32x4{u.o[b][e], u.o[b][e + 1], u.o[b][e + 2], u.o[b][e + 3]};
+  __syncthreads();
+  if (odd_values != 0) {
+    for (int row = row0 + w; row < row1; row += kWaves) selected_row<HD>(a, p, tree, ring, pos, row, t_begin, t_end, first);
+    return;
+  }
+  for (int idx = threadIdx.x; idx < 32 * HD / 4; idx += kThreads) {
+    const int qr = idx / (HD / 4), e = idx % (HD / 4) * 4, row = row0 + qr;
+    if (row >= row1) continue;
+    float mm = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < kWaves; ++x) mm = fmaxf(mm, red_ml[x][qr][0]);
+    float den = 0.f;
+    f32x4 num{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < kWaves; ++x) {
+      const float f = red_ml[x][qr][0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((red_ml[x][qr][0] - mm) * c2);
+      const f32x4 y = *reinterpret_cast<const f32x4*>(red + (x * 32 + qr) * RED + e);
+      den += f * red_ml[x][qr][1];
+      if (f != 0.f) num += f * y;
+    }
+    if (a.nsplit == 1) {
+      const float inv = 1.0f / den;
+      bf16 y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] = from_f32<bf16>(num[j] * inv);
+      *reinterpret_cast<uint2*>(out_row<bf16>(a, p, row) + e) = *reinterpret_cast<const uint2*>(y);
+    } else {
+      const int64_t at = part_row(a, p, row);
+      *reinterpret_cast<f32x4*>(a.part_o + at * HD + e) = num;
+      if (e == 0) {
+        a.part_ml[2 * at] = den == den ? mm * c2 : NAN;
+        a.part_ml[2 * at + 1] = den;
+      }
+    }
+  }
+}
+
+// A unit per wave, the workgroup's NW waves sharing each tile in LDS: for so many rows that reading the cache again for
+// every 32 of them would cost more than it brings.  Tiles alternate between two slots: one is loaded while the
+// other is used, a barrier per tile.
+template <int HD, int NW>
+__global__ void __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) k_swa_tree_wide(const TreeArgs a) {
+  constexpr int NB = HD / 32, TILE = kTileBytes<HD>, SLOT = 2 * TILE, LOADS = SLOT / 1024;
+  static_assert(LOADS % NW == 0, "a tile's loads divide among the waves");
+  __shared__ __align__(1024) char lds[2 * SLOT];
+  __shared__ int tree_odd;  // the new values hold infinities or NaN
+  const Place p = place_of(a);
+  if (!p.valid) return;
+  const int w = uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
+  const int count = a.counts != nullptr ? min(max(uniform(a.counts[p.n]), 0), a.nodes) : a.nodes;
+  const int row0 = p.group * 32 * NW, row1 = min(row0 + 32 * NW, count * a.rep);
+  if (row0 >= row1) return;
+  const bool first = p.split == 0;
+  const bf16* kr = static_cast<const bf16*>(a.k_ring) + p.n * a.ring_n + (int64_t)p.kvh * a.slots * HD;
+  const bf16* vr = static_cast<const bf16*>(a.v_ring) + p.n * a.ring_n + (int64_t)p.kvh * a.slots * HD;
+  const TileLoad<HD> load(lane);
+  const uint32_t lds0 = lds_addr(lds);
+  auto issue = [&](int tile, int slot) {
+#pragma unroll
+    for (int i = 0; i < LOADS / NW; ++i) {
+      const int g = w + NW * i;  // K's loads first
+      const bool is_k = g < LOADS / 2;
+      load.issue(is_k ? kr : vr, a.slots, lds0 + (uint32_t)(slot * SLOT + (is_k ? 0 : TILE)), tile, is_k ? g : g - LOADS / 2,
+                 is_k);
+    }
+  };
+  const int64_t pos = uniform(a.positions[p.n]);
+  const Tree tree = read_tree(a, p.n, count, pos, lane);
+  if (tree.bad) {
+    refuse_rows<bf16, HD>(a, p, row0, row1, NW * 64);
+    return;
+  }
+  if (threadIdx.x == 0) tree_odd = 0;
+  const Ring ring = read_ring(a, pos);
+  const int ntiles = (ring.used + 63) / 64;
+  const int t_begin = (int)((int64_t)ntiles * p.split / a.nsplit), t_end = (int)((int64_t)ntiles * (p.split + 1) / a.nsplit);
+  // the list: the new tokens (the first split's), then the slots' tiles
+  const int lead = first ? 1 : 0, listed = lead + t_end - t_begin;
+  if (first && listed > 1) issue(t_begin, 1);
+  if (!first && listed > 0) issue(t_begin, 0);
+  const bool turned = a.cos_table != nullptr;
+  if (first) {
+    __syncthreads();  // tree_odd is 0
+    new_tile<HD, NW * 64>(a, p, tree, count, pos, lds, &tree_odd);
+  }
+  Unit<HD> u;
+  const bool unit_ok = row0 + 32 * w < row1;
+  u.load(a, p, tree, ring, pos, row0 + 32 * w + r, row1);
+  const float c2 = a.scale * kLog2e;
+  const int lim_any = visible_age(a, ring, 0), lim_all = visible_age(a, ring, tree.deepest);
+  bool odd = first && tree_odd != 0;
+  for (int i = 0; i < listed; ++i) {
+    const bool is_tree = first && i == 0;
+    const int tile = t_begin + i - lead, s0 = tile * 64, slot = i & 1;
+    if (!is_tree) {
+      wait_vmcnt<0>();
+      pin_loads();
+      __builtin_amdgcn_s_barrier();  // the tile is in LDS; every wave is done with the other slot
+      pin_loads();
+      if (i + 1 < listed) issue(tile + 1, slot ^ 1);
+    }
+    if (!unit_ok) continue;
+    f32x16 s[2];
+    u.scores(s, lds0 + (uint32_t)(slot * SLOT), turned);
+    uint64_t any = ~0ull, all = 0;
+    if (!is_tree) {
+      any = seen_slots(a, ring, s0, lim_any);
+      all = seen_slots(a, ring, s0, lim_all);
+    }
+    if (all != ~0ull) mask_tile(s, is_tree ? u.sees : seen_slots(a, ring, s0, u.lim));
+    bf16x8 pw[4];
+    u.softmax(s, pw, c2);
+    if (!is_tree && all != ~0ull)  // every wave writes the same zeros
+      odd |= guard_values<HD>(lds + slot * SLOT + TILE, any, all);
+    u.values(pw, lds0 + (uint32_t)(slot * SLOT + TILE));
+  }
+  if (odd) {
+    const int last = min(row0 + 32 * (w + 1), row1);
+    for (int row = row0 + 32 * w; row < last; ++row) selected_row<HD>(a, p, tree, ring, pos, row, t_begin, t_end, first);
+    return;
+  }
+  const int row = row0 + 32 * w + r;
+  if (row >= row1) return;
+  u.l += other_half(u.l);
+  if (a.nsplit == 1) {
+    const float inv = 1.0f / u.l;
+    bf16* og = out_row<bf16>(a, p, row) + 4 * h;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        bf16 y[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = from_f32<bf16>(u.o[b][e + j] * inv);
+        *reinterpret_cast<uint2*>(og + 32 * b + 2 * e) = *reinterpret_cast<const uint2*>(y);
+      }
+  } else {
+    const int64_t at = part_row(a, p, row);
     if (h == 0) {
-      red_ml[w][r][0] = m[u];
-      red_ml[w][r][1] = l[u];
+      a.part_ml[2 * at] = u.l == u.l ? u.m * c2 : NAN;
+      a.part_ml[2 * at + 1] = u.l;
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int e = 0; e < 16; e += 4)
-        *reinterpret_cast<f32x4*>(red + (w * 32 + r) * RED + 32 * b + 2 * e + 4 * h) =
-            f32x4{o[u][b][e], o[u][b][e + 1], o[u][b][e + 2], o[u][b][e + 3]};
-    __syncthreads();
-    for (int idx = threadIdx.x; idx < 32 * HD / 4; idx += kThreads) {
-      const int qr = idx / (HD / 4), e = idx % (HD / 4) * 4, row = row0 + 32 * u + qr;
-      if (row >= row1) continue;
-      float mm = -INFINITY;
-#pragma unroll
-      for (int x = 0; x < kWaves; ++x) mm = fmaxf(mm, red_ml[x][qr][0]);
-      float den = 0.f;
-      f32x4 num{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int x = 0; x < kWaves; ++x) {
-        const float f = red_ml[x][qr][0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((red_ml[x][qr][0] - mm) * c2);
-        const f32x4 y = *reinterpret_cast<const f32x4*>(red + (x * 32 + qr) * RED + e);
-        den += f * red_ml[x][qr][1];
-        if (f != 0.f) num += f * y;
-      }
-      if (a.nsplit == 1) {
-        const float inv = 1.0f / den;
-        bf16* og = static_cast<bf16*>(a.out) + p.n * a.o_n + row / a.rep * a.o_t + (p.kvh * a.rep + row % a.rep) * a.o_h + e;
-        bf16 y[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = from_f32<bf16>(num[j] * inv);
-        *reinterpret_cast<uint2*>(og) = *reinterpret_cast<const uint2*>(y);
-      } else {
-        const int64_t at = part_row(a, p, row);
-        *reinterpret_cast<f32x4*>(a.part_o + at * HD + e) = num;
-        if (e == 0) {
-          a.part_ml[2 * at] = mm * c2;
-          a.part_ml[2 * at + 1] = den;
-        }
-      }
-    }
+        *reinterpret_cast<f32x4*>(a.part_o + at * HD + 32 * b + 2 * e + 4 * h) =
+            f32x4{u.o[b][e], u.o[b][e + 1], u.o[b][e + 2], u.o[b][e + 3]};
   }
 }
 
@@ -642,7 +855,6 @@ __global__ void __launch_bounds__(kThreads) k_swa_tree_join(const TreeArgs a) {
 template <int HD>
 __global__ void __launch_bounds__(kThreads) k_swa_tree_f32(const TreeArgs a) {
   constexpr int NJ = HD / 16, LK = HD + 4, RED = HD + 4;
-  constexpr float kLog2e = 1.4426950408889634f;
   __shared__ __align__(16) float kt[64 * LK];  // the new keys, rotated; at the end the waves' results
   __shared__ __align__(16) float ps[kWaves][16][20];
   __shared__ float red_ml[kWaves][16][2];
@@ -656,7 +868,7 @@ __global__ void __launch_bounds__(kThreads) k_swa_tree_f32(const TreeArgs a) {
   const int64_t pos = uniform(a.positions[p.n]);
   const Tree tree = read_tree(a, p.n, count, pos, lane);
   if (tree.bad) {
-    refuse_rows<float, HD>(a, p, row0, row1);
+    refuse_rows<float, HD>(a, p, row0, row1, kThreads);
     return;
   }
   const Ring ring = read_ring(a, pos);
@@ -838,19 +1050,20 @@ __global__ void __launch_bounds__(kThreads) k_swa_tree_f32(const TreeArgs a) {
       if (f != 0.f) num += f * kt[(x * 16 + qr) * RED + e];
     }
     if (a.nsplit == 1) {
-      static_cast<float*>(a.out)[p.n * a.o_n + row / a.rep * a.o_t + (p.kvh * a.rep + row % a.rep) * a.o_h + e] = num / den;
+      out_row<float>(a, p, row)[e] = num / den;
     } else {
       const int64_t at = part_row(a, p, row);
       a.part_o[at * HD + e] = num;
       if (e == 0) {
-        a.part_ml[2 * at] = mm * c2;
+        a.part_ml[2 * at] = den == den ? mm * c2 : NAN;
         a.part_ml[2 * at + 1] = den;
       }
     }
   }
 }
 
-// Workgroups' shape: rows of a workgroup, workgroups along a (request, kv head)'s rows, splits of its slots.
+// Workgroups' shape: units of 32 rows that share a workgroup's tiles (1: k_swa_tree_mm, 4 or 8: k_swa_tree_wide; 0: 16
+// fp32 rows), workgroups along a (request, kv head)'s rows, splits of its slots.
 struct TreePlan {
   int units, groups, nsplit;
 };
@@ -860,11 +1073,12 @@ constexpr int kMaxTreeSplits = 64;
 TreePlan plan_tree(int64_t n_req, int64_t n_heads, int64_t n_kv_heads, int64_t nodes, int64_t head_dim, int64_t slots,
                    bool b16) {
   TreePlan p;
-  const int64_t rows = n_heads / n_kv_heads * nodes;
-  p.units = 1;
+  const int64_t rows = n_heads / n_kv_heads * nodes, lists = n_req * n_kv_heads, tiles = (slots + 63) / 64;
+  p.units = b16 ? 1 : 0;
+  if (b16 && rows > 64 && lists * ((rows + 31) / 32) >= 256) p.units = rows > 128 ? 8 : 4;
   const int64_t per = b16 ? 32 * p.units : 16;
   p.groups = (int)((rows + per - 1) / per);
-  const int64_t base = n_req * n_kv_heads * p.groups, tiles = (slots + 63) / 64;
+  const int64_t base = lists * p.groups;
   const int64_t want = head_dim == 64 ? 512 : 256, least = 8;  // workgroups, tiles of a split
   p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({(want + base - 1) / base, tiles / least, (int64_t)kMaxTreeSplits}));
   return p;
@@ -874,10 +1088,14 @@ template <int HD>
 void launch_tree(const TreeArgs& m, const TreePlan& p, bool b16, hipStream_t st) {
   const int64_t lists = (int64_t)m.n_req * m.n_kv_heads * m.nsplit;
   const dim3 grid((unsigned)((lists + kXcds - 1) / kXcds * kXcds * m.groups));
-  if (!b16)
+  if (p.units == 0)
     hipLaunchKernelGGL(k_swa_tree_f32<HD>, grid, dim3(kThreads), 0, st, m);
+  else if (p.units == 1)
+    hipLaunchKernelGGL(k_swa_tree_mm<HD>, grid, dim3(kThreads), 0, st, m);
+  else if (p.units == 4)
+    hipLaunchKernelGGL((k_swa_tree_wide<HD, 4>), grid, dim3(256), 0, st, m);
   else
-    hipLaunchKernelGGL((k_swa_tree_mm<HD, 1>), grid, dim3(kThreads), 0, st, m);
+    hipLaunchKernelGGL((k_swa_tree_wide<HD, 8>), grid, dim3(512), 0, st, m);
   if (m.nsplit > 1) {
     const int64_t n = (int64_t)m.n_req * m.n_kv_heads * m.rows * (HD / 4);
     const dim3 jg((unsigned)((n + kThreads - 1) / kThreads));
