@@ -107,8 +107,14 @@ __device__ __forceinline__ Tree read_tree(const TreeArgs& a, int n, int count, i
 // What a request's cache holds, as ages: slot sinks + i holds the token of age (cur - i) mod window, the
 // newest cached one having age 0.
 struct Ring {
-  int used;   // slots that hold tokens are those below
+  int used;       // slots that hold tokens are those below
   int cur, held;  // of the newest token; ages below `held` exist
+};
+
+// The slots outside every node's view start behind the newest token and may go on from the window's first slot:
+// [from, to) and [sinks, over).
+struct Edge {
+  int from, to, over;
 };
 
 __device__ __forceinline__ Ring read_ring(const TreeArgs& a, int64_t pos) {
@@ -130,6 +136,19 @@ __device__ __forceinline__ uint64_t seen_slots(const TreeArgs& a, const Ring& r,
   const int over = max(start - oldest, 0);  // slots of the part that wraps
   return bit_range(-s0, min(a.sinks, r.used) - s0) | bit_range(max(oldest, start), newest + 1) |
          bit_range(a.slots - s0 - over, a.slots - s0);
+}
+
+__device__ __forceinline__ Edge read_edge(const TreeArgs& a, const Ring& r, int lim_all) {
+  Edge e;
+  e.from = r.used < a.sinks ? r.used : a.sinks + r.cur + 1;
+  e.to = e.from + a.window - max(lim_all, 0);
+  e.over = a.sinks + max(e.to - a.slots, 0);
+  if (r.used < a.sinks) e.to = a.slots;
+  return e;
+}
+// whether every node sees the 64 slots from s0
+__device__ __forceinline__ bool clean_tile(const TreeArgs& a, const Edge& e, int s0) {
+  return s0 + 64 <= a.slots && (s0 + 64 <= e.from || s0 >= e.to) && (e.over == a.sinks || s0 + 64 <= a.sinks || s0 >= e.over);
 }
 
 // This workgroup's work.  Row groups of one (request, kv head, split) read the same slots: their ids are 8
@@ -192,18 +211,20 @@ __device__ __forceinline__ bool finite16(const uint4& v) {  // eight bf16
 template <int HD>
 constexpr int kTileBytes = HD / 64 * 8192;
 
-// The 1 KB loads g of the HD / 8 that bring a tile of 64 slots into LDS, as a row tile (K) or a slab (V).  Slots past the
-// ring read as zeros.
-template <int HD>
+// The 1 KB loads g of the HD / 8 that bring a tile of 64 slots of a (request, kv head)'s keys or values into LDS, as a row
+// tile (K) or a slab (V).  Slots past the ring read as zeros.
+template <int HD, bool K>
 struct TileLoad {
-  int voff_k[2], voff_v;
-  __device__ __forceinline__ explicit TileLoad(int lane)
-      : voff_k{row_src_off(0, lane, HD), row_src_off(1, lane, HD) - 16 * HD}, voff_v(slab_src_off(0, lane, HD)) {}
-  __device__ __forceinline__ void issue(const bf16* ring, int slots, uint32_t dst, int tile, int g, bool is_k) const {
-    const int n = max(min(slots - tile * 64, 64), 0), t = g >> 3, rg = g & 7;
-    const __amdgpu_buffer_rsrc_t rs =
-        buffer_rsrc(ring + (int64_t)tile * 64 * HD + 64 * t, (uint32_t)max(n * HD * 2 - 128 * t, 0));
-    buffer_load_lds_raw(rs, lds_ptr(dst + (uint32_t)(g * 1024)), 16, (is_k ? voff_k[rg & 1] : voff_v) + rg * 16 * HD, 0, 0, 0);
+  __amdgpu_buffer_rsrc_t ring;
+  int even, odd;  // this lane's piece of row groups 0 and 1, less the group's own offset
+  __device__ __forceinline__ TileLoad(const void* base, int slots, int lane)
+      : ring(buffer_rsrc(base, (uint32_t)(slots * HD * 2))),
+        even(K ? row_src_off(0, lane, HD) : slab_src_off(0, lane, HD)),
+        odd(K ? row_src_off(1, lane, HD) - 16 * HD : even) {}
+  __device__ __forceinline__ void issue(uint32_t dst, int tile, int g) const {
+    const int rg = g & 7;
+    buffer_load_lds_raw(ring, lds_ptr(dst + (uint32_t)(g * 1024)), 16,
+                        (rg & 1 ? odd : even) + (tile * 128 * HD + rg * 16 * HD + (g >> 3) * 128), 0, 0, 0);
   }
 };
 
@@ -422,8 +443,10 @@ __device__ __forceinline__ void selected_row(const TreeArgs& a, const Place& p, 
     m = m_new;
   };
   const int64_t base = p.n * a.ring_n + (int64_t)p.kvh * a.slots * HD;
+#pragma unroll 1
   for (int tile = t_begin; tile < t_end; ++tile) {
     uint64_t seen = seen_slots(a, ring, tile * 64, lim);
+#pragma unroll 1
     while (seen != 0) {
       const int64_t at = base + ((int64_t)tile * 64 + __builtin_ctzll(seen)) * HD;
       seen &= seen - 1;
@@ -434,6 +457,7 @@ __device__ __forceinline__ void selected_row(const TreeArgs& a, const Place& p, 
     }
   }
   uint64_t seen = nodes ? sees : 0;
+#pragma unroll 1
   while (seen != 0) {
     const int j = __builtin_ctzll(seen);
     seen &= seen - 1;
@@ -462,9 +486,8 @@ __device__ __forceinline__ void selected_row(const TreeArgs& a, const Place& p, 
 // group.  Whether the values hold infinities or NaN comes back through `odd` (LDS, 0 before); ends with a barrier.
 template <int HD, int THREADS>
 __device__ __forceinline__ void new_tile(const TreeArgs& a, const Place& p, const Tree& tree, int count, int64_t pos,
-                                         char* kt, int* odd) {
+                                         char* kt, char* vt, int* odd) {
   constexpr int HP = HD / 16;  // pairs of 16-byte pieces of a key
-  char* vt = kt + kTileBytes<HD>;
   const bool keep = p.group == 0 && (a.write_ring || a.k_nodes != nullptr);
   const bf16* kn = static_cast<const bf16*>(a.k) + p.n * a.k_n + p.kvh * a.k_h;
   const bf16* vn = static_cast<const bf16*>(a.v) + p.n * a.v_n + p.kvh * a.v_h;
@@ -517,26 +540,19 @@ __device__ __forceinline__ void new_tile(const TreeArgs& a, const Place& p, cons
 template <int HD>
 __device__ __forceinline__ bool guard_values(char* vt, uint64_t any, uint64_t all) {
   const int lane = threadIdx.x & 63;
-  if (any != ~0ull) {
-    for (int t = lane >> 3; t < 64; t += 8)
-      if (!((any >> t) & 1)) {
-#pragma unroll
-        for (int b = 0; b < HD / 64; ++b)
-          *reinterpret_cast<uint4*>(vt + b * 8192 + t * 128 + (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-      }
-  }
+  const uint64_t none = ~any, part = any & ~all;
   bool bad = false;
-  if (any != all) {
-    if (((any & ~all) >> lane) & 1) {
-#pragma unroll
-      for (int b = 0; b < HD / 64; ++b)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) bad |= !finite16(*reinterpret_cast<const uint4*>(vt + b * 8192 + lane * 128 + j * 16));
-    }
-    bad = __any(bad);
+#pragma unroll 1
+  for (int i = 0; i < HD / 8; ++i) {  // 8 rows at a time, a 16-byte piece per lane
+    const int t = 8 * (i & 7) + (lane >> 3);
+    uint4* piece = reinterpret_cast<uint4*>(vt + (i >> 3) * 8192 + t * 128 + (lane & 7) * 16);
+    if ((none >> t) & 1)
+      *piece = make_uint4(0u, 0u, 0u, 0u);
+    else if ((part >> t) & 1)
+      bad |= !finite16(*piece);
   }
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  return bad;
+  return __any(bad);
 }
 
 // The keys of a tile that a unit's rows see, as a mask; -inf for the others' scores.
@@ -566,19 +582,23 @@ __global__ void __launch_bounds__(kThreads, HD == 64 ? 2 : 1) k_swa_tree_mm(cons
   char* kt = lds + w * 2 * TILE;
   char* vt = kt + TILE;
   const uint32_t k_lds = lds_addr(kt), v_lds = k_lds + TILE;
-  const bf16* kr = static_cast<const bf16*>(a.k_ring) + p.n * a.ring_n + (int64_t)p.kvh * a.slots * HD;
-  const bf16* vr = static_cast<const bf16*>(a.v_ring) + p.n * a.ring_n + (int64_t)p.kvh * a.slots * HD;
-  const TileLoad<HD> load(lane);
-  auto issue = [&](const bf16* src, uint32_t dst, int tile, bool is_k) {
+  const int64_t slab = p.n * a.ring_n + (int64_t)p.kvh * a.slots * HD;
+  const TileLoad<HD, true> k_load(static_cast<const bf16*>(a.k_ring) + slab, a.slots, lane);
+  const TileLoad<HD, false> v_load(static_cast<const bf16*>(a.v_ring) + slab, a.slots, lane);
+  auto issue_k = [&](int tile) {
 #pragma unroll
-    for (int g = 0; g < LOADS; ++g) load.issue(src, a.slots, dst, tile, g, is_k);
+    for (int g = 0; g < LOADS; ++g) k_load.issue(k_lds, tile, g);
+  };
+  auto issue_v = [&](int tile) {
+#pragma unroll
+    for (int g = 0; g < LOADS; ++g) v_load.issue(v_lds, tile, g);
   };
   // the tile a wave starts with needs no position in the first split: ask for it at once (the last wave
   // starts with the new tokens there)
   const bool early = first && w < kWaves - 1;
   if (early) {
-    issue(kr, k_lds, w, true);
-    issue(vr, v_lds, w, false);
+    issue_k(w);
+    issue_v(w);
   }
   const int64_t pos = uniform(a.positions[p.n]);
   const Tree tree = read_tree(a, p.n, count, pos, lane);
@@ -600,9 +620,11 @@ __global__ void __launch_bounds__(kThreads, HD == 64 ? 2 : 1) k_swa_tree_mm(cons
   Unit<HD> u;
   u.load(a, p, tree, ring, pos, row0 + r, row1);
   __syncthreads();  // odd_values is 0
-  if (first) new_tile<HD, kThreads>(a, p, tree, count, pos, lds + (kWaves - 1) * 2 * TILE, &odd_values);
+  if (first) new_tile<HD, kThreads>(a, p, tree, count, pos, lds + (kWaves - 1) * 2 * TILE, lds + (kWaves - 1) * 2 * TILE + TILE,
+                                    &odd_values);
   const float c2 = a.scale * kLog2e;
   const int lim_any = visible_age(a, ring, 0), lim_all = visible_age(a, ring, tree.deepest);
+  const Edge edge = read_edge(a, ring, lim_all);
 
   bool loaded = early;  // this wave's next ring tile is on its way
   for (int i = w; has(i); i += kWaves) {
@@ -611,8 +633,8 @@ __global__ void __launch_bounds__(kThreads, HD == 64 ? 2 : 1) k_swa_tree_mm(cons
     const bool more = has(i + kWaves);
     if (!is_tree) {
       if (!loaded) {
-        issue(kr, k_lds, tile, true);
-        issue(vr, v_lds, tile, false);
+        issue_k(tile);
+        issue_v(tile);
       }
       wait_vmcnt<LOADS>();  // K has landed, V may still be on its way
     }
@@ -621,13 +643,9 @@ __global__ void __launch_bounds__(kThreads, HD == 64 ? 2 : 1) k_swa_tree_mm(cons
     pin_loads();
     // every K read is back: the next tile's K on its way
     const int next = more ? tile_at(i + kWaves) : 0;
-    if (more) issue(kr, k_lds, next, true);
-    uint64_t any = ~0ull, all = 0;
-    if (!is_tree) {
-      any = seen_slots(a, ring, s0, lim_any);
-      all = seen_slots(a, ring, s0, lim_all);
-    }
-    if (all != ~0ull) mask_tile(s, is_tree ? u.sees : seen_slots(a, ring, s0, u.lim));
+    if (more) issue_k(next);
+    const bool clean = !is_tree && clean_tile(a, edge, s0);
+    if (!clean) mask_tile(s, is_tree ? u.sees : seen_slots(a, ring, s0, u.lim));
     bf16x8 pw[4];
     u.softmax(s, pw, c2);
     if (!is_tree) {
@@ -636,11 +654,11 @@ __global__ void __launch_bounds__(kThreads, HD == 64 ? 2 : 1) k_swa_tree_mm(cons
       else
         wait_vmcnt<0>();
       pin_loads();
-      if (all != ~0ull && guard_values<HD>(vt, any, all)) odd_values = 1;
+      if (!clean && guard_values<HD>(vt, seen_slots(a, ring, s0, lim_any), seen_slots(a, ring, s0, lim_all))) odd_values = 1;
     }
     u.values(pw, v_lds);
     pin_loads();
-    if (more) issue(vr, v_lds, next, false);
+    if (more) issue_v(next);
     loaded = more;
   }
   if (early && !has(w)) wait_vmcnt<0>();  // an early tile that the request does not have
@@ -661,6 +679,7 @@ __global__ void __launch_bounds__(kThreads, HD == 64 ? 2 : 1) k_swa_tree_mm(cons
           f32x4{u.o[b][e], u.o[b][e + 1], u.o[b][e + 2], u.o[b][e + 3]};
   __syncthreads();
   if (odd_values != 0) {
+#pragma unroll 1
     for (int row = row0 + w; row < row1; row += kWaves) selected_row<HD>(a, p, tree, ring, pos, row, t_begin, t_end, first);
     return;
   }
@@ -696,39 +715,40 @@ __global__ void __launch_bounds__(kThreads, HD == 64 ? 2 : 1) k_swa_tree_mm(cons
   }
 }
 
-// A unit per wave, the workgroup's NW waves sharing each tile in LDS: for so many rows that reading the cache again for
-// every 32 of them would cost more than it brings.  Tiles alternate between two slots: one is loaded while the
-// other is used, a barrier per tile.
-template <int HD, int NW>
-__global__ void __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) k_swa_tree_wide(const TreeArgs a) {
-  constexpr int NB = HD / 32, TILE = kTileBytes<HD>, SLOT = 2 * TILE, LOADS = SLOT / 1024;
-  static_assert(LOADS % NW == 0, "a tile's loads divide among the waves");
-  __shared__ __align__(1024) char lds[2 * SLOT];
-  __shared__ int tree_odd;  // the new values hold infinities or NaN
+// A unit per wave, the workgroup's eight waves sharing each tile in LDS: for so many rows that reading the cache again for
+// every 32 of them would cost more than it brings.  The two waves of a SIMD work half a tile apart, a barrier
+// per half: while one multiplies (values of tile t - 1, then scores of tile t) the other forms its weights, so
+// matrix and vector units are busy at once.  K and V have three slots each: a wave asks for K of tile t + 2
+// and V of tile t + 1 ahead of its scores of tile t (every wave has left what those slots held), and the loads of the
+// tile before are home by the end of that half, one half before the first wave needs them.
+constexpr int kWideWaves = 8;
+
+__device__ __forceinline__ void half_barrier() {
+  pin_loads();
+  __builtin_amdgcn_s_barrier();
+  pin_loads();
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kWideWaves * 64, 1) k_swa_tree_wide(const TreeArgs a) {
+  constexpr int NB = HD / 32, TILE = kTileBytes<HD>, PER = TILE / 1024 / kWideWaves;  // loads of a wave
+  __shared__ __align__(1024) char lds[6 * TILE];  // three K tiles, three V slabs
+  __shared__ int tree_odd;                        // the new values hold infinities or NaN
   const Place p = place_of(a);
   if (!p.valid) return;
   const int w = uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
   const int count = a.counts != nullptr ? min(max(uniform(a.counts[p.n]), 0), a.nodes) : a.nodes;
-  const int row0 = p.group * 32 * NW, row1 = min(row0 + 32 * NW, count * a.rep);
+  const int row0 = p.group * 32 * kWideWaves, row1 = min(row0 + 32 * kWideWaves, count * a.rep);
   if (row0 >= row1) return;
-  const bool first = p.split == 0;
-  const bf16* kr = static_cast<const bf16*>(a.k_ring) + p.n * a.ring_n + (int64_t)p.kvh * a.slots * HD;
-  const bf16* vr = static_cast<const bf16*>(a.v_ring) + p.n * a.ring_n + (int64_t)p.kvh * a.slots * HD;
-  const TileLoad<HD> load(lane);
-  const uint32_t lds0 = lds_addr(lds);
-  auto issue = [&](int tile, int slot) {
-#pragma unroll
-    for (int i = 0; i < LOADS / NW; ++i) {
-      const int g = w + NW * i;  // K's loads first
-      const bool is_k = g < LOADS / 2;
-      load.issue(is_k ? kr : vr, a.slots, lds0 + (uint32_t)(slot * SLOT + (is_k ? 0 : TILE)), tile, is_k ? g : g - LOADS / 2,
-                 is_k);
-    }
-  };
+  const bool first = p.split == 0, late = w >= kWideWaves / 2;
+  const int64_t slab = p.n * a.ring_n + (int64_t)p.kvh * a.slots * HD;
+  const TileLoad<HD, true> k_load(static_cast<const bf16*>(a.k_ring) + slab, a.slots, lane);
+  const TileLoad<HD, false> v_load(static_cast<const bf16*>(a.v_ring) + slab, a.slots, lane);
+  const uint32_t k_lds = lds_addr(lds), v_lds = k_lds + 3 * TILE;
   const int64_t pos = uniform(a.positions[p.n]);
   const Tree tree = read_tree(a, p.n, count, pos, lane);
   if (tree.bad) {
-    refuse_rows<bf16, HD>(a, p, row0, row1, NW * 64);
+    refuse_rows<bf16, HD>(a, p, row0, row1, kWideWaves * 64);
     return;
   }
   if (threadIdx.x == 0) tree_odd = 0;
@@ -737,46 +757,64 @@ __global__ void __launch_bounds__(NW * 64, NW == 8 ? 1 : 2) k_swa_tree_wide(cons
   const int t_begin = (int)((int64_t)ntiles * p.split / a.nsplit), t_end = (int)((int64_t)ntiles * (p.split + 1) / a.nsplit);
   // the list: the new tokens (the first split's), then the slots' tiles
   const int lead = first ? 1 : 0, listed = lead + t_end - t_begin;
-  if (first && listed > 1) issue(t_begin, 1);
-  if (!first && listed > 0) issue(t_begin, 0);
-  const bool turned = a.cos_table != nullptr;
+  // this wave's share of place i
+  auto issue_k = [&](int i) {
+#pragma unroll
+    for (int x = 0; x < PER; ++x) k_load.issue(k_lds + (uint32_t)(i % 3 * TILE), t_begin + i - lead, w + kWideWaves * x);
+  };
+  auto issue_v = [&](int i) {
+#pragma unroll
+    for (int x = 0; x < PER; ++x) v_load.issue(v_lds + (uint32_t)(i % 3 * TILE), t_begin + i - lead, w + kWideWaves * x);
+  };
+  if (!first && listed > 0) {
+    issue_k(0);
+    issue_v(0);
+  }
+  if (listed > 1) issue_k(1);
   if (first) {
     __syncthreads();  // tree_odd is 0
-    new_tile<HD, NW * 64>(a, p, tree, count, pos, lds, &tree_odd);
+    new_tile<HD, kWideWaves * 64>(a, p, tree, count, pos, lds, lds + 3 * TILE, &tree_odd);
   }
   Unit<HD> u;
-  const bool unit_ok = row0 + 32 * w < row1;
   u.load(a, p, tree, ring, pos, row0 + 32 * w + r, row1);
   const float c2 = a.scale * kLog2e;
   const int lim_any = visible_age(a, ring, 0), lim_all = visible_age(a, ring, tree.deepest);
+  const Edge edge = read_edge(a, ring, lim_all);
+  const bool turned = a.cos_table != nullptr;
   bool odd = first && tree_odd != 0;
-  for (int i = 0; i < listed; ++i) {
-    const bool is_tree = first && i == 0;
-    const int tile = t_begin + i - lead, s0 = tile * 64, slot = i & 1;
-    if (!is_tree) {
-      wait_vmcnt<0>();
-      pin_loads();
-      __builtin_amdgcn_s_barrier();  // the tile is in LDS; every wave is done with the other slot
-      pin_loads();
-      if (i + 1 < listed) issue(tile + 1, slot ^ 1);
-    }
-    if (!unit_ok) continue;
+  wait_vmcnt<0>();
+  half_barrier();
+  if (late) half_barrier();
+  for (int t = 0; t < listed; ++t) {
+    if (t + 2 < listed) issue_k(t + 2);
+    if (t + 1 < listed) issue_v(t + 1);
     f32x16 s[2];
-    u.scores(s, lds0 + (uint32_t)(slot * SLOT), turned);
-    uint64_t any = ~0ull, all = 0;
-    if (!is_tree) {
-      any = seen_slots(a, ring, s0, lim_any);
-      all = seen_slots(a, ring, s0, lim_all);
-    }
-    if (all != ~0ull) mask_tile(s, is_tree ? u.sees : seen_slots(a, ring, s0, u.lim));
+    u.scores(s, k_lds + (uint32_t)(t % 3 * TILE), turned);
+    asm volatile("" : "+v"(s[0]), "+v"(s[1]));  // and these in theirs
+    // K of place t + 1 and V of place t have landed
+    if (t + 2 < listed)
+      wait_vmcnt<2 * PER>();
+    else if (t + 1 < listed)
+      wait_vmcnt<PER>();
+    else
+      wait_vmcnt<0>();
+    half_barrier();
+    const int s0 = (t_begin + t - lead) * 64;
+    const bool clean = t >= lead && clean_tile(a, edge, s0);
+    if (!clean) mask_tile(s, t < lead ? u.sees : seen_slots(a, ring, s0, u.lim));
     bf16x8 pw[4];
     u.softmax(s, pw, c2);
-    if (!is_tree && all != ~0ull)  // every wave writes the same zeros
-      odd |= guard_values<HD>(lds + slot * SLOT + TILE, any, all);
-    u.values(pw, lds0 + (uint32_t)(slot * SLOT + TILE));
+    // formed in this half: the barrier alone would not keep the arithmetic from sinking below it
+    asm volatile("" : "+v"(pw[0]), "+v"(pw[1]), "+v"(pw[2]), "+v"(pw[3]));
+    half_barrier();
+    if (t >= lead && !clean)  // every wave writes the same zeros
+      odd |= guard_values<HD>(lds + (3 + t % 3) * TILE, seen_slots(a, ring, s0, lim_any), seen_slots(a, ring, s0, lim_all));
+    u.values(pw, v_lds + (uint32_t)(t % 3 * TILE));
   }
+  if (!late) half_barrier();
   if (odd) {
     const int last = min(row0 + 32 * (w + 1), row1);
+#pragma unroll 1
     for (int row = row0 + 32 * w; row < last; ++row) selected_row<HD>(a, p, tree, ring, pos, row, t_begin, t_end, first);
     return;
   }
@@ -1062,8 +1100,8 @@ __global__ void __launch_bounds__(kThreads) k_swa_tree_f32(const TreeArgs a) {
   }
 }
 
-// Workgroups' shape: units of 32 rows that share a workgroup's tiles (1: k_swa_tree_mm, 4 or 8: k_swa_tree_wide; 0: 16
-// fp32 rows), workgroups along a (request, kv head)'s rows, splits of its slots.
+// Workgroups' shape: units of 32 rows that share a workgroup's tiles (1: k_swa_tree_mm, 8: k_swa_tree_wide; 0: 16 fp32
+// rows), workgroups along a (request, kv head)'s rows, splits of its slots.
 struct TreePlan {
   int units, groups, nsplit;
 };
@@ -1075,7 +1113,7 @@ TreePlan plan_tree(int64_t n_req, int64_t n_heads, int64_t n_kv_heads, int64_t n
   TreePlan p;
   const int64_t rows = n_heads / n_kv_heads * nodes, lists = n_req * n_kv_heads, tiles = (slots + 63) / 64;
   p.units = b16 ? 1 : 0;
-  if (b16 && rows > 64 && lists * ((rows + 31) / 32) >= 256) p.units = rows > 128 ? 8 : 4;
+  if (b16 && rows > 128 && lists * ((rows + 31) / 32) >= 256) p.units = kWideWaves;
   const int64_t per = b16 ? 32 * p.units : 16;
   p.groups = (int)((rows + per - 1) / per);
   const int64_t base = lists * p.groups;
@@ -1092,10 +1130,8 @@ void launch_tree(const TreeArgs& m, const TreePlan& p, bool b16, hipStream_t st)
     hipLaunchKernelGGL(k_swa_tree_f32<HD>, grid, dim3(kThreads), 0, st, m);
   else if (p.units == 1)
     hipLaunchKernelGGL(k_swa_tree_mm<HD>, grid, dim3(kThreads), 0, st, m);
-  else if (p.units == 4)
-    hipLaunchKernelGGL((k_swa_tree_wide<HD, 4>), grid, dim3(256), 0, st, m);
   else
-    hipLaunchKernelGGL((k_swa_tree_wide<HD, 8>), grid, dim3(512), 0, st, m);
+    hipLaunchKernelGGL(k_swa_tree_wide<HD>, grid, dim3(kWideWaves * 64), 0, st, m);
   if (m.nsplit > 1) {
     const int64_t n = (int64_t)m.n_req * m.n_kv_heads * m.rows * (HD / 4);
     const dim3 jg((unsigned)((n + kThreads - 1) / kThreads));
@@ -1126,8 +1162,9 @@ extern "C" int uttt_swa_tree(const uttt_swa_tree_args* a, uttt_stream_t stream) 
                    a->n_heads >= 1 && a->n_heads <= 65535 && a->n_heads % a->n_kv_heads == 0,
                "bad request / head counts");
   UTTT_REQUIRE(a->nodes >= 1 && a->nodes <= kMaxNodes, "nodes must be in [1, %d]", kMaxNodes);
-  UTTT_REQUIRE(a->window >= 1 && a->window <= (1LL << 28) && a->sinks >= 0 && a->sinks <= (1LL << 28),
-               "window or sinks out of range");
+  UTTT_REQUIRE(a->window >= 1 && a->window <= (1LL << 28) && a->sinks >= 0 && a->sinks <= (1LL << 28) &&
+                   (a->window + a->sinks) * a->head_dim * 4 < (1LL << 31),
+               "window or sinks out of range (a request's keys of one head must stay below 2 GB)");
   UTTT_REQUIRE(a->act_dtype == UTTT_DTYPE_F32 || a->act_dtype == UTTT_DTYPE_BF16, "bad act_dtype");
   UTTT_REQUIRE(a->scale > 0.f, "scale must be > 0");
   UTTT_REQUIRE(a->positions && a->q && a->k_new && a->v_new && a->k_ring && a->v_ring && a->out,
