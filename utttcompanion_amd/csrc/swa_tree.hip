@@ -542,7 +542,7 @@ __device__ __forceinline__ bool guard_values(char* vt, uint64_t any, uint64_t al
   const int lane = threadIdx.x & 63;
   const uint64_t none = ~any, part = any & ~all;
   bool bad = false;
-#pragma unroll 1
+#pragma unroll 4
   for (int i = 0; i < HD / 8; ++i) {  // 8 rows at a time, a 16-byte piece per lane
     const int t = 8 * (i & 7) + (lane >> 3);
     uint4* piece = reinterpret_cast<uint4*>(vt + (i >> 3) * 8192 + t * 128 + (lane & 7) * 16);
@@ -717,10 +717,11 @@ __global__ void __launch_bounds__(kThreads, HD == 64 ? 2 : 1) k_swa_tree_mm(cons
 
 // A unit per wave, the workgroup's eight waves sharing each tile in LDS: for so many rows that reading the cache again for
 // every 32 of them would cost more than it brings.  The two waves of a SIMD work half a tile apart, a barrier
-// per half: while one multiplies (values of tile t - 1, then scores of tile t) the other forms its weights, so
-// matrix and vector units are busy at once.  K and V have three slots each: a wave asks for K of tile t + 2
-// and V of tile t + 1 ahead of its scores of tile t (every wave has left what those slots held), and the loads of the
-// tile before are home by the end of that half, one half before the first wave needs them.
+// per half: while one forms scores the other is at its weights and values, so matrix and vector units are busy
+// at once.  (Weights alone against both products, the other cut, leaves the weights' half waiting: 3200 cycles
+// a half at head_dim 128.)  K has three slots and V four: a wave asks for tile t + 2 ahead of its scores of tile t
+// (every wave has left what those slots held), and the tile it asked for before is home by the end of that half,
+// one half before the first wave needs it.
 constexpr int kWideWaves = 8;
 
 __device__ __forceinline__ void half_barrier() {
@@ -732,7 +733,7 @@ __device__ __forceinline__ void half_barrier() {
 template <int HD>
 __global__ void __launch_bounds__(kWideWaves * 64, 1) k_swa_tree_wide(const TreeArgs a) {
   constexpr int NB = HD / 32, TILE = kTileBytes<HD>, PER = TILE / 1024 / kWideWaves;  // loads of a wave
-  __shared__ __align__(1024) char lds[6 * TILE];  // three K tiles, three V slabs
+  __shared__ __align__(1024) char lds[7 * TILE];  // three K tiles, four V slabs
   __shared__ int tree_odd;                        // the new values hold infinities or NaN
   const Place p = place_of(a);
   if (!p.valid) return;
@@ -764,13 +765,16 @@ __global__ void __launch_bounds__(kWideWaves * 64, 1) k_swa_tree_wide(const Tree
   };
   auto issue_v = [&](int i) {
 #pragma unroll
-    for (int x = 0; x < PER; ++x) v_load.issue(v_lds + (uint32_t)(i % 3 * TILE), t_begin + i - lead, w + kWideWaves * x);
+    for (int x = 0; x < PER; ++x) v_load.issue(v_lds + (uint32_t)(i % 4 * TILE), t_begin + i - lead, w + kWideWaves * x);
   };
   if (!first && listed > 0) {
     issue_k(0);
     issue_v(0);
   }
-  if (listed > 1) issue_k(1);
+  if (listed > 1) {
+    issue_k(1);
+    issue_v(1);
+  }
   if (first) {
     __syncthreads();  // tree_odd is 0
     new_tile<HD, kWideWaves * 64>(a, p, tree, count, pos, lds, lds + 3 * TILE, &tree_odd);
@@ -786,16 +790,16 @@ __global__ void __launch_bounds__(kWideWaves * 64, 1) k_swa_tree_wide(const Tree
   half_barrier();
   if (late) half_barrier();
   for (int t = 0; t < listed; ++t) {
-    if (t + 2 < listed) issue_k(t + 2);
-    if (t + 1 < listed) issue_v(t + 1);
+    if (t + 2 < listed) {
+      issue_k(t + 2);
+      issue_v(t + 2);
+    }
     f32x16 s[2];
     u.scores(s, k_lds + (uint32_t)(t % 3 * TILE), turned);
-    asm volatile("" : "+v"(s[0]), "+v"(s[1]));  // and these in theirs
-    // K of place t + 1 and V of place t have landed
-    if (t + 2 < listed)
+    // formed in this half: the barrier alone would not keep the arithmetic from sinking below it
+    asm volatile("" : "+v"(s[0]), "+v"(s[1]));
+    if (t + 2 < listed)  // place t + 1 has landed
       wait_vmcnt<2 * PER>();
-    else if (t + 1 < listed)
-      wait_vmcnt<PER>();
     else
       wait_vmcnt<0>();
     half_barrier();
@@ -804,12 +808,10 @@ __global__ void __launch_bounds__(kWideWaves * 64, 1) k_swa_tree_wide(const Tree
     if (!clean) mask_tile(s, t < lead ? u.sees : seen_slots(a, ring, s0, u.lim));
     bf16x8 pw[4];
     u.softmax(s, pw, c2);
-    // formed in this half: the barrier alone would not keep the arithmetic from sinking below it
-    asm volatile("" : "+v"(pw[0]), "+v"(pw[1]), "+v"(pw[2]), "+v"(pw[3]));
-    half_barrier();
     if (t >= lead && !clean)  // every wave writes the same zeros
-      odd |= guard_values<HD>(lds + (3 + t % 3) * TILE, seen_slots(a, ring, s0, lim_any), seen_slots(a, ring, s0, lim_all));
-    u.values(pw, v_lds + (uint32_t)(t % 3 * TILE));
+      odd |= guard_values<HD>(lds + (3 + t % 4) * TILE, seen_slots(a, ring, s0, lim_any), seen_slots(a, ring, s0, lim_all));
+    u.values(pw, v_lds + (uint32_t)(t % 4 * TILE));
+    half_barrier();
   }
   if (!late) half_barrier();
   if (odd) {
