@@ -125,6 +125,24 @@ def test_many_neighbouring_values_in_one_bin():
     check(x * 1e-30, u, t, k=[7000, 1, 3, 19999], p=[0.1, 0.5, 0.77, 0.999], sure=True)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [5000, 60000])
+def test_few_and_many_ids_are_kept(vocab, dtype):
+    """Cuts that keep few ids of the row, some thousands, and nearly all of it: flat and peaked rows, and rows whose
+    kept ids stand in one place."""
+    g = torch.Generator().manual_seed(vocab)
+    rows = [s * torch.randn(vocab, generator=g) for s in (0.3, 1.0, 2.0, 4.0)]
+    lump = torch.randn(vocab, generator=g) - 20
+    lump[700:1900] += 20  # 1200 neighbours hold the mass
+    x = torch.stack([*rows, lump, lump.flip(0)]).to(dtype).to(DEV)
+    n = x.shape[0]
+    for seed, (k, p) in enumerate([([0] * n, [0.02, 0.3, 0.9, 0.99, 0.9, 0.97]), ([3, 700, 2500, 4900, 1100, 1300], [1.0] * n),
+                                   ([4000] * n, [0.9] * n), ([0] * n, [0.9999] * n)]):
+        u = uniforms(n, 100 + seed)
+        check(x, u, [0.9] * n, k, p)
+        check(x, u, [1.0] * n, k, p, [0.001] * n)
+
+
 @pytest.mark.parametrize("temperature", [2e-5, 1e-3, 50.0, 1e4, math.inf])
 def test_extreme_temperatures(temperature):
     g = torch.Generator().manual_seed(11)

@@ -7,10 +7,13 @@
 //   1. the largest logit (rows that fit are kept in LDS for the passes behind);
 //   2. a histogram of counts and masses over x, of the ids within 16 factors of two of the top (bins of 1/128
 //      of one; when the cut lies further down, a second one of 1/48 over everything), and the whole mass;
-//   3. the mass of 16 stretches of the row (one per wave) ahead of the bin in which the count or the mass
-//      passes its bound, and that bin's ids, which are few: they are ranked against each other.  When there are
-//      many (equal or nearly equal logits), the bin's range of keys is divided further first;
-//   4. the same masses of 16 parts of the stretch that holds the chosen id, and a scan inside one wave.
+//   3. the ids up to the bin in which the count or the mass passes its bound, listed per stretch (16 of the row, one
+//      per wave) and weighed there: the stretches' masses, and that bin's ids, which are ranked against
+//      each other.  When there are many (equal or nearly equal logits), the bin's range of keys is divided
+//      further first;
+//   4. a scan of the list of the stretch that holds the chosen id, inside one wave.
+// Without a cut 3 is a pass that weighs the whole row; without a list of the stretch (no cut, or many ids kept) 4 weighs
+// 16 parts of it first.
 //
 // The sums decide between neighbouring ids, so weights are formed in 64 bits and added as integers in units of
 // 2^-42 of the largest weight: exact whatever the order, so atomics in any order give equal bits.  (fp64 and
@@ -47,6 +50,7 @@ constexpr int kSmpThreads = 1024, kSmpWaves = kSmpThreads / 64;
 constexpr int kBins = 2 * kSmpThreads;  // two per thread in the scan
 constexpr int kList = 256;
 constexpr int kStageBytes = 96 * 1024;  // rows up to this size stay in LDS
+constexpr int kKeptStaged = 256, kKept = 512;
 
 // order-preserving key of a logit that is not NaN; -0 and +0 are equal
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -116,11 +120,22 @@ struct Cut {
   u64 mass;  // of what it keeps
 };
 
+// kept: ids of one wave's stretch that are listed
+template <int KEPT>
 struct Shared {
   u64 mass[kBins];
   uint32_t count[kBins];
-  u64 mass2[kBins];  // of a range of keys inside one bin
-  uint32_t count2[kBins];
+  union {
+    struct {  // of a range of keys inside one bin
+      u64 mass2[kBins];
+      uint32_t count2[kBins];
+    };
+    struct {  // the ids of a wave's stretch that may be kept, in their order
+      float kept_logit[kSmpWaves][KEPT];
+      int kept_id[kSmpWaves][KEPT];
+    };
+  };
+  int kept_n[kSmpWaves];  // -1: the list holds only the last of them
   u64 wave_mass[kSmpWaves], scan_mass[kSmpWaves];
   uint32_t wave_count[kSmpWaves], scan_count[kSmpWaves];
   float wave_best[kSmpWaves];
@@ -180,7 +195,8 @@ __device__ __forceinline__ void scan_ids(const SampleArgs& a, const T* x, int lo
 // STAGED: the row stays in LDS behind the first pass, without the ids that are left out.
 template <typename T, int VEC, bool STAGED>
 __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs a) {
-  __shared__ Shared s;
+  constexpr int KEPT = STAGED ? kKeptStaged : kKept;
+  __shared__ Shared<KEPT> s;
   __shared__ __align__(16) T stage[STAGED ? kStageBytes / sizeof(T) : 1];
   constexpr int W = STAGED || VEC > 4 ? 4 : VEC;  // ids to a lane in the passes behind the first
   constexpr float kFine = 128.f, kCoarse = 48.f;  // bins to a factor of two: kBins / 48 > 42, what weights reach
@@ -332,68 +348,117 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
       __syncthreads();
       return bin;
     };
-    // the ids of one bin with keys in [kmin, kmax]: how many, the first kList, the range of their keys; and per
-    // stretch the mass of the bins ahead
-    auto gather = [&](int bin, uint32_t kmin, uint32_t kmax, bool ahead) __attribute__((always_inline)) {
+    auto add_to_list = [&](uint32_t k, int id, u64 u) __attribute__((always_inline)) {
+      const uint32_t at = atomicAdd(&s.n, 1u);
+      if (at < kList) {
+        s.list_key[at] = k;
+        s.list_id[at] = id;
+        s.list_mass[at] = u;
+      }
+    };
+    auto start_list = [&]() __attribute__((always_inline)) {
       if (tid == 0) {
         s.n = 0;
         s.kmin = 0xffffffffu;
         s.kmax = 0;
       }
       __syncthreads();
-      uint32_t mn = 0xffffffffu, mx = 0;
-      u64 sum = 0;
-      scan(lo, hi, [&](const float(&v)[W], int i) __attribute__((always_inline)) {
-        float d[W], nearest = INFINITY;
-#pragma unroll
-        for (int e = 0; e < W; ++e) {
-          d[e] = place(v[e]);
-          nearest = fminf(nearest, d[e]);
-        }
-        if (!(nearest < (float)(bin + 1))) return;
-        bool here = false;
-        u64 u[W];
-#pragma unroll
-        for (int e = 0; e < W; ++e) u[e] = weight(v[e]);
-#pragma unroll
-        for (int e = 0; e < W; ++e) {
-          sum += d[e] < (float)bin ? u[e] : 0;
-          here |= d[e] >= (float)bin && d[e] < (float)(bin + 1);
-        }
-        if (!here) return;
-#pragma unroll
-        for (int e = 0; e < W; ++e) {
-          if (!(d[e] >= (float)bin && d[e] < (float)(bin + 1))) continue;
-          const uint32_t k = key_of(v[e]);
-          if (k < kmin || k > kmax) continue;
-          mn = min(mn, k);
-          mx = max(mx, k);
-          const uint32_t at = atomicAdd(&s.n, 1u);
-          if (at < kList) {
-            s.list_key[at] = k;
-            s.list_id[at] = i + e;
-            s.list_mass[at] = u[e];
-          }
-        }
-      });
+    };
+    auto end_list = [&](uint32_t mn, uint32_t mx) __attribute__((always_inline)) {
       if (mn <= mx) {
         atomicMin(&s.kmin, mn);
         atomicMax(&s.kmax, mx);
       }
-      if (ahead) {
-        sum = wave_scan(sum);
-        if (lane == 63) {
-          s.wave_mass[w] = sum;
-          s.wave_count[w] = 0;
-        }
-      }
       __syncthreads();
+    };
+    // the ids of one bin with keys in [kmin, kmax]: how many, the first kList, the range of their keys
+    auto gather = [&](int bin, uint32_t kmin, uint32_t kmax) __attribute__((always_inline)) {
+      start_list();
+      uint32_t mn = 0xffffffffu, mx = 0;
+      scan(lo, hi, [&](const float(&v)[W], int i) __attribute__((always_inline)) {
+#pragma unroll 1
+        for (int e = 0; e < W; ++e) {
+          const float ve = e == 0 ? v[0] : e == 1 ? v[1 % W] : e == 2 ? v[2 % W] : v[3 % W];
+          const float d = place(ve);
+          if (!(d >= (float)bin && d < (float)(bin + 1))) continue;
+          const uint32_t k = key_of(ve);
+          if (k < kmin || k > kmax) continue;
+          mn = min(mn, k);
+          mx = max(mx, k);
+          add_to_list(k, i + e, weight(ve));
+        }
+      });
+      end_list(mn, mx);
+    };
+    // the same for a whole bin, and per stretch the mass of the bins ahead: each wave lists its ids up to that bin and
+    // weighs the list when it is full, so weights are formed with all lanes busy
+    auto collect = [&](int bin) __attribute__((always_inline)) {
+      start_list();
+      uint32_t mn = 0xffffffffu, mx = 0;
+      u64 sum = 0;
+      int n = 0;
+      bool whole_list = true;
+      auto weigh = [&]() __attribute__((always_inline)) {
+#pragma unroll 1
+        for (int b = 0; b < n; b += 64) {
+          if (b + lane < n) {
+            const float v = s.kept_logit[w][b + lane];
+            const u64 u = weight(v);
+            if (place(v) < (float)bin) {
+              sum += u;
+            } else {
+              const uint32_t k = key_of(v);
+              mn = min(mn, k);
+              mx = max(mx, k);
+              add_to_list(k, s.kept_id[w][b + lane], u);
+            }
+          }
+        }
+      };
+      scan(lo, hi, [&](const float(&v)[W], int i) __attribute__((always_inline)) {
+        bool in[W];
+        uint32_t mine = 0;
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          in[e] = place(v[e]) < (float)(bin + 1);
+          mine += in[e];
+        }
+        if (!__any(mine != 0)) return;
+        const uint32_t upto = wave_scan(mine);
+        const int more = (int)of_lane(upto, 63);
+        if (n + more > KEPT) {
+          weigh();
+          n = 0;
+          whole_list = false;
+        }
+        int at = n + (int)(upto - mine);
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          if (in[e]) {
+            s.kept_logit[w][at] = v[e];
+            s.kept_id[w][at] = i + e;
+          }
+          at += in[e];
+        }
+        n += more;
+      });
+      weigh();
+      sum = wave_scan(sum);
+      if (lane == 63) {
+        s.wave_mass[w] = sum;
+        s.wave_count[w] = 0;
+        s.kept_n[w] = whole_list ? n : -1;
+      }
+      end_list(mn, mx);
     };
     // the cut inside a bin that find() named
     auto resolve = [&](int bin, bool counts, u64 bound, bool ahead) __attribute__((always_inline)) -> Cut {
       u64 mass0 = s.before_mass;
       uint32_t count0 = s.before_count;
-      gather(bin, 0, 0xffffffffu, ahead);
+      if (ahead)
+        collect(bin);
+      else
+        gather(bin, 0, 0xffffffffu);
       masses = ahead && s.n <= kList;
       uint32_t kmin = s.kmin, kmax = s.kmax;
       while (s.n > kList && kmin != kmax) {
@@ -423,7 +488,7 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
         count0 = s.before_count;
         const uint32_t hi_key = kmax - ((uint32_t)part << shift), width = (1u << shift) - 1;
         const uint32_t lo_key = hi_key - kmin > width ? hi_key - width : kmin;
-        gather(bin, lo_key, hi_key, false);
+        gather(bin, lo_key, hi_key);
         kmin = s.kmin;
         kmax = s.kmax;
       }
@@ -574,22 +639,29 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
     }
     return found;
   };
-  const int p0 = min(pick(true) * stretch, a.limit), p1 = min(p0 + stretch, a.limit);
-  const int part = ((p1 - p0 + kSmpWaves - 1) / kSmpWaves + kStep - 1) / kStep * kStep;
-  {
+  const int q = pick(true);
+  int q0 = 0, q1 = masses ? s.kept_n[q] : -1;
+  const bool listed = q1 >= 0;
+  if (!listed) {
+    const int p0 = min(q * stretch, a.limit), p1 = min(p0 + stretch, a.limit);
+    const int part = ((p1 - p0 + kSmpWaves - 1) / kSmpWaves + kStep - 1) / kStep * kStep;
     const int q_lo = min(p0 + w * part, p1);
     part_mass(q_lo, min(q_lo + part, p1));
+    q0 = min(p0 + pick(false) * part, p1);
+    q1 = min(q0 + part, p1);
   }
-  const int q0 = min(p0 + pick(false) * part, p1), q1 = min(q0 + part, p1);
   if (w != 0) return;
-  // ---- inside one wave: 64 ids at a time
+  // ---- inside one wave: 64 ids at a time, of the stretch's list or of a part of the row
   u64 m = ahead, t = ties_ahead;
   int token = -1;
+#pragma unroll 1
   for (int b = q0; b < q1 && token < 0; b += 64) {
     const int i = b + lane;
     float v[1] = {-INFINITY};
     if (i < q1) {
-      if constexpr (STAGED) {
+      if (listed) {
+        v[0] = s.kept_logit[q][i];
+      } else if constexpr (STAGED) {
         v[0] = to_f32(stage[i]);
       } else {
         v[0] = to_f32(x[i]);
@@ -602,12 +674,15 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
     if (tie) u = t + __popcll(tied & ((1ull << lane) - 1)) < max_ties ? tie_mass : 0;
     const u64 sum = wave_scan(u);
     const u64 over = __ballot(m + sum > want);
-    if (over != 0) token = b + __builtin_ctzll(over);
+    if (over != 0) {
+      token = b + __builtin_ctzll(over);
+      if (listed) token = s.kept_id[q][token];
+    }
     m += of_lane(sum, 63);
     t += __popcll(tied);
   }
   if (lane == 0) {
-    token = token < 0 ? q0 : token;  // integers add up the same way at every level, so one is found
+    token = token < 0 ? 0 : token;  // integers add up the same way at every level, so one is found
     a.out[row] = token;
     // log(w / total): the weight's own exponent, not its rounded units
     if (a.logprob != nullptr)
