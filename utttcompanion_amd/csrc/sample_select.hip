@@ -5,12 +5,12 @@
 // descending, id ascending), so the kept set is a cut (key, ties): the ids whose logit lies above the key's,
 // and the first `ties` of those at it.  Passes over the row, one workgroup each:
 //   1. the largest logit (rows that fit are kept in LDS for the passes behind);
-//   2. a histogram of counts and masses over x, of the ids within 16 factors of two of the top (bins of 1/128
-//      of one; when the cut lies further down, a second one of 1/48 over everything), and the whole mass;
-//   3. the ids up to the bin in which the count or the mass passes its bound, listed per stretch (16 of the row, one
-//      per wave) and weighed there: the stretches' masses, and that bin's ids, which are ranked against
-//      each other.  When there are many (equal or nearly equal logits), the bin's range of keys is divided
-//      further first;
+//   2. the ids within 16 factors of two of the top, listed per stretch of the row (16, one per wave) so that their weights
+//      are formed with all lanes busy; their histogram of counts and masses over x (bins of 1/128 of a factor
+//      of two), and the whole mass.  When the cut lies further down, again over everything, with bins of 1/48;
+//   3. the bin in which the count or the mass passes its bound: the stretches' masses ahead of it from the lists (where one
+//      overflowed, from the row), and its ids, which are ranked against each other.  When they are many (equal or
+//      nearly equal logits), the bin's range of keys is divided further first;
 //   4. a scan of the list of the stretch that holds the chosen id, inside one wave.
 // Without a cut 3 is a pass that weighs the whole row; without a list of the stretch (no cut, or many ids kept) 4 weighs
 // 16 parts of it first.
@@ -48,8 +48,9 @@ struct SampleArgs {
 
 constexpr int kSmpThreads = 1024, kSmpWaves = kSmpThreads / 64;
 constexpr int kBins = 2 * kSmpThreads;  // two per thread in the scan
-constexpr int kList = 256;
-constexpr int kStageBytes = 96 * 1024;  // rows up to this size stay in LDS
+constexpr int kList = kSmpThreads;  // ids that are ranked against each other, one per thread
+constexpr int kDense = 24;  // ids of each 64: from so many on they are weighed in place
+constexpr int kStageBytes = 60 * 1024;  // rows up to this size stay in LDS
 constexpr int kKeptStaged = 256, kKept = 512;
 
 // order-preserving key of a logit that is not NaN; -0 and +0 are equal
@@ -125,16 +126,10 @@ template <int KEPT>
 struct Shared {
   u64 mass[kBins];
   uint32_t count[kBins];
-  union {
-    struct {  // of a range of keys inside one bin
-      u64 mass2[kBins];
-      uint32_t count2[kBins];
-    };
-    struct {  // the ids of a wave's stretch that may be kept, in their order
-      float kept_logit[kSmpWaves][KEPT];
-      int kept_id[kSmpWaves][KEPT];
-    };
-  };
+  u64 mass2[kBins];  // of a range of keys inside one bin
+  uint32_t count2[kBins];
+  float kept_logit[kSmpWaves][KEPT];  // the ids of a wave's stretch that have a bin, in their order
+  int kept_id[kSmpWaves][KEPT];
   int kept_n[kSmpWaves];  // -1: the list holds only the last of them
   u64 wave_mass[kSmpWaves], scan_mass[kSmpWaves];
   uint32_t wave_count[kSmpWaves], scan_count[kSmpWaves];
@@ -198,7 +193,7 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
   constexpr int KEPT = STAGED ? kKeptStaged : kKept;
   __shared__ Shared<KEPT> s;
   __shared__ __align__(16) T stage[STAGED ? kStageBytes / sizeof(T) : 1];
-  constexpr int W = STAGED || VEC > 4 ? 4 : VEC;  // ids to a lane in the passes behind the first
+  constexpr int W = STAGED ? 8 / (int)sizeof(T) : VEC > 4 ? 4 : VEC;  // ids to a lane in the passes behind the first
   constexpr float kFine = 128.f, kCoarse = 48.f;  // bins to a factor of two: kBins / 48 > 42, what weights reach
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const T* x = static_cast<const T*>(a.logits) + (int64_t)row * a.rs;
@@ -213,7 +208,7 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
     if constexpr (STAGED)
       scan_ids<T, W, 1, false>(a, stage, from, to, lane, f);
     else
-      scan_ids<T, W, 4, true>(a, x, from, to, lane, f);
+      scan_ids<T, W, 2, true>(a, x, from, to, lane, f);
   };
 
   // ---- the largest logit; NaN makes it NaN
@@ -283,33 +278,116 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
 
   Cut cut{0, 0x7fffffff, 0};  // keeps everything
   bool masses = false;        // the stretches' masses up to the cut are known
+  int kept = 0;               // ids in this wave's list
+  bool complete = false;      // it holds all it should
   u64 whole = 0;              // the row's mass; at the end the kept ids'
   if (by_count || by_mass) {
-    auto histogram = [&]() __attribute__((always_inline)) {
-      u64 sum = 0;
-      scan(lo, hi, [&](const float(&v)[W], int) __attribute__((always_inline)) {
-        u64 u[W] = {};
-        if (by_mass) {
-#pragma unroll
-          for (int e = 0; e < W; ++e) u[e] = weight(v[e]);
-#pragma unroll
-          for (int e = 0; e < W; ++e) sum += u[e];
+    // f(logits, first id, weights, which of them) for the ids of this wave's list, a lane each
+    auto each_listed = [&](auto&& f) __attribute__((always_inline)) {
+#pragma unroll 1
+      for (int b = 0; b < kept; b += 64)
+        if (b + lane < kept) {
+          const float v[1] = {s.kept_logit[w][b + lane]};
+          const u64 u[1] = {weight(v[0])};
+          const bool in[1] = {true};
+          f(v, s.kept_id[w][b + lane], u, in);
         }
-        float d[W], nearest = INFINITY;
+    };
+    // append the ids of a step that `in` marks to this wave's list, which f takes when they do not fit, and at the end; f
+    // takes a step with many marked ids at once
+    auto append = [&](const float(&v)[W], int i, const bool(&in)[W], auto&& f) __attribute__((always_inline)) {
+      uint32_t mine = 0;
+      int more = 0;
 #pragma unroll
+      for (int e = 0; e < W; ++e) {
+        mine += in[e];
+        more += __popcll(__ballot(in[e]));
+      }
+      if (more == 0) return;
+      if (more >= kDense * W) {
+        u64 u[W];
+#pragma unroll
+        for (int e = 0; e < W; ++e) u[e] = weight(v[e]);
+        f(v, i, u, in);
+        complete = false;
+        return;
+      }
+      const uint32_t upto = wave_scan(mine);
+      if (kept + more > KEPT) {
+        each_listed(f);
+        kept = 0;
+        complete = false;
+      }
+      int at = kept + (int)(upto - mine);
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        if (in[e]) {
+          s.kept_logit[w][at] = v[e];
+          s.kept_id[w][at] = i + e;
+        }
+        at += in[e];
+      }
+      kept += more;
+    };
+    // the same for all ids that have a bin: from the list when it is complete, else from the row
+    auto each_binned = [&](auto&& f) __attribute__((always_inline)) {
+      if (complete) {
+        each_listed(f);
+        return;
+      }
+      scan(lo, hi, [&](const float(&v)[W], int i) __attribute__((always_inline)) {
+#pragma unroll 1
         for (int e = 0; e < W; ++e) {
-          d[e] = place(v[e]);
-          nearest = fminf(nearest, d[e]);
-        }
-        if (nearest < (float)kBins) {
-#pragma unroll
-          for (int e = 0; e < W; ++e)
-            if (d[e] < (float)kBins) {
-              if (by_mass) atomicAdd(&s.mass[(int)d[e]], u[e]);
-              if (by_count) atomicAdd(&s.count[(int)d[e]], 1u);
-            }
+          const float ve = e == 0 ? v[0] : e == 1 ? v[1 % W] : e == 2 ? v[2 % W] : v[3 % W];
+          if (!(place(ve) < (float)kBins)) continue;
+          const float v1[1] = {ve};
+          const u64 u1[1] = {weight(ve)};
+          const bool in1[1] = {true};
+          f(v1, i + e, u1, in1);
         }
       });
+    };
+    // counts and masses of the bins, and the whole mass.  Ids further down add to the whole mass alone, by fp32
+    // exponentials: their errors (2^-23 of each, and random) are far below what a kept id weighs.
+    auto histogram = [&]() __attribute__((always_inline)) {
+      u64 sum = 0;
+      float tail = 0.f;
+      const float cf = (float)c;
+      kept = 0;
+      complete = true;
+      auto count = [&](const auto& v, int, const auto& u, const auto& in) __attribute__((always_inline)) {
+        constexpr int M = sizeof(v) / sizeof(float);
+        if (by_mass) {
+#pragma unroll
+          for (int e = 0; e < M; ++e) {
+            sum += in[e] ? u[e] : 0;
+            if (in[e]) atomicAdd(&s.mass[(int)place(v[e])], u[e]);
+          }
+        }
+        if (by_count) {
+#pragma unroll
+          for (int e = 0; e < M; ++e)
+            if (in[e]) atomicAdd(&s.count[(int)place(v[e])], 1u);
+        }
+      };
+      scan(lo, hi, [&](const float(&v)[W], int i) __attribute__((always_inline)) {
+        bool in[W], all = true;
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          in[e] = place(v[e]) < (float)kBins;
+          all &= in[e];
+        }
+        if (by_mass && !all) {
+#pragma unroll
+          for (int e = 0; e < W; ++e) {
+            const float x = __builtin_amdgcn_exp2f((v[e] - top) * cf);
+            tail += in[e] || !(x >= min_p) ? 0.f : x;
+          }
+        }
+        append(v, i, in, count);
+      });
+      each_listed(count);
+      sum += (u64)((double)tail * 4398046511104.0);
       sum = wave_scan(sum);
       if (lane == 63) s.wave_mass[w] = sum;
       __syncthreads();
@@ -375,79 +453,58 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
     auto gather = [&](int bin, uint32_t kmin, uint32_t kmax) __attribute__((always_inline)) {
       start_list();
       uint32_t mn = 0xffffffffu, mx = 0;
-      scan(lo, hi, [&](const float(&v)[W], int i) __attribute__((always_inline)) {
-#pragma unroll 1
-        for (int e = 0; e < W; ++e) {
-          const float ve = e == 0 ? v[0] : e == 1 ? v[1 % W] : e == 2 ? v[2 % W] : v[3 % W];
-          const float d = place(ve);
-          if (!(d >= (float)bin && d < (float)(bin + 1))) continue;
-          const uint32_t k = key_of(ve);
-          if (k < kmin || k > kmax) continue;
-          mn = min(mn, k);
-          mx = max(mx, k);
-          add_to_list(k, i + e, weight(ve));
-        }
+      each_binned([&](const float(&v)[1], int i, const u64(&u)[1], const bool(&)[1]) __attribute__((always_inline)) {
+        const float d = place(v[0]);
+        if (!(d >= (float)bin && d < (float)(bin + 1))) return;
+        const uint32_t k = key_of(v[0]);
+        if (k < kmin || k > kmax) return;
+        mn = min(mn, k);
+        mx = max(mx, k);
+        add_to_list(k, i, u[0]);
       });
       end_list(mn, mx);
     };
-    // the same for a whole bin, and per stretch the mass of the bins ahead: each wave lists its ids up to that bin and
-    // weighs the list when it is full, so weights are formed with all lanes busy
+    // the same for a whole bin, and per stretch the mass of the bins ahead
     auto collect = [&](int bin) __attribute__((always_inline)) {
       start_list();
       uint32_t mn = 0xffffffffu, mx = 0;
       u64 sum = 0;
-      int n = 0;
-      bool whole_list = true;
-      auto weigh = [&]() __attribute__((always_inline)) {
-#pragma unroll 1
-        for (int b = 0; b < n; b += 64) {
-          if (b + lane < n) {
-            const float v = s.kept_logit[w][b + lane];
-            const u64 u = weight(v);
-            if (place(v) < (float)bin) {
-              sum += u;
-            } else {
-              const uint32_t k = key_of(v);
-              mn = min(mn, k);
-              mx = max(mx, k);
-              add_to_list(k, s.kept_id[w][b + lane], u);
-            }
-          }
+      auto weigh = [&](const auto& v, int i, const auto& u, const auto& in) __attribute__((always_inline)) {
+        constexpr int M = sizeof(v) / sizeof(float);
+        bool here = false, at[M];
+#pragma unroll
+        for (int e = 0; e < M; ++e) {
+          const float d = place(v[e]);
+          sum += in[e] && d < (float)bin ? u[e] : 0;
+          at[e] = in[e] && d >= (float)bin && d < (float)(bin + 1);
+          here |= at[e];
+        }
+        if (!here) return;
+#pragma unroll
+        for (int e = 0; e < M; ++e) {
+          if (!at[e]) continue;
+          const uint32_t k = key_of(v[e]);
+          mn = min(mn, k);
+          mx = max(mx, k);
+          add_to_list(k, i + e, u[e]);
         }
       };
-      scan(lo, hi, [&](const float(&v)[W], int i) __attribute__((always_inline)) {
-        bool in[W];
-        uint32_t mine = 0;
+      if (!complete) {  // list again, now only what may be kept
+        kept = 0;
+        complete = true;
+        scan(lo, hi, [&](const float(&v)[W], int i) __attribute__((always_inline)) {
+          bool in[W];
 #pragma unroll
-        for (int e = 0; e < W; ++e) {
-          in[e] = place(v[e]) < (float)(bin + 1);
-          mine += in[e];
-        }
-        if (!__any(mine != 0)) return;
-        const uint32_t upto = wave_scan(mine);
-        const int more = (int)of_lane(upto, 63);
-        if (n + more > KEPT) {
-          weigh();
-          n = 0;
-          whole_list = false;
-        }
-        int at = n + (int)(upto - mine);
-#pragma unroll
-        for (int e = 0; e < W; ++e) {
-          if (in[e]) {
-            s.kept_logit[w][at] = v[e];
-            s.kept_id[w][at] = i + e;
-          }
-          at += in[e];
-        }
-        n += more;
-      });
-      weigh();
+          for (int e = 0; e < W; ++e) in[e] = place(v[e]) < (float)(bin + 1);
+          append(v, i, in, weigh);
+        });
+      }
+      each_listed(weigh);
       sum = wave_scan(sum);
       if (lane == 63) {
         s.wave_mass[w] = sum;
         s.wave_count[w] = 0;
-        s.kept_n[w] = whole_list ? n : -1;
+        s.kept_n[w] = complete ? kept : -1;
       }
       end_list(mn, mx);
     };
@@ -468,18 +525,14 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
           s.count2[i] = 0;
         }
         __syncthreads();
-        scan(lo, hi, [&](const float(&v)[W], int) __attribute__((always_inline)) {
-#pragma unroll 1
-          for (int e = 0; e < W; ++e) {
-            const float ve = e == 0 ? v[0] : e == 1 ? v[1 % W] : e == 2 ? v[2 % W] : v[3 % W];
-            const float d = place(ve);
-            if (!(d >= (float)bin && d < (float)(bin + 1))) continue;
-            const uint32_t k = key_of(ve);
-            if (k < kmin || k > kmax) continue;
-            const int b = (int)((kmax - k) >> shift);
-            atomicAdd(&s.mass2[b], weight(ve));
-            atomicAdd(&s.count2[b], 1u);
-          }
+        each_binned([&](const float(&v)[1], int, const u64(&u)[1], const bool(&)[1]) __attribute__((always_inline)) {
+          const float d = place(v[0]);
+          if (!(d >= (float)bin && d < (float)(bin + 1))) return;
+          const uint32_t k = key_of(v[0]);
+          if (k < kmin || k > kmax) return;
+          const int b = (int)((kmax - k) >> shift);
+          atomicAdd(&s.mass2[b], u[0]);
+          atomicAdd(&s.count2[b], 1u);
         });
         __syncthreads();
         const int part = find(s.mass2, s.count2, mass0, count0, counts, bound);
