@@ -10,12 +10,18 @@ fast-weight master state (read through per-request activation-dtype copies), its
 and its own ring slots.  One step is, per layer: RMSNorm -> packed QKV GEMM -> ``uttt_swa_decode``
 (RoPE at each request's position, ring write, window attention) -> output GEMM -> RMSNorm ->
 query projection -> per-request fast-weight readout (``uttt_swiglu_readout`` over the stacked
-copies) -> output GEMM; then the final norm, the LM head and greedy selection, all on the
-device, so ``capture()`` can record the whole step into one HIP graph.
+copies) -> output GEMM; then the final norm, the LM head and the next token's selection, greedy or
+sampled (``set_sampling``), all on the device, so ``capture()`` can record the whole step into one
+HIP graph.
+
+Beside the step (not in the reference's decoders): ``verify`` runs a tree of drafted tokens per
+request through the model at once, without writing the rings, ``commit`` makes a path of it part
+of the requests, ``speculate_greedy`` does both, and ``fork`` lets requests take over others'
+caches.
 """
 from __future__ import annotations
 
-from typing import List, Optional, Sequence
+from typing import List, Optional, Sequence, Tuple, Union
 
 import torch
 import torch.nn.functional as F
@@ -59,15 +65,21 @@ class BatchedDecoder:
             self.w_down = torch.cat([st.w_down.detach() for st in states]).to(self.dtype).contiguous()
         attn = model.layers[0].attn
         self.window, self.hkv, self.hd, self.heads = attn.window_size, attn.n_kv_heads, attn.head_dim, attn.n_heads
-        self.rings = [(torch.zeros((self.n, self.hkv, self.window, self.hd), dtype=self.dtype, device=dev),
-                       torch.zeros((self.n, self.hkv, self.window, self.hd), dtype=self.dtype, device=dev))
-                      for _ in model.layers]
+        self.sinks = attn.sinks
+        # every layer's slots in one tensor: commits and forks take all layers in one launch
+        self.slots = self.sinks + self.window
+        self.k_rings, self.v_rings = (torch.zeros((len(model.layers), self.n, self.hkv, self.slots, self.hd),
+                                                  dtype=self.dtype, device=dev) for _ in range(2))
+        self.rings = [(self.k_rings[li], self.v_rings[li]) for li in range(len(model.layers))]
         self.cos, self.sin = attn.rope.tables(max_positions, dev)
         self.positions = torch.zeros(self.n, dtype=torch.int64, device=dev)
         self.host_positions = [0] * self.n
         self.tokens = torch.zeros(self.n, dtype=torch.int64, device=dev)
         self.logits: Optional[Tensor] = None
         self.next_tokens: Optional[Tensor] = None
+        self.logprobs: Optional[Tensor] = None  # of the sampled next tokens, after ``set_sampling``
+        self._sampling: Optional[dict] = None
+        self._nodes: Optional[Tuple[Tensor, Tensor]] = None  # the last verified trees' keys / values
         self._graph = None
         self._ws_attn = torch.zeros(1, dtype=torch.uint8, device=dev)
         self._ws_read = torch.zeros(1, dtype=torch.uint8, device=dev)
@@ -86,6 +98,7 @@ class BatchedDecoder:
         ``window`` keys/values into the ring slots.  Returns the next-token logits (N, V)."""
         if len(prompts) != self.n:
             raise ValueError(f"expected {self.n} prompts, got {len(prompts)}")
+        self._nodes = None
         out_logits = []
         for i, (ids, st) in enumerate(zip(prompts, self._states)):
             ids = ids.to(self.device).view(1, -1)
@@ -97,17 +110,27 @@ class BatchedDecoder:
         self.positions.copy_(torch.tensor(self.host_positions, dtype=torch.int64))
         return torch.cat(out_logits, dim=0)
 
+    def _cached_slots(self, cached: int, length: int) -> Tensor:
+        """The slots of the ``cached`` rows of a request of ``length`` tokens: its first tokens, as
+        far as they are sinks, then its last ones.  Token p has slot p while p < sinks and
+        sinks + (p - sinks) mod window from there."""
+        first = min(self.sinks, cached)
+        tokens = torch.arange(length - (cached - first), length, device=self.device)
+        recent = torch.where(tokens < self.sinks, tokens, self.sinks + (tokens - self.sinks) % self.window)
+        return torch.cat((torch.arange(first, device=self.device), recent)) if first else recent
+
     def _load_request(self, i: int, kv_caches, length: int) -> None:
         """Request i's ring slots from a frozen prefill's per-layer caches (the last <= window
-        rotated keys / values of ``length`` tokens): token p goes to slot p mod window."""
+        rotated keys / values of ``length`` tokens, behind the sinks)."""
         if len(kv_caches) != len(self.rings):
             raise ValueError(f"expected {len(self.rings)} layer caches, got {len(kv_caches)}")
         for (kr, vr), (k, v) in zip(self.rings, kv_caches):
             cached = k.shape[2]
-            if (k.shape != (1, self.hkv, cached, self.hd) or v.shape != k.shape or cached > min(length, self.window)
-                    or cached < min(length, self.window - 1)):
-                raise ValueError("a cache must be (1, n_kv_heads, min(length, window) or window - 1, head_dim)")
-            slots = torch.arange(length - cached, length, device=self.device) % self.window
+            if (k.shape != (1, self.hkv, cached, self.hd) or v.shape != k.shape or cached > min(length, self.slots)
+                    or cached < min(length, self.slots - 1)):
+                raise ValueError("a cache must be (1, n_kv_heads, min(length, sinks + window) or sinks + window - 1, "
+                                 "head_dim)")
+            slots = self._cached_slots(cached, length)
             kr[i].index_copy_(1, slots, k[0].to(device=self.device, dtype=kr.dtype))
             vr[i].index_copy_(1, slots, v[0].to(device=self.device, dtype=vr.dtype))
         self.host_positions[i] = int(length)
@@ -118,6 +141,7 @@ class BatchedDecoder:
         the rings, positions and buffers keep their addresses, so a captured step stays valid."""
         if len(kv_caches_per_request) != self.n or len(lengths) != self.n:
             raise ValueError(f"expected caches and lengths for {self.n} requests")
+        self._nodes = None
         for kr, vr in self.rings:
             kr.zero_()
             vr.zero_()
@@ -129,11 +153,10 @@ class BatchedDecoder:
 
     @torch.no_grad()
     def export_kv_caches(self, i: int = 0) -> List:
-        """Request i's per-layer caches in the eager layout (the last min(position, window)
-        rotated keys / values in token order), e.g. to continue a decode eagerly."""
+        """Request i's per-layer caches in the eager layout (the sinks, then the last rotated keys /
+        values up to the window in token order), e.g. to continue a decode eagerly."""
         pos = self.host_positions[i]
-        kept = min(pos, self.window)
-        slots = torch.arange(pos - kept, pos, device=self.device) % self.window
+        slots = self._cached_slots(min(pos, self.slots), pos)
         return [(kr[i:i + 1].index_select(2, slots), vr[i:i + 1].index_select(2, slots)) for kr, vr in self.rings]
 
     def matches(self, model: uTTTModel, states: Sequence[FastWeightState]) -> bool:
@@ -188,7 +211,8 @@ class BatchedDecoder:
             k = qkv[:, hq:hq + hk].view(n, self.hkv, self.hd)
             v = qkv[:, hq + hk:].view(n, self.hkv, self.hd)
             kr, vr = self.rings[li]
-            att = K.swa_decode(q, k, v, kr, vr, self.positions, self.cos, self.sin, workspace=self._ws_attn)
+            att = K.swa_decode(q, k, v, kr, vr, self.positions, self.cos, self.sin, workspace=self._ws_attn,
+                               sinks=self.sinks)
             h = self._linear(att.reshape(n, -1), attn.wo.weight, residual=h)
             y = self._linear(h, block.uttt.w_q.weight, norm=block.uttt_norm)
             qn = block.uttt.q_norm
@@ -207,16 +231,33 @@ class BatchedDecoder:
             h = self._linear(r.view(n, -1), block.uttt.w_o.weight, residual=h)
         logits = self._linear(h, m.lm_head.weight, norm=m.norm)
         self.logits = logits
-        # temperature-0 selection: PAD / BOS / UNK and ids past the active vocabulary excluded
-        limit = m.active_vocab_limit if m.active_vocab_limit < logits.shape[-1] else None
+        # temperature-0 selection: PAD / BOS / UNK and ids past the active vocabulary excluded,
         # written straight into the next step's input (stepping with `next_tokens` copies
         # nothing), and the positions advance in the same launch
-        self.next_tokens = K.greedy_select(logits, (PAD_ID, BOS_ID, UNK_ID), limit, out=self.tokens,
-                                           advance=self.positions)
+        if self._sampling is None:
+            self.next_tokens = K.greedy_select(logits, (PAD_ID, BOS_ID, UNK_ID), self._active_limit(logits),
+                                               out=self.tokens, advance=self.positions)
+        else:
+            self._sample(logits, advance=self.positions)
+
+    def _active_limit(self, logits: Tensor) -> Optional[int]:
+        limit = self.model.active_vocab_limit
+        return limit if limit < logits.shape[-1] else None
+
+    def _sample(self, logits: Tensor, advance: Optional[Tensor] = None) -> None:
+        s = self._sampling
+        self.next_tokens, _ = K.sample_select(logits, s["uniforms"], s["temperature"], s["top_k"], s["top_p"],
+                                              s["min_p"], (PAD_ID, BOS_ID, UNK_ID), self._active_limit(logits),
+                                              out=self.tokens, logprobs=self.logprobs, advance=advance)
 
     def _warm_workspaces(self) -> None:
         from . import _native as N
-        nbytes = N.load_library().uttt_swa_decode_workspace(self.n, self.heads, self.hkv, self.hd, self.window)
+        lib = N.load_library()
+        if self.sinks:
+            code = N.DTYPE_BF16 if self.dtype == torch.bfloat16 else N.DTYPE_F32
+            nbytes = lib.uttt_swa_tree_workspace(self.n, self.heads, self.hkv, 1, self.hd, self.slots, code)
+        else:
+            nbytes = lib.uttt_swa_decode_workspace(self.n, self.heads, self.hkv, self.hd, self.window)
         self._ws_attn = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=self.device)
         d = self.model.config.d_model
         ff = self.model.config.d_ff_fast
@@ -252,6 +293,9 @@ class BatchedDecoder:
             raise ValueError("a request reached the end of the RoPE table")
         if tokens.data_ptr() != self.tokens.data_ptr():
             self.tokens.copy_(tokens)
+        self._nodes = None
+        if self._sampling is not None:  # ahead of the step, so that a replay draws new ones
+            self._sampling["uniforms"].uniform_(generator=self._sampling["generator"])
         if self._graph is not None:
             self._graph.replay()
         else:
@@ -264,6 +308,8 @@ class BatchedDecoder:
     @torch.no_grad()
     def generate_greedy(self, first_logits: Tensor, steps: int) -> Tensor:
         """Greedy tokens (N, steps) continuing from ``first_logits`` (no EOS stop)."""
+        if self._sampling is not None:
+            raise ValueError("the decoder samples; set_sampling(None) makes its choices greedy again")
         m = self.model
         work = first_logits.float().clone()
         work[:, [PAD_ID, BOS_ID, UNK_ID]] = float("-inf")
@@ -276,3 +322,174 @@ class BatchedDecoder:
             tok = self.next_tokens  # already the next step's input
             out.append(tok.clone())
         return torch.stack(out, dim=1)
+
+    # ------------------------------------------------------------------ sampling
+    @torch.no_grad()
+    def set_sampling(self, temperature: Union[None, float, Sequence[float]], top_k: Union[int, Sequence[int]] = 0,
+                     top_p: Union[float, Sequence[float]] = 1.0, min_p: Union[float, Sequence[float]] = 0.0,
+                     generator: Optional[torch.Generator] = None) -> None:
+        """Let every step choose its next tokens by sampling (``kernels.sample_select``), each setting
+        one number or one per request; ``temperature`` None goes back to greedy choices.  The
+        uniforms come from ``generator`` (of the model's device; the default one otherwise), drawn ahead of each
+        step, so that a captured step draws new ones on each replay.  Settings changed later
+        reach a captured step; changing between greedy and sampled drops it (``capture`` again)."""
+        if temperature is None:
+            if self._sampling is not None:
+                self._sampling, self.logprobs, self._graph = None, None, None
+            return
+        rows = {}
+        for name, value, low, high in (("temperature", temperature, 0.0, float("inf")), ("top_k", top_k, 0, 2 ** 31 - 1),
+                                       ("top_p", top_p, 0.0, 1.0), ("min_p", min_p, 0.0, 1.0)):
+            values = [value] * self.n if isinstance(value, (int, float)) else list(value)
+            if len(values) != self.n:
+                raise ValueError(f"{name} must be one number or one per request")
+            if not all(low <= v <= high and v != float("inf") for v in values):
+                raise ValueError(f"{name} must be finite, at least {low} and at most {high}")
+            if name == "top_p" and min(values) <= 0.0:
+                raise ValueError("top_p must be above 0")
+            rows[name] = torch.tensor(values, dtype=torch.int32 if name == "top_k" else torch.float32)
+        if self._sampling is None:
+            self._sampling = {name: t.to(self.device) for name, t in rows.items()}
+            self._sampling["uniforms"] = torch.zeros(self.n, dtype=torch.float32, device=self.device)
+            self.logprobs = torch.zeros(self.n, dtype=torch.float32, device=self.device)
+            self._graph = None
+        else:
+            for name, t in rows.items():
+                self._sampling[name].copy_(t)
+        self._sampling["generator"] = generator
+
+    @torch.no_grad()
+    def generate_sampled(self, first_logits: Tensor, steps: int) -> Tuple[Tensor, Tensor]:
+        """Sampled tokens (N, steps) continuing from ``first_logits``, and the logarithms (N, steps) of
+        the probabilities they were chosen with (no EOS stop; after ``set_sampling``)."""
+        if self._sampling is None:
+            raise ValueError("set_sampling comes first")
+        self._sampling["uniforms"].uniform_(generator=self._sampling["generator"])
+        self._sample(first_logits)
+        out, logprobs = [self.tokens.clone()], [self.logprobs.clone()]
+        for _ in range(steps - 1):
+            self.step(self.tokens)
+            out.append(self.tokens.clone())
+            logprobs.append(self.logprobs.clone())
+        return torch.stack(out, dim=1), torch.stack(logprobs, dim=1)
+
+    # ------------------------------------------------------------------ drafted tokens
+    @torch.no_grad()
+    def verify(self, tokens: Tensor, parents: Optional[Tensor] = None, counts: Optional[Tensor] = None) -> Tensor:
+        """The logits (N, T, V) behind every node of a tree of drafted tokens per request, all nodes
+        at once: ``tokens`` (N, T) int64, T <= 64, ``parents`` (N, T) int32 (-1: the node follows the request's
+        tokens so far, else an earlier node; None: each follows the one before it), ``counts`` (N,) int32 nodes that
+        exist per request (None: T; the logits behind them mean nothing, and their tokens must be ids of
+        the vocabulary all the same).  Neither the rings nor the positions change: ``commit`` makes a
+        path of the tree part of each request."""
+        if tokens.dim() != 2 or tokens.shape[0] != self.n or not 1 <= tokens.shape[1] <= K.N.MAX_TREE_NODES:
+            raise ValueError(f"tokens must be ({self.n}, 1 to {K.N.MAX_TREE_NODES})")
+        nodes = tokens.shape[1]
+        if max(self.host_positions) + nodes > self.cos.shape[0]:
+            raise ValueError("a request's drafted tokens reach past the end of the RoPE table")
+        m, n = self.model, self.n
+        parents = None if parents is None else parents.to(device=self.device, dtype=torch.int32).contiguous()
+        counts = None if counts is None else counts.to(device=self.device, dtype=torch.int32).contiguous()
+        # the nodes that do not exist are zeros here: the layers read them on their way through
+        made = torch.empty if counts is None else torch.zeros
+        k_nodes, v_nodes = (made((len(m.layers), n, nodes, self.hkv, self.hd), dtype=self.dtype, device=self.device)
+                            for _ in range(2))
+        h = F.embedding(tokens.to(self.device).reshape(-1), m.tok_embeddings.weight)  # (N T, D)
+        hq, hk = self.heads * self.hd, self.hkv * self.hd
+        read_ws = None
+        for li, block in enumerate(m.layers):
+            attn = block.attn
+            qkv = self._linear(h, attn.packed_qkv().to(h.dtype), norm=block.attn_norm).view(n, nodes, -1)
+            q = qkv[..., :hq].unflatten(-1, (self.heads, self.hd))
+            k = qkv[..., hq:hq + hk].unflatten(-1, (self.hkv, self.hd))
+            v = qkv[..., hq + hk:].unflatten(-1, (self.hkv, self.hd))
+            att, _, _ = K.swa_tree(q, k, v, *self.rings[li], self.positions, parents, self.cos, self.sin, self.sinks,
+                                   counts, node_outputs=(k_nodes[li], v_nodes[li]))
+            h = self._linear(att.view(n * nodes, -1), attn.wo.weight, residual=h)
+            y = self._linear(h, block.uttt.w_q.weight, norm=block.uttt_norm)
+            qn = block.uttt.q_norm
+            uq = F.rms_norm(y, (h.shape[-1],), qn.weight.to(h.dtype), qn.eps).view(n, nodes, -1)
+            if read_ws is None:
+                read_ws = K.readout_workspace(uq, self.w_up)
+            r = K.swiglu_readout(uq, self.w_up, self.w_gate, self.w_down, self.ln_weight, self.ln_bias,
+                                 m.fast_weight_pool.eps, workspace=read_ws, sweep_reverse=li % 2 == 1)
+            h = self._linear(r.view(n * nodes, -1), block.uttt.w_o.weight, residual=h)
+        logits = self._linear(h, m.lm_head.weight, norm=m.norm)
+        self._nodes = (k_nodes, v_nodes)
+        return logits.view(n, nodes, -1)
+
+    @torch.no_grad()
+    def commit(self, nodes: Tensor, counts: Tensor) -> None:
+        """Append a path of the last verified trees to each request: the tokens of its nodes
+        nodes[n, :counts[n]], from the first behind the request's tokens on, each the parent of the next (``nodes``
+        (N, A) and ``counts`` (N,), on any device; the counts are read back).  A tree is committed once."""
+        if self._nodes is None:
+            raise ValueError("commit follows verify, once, before anything else changes the requests")
+        k_nodes, v_nodes = self._nodes
+        if nodes.dim() != 2 or nodes.shape[0] != self.n or counts.shape != (self.n,):
+            raise ValueError(f"nodes must be ({self.n}, A) and counts ({self.n},)")
+        path, taken = nodes.to("cpu", torch.int64), counts.to("cpu", torch.int64).tolist()
+        if min(taken) < 0 or max(taken) > path.shape[1]:
+            raise ValueError("counts must be at least 0 and at most the columns of nodes")
+        used = path[torch.arange(path.shape[1])[None, :] < torch.tensor(taken)[:, None]]
+        if used.numel() and not 0 <= int(used.min()) <= int(used.max()) < k_nodes.shape[2]:
+            raise ValueError("nodes must be nodes of the verified trees")
+        self._nodes = None
+        K.kv_commit(k_nodes, v_nodes, path.to(device=self.device, dtype=torch.int32),
+                    torch.tensor(taken, dtype=torch.int32).to(self.device), self.k_rings, self.v_rings, self.positions,
+                    self.sinks, advance=True)
+        self.host_positions = [p + t for p, t in zip(self.host_positions, taken)]
+
+    @torch.no_grad()
+    def speculate_greedy(self, tokens: Tensor, parents: Optional[Tensor] = None,
+                         counts: Optional[Tensor] = None) -> List[List[int]]:
+        """One round of greedy decoding with drafted tokens: node 0 of each request's tree is its next token,
+        chosen already, the others descend from it.  Verifies the trees, takes in each the longest path from
+        node 0 whose every token is the greedy choice behind its parent, commits it and returns, per request, the
+        drafted tokens taken and the greedy choice behind the last of them (the next round's
+        node 0, in ``self.tokens`` too): the tokens that single steps would give, as far as the products of
+        more rows at once round alike.  Trees and the choices behind them are read back."""
+        up = (torch.arange(-1, tokens.shape[1] - 1).expand(self.n, -1) if parents is None else parents.cpu()).tolist()
+        held = [tokens.shape[1]] * self.n if counts is None else counts.tolist()
+        if min(held) < 1 or max(held) > tokens.shape[1] or any(
+                row[0] != -1 or any(not 0 <= p < t for t, p in enumerate(row[1:c], 1)) for row, c in zip(up, held)):
+            raise ValueError("node 0 is each tree's root, and every other node's parent is an earlier node")
+        logits = self.verify(tokens, parents, counts)
+        n, nodes, vocab = logits.shape
+        choice = K.greedy_select(logits.view(n * nodes, vocab), (PAD_ID, BOS_ID, UNK_ID),
+                                 self._active_limit(logits)).view(n, nodes).tolist()
+        drafted = tokens.tolist()
+        paths = []
+        for i in range(n):
+            path = [0]
+            for t in range(1, held[i]):
+                if up[i][t] == path[-1] and drafted[i][t] == choice[i][path[-1]]:
+                    path.append(t)
+            paths.append(path)
+        longest = max(len(p) for p in paths)
+        self.commit(torch.tensor([p + [0] * (longest - len(p)) for p in paths]), torch.tensor([len(p) for p in paths]))
+        self.tokens.copy_(torch.tensor([choice[i][p[-1]] for i, p in enumerate(paths)]))
+        return [[drafted[i][t] for t in p[1:]] + [choice[i][p[-1]]] for i, p in enumerate(paths)]
+
+    # ------------------------------------------------------------------ requests taken over
+    @torch.no_grad()
+    def fork(self, sources: Sequence[int]) -> None:
+        """Request i goes on from request sources[i], as that was before the call: its cache and
+        position (``kernels.kv_fork``, in place), the token chosen last, its logits and its fast
+        weights.  Sampling settings stay with the slot.  Buffers keep their addresses, so a
+        captured step stays valid."""
+        src = [int(s) for s in sources]
+        if len(src) != self.n or min(src) < 0 or max(src) >= self.n:
+            raise ValueError(f"sources must be {self.n} requests' indexes")
+        self._nodes = None
+        index = torch.tensor(src, dtype=torch.int32).to(self.device)
+        K.kv_fork(self.k_rings, self.v_rings, index, self.positions)
+        follow = [self.tokens] if self.logits is None else [self.tokens, self.logits]
+        if any(self._states[i] is not self._states[s] for i, s in enumerate(src)):
+            follow += [self.w_up, self.w_gate, self.w_down]
+        index = index.long()
+        for t in follow:
+            t.copy_(t.index_select(0, index))
+        self.host_positions = [self.host_positions[s] for s in src]
+        self._states = [self._states[s] for s in src]
+        self._key = self._state_key(self._states)

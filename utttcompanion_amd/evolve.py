@@ -163,7 +163,7 @@ def ragged_test_time_update(model: uTTTModel, interactions: Sequence[Tensor],
     dt = h.dtype
     n_layers = len(model.layers)
     attn0 = model.layers[0].attn
-    hd, hkv, win = attn0.head_dim, attn0.n_kv_heads, attn0.window_size
+    hd, hkv, win, sinks = attn0.head_dim, attn0.n_kv_heads, attn0.window_size, attn0.sinks
     k_bufs = [torch.empty((n, hkv, seq, hd), dtype=dt, device=dev) for _ in range(n_layers)]
     v_bufs = [torch.empty_like(kb) for kb in k_bufs]
 
@@ -212,7 +212,7 @@ def ragged_test_time_update(model: uTTTModel, interactions: Sequence[Tensor],
                 kb, vb = k_bufs[li][:rows], v_bufs[li][:rows]
                 q = attn.project(hid, off, kb, vb, off, norm=block.attn_norm)
                 att = torch.empty((rows, c, attn.n_heads, hd), dtype=dt, device=dev)
-                K.swa_prefill(q.transpose(1, 2), kb, vb, win, off, out=att.transpose(1, 2), kv_len=end)
+                K.swa_prefill(q.transpose(1, 2), kb, vb, win, off, out=att.transpose(1, 2), kv_len=end, sinks=sinks)
                 hid = linear_residual(hid, att.view(rows, c, -1), attn.wo.weight)
                 uq, uk, uv, eta, alpha = block.uttt.projections(hid, norm=block.uttt_norm)
                 prep = K.prepare_chunk_update(uq, uk, uv, eta, alpha, *(snap if li == 0 else cursor), ln_w, ln_b,
@@ -235,7 +235,7 @@ def ragged_test_time_update(model: uTTTModel, interactions: Sequence[Tensor],
             kb, vb = k_bufs[li][:rows], v_bufs[li][:rows]
             q = attn.project(hid, off, kb, vb, off, norm=block.attn_norm)
             att = torch.empty((rows, c, attn.n_heads, hd), dtype=dt, device=dev)
-            K.swa_prefill(q.transpose(1, 2), kb, vb, win, off, out=att.transpose(1, 2), kv_len=end)
+            K.swa_prefill(q.transpose(1, 2), kb, vb, win, off, out=att.transpose(1, 2), kv_len=end, sinks=sinks)
             hid = linear_residual(hid, att.view(rows, c, -1), attn.wo.weight)
             uq, uk, uv, eta, alpha = block.uttt.projections(hid, norm=block.uttt_norm)
             ready = torch.cuda.Event()

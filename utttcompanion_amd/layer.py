@@ -381,12 +381,34 @@ def apply_rope(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor) -> Tuple[Tensor, 
     return q * cos + rot(q) * sin, k * cos + rot(k) * sin
 
 
+def kept_rows(buf: Tensor, window: int, sinks: int) -> Tensor:
+    """The rows of a (B, Hkv, tokens, hd) KV buffer that a cache keeps: all of them while they are at
+    most sinks + window, else the first ``sinks`` and the last ``window`` (a copy)."""
+    if buf.shape[2] <= sinks + window:
+        return buf
+    if not sinks:
+        return buf[:, :, -window:].contiguous()
+    return torch.cat((buf[:, :, :sinks], buf[:, :, -window:]), dim=2)
+
+
+def history_rows(cached: int, window: int, sinks: int) -> Tuple[int, int]:
+    """(leading rows, trailing rows) of a cache of ``cached`` rows that the next token can see: the
+    sinks, and of the rest the last window - 1."""
+    first = min(sinks, cached)
+    return first, min(cached - first, window - 1)
+
+
 class SlidingWindowAttention(nn.Module):
-    """Local sliding-window GQA with RoPE and a bounded KV cache (reference :961-1168)."""
+    """Local sliding-window GQA with RoPE and a bounded KV cache (reference :961-1168).  With
+    ``sinks`` the first tokens of a sequence stay visible beside the window and in the cache
+    (not in the reference)."""
 
     def __init__(self, d_model: int, n_heads: int, n_kv_heads: int, window_size: int = 512,
-                 max_seq_len: int = 4096, rope_theta: float = 10000.0, dropout: float = 0.0) -> None:
+                 max_seq_len: int = 4096, rope_theta: float = 10000.0, dropout: float = 0.0,
+                 sinks: int = 0) -> None:
         super().__init__()
+        if sinks < 0:
+            raise ValueError("sinks must be >= 0")
         if d_model % n_heads or n_heads % n_kv_heads:
             raise ValueError("d_model must divide by n_heads and n_heads by n_kv_heads")
         self.d_model = d_model
@@ -395,6 +417,7 @@ class SlidingWindowAttention(nn.Module):
         self.n_rep = n_heads // n_kv_heads
         self.head_dim = d_model // n_heads
         self.window_size = window_size
+        self.sinks = sinks
         self.dropout = dropout
         self.wq = nn.Linear(d_model, n_heads * self.head_dim, bias=False)
         self.wk = nn.Linear(d_model, n_kv_heads * self.head_dim, bias=False)
@@ -472,24 +495,33 @@ class SlidingWindowAttention(nn.Module):
 
     def forward(self, x: Tensor, kv_cache: Optional[Tuple[Tensor, Tensor]] = None,
                 start_pos: int = 0) -> Tuple[Tensor, Tuple[Tensor, Tensor]]:
-        """Attention over the window; returns (out, cache of the last <= window rotated k/v)."""
+        """Attention over the window (and the sinks); returns (out, cache of the last <= window
+        rotated k/v, behind the first ``sinks`` of them)."""
         if self.training and torch.is_grad_enabled():
             raise ValueError("the HIP attention path is inference-only")
         bsz, seq, _ = x.shape
-        hd, hkv, win = self.head_dim, self.n_kv_heads, self.window_size
-        hist = 0
+        hd, hkv, win, sinks = self.head_dim, self.n_kv_heads, self.window_size, self.sinks
+        first = recent = 0
         if kv_cache is not None:
-            hist = min(kv_cache[0].shape[2], win - 1)
+            first, recent = history_rows(kv_cache[0].shape[2], win, sinks)
+        hist = first + recent
         kv_len = hist + seq
         k_buf = torch.empty((bsz, hkv, kv_len, hd), dtype=x.dtype, device=x.device)
         v_buf = torch.empty_like(k_buf)
-        history = None if not hist else (kv_cache[0][:, :, -hist:], kv_cache[1][:, :, -hist:])
+        history = None if not recent else (kv_cache[0][:, :, -recent:], kv_cache[1][:, :, -recent:])
         cache, trimmed = (k_buf, v_buf), None
-        if kv_len > win:
-            cache = trimmed = tuple(torch.empty((bsz, hkv, win, hd), dtype=x.dtype, device=x.device) for _ in range(2))
+        if kv_len > sinks + win:
+            cache = tuple(torch.empty((bsz, hkv, sinks + win, hd), dtype=x.dtype, device=x.device) for _ in range(2))
+            trimmed = tuple(t[:, :, sinks:] for t in cache) if sinks else cache
+        if first:  # the sinks' rows stay in front of the window's
+            k_buf[:, :, :first].copy_(kv_cache[0][:, :, :first])
+            v_buf[:, :, :first].copy_(kv_cache[1][:, :, :first])
         q = self.project(x, start_pos, k_buf, v_buf, hist, history=history, out=trimmed)
+        if sinks and trimmed is not None:
+            cache[0][:, :, :sinks].copy_(k_buf[:, :, :sinks])
+            cache[1][:, :, :sinks].copy_(v_buf[:, :, :sinks])
         attn = torch.empty((bsz, seq, self.n_heads, hd), dtype=x.dtype, device=x.device)
-        K.swa_prefill(q.transpose(1, 2), k_buf, v_buf, win, hist, out=attn.transpose(1, 2))
+        K.swa_prefill(q.transpose(1, 2), k_buf, v_buf, win, hist, out=attn.transpose(1, 2), sinks=sinks)
         return self.wo(attn.view(bsz, seq, self.d_model)), cache
 
 
@@ -629,12 +661,12 @@ class uTTTBlock(nn.Module):
     def __init__(self, layer_idx: int, d_model: int, n_heads: int, n_kv_heads: int, window_size: int = 512,
                  chunk_size: int = 64, base_inner_lr: float = 0.015, base_weight_decay: float = 0.005,
                  max_seq_len: int = 4096, rope_theta: float = 10000.0, rms_norm_eps: float = 1e-5,
-                 dropout: float = 0.0) -> None:
+                 dropout: float = 0.0, sinks: int = 0) -> None:
         super().__init__()
         self.layer_idx = layer_idx
         self.attn_norm = RMSNorm(d_model, eps=rms_norm_eps)
         self.attn = SlidingWindowAttention(d_model, n_heads, n_kv_heads, window_size, max_seq_len, rope_theta,
-                                           dropout)
+                                           dropout, sinks)
         self.uttt_norm = RMSNorm(d_model, eps=rms_norm_eps)
         self.uttt = uTTTLayer(d_model, chunk_size, base_inner_lr, base_weight_decay, rms_norm_eps)
 

@@ -30,7 +30,8 @@ import torch.nn.functional as F
 from . import _native as N
 from . import kernels as K
 from .prefill_plan import PrefillPlan, plan_supported
-from .layer import FastWeightState, RMSNorm, SharedFastWeightPool, linear_residual, require_write_chunk, uTTTBlock
+from .layer import (FastWeightState, RMSNorm, SharedFastWeightPool, history_rows, kept_rows, linear_residual,
+                    require_write_chunk, uTTTBlock)
 
 Tensor = torch.Tensor
 _NAMES = ("w_up", "w_gate", "w_down", "s_up", "s_gate", "s_down")
@@ -75,6 +76,7 @@ class uTTTConfig:
     dspark_conf_threshold: float = 0.82
     tokenizer_json: Optional[str] = None
     repetition_penalty: float = 1.0
+    attention_sinks: int = 0  # first tokens that stay visible beside the window (not in the reference)
 
     def to_dict(self) -> Dict[str, Any]:
         return asdict(self)
@@ -130,7 +132,7 @@ class uTTTModel(nn.Module):
         self.layers = nn.ModuleList([
             uTTTBlock(i, config.d_model, config.n_heads, config.n_kv_heads, config.sliding_window_size,
                       config.chunk_size, config.base_inner_lr, config.base_weight_decay, config.max_seq_len,
-                      config.rope_theta, config.rms_norm_eps, config.dropout)
+                      config.rope_theta, config.rms_norm_eps, config.dropout, config.attention_sinks)
             for i in range(config.n_layers)])
         self.norm = RMSNorm(config.d_model, eps=config.rms_norm_eps)
         self.lm_head = nn.Linear(config.d_model, config.vocab_size, bias=False)
@@ -245,7 +247,8 @@ class uTTTModel(nn.Module):
         (all readouts read the chunk-start state, reference uttt_model.py:519-608), then one
         ``uttt_chunk_chain`` launch applies the layers' chained updates to the state in place.
         Returns (hidden (B, T, D), final state tensors (6,), per-layer surprise (L,) fp32
-        device tensor, per-layer KV caches (last <= window rotated keys/values)).
+        device tensor, per-layer KV caches (last <= window rotated keys/values, behind the
+        sinks')).
         """
         cfg = self.config
         if cfg.write_schedule != "sequential":
@@ -258,18 +261,21 @@ class uTTTModel(nn.Module):
         n_layers, c = len(self.layers), cfg.chunk_size
         n_chunks = (seq + c - 1) // c
         attn0 = self.layers[0].attn
-        hd, hkv, win = attn0.head_dim, attn0.n_kv_heads, attn0.window_size
+        hd, hkv, win, sinks = attn0.head_dim, attn0.n_kv_heads, attn0.window_size, attn0.sinks
 
-        hist = 0
+        first = hist = 0
         if kv_caches is not None:
-            hist = min(kv_caches[0][0].shape[2], win - 1)
+            first, recent = history_rows(kv_caches[0][0].shape[2], win, sinks)
+            hist = first + recent
         k_bufs, v_bufs = [], []
         for li in range(n_layers):
             kb = torch.empty((bsz, hkv, hist + seq, hd), dtype=h.dtype, device=dev)
             vb = torch.empty_like(kb)
-            if hist:
-                kb[:, :, :hist].copy_(kv_caches[li][0][:, :, -hist:])
-                vb[:, :, :hist].copy_(kv_caches[li][1][:, :, -hist:])
+            for buf, kept in ((kb, 0), (vb, 1)):
+                if first:
+                    buf[:, :, :first].copy_(kv_caches[li][kept][:, :, :first])
+                if hist > first:
+                    buf[:, :, first:hist].copy_(kv_caches[li][kept][:, :, first - hist:])
             k_bufs.append(kb)
             v_bufs.append(vb)
 
@@ -329,8 +335,7 @@ class uTTTModel(nn.Module):
                     N.check(N.load_library().uttt_stream_wait_event(main.cuda_stream, pending),
                             "uttt_stream_wait_event")
             per_layer = (surprises * counts[:, None]).sum(dim=0) / counts.sum().clamp_min(1.0)
-            caches = [(kb[:, :, -win:].contiguous(), vb[:, :, -win:].contiguous()) if kb.shape[2] > win
-                      else (kb, vb) for kb, vb in zip(k_bufs, v_bufs)]
+            caches = [(kept_rows(kb, win, sinks), kept_rows(vb, win, sinks)) for kb, vb in zip(k_bufs, v_bufs)]
             return h, cur, per_layer, caches
         ws_chain = ws_read = None
         # bf16: each layer's readout also forms the chain's products of that layer's keys with
@@ -354,7 +359,7 @@ class uTTTModel(nn.Module):
                 q = attn.project(hid, start_pos + off, k_bufs[li], v_bufs[li], hist + off, norm=block.attn_norm)
                 att = torch.empty((bsz, end - off, attn.n_heads, hd), dtype=h.dtype, device=dev)
                 K.swa_prefill(q.transpose(1, 2), k_bufs[li], v_bufs[li], win, hist + off,
-                              out=att.transpose(1, 2), kv_len=hist + end)
+                              out=att.transpose(1, 2), kv_len=hist + end, sinks=sinks)
                 hid = linear_residual(hid, att.view(bsz, end - off, -1), attn.wo.weight)
                 uq, uk, uv, eta, alpha = block.uttt.projections(hid, norm=block.uttt_norm)
                 ready = torch.cuda.Event()
@@ -388,8 +393,7 @@ class uTTTModel(nn.Module):
             pieces.append(hid)
             yield ci
         per_layer = (surprises * counts[:, None]).sum(dim=0) / counts.sum().clamp_min(1.0)
-        caches = [(kb[:, :, -win:].contiguous(), vb[:, :, -win:].contiguous()) if kb.shape[2] > win else (kb, vb)
-                  for kb, vb in zip(k_bufs, v_bufs)]
+        caches = [(kept_rows(kb, win, sinks), kept_rows(vb, win, sinks)) for kb, vb in zip(k_bufs, v_bufs)]
         return torch.cat(pieces, dim=1), cur, per_layer, caches
 
     def _prefill_per_layer_updates(self, h: Tensor, cur: Tuple[Tensor, ...], ln_w: Tensor, ln_b: Tensor,
@@ -410,7 +414,7 @@ class uTTTModel(nn.Module):
         c, n_layers = cfg.chunk_size, len(self.layers)
         n_chunks = (seq + c - 1) // c
         attn0 = self.layers[0].attn
-        hd, win = attn0.head_dim, attn0.window_size
+        hd, win, sinks = attn0.head_dim, attn0.window_size, attn0.sinks
         pool = self.fast_weight_pool
         clip = float(pool.max_inner_grad_norm or 0.0)
         sets = [tuple(cur), tuple(torch.empty_like(t) for t in cur)]
@@ -431,7 +435,7 @@ class uTTTModel(nn.Module):
                 q = attn.project(hid, start_pos + off, k_bufs[li], v_bufs[li], hist + off, norm=block.attn_norm)
                 att = torch.empty((bsz, end - off, attn.n_heads, hd), dtype=h.dtype, device=h.device)
                 K.swa_prefill(q.transpose(1, 2), k_bufs[li], v_bufs[li], win, hist + off, out=att.transpose(1, 2),
-                              kv_len=hist + end)
+                              kv_len=hist + end, sinks=sinks)
                 hid = linear_residual(hid, att.view(bsz, end - off, -1), attn.wo.weight)
                 uq, uk, uv, eta, alpha = block.uttt.projections(hid, norm=block.uttt_norm)
                 src = snap if li == 0 else cursor  # layer 0 writes the chunk-start state out of place
@@ -446,8 +450,7 @@ class uTTTModel(nn.Module):
             pieces.append(hid)
             yield ci
         per_layer = (surprises * counts[:, None]).sum(dim=0) / counts.sum().clamp_min(1.0)
-        caches = [(kb[:, :, -win:].contiguous(), vb[:, :, -win:].contiguous()) if kb.shape[2] > win else (kb, vb)
-                  for kb, vb in zip(k_bufs, v_bufs)]
+        caches = [(kept_rows(kb, win, sinks), kept_rows(vb, win, sinks)) for kb, vb in zip(k_bufs, v_bufs)]
         return torch.cat(pieces, dim=1), sets[start_set], per_layer, caches
 
     def _chain_stream(self, device: torch.device) -> "torch.cuda.Stream":

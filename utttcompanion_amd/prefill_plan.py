@@ -25,12 +25,12 @@ from . import kernels as K
 
 def plan_supported(model, h: Tensor, copies) -> bool:
     """Whether ``uttt_prefill_chunk`` runs this prefill: bf16 activations with the state's bf16
-    copies (the shared-weight-read schedule) and slow-weight products whose k is a multiple of
-    64."""
+    copies (the shared-weight-read schedule), slow-weight products whose k is a multiple of
+    64, and attention without sinks (its prepared calls carry none)."""
     if h.dtype != torch.bfloat16 or copies is None or h.device.type != "cuda":
         return False
     attn = model.layers[0].attn
-    return (model.config.d_model % 64 == 0 and (attn.n_heads * attn.head_dim) % 64 == 0
+    return (attn.sinks == 0 and model.config.d_model % 64 == 0 and (attn.n_heads * attn.head_dim) % 64 == 0
             and len(model.layers) <= N.MAX_CHAIN)
 
 
