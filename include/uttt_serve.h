@@ -38,7 +38,8 @@ int uttt_serve_abi_version(void);
  *    uniform * total (uniforms are taken into [0, 1), NaN as 0); logprob is log(w_out / total).
  *    A temperature that is not above 1e-5 takes the argmax (uttt_greedy_select's rules), logprob 0; so does,
  *    with logprob NaN, a row whose largest logit is not finite (NaN, +inf, or nothing allowed above -inf).
- *    Sums are formed in fixed point, so equal inputs give equal bits whatever the order.
+ *    Sums are formed in fixed point (weights in steps of 2^-42, by fp32 exponentials), so equal inputs give
+ *    equal bits whatever the order.
  * ------------------------------------------------------------------------- */
 typedef struct {
   int64_t rows, vocab; /* vocab <= 2^20 */
@@ -78,6 +79,8 @@ int uttt_swa_prefill_sinks(const uttt_swa_prefill_args* args, int64_t sinks, utt
  *    counts (optional): only the first counts[n] nodes of request n exist, rows behind them are neither read
  *    nor written.  A request with a negative position, a position past the tables, or a node whose parent is
  *    neither -1 nor an earlier node gets NaN outputs and no key or value is written.
+ *    One head's slots of one request, taken as fp32, stay below 2 GB: (window + sinks) head_dim < 2^29.  Requests
+ *    may share a ring (stride 0) where none is written.
  * ------------------------------------------------------------------------- */
 typedef struct {
   int64_t n_req, n_heads, n_kv_heads, nodes, head_dim; /* head_dim 64 or 128; nodes in 1..64 */
@@ -106,7 +109,8 @@ int uttt_swa_tree(const uttt_swa_tree_args* args, uttt_stream_t stream);
  * 4. The accepted nodes of each request into its rings, all layers in one launch: node nodes[n][a], for
  *    a < counts[n], becomes the token at position positions[n] + a.  advance: positions[n] += counts[n]
  *    afterwards.  counts are taken into [0, path]; a node id outside [0, n_nodes) leaves its slot
- *    as it was; a request with a negative position is left as it was.
+ *    as it was; a request with a negative position is left as it was.  Where a path is longer than
+ *    the window, the last token of a slot stays.
  * ------------------------------------------------------------------------- */
 typedef struct {
   int64_t layers, n_req, n_kv_heads, n_nodes, path, head_dim; /* path: length of a row of `nodes` */

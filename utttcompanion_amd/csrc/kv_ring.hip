@@ -105,6 +105,14 @@ __global__ void __launch_bounds__(kMaxFork) k_kv_fork_positions(int64_t* positio
   if (moved) positions[n] = p;
 }
 
+// Whether the requests' slabs of all layers, which the call writes, lie apart.
+bool slabs_apart(int64_t layers, int64_t stride_l, int64_t n_req, int64_t stride_n, int64_t slab) {
+  if (n_req == 1 || layers == 1)
+    return (n_req == 1 || stride_n >= slab) && (layers == 1 || stride_l >= slab);
+  return stride_l >= stride_n ? stride_n >= slab && stride_l / n_req >= stride_n
+                              : stride_l >= slab && stride_n / layers >= stride_l;
+}
+
 }  // namespace
 }  // namespace uttt
 
@@ -128,6 +136,10 @@ extern "C" int uttt_kv_commit(const uttt_kv_commit_args* a, uttt_stream_t stream
                    a->nodes_stride_l % vec == 0 && a->nodes_stride_n % vec == 0 && a->ring_stride_l % vec == 0 &&
                    a->ring_stride_n % vec == 0,
                "nodes and rings must be 16-byte aligned with strides of whole pieces");
+  UTTT_REQUIRE((double)a->n_kv_heads * (double)(a->sinks + a->window) * (double)a->head_dim < (double)(1LL << 60) &&
+                   slabs_apart(a->layers, a->ring_stride_l, a->n_req, a->ring_stride_n,
+                               a->n_kv_heads * (a->sinks + a->window) * a->head_dim),
+               "the requests' rings must not overlap");
   CommitArgs m{};
   m.layers = (int)a->layers; m.heads = (int)a->n_kv_heads; m.n_nodes = (int)a->n_nodes; m.path = (int)a->path;
   m.pieces = (int)(a->head_dim / vec);
@@ -162,6 +174,9 @@ extern "C" int uttt_kv_fork(const uttt_kv_fork_args* a, uttt_stream_t stream) {
   UTTT_REQUIRE(a->sources && a->k_ring && a->v_ring && a->positions, "pointers must be non-NULL");
   UTTT_REQUIRE(aligned16(a->k_ring) && aligned16(a->v_ring) && a->ring_stride_l % vec == 0 && a->ring_stride_n % vec == 0,
                "rings must be 16-byte aligned with strides of whole pieces");
+  UTTT_REQUIRE((double)a->n_kv_heads * (double)a->slots * (double)a->head_dim < (double)(1LL << 60) &&
+                   slabs_apart(a->layers, a->ring_stride_l, a->n_req, a->ring_stride_n, a->n_kv_heads * a->slots * a->head_dim),
+               "the requests' rings must not overlap");
   // 16-byte pieces while 64 requests' pieces fit a thread's registers, 8-byte ones beyond
   const int64_t piece = a->n_req <= 64 ? 16 : 8, per = piece / size;
   ForkArgs m{};

@@ -1184,6 +1184,8 @@ extern "C" int uttt_swa_tree(const uttt_swa_tree_args* a, uttt_stream_t stream) 
                "operands must be 16-byte aligned with strides of whole 16-byte pieces");
   const bool b16 = a->act_dtype == UTTT_DTYPE_BF16;
   const int64_t slots = a->window + a->sinks;
+  UTTT_REQUIRE(!a->write_ring || a->n_req == 1 || a->ring_stride_n >= a->n_kv_heads * slots * a->head_dim,
+               "the requests' rings must not overlap");
   const TreePlan p = plan_tree(a->n_req, a->n_heads, a->n_kv_heads, a->nodes, a->head_dim, slots, b16);
   UTTT_REQUIRE((a->n_req * a->n_kv_heads * p.nsplit + kXcds) * p.groups <= 0x7fffffffLL &&
                    a->n_req * a->n_heads * a->nodes * (a->head_dim / 4) / kThreads < 0x7fffffffLL,
