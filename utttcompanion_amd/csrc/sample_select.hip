@@ -145,21 +145,21 @@ struct Shared {
   int cut_ties;
 };
 
-// ids that are left out read as -inf
+// ids that are left out, and those below 0, read as -inf
 template <int VEC>
 __device__ __forceinline__ void leave_out(const SampleArgs& a, float (&v)[VEC], int i) {
 #pragma unroll
   for (int e = 0; e < VEC; ++e) {
-    bool out = i + e < 64 && ((a.low >> (i + e)) & 1);
+    bool out = i + e < 64 && (i + e < 0 || ((a.low >> (i + e)) & 1));
     for (int k = 0; k < a.n_high; ++k) out |= i + e == a.high[k];
     v[e] = out ? -INFINITY : v[e];
   }
 }
 
-// f(values, first id) for ids [lo, hi) of the row in order, VEC to a lane; U steps of 64 VEC ids in flight.  What a step
-// has past hi reads as -inf.
+// f(values, first id) for places [lo, hi) of the row in order, VEC to a lane; U steps of 64 VEC in flight.  The id is the
+// place less `off`.  What a step has past hi reads as -inf.
 template <typename T, int VEC, int U, bool RAW, typename F>
-__device__ __forceinline__ void scan_ids(const SampleArgs& a, const T* x, int lo, int hi, int lane, F&& f) {
+__device__ __forceinline__ void scan_ids(const SampleArgs& a, const T* x, int off, int lo, int hi, int lane, F&& f) {
   typedef T vec_t __attribute__((ext_vector_type(VEC)));
 #pragma unroll 1
   for (int b = lo; b < hi; b += 64 * VEC * U) {
@@ -177,44 +177,50 @@ __device__ __forceinline__ void scan_ids(const SampleArgs& a, const T* x, int lo
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = b + (u * 64 + lane) * VEC;
+      const int i = b + (u * 64 + lane) * VEC - off;
       float y[VEC];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) y[e] = to_f32((T)v[u][e]);
-      if (RAW && (b < 64 || a.n_high > 0)) leave_out<VEC>(a, y, i);
+      if (RAW && (b < 64 + off || a.n_high > 0)) leave_out<VEC>(a, y, i);
       f(y, i);
     }
   }
 }
 
 // STAGED: the row stays in LDS behind the first pass, without the ids that are left out.
-template <typename T, int VEC, bool STAGED>
+template <typename T, bool STAGED>
 __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs a) {
-  constexpr int KEPT = STAGED ? kKeptStaged : kKept;
+  constexpr int KEPT = STAGED ? kKeptStaged : kKept, VEC = 16 / (int)sizeof(T);
   __shared__ Shared<KEPT> s;
   __shared__ __align__(16) T stage[STAGED ? kStageBytes / sizeof(T) : 1];
   constexpr int W = STAGED ? 8 / (int)sizeof(T) : VEC > 4 ? 4 : VEC;  // ids to a lane in the passes behind the first
   constexpr float kFine = 128.f, kCoarse = 48.f;  // bins to a factor of two: kBins / 48 > 42, what weights reach
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // Places count from the 16-byte boundary at or before the row's first id, so that rows of any alignment are read in
+  // whole 16-byte pieces (256 rows of 131071 fp32 at temperature 0.7: one id at
+  // a time 123 us, so 80); ids from the place `off` on.
   const T* x = static_cast<const T*>(a.logits) + (int64_t)row * a.rs;
+  const int off = __builtin_amdgcn_readfirstlane((int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T)));
+  const int places = a.limit + off;
+  x -= off;
   // a wave's stretch of the row
-  constexpr int kStep = 64 * (VEC > W ? VEC : W);
-  const int stretch = ((a.limit + kSmpWaves - 1) / kSmpWaves + kStep - 1) / kStep * kStep;
-  const int lo = min(w * stretch, a.limit), hi = min(lo + stretch, a.limit);
+  constexpr int kStep = 64;  // whole pieces; short rows still reach many waves
+  const int stretch = ((places + kSmpWaves - 1) / kSmpWaves + kStep - 1) / kStep * kStep;
+  const int lo = min(w * stretch, places), hi = min(lo + stretch, places);
   const float temp = a.temperature[row], uniform = a.uniforms[row];
   const int top_k = a.top_k != nullptr ? a.top_k[row] : 0;
   const float top_p = a.top_p != nullptr ? a.top_p[row] : 1.f, min_p = a.min_p != nullptr ? a.min_p[row] : 0.f;
   auto scan = [&](int from, int to, auto&& f) __attribute__((always_inline)) {
     if constexpr (STAGED)
-      scan_ids<T, W, 1, false>(a, stage, from, to, lane, f);
+      scan_ids<T, W, 1, false>(a, stage, off, from, to, lane, f);
     else
-      scan_ids<T, W, 2, true>(a, x, from, to, lane, f);
+      scan_ids<T, W, 2, true>(a, x, off, from, to, lane, f);
   };
 
   // ---- the largest logit; NaN makes it NaN
   float top = -INFINITY;
   bool nan = false;
-  scan_ids<T, VEC, 4, true>(a, x, lo, hi, lane, [&](const float(&v)[VEC], int i) __attribute__((always_inline)) {
+  scan_ids<T, VEC, 4, true>(a, x, off, lo, hi, lane, [&](const float(&v)[VEC], int i) __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       top = fmaxf(top, v[e]);
@@ -225,7 +231,7 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
       vec_t y;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) y[e] = from_f32<T>(v[e]);
-      if (i < hi) *reinterpret_cast<vec_t*>(stage + i) = y;  // past the last id: -inf
+      if (i + off < hi) *reinterpret_cast<vec_t*>(stage + (i + off)) = y;  // past the last id: -inf
     }
   });
 #pragma unroll
@@ -257,7 +263,7 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
     if (best != 0x7fffffff) atomicMin(&s.best, best);
     __syncthreads();
     if (tid == 0) {
-      a.out[row] = s.best == 0x7fffffff ? 0 : s.best;
+      a.out[row] = s.best == 0x7fffffff ? 0 : max(s.best, 0);  // below 0 where all are -inf
       if (a.logprob != nullptr) a.logprob[row] = greedy ? 0.f : NAN;
       if (a.advance != nullptr) a.advance[row] += 1;
     }
@@ -268,8 +274,9 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
   const bool by_count = top_k > 0 && top_k < a.limit, by_mass = top_p < 1.f;
   const u64 least = min_p > 0.f ? (u64)__builtin_ceil(fmin((double)min_p, 1.0) * 4398046511104.0) : 1;
   auto weight = [&](float v) __attribute__((always_inline)) -> u64 {
-    const u64 u = weight_units(((double)v - dtop) * c);
-    return least <= 1 || u >= least ? u : 0;
+    u64 u = weight_units(((double)v - dtop) * c);
+    if (least > 1) u = u >= least ? u : 0;
+    return u;
   };
   float per_unit = fminf((float)c * kFine, 3e38f);  // bins to a unit of the logits
   float last = (float)kBins;                        // ids in bins from here on are not counted, or with ...
@@ -591,7 +598,7 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
         r.mass = mass0 + s.kept;
       }
       if (masses && tid < n) {  // the bin's own part of the stretches' masses, and its ids at the cut
-        const int q = s.list_id[tid] / stretch;
+        const int q = (s.list_id[tid] + off) / stretch;
         if (s.list_key[tid] > r.key) atomicAdd(&s.wave_mass[q], s.list_mass[tid]);
         if (s.list_key[tid] == r.key) atomicAdd(&s.wave_count[q], 1u);
       }
@@ -696,7 +703,7 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
   int q0 = 0, q1 = masses ? s.kept_n[q] : -1;
   const bool listed = q1 >= 0;
   if (!listed) {
-    const int p0 = min(q * stretch, a.limit), p1 = min(p0 + stretch, a.limit);
+    const int p0 = min(q * stretch, places), p1 = min(p0 + stretch, places);
     const int part = ((p1 - p0 + kSmpWaves - 1) / kSmpWaves + kStep - 1) / kStep * kStep;
     const int q_lo = min(p0 + w * part, p1);
     part_mass(q_lo, min(q_lo + part, p1));
@@ -718,7 +725,7 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
         v[0] = to_f32(stage[i]);
       } else {
         v[0] = to_f32(x[i]);
-        leave_out<1>(a, v, i);
+        leave_out<1>(a, v, i - off);
       }
     }
     u64 u = v[0] > at_cut ? weight(v[0]) : 0;
@@ -729,7 +736,7 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
     const u64 over = __ballot(m + sum > want);
     if (over != 0) {
       token = b + __builtin_ctzll(over);
-      if (listed) token = s.kept_id[q][token];
+      token = listed ? s.kept_id[q][token] : token - off;
     }
     m += of_lane(sum, 63);
     t += __popcll(tied);
@@ -738,26 +745,21 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
     token = token < 0 ? 0 : token;  // integers add up the same way at every level, so one is found
     a.out[row] = token;
     // log(w / total): the weight's own exponent, not its rounded units
+    float divisor = temp;
+    asm volatile("" : "+v"(divisor));  // its 64-bit form is made here, not kept in registers through the passes
     if (a.logprob != nullptr)
-      a.logprob[row] = (float)(((double)to_f32(x[token]) - dtop) / (double)temp - log((double)whole * 0x1p-42));
+      a.logprob[row] = (float)(((double)to_f32(x[token + off]) - dtop) / (double)divisor - log((double)whole * 0x1p-42));
     if (a.advance != nullptr) a.advance[row] += 1;
   }
 }
 
 template <typename T>
 void launch_sample(const SampleArgs& s, int64_t rows, hipStream_t st) {
-  constexpr int VEC = 16 / (int)sizeof(T);
   const dim3 grid((unsigned)rows), block(kSmpThreads);
-  const bool vec = aligned16(s.logits) && (rows == 1 || s.rs % VEC == 0);
-  const bool staged = (int64_t)s.limit * (int64_t)sizeof(T) <= kStageBytes - 16;
-  if (vec && staged)
-    hipLaunchKernelGGL((k_sample_select<T, VEC, true>), grid, block, 0, st, s);
-  else if (vec)
-    hipLaunchKernelGGL((k_sample_select<T, VEC, false>), grid, block, 0, st, s);
-  else if (staged)
-    hipLaunchKernelGGL((k_sample_select<T, 1, true>), grid, block, 0, st, s);
+  if ((int64_t)s.limit * (int64_t)sizeof(T) <= kStageBytes - 16)
+    hipLaunchKernelGGL((k_sample_select<T, true>), grid, block, 0, st, s);
   else
-    hipLaunchKernelGGL((k_sample_select<T, 1, false>), grid, block, 0, st, s);
+    hipLaunchKernelGGL((k_sample_select<T, false>), grid, block, 0, st, s);
 }
 
 }  // namespace

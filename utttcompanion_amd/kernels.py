@@ -11,6 +11,7 @@ reference's PyTorch path).
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 from typing import Optional, Sequence, Tuple
 
@@ -1474,6 +1475,11 @@ def _per_request(t: Tensor, n: int, dtype: torch.dtype, name: str) -> int:
     return t.data_ptr()
 
 
+@functools.lru_cache(maxsize=256)
+def _tree_workspace(*sizes: int) -> int:
+    return N.load_library().uttt_swa_tree_workspace(*sizes)
+
+
 def _tree_call(q: Tensor, k_new: Tensor, v_new: Tensor, k_ring: Tensor, v_ring: Tensor, positions: Tensor,
                parents: Optional[Tensor], cos: Optional[Tensor], sin: Optional[Tensor], sinks: int,
                counts: Optional[Tensor], out: Optional[Tensor], workspace: Optional[Tensor], write_ring: bool,
@@ -1546,7 +1552,7 @@ def _tree_call(q: Tensor, k_new: Tensor, v_new: Tensor, k_ring: Tensor, v_ring: 
     k_new, *k_at = _heads(k_new, mask)
     v_new, *v_at = _heads(v_new, mask)
     lib = N.load_library()
-    nbytes = lib.uttt_swa_tree_workspace(n, heads, hkv, nodes, hd, slots, code)
+    nbytes = _tree_workspace(n, heads, hkv, nodes, hd, slots, code)
     p_ws = 0
     if workspace is not None:
         if workspace.numel() * workspace.element_size() < nbytes:
