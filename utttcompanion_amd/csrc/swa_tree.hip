@@ -887,14 +887,30 @@ __global__ void __launch_bounds__(kThreads) k_swa_tree_join(const TreeArgs a) {
   for (int j = 0; j < 4; ++j) og[j] = from_f32<T>(num[j] * inv);
 }
 
+// the largest of 16 lanes, in all of them, through DPP rotations
+__device__ __forceinline__ float row_max(float v) {
+  auto turned = [](float x, auto by) __attribute__((always_inline)) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x120 + decltype(by)::value, 0xF, 0xF, false));
+  };
+  v = fmaxf(v, turned(v, std::integral_constant<int, 8>{}));
+  v = fmaxf(v, turned(v, std::integral_constant<int, 4>{}));
+  v = fmaxf(v, turned(v, std::integral_constant<int, 2>{}));
+  return fmaxf(v, turned(v, std::integral_constant<int, 1>{}));
+}
+
 // fp32 operands: the same walk with v_mfma_f32_16x16x4f32 and operands straight from memory into registers, for
 // research and parity runs.  A workgroup takes 16 rows; its waves take 16 keys each of a 64-key tile and meet at the
 // end.  A lane's float4 along a row serves four k steps (dims 16 j + 4 g + i for lane group g, step i), and
 // the weights pass through LDS from the scores' layout (a lane: four queries, one key) to the A operand's
-// (one query, four keys).
+// (one query, four keys).  Few requests are bound by the tiles' latency, so a tile's loads are issued at once and
+// without branches, for head_dim 64 (where registers allow it beside two waves of a SIMD) the keys a tile ahead, and
+// tiles that every row sees whole skip all masks: one request over 512 slots 34 -> 16 us, 32 over 4096 of head_dim
+// 128 227 -> 91 us (5.0 TB/s), 16 trees of 64 nodes over as many 743 -> 440 us (66 TFLOP/s, the 16 rows of a
+// workgroup use each key for 16 products only).
 template <int HD>
-__global__ void __launch_bounds__(kThreads) k_swa_tree_f32(const TreeArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) k_swa_tree_f32(const TreeArgs a) {
   constexpr int NJ = HD / 16, LK = HD + 4, RED = HD + 4;
+  constexpr bool AHEAD = HD == 64;
   __shared__ __align__(16) float kt[64 * LK];  // the new keys, rotated; at the end the waves' results
   __shared__ __align__(16) float ps[kWaves][16][20];
   __shared__ float red_ml[kWaves][16][2];
@@ -937,41 +953,33 @@ __global__ void __launch_bounds__(kThreads) k_swa_tree_f32(const TreeArgs a) {
       }
     }
   }
-  // scores' layout: this lane's rows 4 g + i
-  int lim[4];
-  uint64_t sees[4];
+  // scores' layout: the nodes of this lane's rows 4 g + i, a byte each
+  uint32_t of_rows = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int t = min(row0 + 4 * g + i, row1 - 1) / a.rep;
-    lim[i] = visible_age(a, ring, __shfl(tree.depth, t, 64));
-    sees[i] = shfl64(tree.sees, t);
-  }
+  for (int i = 0; i < 4; ++i) of_rows |= (uint32_t)(min(row0 + 4 * g + i, row1 - 1) / a.rep) << (8 * i);
   const int lim_any = visible_age(a, ring, 0), lim_all = visible_age(a, ring, tree.deepest);
   const float* kn = static_cast<const float*>(a.k) + p.n * a.k_n + p.kvh * a.k_h;
   const float* vn = static_cast<const float*>(a.v) + p.n * a.v_n + p.kvh * a.v_h;
   if (first) {
     const bool keep = p.group == 0 && (a.write_ring || a.k_nodes != nullptr);
-    for (int idx = threadIdx.x; idx < 64 * HD / 2; idx += kThreads) {
-      const int t = idx / (HD / 2), e = idx % (HD / 2);  // a wave stays within one or two nodes
+    for (int base = 0; base < count * (HD / 2); base += kThreads) {  // scores with rows past the nodes are masked
+      const int idx = base + threadIdx.x, t = idx / (HD / 2), e = idx % (HD / 2);  // a wave stays within one or two nodes
       const int d = __shfl(tree.depth, t, 64);
-      float lo = 0.f, hi = 0.f;
-      if (t < count) {
-        lo = kn[t * a.k_t + e];
-        hi = kn[t * a.k_t + HD / 2 + e];
-        if (turned) {
-          const float ce = a.cos_table[(pos + d) * HD + e], se = a.sin_table[(pos + d) * HD + e];
-          const float x = lo, y = hi;
-          lo = x * ce - y * se;
-          hi = y * ce + x * se;
-        }
-        if (keep) {
-          float* to = node_row<float, HD>(a, p, a.k_nodes, a.k_ring, t, pos);
-          to[e] = lo;
-          to[HD / 2 + e] = hi;
-          to = node_row<float, HD>(a, p, a.v_nodes, a.v_ring, t, pos);
-          to[e] = vn[t * a.v_t + e];
-          to[HD / 2 + e] = vn[t * a.v_t + HD / 2 + e];
-        }
+      if (t >= count) continue;
+      float lo = kn[t * a.k_t + e], hi = kn[t * a.k_t + HD / 2 + e];
+      if (turned) {
+        const float ce = a.cos_table[(pos + d) * HD + e], se = a.sin_table[(pos + d) * HD + e];
+        const float x = lo, y = hi;
+        lo = x * ce - y * se;
+        hi = y * ce + x * se;
+      }
+      if (keep) {
+        float* to = node_row<float, HD>(a, p, a.k_nodes, a.k_ring, t, pos);
+        to[e] = lo;
+        to[HD / 2 + e] = hi;
+        to = node_row<float, HD>(a, p, a.v_nodes, a.v_ring, t, pos);
+        to[e] = vn[t * a.v_t + e];
+        to[HD / 2 + e] = vn[t * a.v_t + HD / 2 + e];
       }
       kt[t * LK + e] = lo;
       kt[t * LK + HD / 2 + e] = hi;
@@ -991,48 +999,62 @@ __global__ void __launch_bounds__(kThreads) k_swa_tree_f32(const TreeArgs a) {
 #pragma unroll
   for (int j = 0; j < NJ; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  for (int tile = first ? t_begin - 1 : t_begin; tile < t_end; ++tile) {
+  // A tile's keys, dims 16 j + 4 g + i of key c, come a tile ahead, its values, dims 16 j + c of keys 4 g + i, while its
+  // scores are formed: every load is made, from a slot that exists, and what no row sees is left out behind it.
+  const Edge edge = read_edge(a, ring, lim_all);
+  f32x4 k_next[NJ];
+  auto fetch_keys = [&](int tile) __attribute__((always_inline)) {
+    if (tile < t_begin) return;
+    const float* row = kr + (int64_t)min(tile * 64 + 16 * w + c, a.slots - 1) * HD + 4 * g;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) k_next[j] = *reinterpret_cast<const f32x4*>(row + 16 * j);
+  };
+  const int t_first = first ? t_begin - 1 : t_begin;
+  if (AHEAD) fetch_keys(t_first);
+  for (int tile = t_first; tile < t_end; ++tile) {
     const bool is_tree = tile < t_begin;
     const int s0 = is_tree ? 16 * w : tile * 64 + 16 * w;  // this wave's 16 keys
-    // which of them some row sees, and all
-    const uint32_t any = (uint32_t)(is_tree ? bit_range(0, count - s0) : seen_slots(a, ring, s0, lim_any)) & 0xffffu;
-    const uint32_t all = is_tree ? 0u : (uint32_t)seen_slots(a, ring, s0, lim_all) & 0xffffu;
-    if (any == 0) continue;
-    const bool any_c = (any >> c) & 1;
-    f32x4 s{0.f, 0.f, 0.f, 0.f};
+    if (!AHEAD) fetch_keys(tile);
+    f32x4 k[NJ], v[NJ];
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      f32x4 k{0.f, 0.f, 0.f, 0.f};
-      if (is_tree)
-        k = *reinterpret_cast<const f32x4*>(kt + (s0 + c) * LK + 16 * j + 4 * g);
-      else if (any_c)
-        k = *reinterpret_cast<const f32x4*>(kr + (int64_t)(s0 + c) * HD + 16 * j + 4 * g);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s = __builtin_amdgcn_mfma_f32_16x16x4f32(q[j][i], k[i], s, 0, 0, 0);
+    for (int j = 0; j < NJ; ++j) k[j] = k_next[j];
+    const bool clean = !is_tree && clean_tile(a, edge, tile * 64);
+    uint32_t any = 0xffffu, all = 0xffffu;  // which of the keys some row sees, and all
+    if (!clean) {
+      any = (uint32_t)(is_tree ? bit_range(0, count - s0) : seen_slots(a, ring, s0, lim_any)) & 0xffffu;
+      all = is_tree ? 0u : (uint32_t)seen_slots(a, ring, s0, lim_all) & 0xffffu;
     }
-    // values: keys 4 g + i, dims 16 j + c
-    f32x4 v[NJ];
-    bool odd = false;
+    if (any == 0) {
+      if (AHEAD && tile + 1 < t_end) fetch_keys(tile + 1);
+      continue;
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int key = s0 + 4 * g + i;
-      const bool ok = (any >> (4 * g + i)) & 1, part = !((all >> (4 * g + i)) & 1);
-      const float* row = is_tree ? vn + key * a.v_t : vr + (int64_t)key * HD;
+      const float* row = is_tree ? vn + min(key, count - 1) * a.v_t : vr + (int64_t)min(key, a.slots - 1) * HD;
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        v[j][i] = ok ? row[16 * j + c] : 0.f;
-        odd |= part && !(fabsf(v[j][i]) < INFINITY);
-      }
+      for (int j = 0; j < NJ; ++j) v[j][i] = row[16 * j + c];
     }
-    odd = __any(odd);
+    if (AHEAD && tile + 1 < t_end) fetch_keys(tile + 1);
+    if (is_tree) {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) k[j] = *reinterpret_cast<const f32x4*>(kt + (s0 + c) * LK + 16 * j + 4 * g);
+    }
+    f32x4 s{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s = __builtin_amdgcn_mfma_f32_16x16x4f32(q[j][i], k[j][i], s, 0, 0, 0);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const bool vis = ((is_tree ? sees[i] >> s0 : seen_slots(a, ring, s0, lim[i])) >> c) & 1;
-      s[i] = vis ? s[i] : -INFINITY;
-      float mx = s[i];
-#pragma unroll
-      for (int off = 1; off < 16; off <<= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
-      const float m_new = fmaxf(m[i], mx);
+      if (!clean) {
+        const int t = (of_rows >> (8 * i)) & 63;
+        const uint64_t seen =
+            is_tree ? shfl64(tree.sees, t) >> s0 : seen_slots(a, ring, s0, visible_age(a, ring, __shfl(tree.depth, t, 64)));
+        const bool vis = (seen >> c) & 1;
+        s[i] = vis ? s[i] : -INFINITY;
+      }
+      const float m_new = fmaxf(m[i], row_max(s[i]));
       const float corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m[i] - m_new) * c2);
       m[i] = m_new;
       const float x = s[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((s[i] - m_new) * c2);
@@ -1040,6 +1062,19 @@ __global__ void __launch_bounds__(kThreads) k_swa_tree_f32(const TreeArgs a) {
 #pragma unroll
       for (int j = 0; j < NJ; ++j) o[j][i] *= corr;
       ps[w][4 * g + i][c] = x;
+    }
+    bool odd = false;
+    if (!clean) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool ok = (any >> (4 * g + i)) & 1, part = !((all >> (4 * g + i)) & 1);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          v[j][i] = ok ? v[j][i] : 0.f;
+          odd |= part && !(fabsf(v[j][i]) < INFINITY);
+        }
+      }
+      odd = __any(odd);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_wave_barrier();
@@ -1119,7 +1154,14 @@ TreePlan plan_tree(int64_t n_req, int64_t n_heads, int64_t n_kv_heads, int64_t n
   const int64_t per = b16 ? 32 * p.units : 16;
   p.groups = (int)((rows + per - 1) / per);
   const int64_t base = lists * p.groups;
-  const int64_t want = head_dim == 64 ? 512 : 256, least = 8;  // workgroups, tiles of a split
+  // As many splits as bring the launch to `want` workgroups, of at least `least` tiles each.  A split costs its part of
+  // the second launch, a tile its latency, so the slower walks (fp32, head_dim 128) take shorter splits.  Measured, us:
+  //   want of half / this / twice: 32 decoding requests over 4096 slots of head_dim 128, bf16 49.2 / 47.1 / 50.7; 16 trees of
+  //     64 nodes over as many 97.5 / 76.9 / 92.0
+  //   least of 4 / 8: fp32, one request over 512 slots 16.0 / 20.8, 3 over 761 of head_dim 128 22.2 / 35.4; bf16 of
+  //     head_dim 128, 3 over 761 16.8 / 19.9, one tree of 8 nodes over 1024 19.3 / 20.5, one request over 4096 22.4 / 21.1;
+  //     bf16 of head_dim 64, one request over 512 12.2 / 11.6, 5 trees of 38 nodes over 697 15.4 / 11.9
+  const int64_t want = head_dim == 64 ? 512 : 256, least = b16 && head_dim == 64 ? 8 : 4;
   p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({(want + base - 1) / base, tiles / least, (int64_t)kMaxTreeSplits}));
   return p;
 }
