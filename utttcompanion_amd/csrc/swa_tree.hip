@@ -1150,19 +1150,24 @@ TreePlan plan_tree(int64_t n_req, int64_t n_heads, int64_t n_kv_heads, int64_t n
   TreePlan p;
   const int64_t rows = n_heads / n_kv_heads * nodes, lists = n_req * n_kv_heads, tiles = (slots + 63) / 64;
   p.units = b16 ? 1 : 0;
-  if (b16 && rows > 128 && lists * ((rows + 31) / 32) >= 256) p.units = kWideWaves;
+  // Many rows of many lists share their tiles (16 trees of 64 nodes over 4096 slots of head_dim 128: 109 us apart, 75 shared;
+  // of 40 nodes 99, 67; 8 trees of 64 57, 55; below, units alone: 4 trees of 64 41 apart, 50 shared, 16 of 24 56, 61; a unit of
+  // head_dim 64 has half the work for a barrier: 16 of 64 43 apart, 63 shared)
+  if (b16 && head_dim == 128 && rows > 128 && lists * ((rows + 31) / 32) >= 256) p.units = kWideWaves;
   const int64_t per = b16 ? 32 * p.units : 16;
   p.groups = (int)((rows + per - 1) / per);
   const int64_t base = lists * p.groups;
-  // As many splits as bring the launch to `want` workgroups, of at least `least` tiles each.  A split costs its part of
-  // the second launch, a tile its latency, so the slower walks (fp32, head_dim 128) take shorter splits.  Measured, us:
-  //   want of half / this / twice: 32 decoding requests over 4096 slots of head_dim 128, bf16 49.2 / 47.1 / 50.7; 16 trees of
-  //     64 nodes over as many 97.5 / 76.9 / 92.0
+  // Splits that fill the card's `want` places for workgroups once, of at least `least` tiles each: a split costs its part of
+  // the second launch, and a second round of workgroups as much as the first.  A tile of the slower walks (fp32,
+  // head_dim 128) is worth a shorter split.  Measured, us:
+  //   want of half / this / twice: 32 decoding requests over 4096 slots of head_dim 128, bf16 49.2 / 47.1 / 50.7; 16 trees
+  //     of 64 nodes over as many 97.5 / 76.9 / 92.0
+  //   192 workgroups of head_dim 128 left whole / in two (16 trees of 24 nodes): 55 / 69
   //   least of 4 / 8: fp32, one request over 512 slots 16.0 / 20.8, 3 over 761 of head_dim 128 22.2 / 35.4; bf16 of
   //     head_dim 128, 3 over 761 16.8 / 19.9, one tree of 8 nodes over 1024 19.3 / 20.5, one request over 4096 22.4 / 21.1;
   //     bf16 of head_dim 64, one request over 512 12.2 / 11.6, 5 trees of 38 nodes over 697 15.4 / 11.9
   const int64_t want = head_dim == 64 ? 512 : 256, least = b16 && head_dim == 64 ? 8 : 4;
-  p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({(want + base - 1) / base, tiles / least, (int64_t)kMaxTreeSplits}));
+  p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({want / base, tiles / least, (int64_t)kMaxTreeSplits}));
   return p;
 }
 
@@ -1174,7 +1179,7 @@ void launch_tree(const TreeArgs& m, const TreePlan& p, bool b16, hipStream_t st)
     hipLaunchKernelGGL(k_swa_tree_f32<HD>, grid, dim3(kThreads), 0, st, m);
   else if (p.units == 1)
     hipLaunchKernelGGL(k_swa_tree_mm<HD>, grid, dim3(kThreads), 0, st, m);
-  else
+  else if constexpr (HD == 128)
     hipLaunchKernelGGL(k_swa_tree_wide<HD>, grid, dim3(kWideWaves * 64), 0, st, m);
   if (m.nsplit > 1) {
     const int64_t n = (int64_t)m.n_req * m.n_kv_heads * m.rows * (HD / 4);
