@@ -71,7 +71,7 @@ def test_commit_node_ids_out_of_range_and_strided_operands():
 
 @pytest.mark.parametrize("dtype", BOTH)
 @pytest.mark.parametrize("layers,n,hkv,hd,slots", [(1, 1, 1, 64, 5), (2, 3, 2, 64, 20), (3, 5, 1, 128, 33), (2, 16, 4, 64, 68),
-                                                   (1, 17, 2, 8, 9), (2, 64, 1, 64, 12), (1, 65, 2, 64, 11), (1, 128, 1, 64, 7)])
+                                                   (1, 17, 2, 8, 9), (2, 32, 1, 64, 12), (1, 33, 2, 64, 9), (2, 64, 1, 64, 12), (1, 65, 2, 64, 11), (1, 128, 1, 64, 7)])
 def test_fork_any_map(layers, n, hkv, hd, slots, dtype):
     from utttcompanion_amd import kernels as K
     g = torch.Generator().manual_seed(n)

@@ -26,7 +26,9 @@ struct CommitArgs {
 };
 
 // One 16-byte piece of a key and of the value beside it per thread, a node's row of a head in consecutive
-// threads; grid (pieces of all layers and path steps, requests).
+// threads, all layers in one launch: bound by the bytes where there are many (24 layers, 32 requests, paths of up to
+// 64 nodes of 4 heads x 128 bf16 21 us, 4.7 TB/s), by the launch where there are few (2.3 us).
+// Grid (pieces of all layers and path steps, requests).
 __global__ void __launch_bounds__(kThreads) k_kv_commit(const CommitArgs a) {
   const int n = blockIdx.y;
   const int64_t pos = a.positions[n];
@@ -68,8 +70,9 @@ struct ForkArgs {
 };
 
 // A thread owns one piece of a slab, in every request: it loads the pieces of all requests that move
-// before it stores any, and no other thread touches them, so any map of sources is safe in place.
-// grid (pieces of a slab, 2 x layers).
+// before it stores any, and no other thread touches them, so any map of sources is safe in place, without scratch
+// memory.  Bound by the bytes: 16 requests of 24 layers of 4 heads x 1028 slots x 128 bf16 exchanged at random take FORKUS
+// us, FORKTB TB/s read and written.  grid (pieces of a slab, 2 x layers).
 template <typename V, int N>
 __global__ void __launch_bounds__(kThreads) k_kv_fork(const ForkArgs a) {
   const int64_t c = (int64_t)blockIdx.x * kThreads + threadIdx.x;
@@ -177,8 +180,11 @@ extern "C" int uttt_kv_fork(const uttt_kv_fork_args* a, uttt_stream_t stream) {
   UTTT_REQUIRE((double)a->n_kv_heads * (double)a->slots * (double)a->head_dim < (double)(1LL << 60) &&
                    slabs_apart(a->layers, a->ring_stride_l, a->n_req, a->ring_stride_n, a->n_kv_heads * a->slots * a->head_dim),
                "the requests' rings must not overlap");
-  // 16-byte pieces while 64 requests' pieces fit a thread's registers, 8-byte ones beyond
-  const int64_t piece = a->n_req <= 64 ? 16 : 8, per = piece / size;
+  // A thread holds a piece of every request, so the kernel for more requests has more registers and fewer waves, and pieces
+  // shrink so that 128 of them fit.  12 layers of 4 heads x 516 slots x 64 bf16, us, the kernel of its size and the next
+  // larger: 16 requests 18 and 57 (of 64), 32 requests 55 and 89, 64 requests with pieces of 8 bytes 189 and of 16 191,
+  // 128 with 4 bytes 540 and with 8 602 (one for up to 4 requests gave 8.8 for 9.0 and is not kept).
+  const int64_t piece = a->n_req <= 32 ? 16 : a->n_req <= 64 ? 8 : 4, per = piece / size;
   ForkArgs m{};
   m.n_req = (int)a->n_req; m.row_pieces = (int)(a->head_dim / per);
   m.slots = a->slots; m.slab = a->n_kv_heads * a->slots * m.row_pieces;
@@ -190,14 +196,14 @@ extern "C" int uttt_kv_fork(const uttt_kv_fork_args* a, uttt_stream_t stream) {
   UTTT_REQUIRE(blocks <= 0x7fffffffLL, "slabs too large for one launch");
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)blocks, (unsigned)(2 * a->layers));
-  if (a->n_req <= 4)
-    hipLaunchKernelGGL((k_kv_fork<u32x4, 4>), grid, dim3(kThreads), 0, st, m);
-  else if (a->n_req <= 16)
+  if (a->n_req <= 16)
     hipLaunchKernelGGL((k_kv_fork<u32x4, 16>), grid, dim3(kThreads), 0, st, m);
+  else if (a->n_req <= 32)
+    hipLaunchKernelGGL((k_kv_fork<u32x4, 32>), grid, dim3(kThreads), 0, st, m);
   else if (a->n_req <= 64)
-    hipLaunchKernelGGL((k_kv_fork<u32x4, 64>), grid, dim3(kThreads), 0, st, m);
+    hipLaunchKernelGGL((k_kv_fork<u32x2, 64>), grid, dim3(kThreads), 0, st, m);
   else
-    hipLaunchKernelGGL((k_kv_fork<u32x2, 128>), grid, dim3(kThreads), 0, st, m);
+    hipLaunchKernelGGL((k_kv_fork<uint32_t, 128>), grid, dim3(kThreads), 0, st, m);
   hipLaunchKernelGGL(k_kv_fork_positions, dim3(1), dim3(kMaxFork), 0, st, a->positions, a->sources, (int)a->n_req);
   return launch_status("uttt_kv_fork");
 }
