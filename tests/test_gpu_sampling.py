@@ -22,7 +22,8 @@ def check(x, u, t, k=None, p=None, m=None, banned=(), limit=None, sure=True):
     """Tokens equal the definition's and log-probabilities are within their rounding.  Weights are whole units of
     2^-42 of the largest one and off by half a unit and by 2^-42 of themselves, so mass sums over V ids are within
     V 2^-41 largest weights of exact: a u * total nearer than that to a border could take either side (``sure``:
-    none is)."""
+    none is).  top_p's bound is a share of the whole mass, to which ids more than 16 factors of two down add by fp32
+    exponentials, within 2^-36 of the largest weight each: no case here has its cut that near another id."""
     tok, lp = call(x, u, t, k, p, m, banned=banned, active_limit=limit)
     tok, lp, cpu = tok.cpu(), lp.cpu(), x.float().cpu()
     vocab = x.shape[1]
@@ -141,6 +142,20 @@ def test_few_and_many_ids_are_kept(vocab, dtype):
         u = uniforms(n, 100 + seed)
         check(x, u, [0.9] * n, k, p)
         check(x, u, [1.0] * n, k, p, [0.001] * n)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [4001, 70001])
+def test_cuts_far_below_the_top(vocab, dtype):
+    """A top_k among ids that weigh next to nothing, or nothing (more than 43 factors of two down), and a top_p near 1 of
+    a row with one id far above the others, which hold most of the mass."""
+    g = torch.Generator().manual_seed(vocab)
+    x = (3 * torch.randn((5, vocab), generator=g)).to(dtype)
+    x[2:, 17] = 30.0
+    x = x.to(DEV)
+    t = [0.3, 0.12, 2.5, 2.8, 3.0]
+    for k, p in (([200, 900, 0, 0, 3000], None), ([200, 900, 0, 40, 3000], [0.7, 0.9, 0.995, 0.9999, 0.98]), (None, [0.9999, 0.5, 0.9, 0.99, 0.6])):
+        check(x, uniforms(5, 31), t, k, p)
 
 
 @pytest.mark.parametrize("temperature", [2e-5, 1e-3, 50.0, 1e4, math.inf])

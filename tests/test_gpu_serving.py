@@ -244,6 +244,37 @@ def test_speculated_tokens_equal_single_steps(sinks, nodes):
             assert t == truth[i][len(have[i]) - 1]
 
 
+def test_of_equal_siblings_the_longer_way_is_taken():
+    """Two drafts that begin alike, the first of them ending at once."""
+    model, states, prompts = make()
+    plain, first = decoder(model, states, prompts)
+    truth = plain.generate_greedy(first, 6).tolist()
+    dec, _ = decoder(model, states, prompts)
+    tokens = torch.tensor([[t[0], t[1], t[1], t[2], t[3]] for t in truth])
+    new = dec.speculate_greedy(tokens, torch.tensor([[-1, 0, 0, 2, 3]] * 4))
+    assert new == [t[1:5] for t in truth]
+    assert dec.host_positions == [len(p) + 4 for p in prompts]
+
+
+@pytest.mark.parametrize("chunk", [16, 80])
+def test_ragged_writes_with_sinks_equal_single_ones(chunk):
+    """Requests of several lengths in one chunk loop against each alone, through the layer chain and, for chunks past
+    64 tokens, one update per layer (the bound of the same comparison without sinks)."""
+    from utttcompanion_amd import uTTTConfig, uTTTModel
+    torch.manual_seed(0)
+    model = uTTTModel(uTTTConfig(**dict(BASE, chunk_size=chunk), attention_sinks=5)).eval().to(DEV)
+    g = torch.Generator().manual_seed(1)
+    turns = [torch.randint(6, 256, (n,), generator=g) for n in (200, 33, 90)]
+    one = lambda: model.init_fast_state(1, device=DEV, dtype=torch.float32, detach=True)
+    together = model.test_time_update_batched(turns, [one() for _ in turns])
+    for ids, (state, surprise, _) in zip(turns, together):
+        want, want_surprise, _ = model.test_time_update(ids.view(1, -1).to(DEV), one())
+        assert abs(surprise - want_surprise) <= 1e-5 * max(1.0, abs(want_surprise))
+        for name in ("w_up", "w_gate", "w_down", "s_up", "s_gate", "s_down"):
+            a, b = getattr(state, name).double(), getattr(want, name).double()
+            assert float((a - b).norm()) <= 1e-5 * float(b.norm()), name
+
+
 def test_verified_logits_equal_steps_and_leave_the_requests_alone():
     model, states, prompts = make(5, torch.bfloat16, slow_std=0.02)
     dec, first = decoder(model, states, prompts)
@@ -277,7 +308,12 @@ def test_forked_requests_go_on_as_their_source():
         assert torch.equal(dec.k_rings[:, i, :, :used], rings[:, s, :, :used])
     assert torch.equal(dec.logits, logits[src])
     assert torch.equal(dec.generate_greedy(dec.logits, 10), want[src])
-    assert dec.matches(model, [states[s] for s in src])
+    dec.set_sampling(1.0)
+    dec.generate_sampled(dec.logits, 2)
+    chosen, weighed = dec.tokens.clone(), dec.logprobs.clone()
+    dec.fork([0, 0, 3, 2])
+    assert torch.equal(dec.tokens, chosen[[0, 0, 3, 2]]) and torch.equal(dec.logprobs, weighed[[0, 0, 3, 2]])
+    assert dec.matches(model, [states[src[s]] for s in (0, 0, 3, 2)])
 
 
 def test_decoder_refusals():

@@ -5,15 +5,21 @@
 // descending, id ascending), so the kept set is a cut (key, ties): the ids whose logit lies above the key's,
 // and the first `ties` of those at it.  Passes over the row, one workgroup each:
 //   1. the largest logit (rows that fit are kept in LDS for the passes behind);
-//   2. the ids within 16 factors of two of the top, listed per stretch of the row (16, one per wave) so that their weights
-//      are formed with all lanes busy; their histogram of counts and masses over x (bins of 1/128 of a factor
-//      of two), and the whole mass.  When the cut lies further down, again over everything, with bins of 1/48;
+//   2. the ids within 16 factors of two of the top (up to 24 where the row is flat), listed per stretch of the row (16, one
+//      per wave) so that their weights are formed with all lanes busy; their histogram of counts and masses over x (2048
+//      bins), and the whole mass.  When the cut lies further down, again over all ids whose weight is not 0;
 //   3. the bin in which the count or the mass passes its bound: the stretches' masses ahead of it from the lists (where one
 //      overflowed, from the row), and its ids, which are ranked against each other.  When they are many (equal or
 //      nearly equal logits), the bin's range of keys is divided further first;
 //   4. a scan of the list of the stretch that holds the chosen id, inside one wave.
 // Without a cut 3 is a pass that weighs the whole row; without a list of the stretch (no cut, or many ids kept) 4 weighs
 // 16 parts of it first.
+//
+// Bound by the arithmetic of the weights: some 32 instructions an id, 0.85 us a pass over 131072 of them on the one compute
+// unit that has a row, beside 20 us to read it.  One row of 32000 bf16 takes 15.6 us (2.8 for pass 1, 6 for pass 2, 3 for
+// 3), 256 rows of 131072 fp32 with mixed settings 152 us, the flattest of them (temperature 1.5, top_p near 1) last:
+// a row of temperature 0.7 is done after 50.  Finding the cut's bin from counts alone, to weigh each id once, was slower
+// (199 us): it has to weigh every id with a bin again, not only those that may be kept.
 //
 // The sums decide between neighbouring ids, so weights are formed in 64 bits and added as integers in units of
 // 2^-42 of the largest weight: exact whatever the order, so atomics in any order give equal bits.  (fp64 and
@@ -49,8 +55,11 @@ struct SampleArgs {
 constexpr int kSmpThreads = 1024, kSmpWaves = kSmpThreads / 64;
 constexpr int kBins = 2 * kSmpThreads;  // two per thread in the scan
 constexpr int kList = kSmpThreads;  // ids that are ranked against each other, one per thread
-constexpr int kDense = 24;  // ids of each 64: from so many on they are weighed in place
-constexpr int kStageBytes = 60 * 1024;  // rows up to this size stay in LDS
+// Ids of each 64: from so many on they are weighed in place.  From 8, 24, 48 on: 256 x 131072 152, 149, 148 us, 64 x 50000
+// 53.0, 52.5, 53.8.
+constexpr int kDense = 24;
+// Rows up to this size stay in LDS.  Staged and not: 1 x 32000 15.9 and 16.2 us, 64 x 32000 mixed 28.8 and 30.1.
+constexpr int kStageBytes = 60 * 1024;
 constexpr int kKeptStaged = 256, kKept = 512;
 
 // order-preserving key of a logit that is not NaN; -0 and +0 are equal
@@ -133,7 +142,7 @@ struct Shared {
   int kept_n[kSmpWaves];  // -1: the list holds only the last of them
   u64 wave_mass[kSmpWaves], scan_mass[kSmpWaves];
   uint32_t wave_count[kSmpWaves], scan_count[kSmpWaves];
-  float wave_best[kSmpWaves];
+  float wave_best[kSmpWaves], wave_sum[kSmpWaves];
   uint32_t list_key[kList];
   int list_id[kList];
   u64 list_mass[kList];
@@ -194,7 +203,7 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
   __shared__ Shared<KEPT> s;
   __shared__ __align__(16) T stage[STAGED ? kStageBytes / sizeof(T) : 1];
   constexpr int W = STAGED ? 8 / (int)sizeof(T) : VEC > 4 ? 4 : VEC;  // ids to a lane in the passes behind the first
-  constexpr float kFine = 128.f, kCoarse = 48.f;  // bins to a factor of two: kBins / 48 > 42, what weights reach
+  constexpr float kFarthest = 43.5f;  // factors of two below the top from where on weights are 0 units, half of 2^-42 not reached
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   // Places count from the 16-byte boundary at or before the row's first id, so that rows of any alignment are read in
   // whole 16-byte pieces (256 rows of 131071 fp32 at temperature 0.7: one id at
@@ -218,13 +227,14 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
   };
 
   // ---- the largest logit; NaN makes it NaN
-  float top = -INFINITY;
+  float top = -INFINITY, mean = 0.f;
   bool nan = false;
   scan_ids<T, VEC, 4, true>(a, x, off, lo, hi, lane, [&](const float(&v)[VEC], int i) __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       top = fmaxf(top, v[e]);
       nan |= v[e] != v[e];
+      mean += v[e] > -INFINITY ? v[e] : 0.f;
     }
     if constexpr (STAGED) {
       typedef T vec_t __attribute__((ext_vector_type(VEC)));
@@ -235,9 +245,15 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
     }
   });
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+  for (int off = 32; off > 0; off >>= 1) {
+    top = fmaxf(top, __shfl_xor(top, off, 64));
+    mean += __shfl_xor(mean, off, 64);
+  }
   if (__any(nan)) top = NAN;
-  if (lane == 0) s.wave_best[w] = top;
+  if (lane == 0) {
+    s.wave_best[w] = top;
+    s.wave_sum[w] = mean;
+  }
   for (int i = tid; i < kBins; i += kSmpThreads) {
     s.mass[i] = 0;
     s.count[i] = 0;
@@ -245,12 +261,14 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
   if (tid == 0) s.best = 0x7fffffff;
   __syncthreads();
   top = -INFINITY;
+  mean = 0.f;
   nan = false;
 #pragma unroll 4
   for (int q = 0; q < kSmpWaves; ++q) {
     const float v = s.wave_best[q];
     nan |= v != v;
     top = fmaxf(top, v);
+    mean += s.wave_sum[q];
   }
   const bool greedy = !(temp > 1e-5f);
   if (greedy || nan || !(fabsf(top) < INFINITY)) {  // the lowest id of the largest value (NaN above all)
@@ -278,10 +296,15 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
     if (least > 1) u = u >= least ? u : 0;
     return u;
   };
-  float per_unit = fminf((float)c * kFine, 3e38f);  // bins to a unit of the logits
-  float last = (float)kBins;                        // ids in bins from here on are not counted, or with ...
-  bool clamp = false;                               // ... clamp put into the last bin
-  auto place = [&](float v) __attribute__((always_inline)) { return clamp && v > -INFINITY ? fminf((top - v) * per_unit, last) : (top - v) * per_unit; };
+  // The bins of the first round reach 16 factors of two down, in which a cut lies that most of the mass is ahead of; where
+  // the row's mean is that near, so that much of the mass is around it, 4 past the mean; and 2/5 of the way to the mean
+  // for top_k, whose ids may weigh next to nothing.  Reaching 16 always, rows whose cut lay further down took both
+  // rounds, and the slowest of 256 x 131072 mixed ones 226 to 271 us, for 133 to 162 so.
+  const float to_mean = (top - mean / (float)a.limit) * (float)c;
+  float reach = to_mean < 20.f ? fmaxf(16.f, to_mean + 4.f) : 16.f;
+  if (by_count && to_mean > 40.f) reach = fminf(0.4f * to_mean, kFarthest);
+  float per_unit = fminf((float)c * ((float)kBins / reach), 3e38f);  // bins to a unit of the logits
+  auto place = [&](float v) __attribute__((always_inline)) { return (top - v) * per_unit; };
 
   Cut cut{0, 0x7fffffff, 0};  // keeps everything
   bool masses = false;        // the stretches' masses up to the cut are known
@@ -356,7 +379,7 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
     };
     // counts and masses of the bins, and the whole mass.  Ids further down add to the whole mass alone, by fp32
     // exponentials: their errors (2^-23 of each, and random) are far below what a kept id weighs.
-    auto histogram = [&]() __attribute__((always_inline)) {
+    auto histogram = [&](bool far) __attribute__((always_inline)) {
       u64 sum = 0;
       float tail = 0.f;
       const float cf = (float)c;
@@ -384,7 +407,7 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
           in[e] = place(v[e]) < (float)kBins;
           all &= in[e];
         }
-        if (by_mass && !all) {
+        if (by_mass && !far && !all) {
 #pragma unroll
           for (int e = 0; e < W; ++e) {
             const float x = __builtin_amdgcn_exp2f((v[e] - top) * cf);
@@ -607,7 +630,7 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
     };
 #pragma unroll 1
     for (int round = 0; round < 2; ++round) {
-      histogram();
+      histogram(round == 1);
       u64 bound = (u64)((double)fmaxf(top_p, 0.f) * (double)whole);  // top_p of the row's mass
       bool found = true;
       if (by_count) {
@@ -616,7 +639,7 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
           cut = resolve(bin, true, (u64)top_k, !by_mass);
           bound = (u64)((double)fmaxf(top_p, 0.f) * (double)cut.mass);  // or of what top_k keeps
         } else {
-          found = false;  // it lies further down, or there are fewer ids than top_k
+          found = false;  // it lies further down, or among ids of weight 0, or there are fewer ids than top_k
         }
       }
       if (by_mass && (found || round == 1)) {
@@ -631,9 +654,7 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
         }
       }
       if (found || round == 1) break;
-      per_unit = fminf((float)c * kCoarse, 3e38f);
-      last = (float)(kBins - 1);
-      clamp = true;
+      per_unit = fminf((float)c * ((float)kBins / kFarthest), 3e38f);
       __syncthreads();
       for (int i = tid; i < kBins; i += kSmpThreads) {
         s.mass[i] = 0;

@@ -461,11 +461,15 @@ class BatchedDecoder:
         drafted = tokens.tolist()
         paths = []
         for i in range(n):
-            path = [0]
+            depth, deepest = [1] + [0] * (nodes - 1), 0  # of the nodes that agree with the choices; 0: not one
             for t in range(1, held[i]):
-                if up[i][t] == path[-1] and drafted[i][t] == choice[i][path[-1]]:
-                    path.append(t)
-            paths.append(path)
+                if depth[up[i][t]] and drafted[i][t] == choice[i][up[i][t]]:
+                    depth[t] = depth[up[i][t]] + 1
+                    deepest = t if depth[t] > depth[deepest] else deepest
+            path = [deepest]
+            while path[-1] > 0:
+                path.append(up[i][path[-1]])
+            paths.append(path[::-1])
         longest = max(len(p) for p in paths)
         self.commit(torch.tensor([p + [0] * (longest - len(p)) for p in paths]), torch.tensor([len(p) for p in paths]))
         self.tokens.copy_(torch.tensor([choice[i][p[-1]] for i, p in enumerate(paths)]))
@@ -475,8 +479,8 @@ class BatchedDecoder:
     @torch.no_grad()
     def fork(self, sources: Sequence[int]) -> None:
         """Request i goes on from request sources[i], as that was before the call: its cache and
-        position (``kernels.kv_fork``, in place), the token chosen last, its logits and its fast
-        weights.  Sampling settings stay with the slot.  Buffers keep their addresses, so a
+        position (``kernels.kv_fork``, in place), the token chosen last with its log-probability, its logits
+        and its fast weights.  Sampling settings stay with the slot.  Buffers keep their addresses, so a
         captured step stays valid."""
         src = [int(s) for s in sources]
         if len(src) != self.n or min(src) < 0 or max(src) >= self.n:
@@ -484,7 +488,7 @@ class BatchedDecoder:
         self._nodes = None
         index = torch.tensor(src, dtype=torch.int32).to(self.device)
         K.kv_fork(self.k_rings, self.v_rings, index, self.positions)
-        follow = [self.tokens] if self.logits is None else [self.tokens, self.logits]
+        follow = [t for t in (self.tokens, self.logits, self.logprobs) if t is not None]
         if any(self._states[i] is not self._states[s] for i, s in enumerate(src)):
             follow += [self.w_up, self.w_gate, self.w_down]
         index = index.long()
