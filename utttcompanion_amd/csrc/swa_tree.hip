@@ -9,7 +9,9 @@
 // v_mfma_f32_32x32x16_bf16 with the scores transposed (S^T = K Q^T: a query per lane, its softmax inside
 // the lane and one exchange with the lane 32 away; the rounded weights are the B operand of O^T = V^T P^T as
 // they lie).  The new tokens' keys are one more tile, rotated by the whole workgroup into the last wave's
-// buffers.  The waves' results meet in LDS, the splits' in a second launch.
+// buffers.  The waves' results meet in LDS, the splits' in a second launch.  Long caches are bound by their bytes (32
+// requests over 4096 slots of head_dim 128, bf16: 44 us and 4 for the join, 5.1 TB/s), single requests by the chain
+// of latencies (one over 512 slots of head_dim 64: 11.4 us).
 //
 // Roundings: weights to bf16 as a MFMA operand (sums are formed from the unrounded ones); rotated
 // queries are carried as two bf16 terms, so they cost no accuracy beside the keys' own bf16; the new keys are rotated
@@ -721,7 +723,8 @@ __global__ void __launch_bounds__(kThreads, HD == 64 ? 2 : 1) k_swa_tree_mm(cons
 // at once.  (Weights alone against both products, the other cut, leaves the weights' half waiting: 3200 cycles
 // a half at head_dim 128.)  K has three slots and V four: a wave asks for tile t + 2 ahead of its scores of tile t
 // (every wave has left what those slots held), and the tile it asked for before is home by the end of that half,
-// one half before the first wave needs it.
+// one half before the first wave needs it.  16 trees of 64 nodes, 4096 slots: 67 us (435 TFLOP/s; MFMA busy for a
+// quarter of it, the softmax's vector work for as much again) and 8 for the join.
 constexpr int kWideWaves = 8;
 
 __device__ __forceinline__ void half_barrier() {
