@@ -47,7 +47,7 @@ typedef struct {
   int32_t n_banned;    /* <= 8 */
   int32_t banned[8];
   int64_t active_limit; /* < 0 or >= vocab: no limit */
-  const void* logits; int64_t row_stride;
+  const void* logits; int64_t row_stride; /* >= vocab, or 0: one row for all */
   const float* uniforms;    /* (rows,) */
   const float* temperature; /* (rows,) */
   const int32_t* top_k;     /* (rows,) or NULL: off */

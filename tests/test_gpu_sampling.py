@@ -87,6 +87,12 @@ def test_banned_ids_limit_and_strides(dtype):
     assert none.tolist() == [0] * rows and bool(lp.isnan().all())
 
 
+def test_one_row_for_several_samplers():
+    g = torch.Generator().manual_seed(8)
+    x = (3 * torch.randn((1, 4001), generator=g)).to(DEV)
+    check(x.expand(5, -1), uniforms(5, 9), [0.0, 0.5, 0.9, 1.2, 1.2], k=[0, 0, 40, 0, 7], p=[0.9] * 5)
+
+
 def test_equal_logits_share_the_mass_and_ties_go_to_the_lowest_ids():
     rows, vocab = 8, 1000
     x = torch.full((rows, vocab), -2.5, device=DEV)

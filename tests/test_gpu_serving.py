@@ -337,6 +337,9 @@ def test_decoder_refusals():
             dec.verify(tokens)
     with pytest.raises(ValueError):
         dec.speculate_greedy(i64(4, 3), torch.tensor([[-1, 0, 2]] * 4))
+    for tokens in (i64(4), i64(3, 2), i64(4, 0)):
+        with pytest.raises(ValueError):
+            dec.speculate_greedy(tokens)
     dec.verify(i64(4, 3))
     for nodes, counts in ((i64(4, 2) * 3, i64(4)), (i64(4, 2), i64(4) * 3), (i64(4, 2), -i64(4)), (i64(3, 2), i64(3))):
         with pytest.raises(ValueError):

@@ -799,7 +799,7 @@ extern "C" int uttt_sample_select(const uttt_sample_args* a, uttt_stream_t strea
   for (int k = 0; k < a->n_banned; ++k) UTTT_REQUIRE(a->banned[k] >= 0, "excluded ids must be >= 0");
   UTTT_REQUIRE(a->logits != nullptr && a->out != nullptr && a->uniforms != nullptr && a->temperature != nullptr,
                "logits, uniforms, temperature and out must be non-NULL");
-  UTTT_REQUIRE(a->row_stride >= a->vocab, "the row stride must cover vocab");
+  UTTT_REQUIRE(a->row_stride >= a->vocab || a->row_stride == 0, "the row stride must cover vocab, or be 0 for one row for all");
   SampleArgs s{};
   s.vocab = (int)a->vocab;
   for (int k = 0; k < a->n_banned; ++k) {

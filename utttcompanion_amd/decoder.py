@@ -449,6 +449,8 @@ class BatchedDecoder:
         drafted tokens taken and the greedy choice behind the last of them (the next round's
         node 0, in ``self.tokens`` too): the tokens that single steps would give, as far as the products of
         more rows at once round alike.  Trees and the choices behind them are read back."""
+        if tokens.dim() != 2 or tokens.shape[0] != self.n or tokens.shape[1] < 1:
+            raise ValueError(f"tokens must be ({self.n}, nodes)")
         up = (torch.arange(-1, tokens.shape[1] - 1).expand(self.n, -1) if parents is None else parents.cpu()).tolist()
         held = [tokens.shape[1]] * self.n if counts is None else counts.tolist()
         if min(held) < 1 or max(held) > tokens.shape[1] or any(

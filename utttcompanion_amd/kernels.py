@@ -997,8 +997,8 @@ def sample_select(logits: Tensor, uniforms: Tensor, temperature: Tensor, top_k: 
                   active_limit: Optional[int] = None, out: Optional[Tensor] = None,
                   logprobs: Optional[Tensor] = None, advance: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
     """Sampled next tokens (rows,) int64 and the logarithms (rows,) fp32 of their probabilities from
-    logits (rows, vocab) bf16 / fp32 (``uttt_sample_select``), each row with its own settings, all on the
-    device: ``temperature``, ``top_p``, ``min_p`` (rows,) fp32 and ``top_k`` (rows,) int32.  The ``banned``
+    logits (rows, vocab) bf16 / fp32 (``uttt_sample_select``; one row expanded to all is read once per
+    row), each row with its own settings, all on the device: ``temperature``, ``top_p``, ``min_p`` (rows,) fp32 and ``top_k`` (rows,) int32.  The ``banned``
     ids and those at or past ``active_limit`` are left out first, then, in the order (logit descending, id
     ascending) with weights exp((x - max x) / temperature), the first ``top_k`` ids stay (<= 0: all),
     those of at least ``min_p`` times the largest weight, and those whose mass ahead is at most
