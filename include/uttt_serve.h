@@ -63,7 +63,9 @@ int uttt_sample_select(const uttt_sample_args* args, uttt_stream_t stream);
 /* ---------------------------------------------------------------------------
  * 2. uttt_swa_prefill whose first `sinks` keys stay visible: query i (key index p = q_offset + i) sees key
  *    j <= p iff p - j < window or j < sinks.  sinks 0 is uttt_swa_prefill.  A continued prompt passes its
- *    cache's sink keys first, then the recent ones, then its own.
+ *    cache's sink keys first, then the recent ones, then its own.  As in uttt_swa_prefill, values that only some
+ *    queries of a tile see (a 64-key tile, the queries of a workgroup) must be finite: their weight of 0 meets them
+ *    for the others.  Keys that no query of the call sees may hold anything.
  * ------------------------------------------------------------------------- */
 size_t uttt_swa_prefill_sinks_workspace(int64_t batch, int64_t n_heads, int64_t q_len, int64_t kv_len,
                                         int64_t head_dim, int64_t window, int64_t sinks);

@@ -1043,11 +1043,16 @@ __global__ void __launch_bounds__(kThreads, 2) k_swa_tree_f32(const TreeArgs a) 
 #pragma unroll
       for (int j = 0; j < NJ; ++j) k[j] = *reinterpret_cast<const f32x4*>(kt + (s0 + c) * LK + 16 * j + 4 * g);
     }
-    f32x4 s{0.f, 0.f, 0.f, 0.f};
+    // two sums side by side: half as long a chain, and half as many roundings in a row
+    f32x4 s{0.f, 0.f, 0.f, 0.f}, s_odd{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
+    for (int j = 0; j < NJ; j += 2)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s = __builtin_amdgcn_mfma_f32_16x16x4f32(q[j][i], k[j][i], s, 0, 0, 0);
+      for (int i = 0; i < 4; ++i) {
+        s = __builtin_amdgcn_mfma_f32_16x16x4f32(q[j][i], k[j][i], s, 0, 0, 0);
+        s_odd = __builtin_amdgcn_mfma_f32_16x16x4f32(q[j + 1][i], k[j + 1][i], s_odd, 0, 0, 0);
+      }
+    s += s_odd;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (!clean) {
@@ -1058,9 +1063,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_swa_tree_f32(const TreeArgs a) 
         s[i] = vis ? s[i] : -INFINITY;
       }
       const float m_new = fmaxf(m[i], row_max(s[i]));
-      const float corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m[i] - m_new) * c2);
+      const float m_scaled = m_new * c2;  // its rounding is the row's, the exponents have one of their own
+      const float corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(__builtin_fmaf(m[i], c2, -m_scaled));
       m[i] = m_new;
-      const float x = s[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((s[i] - m_new) * c2);
+      const float x = s[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c2, -m_scaled));
       l[i] = l[i] * corr + x;  // this lane's keys; the lanes of a row meet at the end
 #pragma unroll
       for (int j = 0; j < NJ; ++j) o[j][i] *= corr;

@@ -1298,7 +1298,8 @@ def swa_prefill(q: Tensor, k: Tensor, v: Tensor, window: int, q_offset: int,
     """q (B, H, Tq, hd), k/v (B, Hkv, Tkv, hd) (any strides with hd contiguous).  Query i sits
     at key index q_offset + i and sees key j iff 0 <= q_offset + i - j < window.  With ``sinks``
     the first keys stay visible (0 <= q_offset + i - j and j < sinks) beside the window
-    (``uttt_swa_prefill_sinks``; not with ``build_only``, whose arguments carry no sinks).  ``out``
+    (``uttt_swa_prefill_sinks``; not with ``build_only``, whose arguments carry no sinks).  Values
+    that some queries see have to be finite (the others' weights of 0 may meet them).  ``out``
     (B, H, Tq, hd) may be a strided view, e.g. of a (B, Tq, H, hd) buffer.  Without a
     ``workspace`` the call uses one zero-filled buffer per device, shared by every call: calls on
     concurrent streams must each pass their own.  ``build_only``
