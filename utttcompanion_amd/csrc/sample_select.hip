@@ -218,7 +218,8 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
   const int lo = min(w * stretch, places), hi = min(lo + stretch, places);
   const float temp = a.temperature[row], uniform = a.uniforms[row];
   const int top_k = a.top_k != nullptr ? a.top_k[row] : 0;
-  const float top_p = a.top_p != nullptr ? a.top_p[row] : 1.f, min_p = a.min_p != nullptr ? a.min_p[row] : 0.f;
+  const float top_p = a.top_p != nullptr ? a.top_p[row] : 1.f, min_given = a.min_p != nullptr ? a.min_p[row] : 0.f;
+  const float min_p = min_given > 0.f ? fminf(min_given, 1.f) : 0.f;  // NaN is off
   auto scan = [&](int from, int to, auto&& f) __attribute__((always_inline)) {
     if constexpr (STAGED)
       scan_ids<T, W, 1, false>(a, stage, off, from, to, lane, f);
@@ -290,7 +291,7 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
 
   const double c = 1.4426950408889634 / (double)temp, dtop = (double)top;
   const bool by_count = top_k > 0 && top_k < a.limit, by_mass = top_p < 1.f;
-  const u64 least = min_p > 0.f ? (u64)__builtin_ceil(fmin((double)min_p, 1.0) * 4398046511104.0) : 1;
+  const u64 least = min_p > 0.f ? (u64)__builtin_ceil((double)min_p * 4398046511104.0) : 1;
   auto weight = [&](float v) __attribute__((always_inline)) -> u64 {
     u64 u = weight_units(((double)v - dtop) * c);
     if (least > 1) u = u >= least ? u : 0;
