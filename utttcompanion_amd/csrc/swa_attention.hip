@@ -1244,7 +1244,8 @@ extern "C" int uttt_swa_prefill(const uttt_swa_prefill_args* a, uttt_stream_t st
 extern "C" int uttt_swa_prefill_sinks(const uttt_swa_prefill_args* a, int64_t sinks, uttt_stream_t stream) {
   UTTT_REQUIRE(a != nullptr, "args is NULL");
   UTTT_REQUIRE(sinks >= 0 && a->kv_len < (1LL << 31), "sinks must be >= 0 and kv_len below 2^31");
-  return swa_prefill(a, sinks, static_cast<hipStream_t>(stream), "uttt_swa_prefill_sinks");
+  // the kernels take differences of sinks and key indexes in 32 bits
+  return swa_prefill(a, std::min(sinks, std::max<int64_t>(a->kv_len, 0)), static_cast<hipStream_t>(stream), "uttt_swa_prefill_sinks");
 }
 
 extern "C" size_t uttt_swa_decode_workspace(int64_t n_req, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
