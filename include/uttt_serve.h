@@ -38,8 +38,8 @@ int uttt_serve_abi_version(void);
  *    uniform * total (uniforms are taken into [0, 1), NaN as 0); logprob is log(w_out / total).
  *    A temperature that is not above 1e-5 takes the argmax (uttt_greedy_select's rules), logprob 0; so does,
  *    with logprob NaN, a row whose largest logit is not finite (NaN, +inf, or nothing allowed above -inf).
- *    Sums are formed in fixed point (weights in steps of 2^-42, by fp32 exponentials), so equal inputs give
- *    equal bits whatever the order.
+ *    Sums are formed in fixed point (weights from 64-bit arithmetic, each to a whole step of 2^-42 of the largest),
+ *    so equal inputs give equal bits whatever the order, the alignment and the other rows.
  * ------------------------------------------------------------------------- */
 typedef struct {
   int64_t rows, vocab; /* vocab <= 2^20 */
