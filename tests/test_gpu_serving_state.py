@@ -1,0 +1,53 @@
+"""What a decoder's calls leave in its state: the tokens, log-probabilities and logits that the next call goes on from."""
+import pytest
+import torch
+
+from test_gpu_serving import decoder, drafts, make
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("sinks", [0, 5])
+def test_capture_keeps_what_was_chosen(sinks, dtype):
+    """Recording a step between two steps changes nothing that was there: tokens, log-probabilities and logits, and the
+    steps that follow are those without it."""
+    model, states, prompts = make(sinks, dtype)
+    runs = []
+    for captured in (False, True):
+        dec, first = decoder(model, states, prompts)
+        dec.generate_greedy(first, 5)
+        dec.set_sampling(0.9, top_p=0.8, generator=torch.Generator(DEV).manual_seed(4))
+        trail = []
+        for _ in range(2):  # again: over a step that is recorded already
+            for _ in range(3):
+                if captured:
+                    held = dec.tokens.clone(), dec.logits.clone(), dec.positions.clone(), dec.k_rings.clone(), dec.v_rings.clone()
+                    logprobs = dec.logprobs.clone()
+                    dec.capture()
+                    now = dec.tokens, dec.logits, dec.positions, dec.k_rings, dec.v_rings
+                    assert all(torch.equal(a, b) for a, b in zip(now, held)) and torch.equal(dec.logprobs, logprobs)
+                dec.step(dec.next_tokens)
+                trail += [dec.tokens.clone(), dec.logprobs.clone(), dec.logits.clone()]
+            dec.fork([1, 0, 3, 3])
+            trail += [dec.tokens.clone(), dec.logprobs.clone(), dec.logits.clone()]
+        dec.set_sampling(None)
+        if captured:
+            dec.capture()
+        for _ in range(3):
+            dec.step(dec.tokens)
+            trail += [dec.tokens.clone(), dec.logits.clone()]
+        runs.append(trail)
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def test_capture_before_the_first_step_leaves_no_logits():
+    model, states, prompts = make()
+    dec, first = decoder(model, states, prompts)
+    dec.capture()
+    assert dec.logits is None and dec.next_tokens is None and dec.tokens.tolist() == [0] * 4
+    twin, _ = decoder(model, states, prompts)
+    token = first.argmax(1)
+    assert torch.equal(dec.step(token), twin.step(token)) and torch.equal(dec.next_tokens, twin.next_tokens)
+    assert dec.next_tokens.data_ptr() == dec.tokens.data_ptr()

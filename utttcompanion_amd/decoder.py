@@ -81,6 +81,7 @@ class BatchedDecoder:
         self._sampling: Optional[dict] = None
         self._nodes: Optional[Tuple[Tensor, Tensor]] = None  # the last verified trees' keys / values
         self._graph = None
+        self._graph_logits: Optional[Tensor] = None  # where the recorded step leaves its logits
         self._ws_attn = torch.zeros(1, dtype=torch.uint8, device=dev)
         self._ws_read = torch.zeros(1, dtype=torch.uint8, device=dev)
         self._states = list(states)
@@ -267,21 +268,23 @@ class BatchedDecoder:
 
     @torch.no_grad()
     def capture(self) -> None:
-        """Record one step into a HIP graph (after ``prefill``); ``step`` then replays it."""
+        """Record one step into a HIP graph (after ``prefill``, or between steps); ``step`` then replays it.  What the
+        decoder holds stays as it was: caches, positions, the tokens chosen last and their logits."""
         self._warm_workspaces()
-        saved = (self.positions.clone(), [(k.clone(), v.clone()) for k, v in self.rings])
+        held = [t for t in (self.positions, self.tokens, self.logprobs, self.k_rings, self.v_rings) if t is not None]
+        saved = [t.clone() for t in held]
+        chosen, logits = self.next_tokens, self.logits
         self._step_body()  # warm-up outside the graph (packs, tables, allocator)
         torch.cuda.synchronize()
-        self.positions.copy_(saved[0])
-        for (k, v), (k0, v0) in zip(self.rings, saved[1]):
-            k.copy_(k0)
-            v.copy_(v0)
+        for t, t0 in zip(held, saved):
+            t.copy_(t0)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             self._step_body()
         torch.cuda.synchronize()
-        # capture ran no kernels; positions and rings are as before
-        self._graph = graph
+        # capture ran no kernels: the logits recorded last are none yet
+        self._graph, self._graph_logits = graph, self.logits
+        self.next_tokens, self.logits = chosen, logits
 
     @torch.no_grad()
     def step(self, tokens: Tensor) -> Tensor:
@@ -298,6 +301,7 @@ class BatchedDecoder:
             self._sampling["uniforms"].uniform_(generator=self._sampling["generator"])
         if self._graph is not None:
             self._graph.replay()
+            self.next_tokens, self.logits = self.tokens, self._graph_logits
         else:
             if self._ws_attn.numel() == 1:
                 self._warm_workspaces()
