@@ -51,3 +51,19 @@ def test_capture_before_the_first_step_leaves_no_logits():
     token = first.argmax(1)
     assert torch.equal(dec.step(token), twin.step(token)) and torch.equal(dec.next_tokens, twin.next_tokens)
     assert dec.next_tokens.data_ptr() == dec.tokens.data_ptr()
+
+
+def test_speculation_is_refused_while_the_decoder_samples():
+    """As greedy generation is: a round would take greedy choices, whatever the settings.  Nothing has changed then."""
+    model, states, prompts = make()
+    dec, first = decoder(model, states, prompts)
+    dec.set_sampling(0.8)
+    dec.generate_sampled(first, 3)
+    held = dec.tokens.clone(), dec.positions.clone(), dec.k_rings.clone(), dec.logprobs.clone()
+    with pytest.raises(ValueError, match="samples"):
+        dec.speculate_greedy(dec.tokens[:, None])
+    with pytest.raises(ValueError, match="samples"):
+        dec.speculate_greedy(torch.ones(4, 3, dtype=torch.int64), torch.tensor([[-1, 0, 0]] * 4))
+    assert all(torch.equal(a, b) for a, b in zip((dec.tokens, dec.positions, dec.k_rings, dec.logprobs), held))
+    dec.set_sampling(None)
+    dec.speculate_greedy(dec.tokens[:, None])

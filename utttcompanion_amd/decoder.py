@@ -452,7 +452,10 @@ class BatchedDecoder:
         node 0 whose every token is the greedy choice behind its parent, commits it and returns, per request, the
         drafted tokens taken and the greedy choice behind the last of them (the next round's
         node 0, in ``self.tokens`` too): the tokens that single steps would give, as far as the products of
-        more rows at once round alike.  Trees and the choices behind them are read back."""
+        more rows at once round alike.  Trees and the choices behind them are read back.  Refused, as
+        ``generate_greedy`` is, while the decoder samples."""
+        if self._sampling is not None:
+            raise ValueError("the decoder samples; set_sampling(None) makes its choices greedy again")
         if tokens.dim() != 2 or tokens.shape[0] != self.n or tokens.shape[1] < 1:
             raise ValueError(f"tokens must be ({self.n}, nodes)")
         up = (torch.arange(-1, tokens.shape[1] - 1).expand(self.n, -1) if parents is None else parents.cpu()).tolist()
