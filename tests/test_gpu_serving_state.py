@@ -67,3 +67,45 @@ def test_speculation_is_refused_while_the_decoder_samples():
     assert all(torch.equal(a, b) for a, b in zip((dec.tokens, dec.positions, dec.k_rings, dec.logprobs), held))
     dec.set_sampling(None)
     dec.speculate_greedy(dec.tokens[:, None])
+
+
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("sinks", [0, 5])
+def test_speculation_leaves_the_logits_behind_its_last_token(sinks, captured):
+    """As a step does: generating from ``logits``, stepping on, and forks of the requests go on as single steps would."""
+    import random
+    model, states, prompts = make(sinks)
+    plain, first = decoder(model, states, prompts)
+    truth = plain.generate_greedy(first, 40).tolist()
+    for after in ("generate", "step", "fork"):
+        dec, first = decoder(model, states, prompts)
+        if captured:
+            dec.capture()
+        rng, have = random.Random(3), [[t[0]] for t in truth]
+        for _ in range(3):
+            trees = [drafts(truth, len(have[i]) - 1, i, rng, 5) for i in range(4)]
+            tokens, parents = torch.tensor([t for t, _ in trees]), torch.tensor([p for _, p in trees], dtype=torch.int32)
+            verified = dec.verify(tokens, parents)
+            new = dec.speculate_greedy(tokens, parents)
+            for i, row in enumerate(new):
+                node = 0  # the last one taken
+                for token in row[:-1]:
+                    node = next(j for j in range(5) if parents[i, j] == node and tokens[i, j] == token)
+                assert torch.equal(dec.logits[i], verified[i, node]), i
+                have[i] += row
+            assert dec.next_tokens.tolist() == dec.tokens.tolist() == [h[-1] for h in have]
+            if captured:  # a replay between the rounds
+                dec.step(dec.next_tokens)
+                for h, t in zip(have, dec.tokens.tolist()):
+                    h.append(t)
+        assert have == [t[:len(h)] for t, h in zip(truth, have)]
+        src = [0, 1, 2, 3]
+        if after == "step":
+            dec.step(dec.tokens)
+            have = [h + [t] for h, t in zip(have, dec.tokens.tolist())]
+        elif after == "fork":
+            src = [2, 2, 0, 1]
+            dec.fork(src)
+        got = dec.generate_greedy(dec.logits, 6).tolist()
+        # the first token from the logits is the last one chosen
+        assert got == [truth[s][len(have[s]) - 1:len(have[s]) + 5] for s in src], after

@@ -426,7 +426,8 @@ class BatchedDecoder:
     def commit(self, nodes: Tensor, counts: Tensor) -> None:
         """Append a path of the last verified trees to each request: the tokens of its nodes
         nodes[n, :counts[n]], from the first behind the request's tokens on, each the parent of the next (``nodes``
-        (N, A) and ``counts`` (N,), on any device; the counts are read back).  A tree is committed once."""
+        (N, A) and ``counts`` (N,), on any device; the counts are read back).  A tree is committed once.  The next token is
+        the caller's to choose, from ``verify``'s logits: ``self.tokens`` and ``self.logits`` stay the last step's."""
         if self._nodes is None:
             raise ValueError("commit follows verify, once, before anything else changes the requests")
         k_nodes, v_nodes = self._nodes
@@ -451,7 +452,7 @@ class BatchedDecoder:
         chosen already, the others descend from it.  Verifies the trees, takes in each the longest path from
         node 0 whose every token is the greedy choice behind its parent, commits it and returns, per request, the
         drafted tokens taken and the greedy choice behind the last of them (the next round's
-        node 0, in ``self.tokens`` too): the tokens that single steps would give, as far as the products of
+        node 0, in ``self.tokens`` too, with ``self.logits`` what it was chosen from): the tokens that single steps would give, as far as the products of
         more rows at once round alike.  Trees and the choices behind them are read back.  Refused, as
         ``generate_greedy`` is, while the decoder samples."""
         if self._sampling is not None:
@@ -482,6 +483,8 @@ class BatchedDecoder:
         longest = max(len(p) for p in paths)
         self.commit(torch.tensor([p + [0] * (longest - len(p)) for p in paths]), torch.tensor([len(p) for p in paths]))
         self.tokens.copy_(torch.tensor([choice[i][p[-1]] for i, p in enumerate(paths)]))
+        last = torch.tensor([i * nodes + p[-1] for i, p in enumerate(paths)])
+        self.next_tokens, self.logits = self.tokens, logits.view(n * nodes, vocab).index_select(0, last.to(self.device))
         return [[drafted[i][t] for t in p[1:]] + [choice[i][p[-1]]] for i, p in enumerate(paths)]
 
     # ------------------------------------------------------------------ requests taken over
