@@ -1022,6 +1022,8 @@ def sample_select(logits: Tensor, uniforms: Tensor, temperature: Tensor, top_k: 
     p_p = _row_setting(top_p, rows, f32, "top_p")
     p_m = _row_setting(min_p, rows, f32, "min_p")
     p_a = _row_setting(advance, rows, i64, "advance")
+    if torch.is_grad_enabled():
+        _forward_only(logits, temperature, top_p, min_p)
     index = _gpu_index(logits, uniforms, temperature, top_k, top_p, min_p, advance, out, logprobs)
     if out is None:
         out = logits.new_empty(rows, dtype=i64)
