@@ -109,3 +109,33 @@ def test_speculation_leaves_the_logits_behind_its_last_token(sinks, captured):
         got = dec.generate_greedy(dec.logits, 6).tolist()
         # the first token from the logits is the last one chosen
         assert got == [truth[s][len(have[s]) - 1:len(have[s]) + 5] for s in src], after
+
+
+@pytest.mark.parametrize("sinks", [0, 5])
+def test_committed_bf16_nodes_are_the_steps_up_to_their_roundings(sinks):
+    """The same tokens stepped one by one, and verified and committed at once.  Of the first layer, whose inputs are equal,
+    with u = 2^-8: the projections are within one rounding on each side, 2 u of a key's element; the rotation rounds once in
+    the tree and, without sinks, three times in a step: of each product (together at most sqrt 2 of the pair's length h) and
+    of the sum.  So the keys are within (2 sqrt 2 + sqrt 2 + 2) u h and the values within 2 u, and 2^-16 for the fp32 sums of
+    128 products of about 2 in all; what follows, within the bound that holds between bf16 steps and eager bf16 forwards."""
+    model, states, prompts = make(sinks, torch.bfloat16, slow_std=0.02)
+    stepped, _ = decoder(model, states, prompts)
+    drafted, _ = decoder(model, states, prompts)
+    ids = torch.randint(6, 256, (4, 8), generator=torch.Generator().manual_seed(5)).to(DEV)
+    for t in range(8):
+        logits = stepped.step(ids[:, t])
+    verified = drafted.verify(ids)
+    drafted.commit(torch.arange(8).expand(4, -1), torch.full((4,), 8))
+    assert drafted.host_positions == stepped.host_positions and torch.equal(drafted.positions, stepped.positions)
+    torch.testing.assert_close(verified[:, -1].float(), logits.float(), atol=0.015, rtol=0.025)
+    a, b = stepped.k_rings[0].double(), drafted.k_rings[0].double()
+    lo, hi = a.chunk(2, -1)
+    length = torch.hypot(lo, hi).repeat(1, 1, 1, 2)
+    u, root = 2.0 ** -8, 2.0 ** 0.5
+    assert bool(((a - b).abs() <= (3 * root + 2) * u * length + 2.0 ** -16).all())
+    a, b = stepped.v_rings[0].double(), drafted.v_rings[0].double()
+    assert bool(((a - b).abs() <= 2 * u * torch.maximum(a.abs(), b.abs()) + 2.0 ** -16).all())
+    for x, y in ((stepped.k_rings, drafted.k_rings), (stepped.v_rings, drafted.v_rings)):
+        torch.testing.assert_close(x, y, atol=0.015, rtol=0.025)
+    more = torch.randint(6, 256, (4,), generator=torch.Generator().manual_seed(6)).to(DEV)
+    torch.testing.assert_close(stepped.step(more).float(), drafted.step(more).float(), atol=0.015, rtol=0.025)

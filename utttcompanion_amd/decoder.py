@@ -451,9 +451,10 @@ class BatchedDecoder:
         """One round of greedy decoding with drafted tokens: node 0 of each request's tree is its next token,
         chosen already, the others descend from it.  Verifies the trees, takes in each the longest path from
         node 0 whose every token is the greedy choice behind its parent, commits it and returns, per request, the
-        drafted tokens taken and the greedy choice behind the last of them (the next round's
-        node 0, in ``self.tokens`` too, with ``self.logits`` what it was chosen from): the tokens that single steps would give, as far as the products of
-        more rows at once round alike.  Trees and the choices behind them are read back.  Refused, as
+        drafted tokens taken and the greedy choice behind the last of them (the next round's node 0, in
+        ``self.tokens`` too, with ``self.logits`` what it was chosen from): the tokens that single steps would give,
+        as far as the products of more rows at once, and in bf16 the tree's rotations (rounded once, a step's without
+        sinks after each operation), round alike.  Trees and the choices behind them are read back.  Refused, as
         ``generate_greedy`` is, while the decoder samples."""
         if self._sampling is not None:
             raise ValueError("the decoder samples; set_sampling(None) makes its choices greedy again")
