@@ -5,9 +5,10 @@
 // descending, id ascending), so the kept set is a cut (key, ties): the ids whose logit lies above the key's,
 // and the first `ties` of those at it.  Passes over the row, one workgroup each:
 //   1. the largest logit (rows that fit are kept in LDS for the passes behind);
-//   2. the ids within 16 factors of two of the top (up to 24 where the row is flat), listed per stretch of the row (16, one
-//      per wave) so that their weights are formed with all lanes busy; their histogram of counts and masses over x (2048
-//      bins), and the whole mass.  When the cut lies further down, again over all ids whose weight is not 0;
+//   2. the ids within 16 factors of two of the top (up to 24 where the row is flat, 43.5 where a top_k may lie there), listed
+//      per stretch of the row (16, one per wave) so that their weights are formed with all lanes busy; their histogram of
+//      counts and masses over x (2048 bins); and where top_p takes its share of it, the mass of the whole row, all of whose ids
+//      are weighed for it.  When the cut lies further down, again over all ids whose weight is not 0;
 //   3. the bin in which the count or the mass passes its bound: the stretches' masses ahead of it from the lists (where one
 //      overflowed, from the row), and its ids, which are ranked against each other.  When they are many (equal or
 //      nearly equal logits), the bin's range of keys is divided further first;
@@ -15,11 +16,11 @@
 // Without a cut 3 is a pass that weighs the whole row; without a list of the stretch (no cut, or many ids kept) 4 weighs
 // 16 parts of it first.
 //
-// Bound by the arithmetic of the weights: some 32 instructions an id, 0.85 us a pass over 131072 of them on the one compute
-// unit that has a row, beside 20 us to read it.  One row of 32000 bf16 takes 15.6 us (2.8 for pass 1, 6 for pass 2, 3 for
-// 3), 256 rows of 131072 fp32 with mixed settings 152 us, the flattest of them (temperature 1.5, top_p near 1) last:
-// a row of temperature 0.7 is done after 50.  Finding the cut's bin from counts alone, to weigh each id once, was slower
-// (199 us): it has to weigh every id with a bin again, not only those that may be kept.
+// Bound by the arithmetic of the weights: some 25 instructions an id, 18 us a pass over 131072 of them on the one compute
+// unit that has a row, beside 20 us to read it.  One row of 21478 bf16 takes 20 us (2.8 for pass 1, 10 for pass 2, 3 for 3),
+// 256 rows of 131072 fp32 with mixed settings 117 to 164 us by their settings, the flattest of them (temperature 1.5, top_p
+// near 1) last; all at temperature 0.7 and top_p 0.9 95 us.  Finding the cut's bin from counts alone, to weigh each id once, was
+// slower (199 us for 150): it has to weigh every id with a bin again, not only those that may be kept.
 //
 // The sums decide between neighbouring ids, so weights are formed in 64 bits and added as integers in units of
 // 2^-42 of the largest weight: exact whatever the order, so atomics in any order give equal bits.  (fp64 and
@@ -55,10 +56,10 @@ struct SampleArgs {
 constexpr int kSmpThreads = 1024, kSmpWaves = kSmpThreads / 64;
 constexpr int kBins = 2 * kSmpThreads;  // two per thread in the scan
 constexpr int kList = kSmpThreads;  // ids that are ranked against each other, one per thread
-// Ids of each 64: from so many on they are weighed in place.  From 8, 24, 48 on: 256 x 131072 152, 149, 148 us, 64 x 50000
-// 53.0, 52.5, 53.8.
+// Ids of each 64: from so many on they are weighed in place.  From 8, 24, 48 on: 256 x 131072 mixed 137, 133, 129 us (other
+// settings 181, 163, 163), 64 x 50000 46.7, 46.3, 46.3.
 constexpr int kDense = 24;
-// Rows up to this size stay in LDS.  Staged and not: 1 x 32000 15.9 and 16.2 us, 64 x 32000 mixed 28.8 and 30.1.
+// Rows up to this size stay in LDS.  Staged and not: 1 x 21478 20.0 and 20.1 us, 64 x 30000 mixed 34.9 and 36.4.
 constexpr int kStageBytes = 60 * 1024;
 constexpr int kKeptStaged = 256, kKept = 512;
 
@@ -206,8 +207,8 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
   constexpr float kFarthest = 43.5f;  // factors of two below the top from where on weights are 0 units, half of 2^-42 not reached
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   // Places count from the 16-byte boundary at or before the row's first id, so that rows of any alignment are read in
-  // whole 16-byte pieces (256 rows of 131071 fp32 at temperature 0.7: one id at
-  // a time 123 us, so 80); ids from the place `off` on.
+  // whole 16-byte pieces (256 rows of 131071 fp32 at temperature 0.7: 43 us less than
+  // one id at a time); ids from the place `off` on.
   const T* x = static_cast<const T*>(a.logits) + (int64_t)row * a.rs;
   const int off = __builtin_amdgcn_readfirstlane((int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T)));
   const int places = a.limit + off;
@@ -299,8 +300,9 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
   };
   // The bins of the first round reach 16 factors of two down, in which a cut lies that most of the mass is ahead of; where
   // the row's mean is that near, so that much of the mass is around it, 4 past the mean; and 2/5 of the way to the mean
-  // for top_k, whose ids may weigh next to nothing.  Reaching 16 always, rows whose cut lay further down took both
-  // rounds, and the slowest of 256 x 131072 mixed ones 226 to 271 us, for 133 to 162 so.
+  // for top_k, whose ids may weigh next to nothing.  Reaching 16 always, rows whose cut lies further down take both
+  // rounds: 256 x 131072 of deviation 3 at temperature 1.5 and top_p 0.99 230 us, for 154 so; with top_k 50 at temperature 0.2 87, for
+  // 64 (64 x 32000 26.5, for 27.5).
   const float to_mean = (top - mean / (float)a.limit) * (float)c;
   float reach = to_mean < 20.f ? fmaxf(16.f, to_mean + 4.f) : 16.f;
   if (by_count && to_mean > 40.f) reach = fminf(0.4f * to_mean, kFarthest);
@@ -381,7 +383,7 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
     };
     // Counts and masses of the bins, and the whole mass.  Ids further down are a part of that (`tail`; else they have no weight,
     // min_p leaves them out, or top_p's share is not of them), so every id is weighed then.  fp32 exponentials for them were
-    // faster (1 x 32000 16 us for 20, 256 x 131072 at temperature 0.7 77 for 93) and moved cuts.
+    // faster (1 x 21478 16.5 us for 20, 256 x 131072 at temperature 0.7 77 for 95) and moved cuts.
     auto histogram = [&](bool tail) __attribute__((always_inline)) {
       u64 sum = 0;
       kept = 0;
