@@ -86,3 +86,18 @@ def test_cuts_above_a_heavy_tail_are_the_definitions_at_any_alignment(vocab, dty
     assert sure > rows // 2 and deep > rows // 2
     for off, (t, l) in enumerate(runs):
         assert t.tolist() == tok.tolist() and l.tolist() == lp.tolist(), off
+
+
+@pytest.mark.parametrize("temperature", [2e37, 1e38, 3e38, math.inf])
+def test_logits_further_apart_than_the_largest_number(temperature):
+    """The differences of logits at both ends of the type do not fit it, and at such temperatures they weigh something."""
+    from test_gpu_sampling import check, uniforms
+    g = torch.Generator().manual_seed(21)
+    x = 3.3e38 * (2 * torch.rand((4, 500), generator=g) - 1)
+    x[1, ::3] = torch.finfo(torch.float32).min
+    x[2, 100:] = -math.inf
+    x[3] = 3.4e38 * torch.where(torch.rand(500, generator=g) < 0.5, 1.0, -1.0)
+    x = x.to(DEV)
+    for seed, kw in enumerate((dict(), dict(p=[0.3, 0.99, 0.7, 0.9]), dict(k=[400, 40, 3, 300]), dict(m=[0.01, 0.2, 0.0, 0.5]),
+                               dict(k=[450, 7, 90, 400], p=[0.999, 0.9, 0.95, 0.8]))):
+        check(x, uniforms(4, 40 + seed), [temperature] * 4, **kw)

@@ -306,8 +306,10 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
   const float to_mean = (top - mean / (float)a.limit) * (float)c;
   float reach = to_mean < 20.f ? fmaxf(16.f, to_mean + 4.f) : 16.f;
   if (by_count && to_mean > 40.f) reach = fminf(0.4f * to_mean, kFarthest);
-  float per_unit = fminf((float)c * ((float)kBins / reach), 3e38f);  // bins to a unit of the logits
-  auto place = [&](float v) __attribute__((always_inline)) { return (top - v) * per_unit; };
+  // half the difference: a whole one may pass the type's largest number, where a high temperature still gives it weight
+  float per_half = (float)c * (2.f * (float)kBins / reach);  // bins to two units of the logits
+  const float half_top = 0.5f * top;
+  auto place = [&](float v) __attribute__((always_inline)) { return __builtin_fmaf(v, -0.5f, half_top) * per_half; };
 
   Cut cut{0, 0x7fffffff, 0};  // keeps everything
   bool masses = false;        // the stretches' masses up to the cut are known
@@ -656,7 +658,7 @@ __global__ void __launch_bounds__(kSmpThreads) k_sample_select(const SampleArgs 
         }
       }
       if (found || round == 1) break;
-      per_unit = fminf((float)c * ((float)kBins / kFarthest), 3e38f);
+      per_half = (float)c * (2.f * (float)kBins / kFarthest);
       __syncthreads();
       for (int i = tid; i < kBins; i += kSmpThreads) {
         s.mass[i] = 0;
