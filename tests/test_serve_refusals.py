@@ -17,3 +17,10 @@ def test_sampling_refuses_operands_that_ask_for_gradients():
             call()
         with torch.no_grad(), pytest.raises(ValueError, match="no CPU path"):
             call()
+
+
+@pytest.mark.parametrize("ids", [(-1,), (3, 2 ** 31), (2 ** 40,)])
+def test_sampling_refuses_banned_ids_that_are_none(ids):
+    x, u = torch.zeros(2, 100), torch.ones(2)
+    with pytest.raises(ValueError, match="excluded ids"):
+        K.sample_select(x, u, u, banned=ids)

@@ -1009,8 +1009,11 @@ def sample_select(logits: Tensor, uniforms: Tensor, temperature: Tensor, top_k: 
     takes it too, log-probability NaN.  ``advance`` as in ``greedy_select``."""
     if logits.dim() != 2 or logits.stride(1) != 1:
         raise ValueError("logits must be (rows, vocab) with unit column stride")
-    if len(banned) > 8:
+    ids = [int(b) for b in banned]
+    if len(ids) > 8:
         raise ValueError("at most 8 excluded ids")
+    if ids and not 0 <= min(ids) <= max(ids) < 1 << 31:
+        raise ValueError("excluded ids must be at least 0 and below 2^31")
     rows, vocab = logits.shape
     if not 1 <= vocab <= 1 << 20:
         raise ValueError("sampling takes vocabularies of 1 to 2^20 ids")
@@ -1032,7 +1035,6 @@ def sample_select(logits: Tensor, uniforms: Tensor, temperature: Tensor, top_k: 
     p_o, p_l = _row_setting(out, rows, i64, "out"), _row_setting(logprobs, rows, f32, "logprobs")
     if rows == 0:
         return out, logprobs
-    ids = [int(b) for b in banned]
     stride = logits.stride(0) if rows > 1 else vocab
     packed = N.pack_sample(rows, vocab, code, len(ids), *ids, *([0] * (8 - len(ids))),
                            -1 if active_limit is None else int(active_limit), logits.data_ptr(), stride,
