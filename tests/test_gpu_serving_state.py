@@ -139,3 +139,30 @@ def test_committed_bf16_nodes_are_the_steps_up_to_their_roundings(sinks):
         torch.testing.assert_close(x, y, atol=0.015, rtol=0.025)
     more = torch.randint(6, 256, (4,), generator=torch.Generator().manual_seed(6)).to(DEV)
     torch.testing.assert_close(stepped.step(more).float(), drafted.step(more).float(), atol=0.015, rtol=0.025)
+
+
+@pytest.mark.parametrize("sinks", [0, 5])
+def test_nodes_that_were_not_computed_are_loud_when_committed(sinks):
+    """A request whose parents are no earlier nodes has NaN logits, and nodes behind ``counts`` do not exist: neither has keys
+    or values, and committing one all the same puts NaN into that request's cache, not whatever memory held."""
+    model, states, prompts = make(sinks)
+    dec, _ = decoder(model, states, prompts)
+    twin, _ = decoder(model, states, prompts)
+    at = list(dec.host_positions)
+    tokens = torch.randint(6, 256, (4, 3), generator=torch.Generator().manual_seed(8))
+    parents = torch.tensor([[-1, 0, 1]] * 4, dtype=torch.int32)
+    want = twin.verify(tokens, parents)
+    bad = parents.clone()
+    bad[2, 1] = 2
+    counts = torch.tensor([3, 2, 3, 3], dtype=torch.int32)
+    logits = dec.verify(tokens, bad, counts)
+    assert bool(logits[2].isnan().all()) and torch.equal(logits[[0, 3]], want[[0, 3]]) and torch.equal(logits[1, :2], want[1, :2])
+    path = torch.tensor([[0, 1, 2]] * 4)
+    dec.commit(path, torch.tensor([3, 3, 2, 3]))
+    twin.commit(path, torch.tensor([3, 3, 2, 3]))
+    slots = lambda i, n: dec._cached_slots(min(at[i] + n, dec.slots), at[i] + n)[-n:]  # noqa: E731
+    for mine, theirs in ((dec.k_rings, twin.k_rings), (dec.v_rings, twin.v_rings)):
+        assert torch.equal(mine[:, [0, 3]], theirs[:, [0, 3]])
+        assert bool(mine[:, 2].index_select(2, slots(2, 2)).isnan().all())
+        new = mine[:, 1].index_select(2, slots(1, 3))
+        assert bool(new[:, :, 2].isnan().all()) and torch.equal(new[:, :, :2], theirs[:, 1].index_select(2, slots(1, 3))[:, :, :2])

@@ -394,10 +394,11 @@ class BatchedDecoder:
         m, n = self.model, self.n
         parents = None if parents is None else parents.to(device=self.device, dtype=torch.int32).contiguous()
         counts = None if counts is None else counts.to(device=self.device, dtype=torch.int32).contiguous()
-        # the nodes that do not exist are zeros here: the layers read them on their way through
-        made = torch.empty if counts is None else torch.zeros
-        k_nodes, v_nodes = (made((len(m.layers), n, nodes, self.hkv, self.hd), dtype=self.dtype, device=self.device)
-                            for _ in range(2))
+        shape = (len(m.layers), n, nodes, self.hkv, self.hd)
+        k_nodes, v_nodes = (torch.empty(shape, dtype=self.dtype, device=self.device) for _ in range(2))
+        if parents is not None or counts is not None:  # nodes that are not computed: loud, should they be committed
+            k_nodes.fill_(float("nan"))
+            v_nodes.fill_(float("nan"))
         h = F.embedding(tokens.to(self.device).reshape(-1), m.tok_embeddings.weight)  # (N T, D)
         hq, hk = self.heads * self.hd, self.hkv * self.hd
         read_ws = None
