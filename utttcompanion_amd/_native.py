@@ -1,4 +1,4 @@
-"""ctypes binding of libuttt_amd.so (the C ABI declared in include/uttt_amd.h and include/uttt_serve.h).
+"""ctypes binding of libuttt_amd.so (the C ABI declared in include/uttt_amd.h, uttt_serve.h and uttt_decode.h).
 
 The library is loaded lazily on first use and there is no fallback: a missing or
 stale library raises ``RuntimeError`` naming the build command.
@@ -26,6 +26,8 @@ def _header_abi_version(path: str = HEADER_PATH, name: str = "UTTT_ABI_VERSION")
 ABI_VERSION = _header_abi_version()
 SERVE_HEADER_PATH = os.path.join(os.path.dirname(HEADER_PATH), "uttt_serve.h")
 SERVE_ABI_VERSION = _header_abi_version(SERVE_HEADER_PATH, "UTTT_SERVE_ABI_VERSION")
+DECODE_HEADER_PATH = os.path.join(os.path.dirname(HEADER_PATH), "uttt_decode.h")
+DECODE_ABI_VERSION = _header_abi_version(DECODE_HEADER_PATH, "UTTT_DECODE_ABI_VERSION")
 MAX_CHAIN = 64
 MAX_UPDATE_TOKENS = 512  # UTTT_MAX_UPDATE_TOKENS: longest chunk one uttt_chunk_update writes
 DTYPE_F32 = 0
@@ -33,6 +35,7 @@ DTYPE_BF16 = 1
 UPDATE_PHASES = 5
 MAX_TREE_NODES = 64  # of one request's draft (uttt_swa_tree)
 MAX_FORK_REQUESTS = 128  # of one uttt_kv_fork
+MAX_BEAMS = 32  # of one group (uttt_beam_select)
 
 _P = C.c_void_p
 _I64 = C.c_int64
@@ -332,6 +335,80 @@ class KvForkArgs(C.Structure):
     ]
 
 
+# include/uttt_decode.h: decoding in 4 bits and beam search, with a version of their own
+
+
+class Linear4Args(C.Structure):
+    _fields_ = [
+        ("m", _I64), ("n", _I64), ("k", _I64), ("act_dtype", _I32), ("x_eps", _F),
+        ("x", _P), ("x_row_stride", _I64), ("w", _P),
+        ("residual", _P), ("residual_row_stride", _I64), ("out", _P), ("out_row_stride", _I64),
+    ]
+
+
+class Readout4Args(C.Structure):
+    _fields_ = [
+        ("batch", _I64), ("tokens", _I64), ("d_model", _I64), ("d_ff", _I64), ("act_dtype", _I32), ("eps", _F),
+        ("x", _P), ("x_stride_b", _I64), ("x_stride_t", _I64),
+        ("w_up", _P), ("w_gate", _P), ("w_down", _P),
+        ("w_up_stride", _I64), ("w_gate_stride", _I64), ("w_down_stride", _I64),
+        ("ln_weight", _P), ("ln_bias", _P), ("x_norm_weight", _P), ("x_norm_eps", _F),
+        ("out", _P), ("out_stride_b", _I64), ("out_stride_t", _I64),
+        ("workspace", _P), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class SwaTree4Args(C.Structure):
+    _fields_ = [
+        ("n_req", _I64), ("n_heads", _I64), ("n_kv_heads", _I64), ("nodes", _I64), ("head_dim", _I64),
+        ("window", _I64), ("sinks", _I64), ("act_dtype", _I32), ("scale", _F),
+        ("positions", _P), ("parents", _P), ("counts", _P),
+        ("cos_table", _P), ("sin_table", _P), ("table_len", _I64),
+        ("q", _P), ("q_stride_n", _I64), ("q_stride_t", _I64), ("q_stride_h", _I64),
+        ("k_new", _P), ("k_stride_n", _I64), ("k_stride_t", _I64), ("k_stride_h", _I64),
+        ("v_new", _P), ("v_stride_n", _I64), ("v_stride_t", _I64), ("v_stride_h", _I64),
+        ("cache", _P), ("cache_stride_n", _I64),
+        ("out", _P), ("o_stride_n", _I64), ("o_stride_t", _I64), ("o_stride_h", _I64),
+        ("k_nodes", _P), ("v_nodes", _P), ("nodes_stride_n", _I64),
+        ("workspace", _P), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class KvCommit4Args(C.Structure):
+    _fields_ = [
+        ("layers", _I64), ("n_req", _I64), ("n_kv_heads", _I64), ("n_nodes", _I64), ("path", _I64), ("head_dim", _I64),
+        ("window", _I64), ("sinks", _I64), ("act_dtype", _I32), ("advance", _I32),
+        ("k_nodes", _P), ("v_nodes", _P),
+        ("nodes_stride_l", _I64), ("nodes_stride_n", _I64), ("nodes_stride_t", _I64), ("nodes_stride_h", _I64),
+        ("nodes", _P), ("path_stride", _I64), ("counts", _P),
+        ("cache", _P), ("cache_stride_l", _I64), ("cache_stride_n", _I64), ("positions", _P),
+    ]
+
+
+class KvValues4Args(C.Structure):
+    _fields_ = [
+        ("layers", _I64), ("n_req", _I64), ("n_kv_heads", _I64), ("head_dim", _I64), ("window", _I64), ("sinks", _I64),
+        ("act_dtype", _I32), ("cache", _P), ("cache_stride_l", _I64), ("cache_stride_n", _I64), ("k", _P), ("v", _P),
+    ]
+
+
+class KvFork4Args(C.Structure):
+    _fields_ = [
+        ("layers", _I64), ("n_req", _I64), ("n_kv_heads", _I64), ("head_dim", _I64), ("window", _I64), ("sinks", _I64),
+        ("sources", _P), ("cache", _P), ("cache_stride_l", _I64), ("cache_stride_n", _I64), ("positions", _P),
+    ]
+
+
+class BeamSelectArgs(C.Structure):
+    _fields_ = [
+        ("rows", _I64), ("vocab", _I64), ("beams", _I64), ("dtype", _I32), ("n_banned", _I32),
+        ("banned", _I32 * 8), ("active_limit", _I64), ("eos", _I64), ("pad", _I64),
+        ("logits", _P), ("row_stride", _I64), ("scores", _P), ("ended_in", _P),
+        ("tokens", _P), ("sources", _P), ("out_scores", _P), ("ended_out", _P),
+        ("workspace", _P), ("workspace_bytes", C.c_size_t),
+    ]
+
+
 def _packer(args):
     """A function of an argument block's fields, in order (pointers as integers), to its bytes: what a call costs the
     host is mostly Python, and one pack is several times cheaper than setting forty ctypes fields."""
@@ -346,6 +423,13 @@ pack_sample = _packer(SampleArgs)
 pack_swa_tree = _packer(SwaTreeArgs)
 pack_kv_commit = _packer(KvCommitArgs)
 pack_kv_fork = _packer(KvForkArgs)
+pack_linear4 = _packer(Linear4Args)
+pack_readout4 = _packer(Readout4Args)
+pack_swa_tree4 = _packer(SwaTree4Args)
+pack_kv_commit4 = _packer(KvCommit4Args)
+pack_kv_values4 = _packer(KvValues4Args)
+pack_kv_fork4 = _packer(KvFork4Args)
+pack_beam_select = _packer(BeamSelectArgs)
 
 # the argument blocks of these calls may come as bytes
 SERVE_SIGNATURES = {
@@ -357,6 +441,20 @@ SERVE_SIGNATURES = {
     "uttt_swa_tree": (C.c_int, [_P, _P]),
     "uttt_kv_commit": (C.c_int, [_P, _P]),
     "uttt_kv_fork": (C.c_int, [_P, _P]),
+}
+
+DECODE_SIGNATURES = {
+    "uttt_decode_abi_version": (C.c_int, []),
+    "uttt_linear4": (C.c_int, [_P, _P]),
+    "uttt_readout4_workspace": (C.c_size_t, [_I64, _I64, _I64, _I64]),
+    "uttt_readout4": (C.c_int, [_P, _P]),
+    "uttt_swa_tree4_workspace": (C.c_size_t, [_I64, _I64, _I64, _I64, _I64, _I64, _I64]),
+    "uttt_swa_tree4": (C.c_int, [_P, _P]),
+    "uttt_kv_commit4": (C.c_int, [_P, _P]),
+    "uttt_kv_values4": (C.c_int, [_P, _P]),
+    "uttt_kv_fork4": (C.c_int, [_P, _P]),
+    "uttt_beam_select_workspace": (C.c_size_t, [_I64, _I64, _I64]),
+    "uttt_beam_select": (C.c_int, [_P, _P]),
 }
 
 _lib = None
@@ -382,7 +480,10 @@ def load_library(path: str = LIB_PATH) -> C.CDLL:
         serve = lib.uttt_serve_abi_version() if hasattr(lib, "uttt_serve_abi_version") else 0
         if serve != SERVE_ABI_VERSION:
             raise RuntimeError(f"{path} has serving ABI version {serve}, expected {SERVE_ABI_VERSION}: rebuild it")
-        for name, (res, argt) in {**SIGNATURES, **SERVE_SIGNATURES}.items():
+        decode = lib.uttt_decode_abi_version() if hasattr(lib, "uttt_decode_abi_version") else 0
+        if decode != DECODE_ABI_VERSION:
+            raise RuntimeError(f"{path} has decoding ABI version {decode}, expected {DECODE_ABI_VERSION}: rebuild it")
+        for name, (res, argt) in {**SIGNATURES, **SERVE_SIGNATURES, **DECODE_SIGNATURES}.items():
             fn = getattr(lib, name)
             fn.restype = res
             fn.argtypes = argt

@@ -13,7 +13,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import math
-from typing import Optional, Sequence, Tuple
+from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -1665,6 +1665,440 @@ def kv_fork(k_ring: Tensor, v_ring: Tensor, sources: Tensor, positions: Tensor) 
     packed = N.pack_kv_fork(layers, n, hkv, slots, hd, code, p_src, k_ring.data_ptr(), v_ring.data_ptr(), ring_l, ring_n,
                             p_pos)
     _serve_call(N.load_library().uttt_kv_fork, packed, index, "uttt_kv_fork")
+
+
+# ---------------------------------------------------------------------------
+# decoding in 4 bits (include/uttt_decode.h): groups of 32 neighbours share a bf16 scale, values are one of 15 levels
+# ---------------------------------------------------------------------------
+
+FP4_GROUP = 32
+FP4_LEVELS = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+class Weight4(NamedTuple):
+    """A weight (n, k), or a batch of them, in 4 bits as ``pack_weight4`` lays it out: ``data`` uint8 ([B,] ceil(n / 16),
+    ceil(k / 128), 1152)."""
+    data: Tensor
+    n: int
+    k: int
+
+
+def pack_weight4(weight: Tensor) -> Weight4:
+    """``weight`` ([B,] n, k), products running along k, in 4 bits: per row, 32 neighbours share the scale
+    s = bf16(largest magnitude * fp32(1 / 6)) (0 below 2^-126; NaN where a value is not finite) and each takes the level of
+    ``FP4_LEVELS`` next to |w| / s (the even one of two as near) with its sign.  Once per weight, on its own
+    device; a matrix at a time is held in fp32 besides."""
+    if weight.dim() not in (2, 3) or 0 in weight.shape or not weight.is_floating_point():
+        raise ValueError(f"weight must be a floating ([B,] n, k) tensor, got {tuple(weight.shape)} {weight.dtype}")
+    if weight.dim() == 3:
+        return Weight4(torch.stack([pack_weight4(w).data for w in weight]), *weight.shape[1:])
+    n, k = weight.shape
+    tiles, blocks = -(-n // 16), -(-k // 128)
+    data = torch.empty((tiles, blocks, 1152), dtype=torch.uint8, device=weight.device)
+    w = torch.zeros((16 * tiles, 128 * blocks), dtype=torch.float32, device=weight.device)
+    w[:n, :k] = weight.detach()
+    groups = w.view(tiles, 16, blocks, 4, FP4_GROUP)
+    largest = groups.abs().amax(-1)
+    scale = (largest * torch.tensor(1.0 / 6.0, dtype=torch.float32, device=w.device)).to(torch.bfloat16)
+    scale = torch.where(scale < 2.0 ** -126, torch.zeros_like(scale), scale)
+    scale = torch.where(torch.isfinite(largest), scale, torch.full_like(scale, math.nan))
+    wide = scale.float()[..., None]
+    t = torch.where(wide > 0, groups.abs() / torch.where(wide > 0, wide, 1.0), 0.0)
+    code = torch.zeros_like(t, dtype=torch.uint8)
+    for i, (low, high) in enumerate(zip(FP4_LEVELS, FP4_LEVELS[1:])):
+        middle = (low + high) / 2
+        code += t > middle if i % 2 == 0 else t >= middle
+    code += ((groups < 0) & (code > 0)).to(torch.uint8) * 8
+    code = code.view(tiles, 16, blocks, 4, 4, 8).permute(0, 2, 4, 1, 3, 5)  # tile, block, h, row, group, j
+    data[..., :1024] = (code[..., 0::2] | code[..., 1::2] << 4).reshape(tiles, blocks, 1024)
+    data[..., 1024:] = scale.permute(0, 2, 1, 3).contiguous().view(torch.uint8).view(tiles, blocks, 128)
+    return Weight4(data, n, k)
+
+
+def _weight4(w: Weight4, n: int, k: int, name: str, batch: Optional[int] = None) -> Tuple[int, int]:
+    """The address and the batch's stride in bytes (0: one matrix) of a packed weight that has to be (n, k)."""
+    data = w.data
+    shape = data.shape
+    if w.n != n or w.k != k or shape[-3:] != ((n + 15) // 16, (k + 127) // 128, 1152) or data.dtype is not torch.uint8:
+        raise ValueError(f"{name} must be a packed weight of ({n}, {k}), got ({w.n}, {w.k}) with {tuple(shape)} {data.dtype}")
+    address = data.data_ptr()
+    inner = data.stride()[-3:]
+    if inner != (shape[-2] * 1152, 1152, 1) or address & 15:
+        raise ValueError(f"{name} must lie together, 16-byte aligned")
+    if len(shape) == 3:
+        return address, 0
+    if len(shape) != 4 or batch is None or shape[0] not in (1, batch):
+        raise ValueError(f"{name} must hold one matrix" + ("" if batch is None else f" or {batch}"))
+    stride = data.stride(0) if shape[0] > 1 else 0
+    if stride & 15:
+        raise ValueError(f"{name} must lie together, 16-byte aligned")
+    return address, stride
+
+
+def linear4(x: Tensor, weight: Weight4, out: Optional[Tensor] = None, residual: Optional[Tensor] = None,
+            x_eps: float = 0.0) -> Tensor:
+    """out = x weight^T (+ residual) with a weight in 4 bits (``uttt_linear4``; ``pack_weight4``): the decode step's
+    projections and LM head (reference engine/inference.py:263-276).  x (m, k) bf16 or fp32, any m, k and row stride;
+    ``residual`` (m, n) may be ``out`` itself.  ``x_eps`` > 0 RMS-normalises x's rows first (pack the weight with
+    the norm weight multiplied into its columns).  Products are of x's whole values, sums fp32, rounded once."""
+    if x.dim() != 2 or x.shape[1] != weight.k:
+        raise ValueError(f"x must be (m, {weight.k}), got {tuple(x.shape)}")
+    m, k = x.shape
+    n = weight.n
+    dt = x.dtype
+    code = _act_code(dt)
+    p_w, _ = _weight4(weight, n, k, "weight")
+    x_eps = float(x_eps)
+    if not 0.0 <= x_eps < math.inf:
+        raise ValueError("x_eps must be finite and >= 0")
+    if torch.is_grad_enabled():
+        _forward_only(x, residual)
+    index = _gpu_index(x, weight.data, out, residual)
+    if k > 1 and x.stride(1) != 1 or m > 1 and x.stride(0) < k:
+        x = x.contiguous()
+    if out is None:
+        out = x.new_empty((m, n))
+    elif out.shape != (m, n) or out.dtype is not dt or n > 1 and out.stride(1) != 1 or m > 1 and out.stride(0) < n:
+        raise ValueError(f"out must be ({m}, {n}) of x's dtype with unit column stride and rows apart")
+    p_r = r_stride = 0
+    if residual is not None:
+        if residual.shape != (m, n) or residual.dtype is not dt or n > 1 and residual.stride(1) != 1:
+            raise ValueError(f"residual must be ({m}, {n}) of x's dtype with unit column stride")
+        if m > 1 and residual.stride(0) < n:
+            residual = residual.contiguous()
+        p_r, r_stride = residual.data_ptr(), residual.stride(0)
+    if m == 0:
+        return out
+    packed = N.pack_linear4(m, n, k, code, x_eps, x.data_ptr(), x.stride(0), p_w, p_r, r_stride, out.data_ptr(), out.stride(0))
+    _serve_call(N.load_library().uttt_linear4, packed, index, "uttt_linear4")
+    return out
+
+
+@functools.lru_cache(maxsize=256)
+def _readout4_workspace(*sizes: int) -> int:
+    return N.load_library().uttt_readout4_workspace(*sizes)
+
+
+def readout4(x: Tensor, w_up: Weight4, w_gate: Weight4, w_down: Weight4, ln_weight: Tensor, ln_bias: Tensor,
+             eps: float = 1e-5, x_norm: Optional[Tuple[Tensor, float]] = None, out: Optional[Tensor] = None,
+             workspace: Optional[Tensor] = None) -> Tensor:
+    """``swiglu_readout`` through fast weights in 4 bits (``uttt_readout4``): x (B, T, D) bf16 or fp32, ``w_up`` and ``w_gate``
+    packed from (d_ff, D) matrices, ``w_down`` from (D, d_ff) ones -- the transposes of a state's, products running along
+    the last axis -- one per row or one for all.  ``x_norm`` = (weight, eps) reads out RMSNorm(x) with that weight
+    instead of x.  ``workspace``: uint8, of ``readout4_workspace`` bytes; calls that share one must be ordered."""
+    if x.dim() != 3:
+        raise ValueError(f"x must be (B, T, D), got {tuple(x.shape)}")
+    bsz, tokens, dim = x.shape
+    ff = w_up.n
+    dt = x.dtype
+    code = _act_code(dt)
+    if dim % 64 or ff % 64 or not 64 <= dim <= 4096 or ff < 64:
+        raise ValueError(f"d_model and d_ff must be multiples of 64 (d_model <= 4096); got {dim}, {ff}")
+    p_up, s_up = _weight4(w_up, ff, dim, "w_up", bsz)
+    p_gate, s_gate = _weight4(w_gate, ff, dim, "w_gate", bsz)
+    p_down, s_down = _weight4(w_down, dim, ff, "w_down", bsz)
+    gain, x_eps = (None, 0.0) if x_norm is None else (x_norm[0], float(x_norm[1]))
+    for name, t in (("ln_weight", ln_weight), ("ln_bias", ln_bias)) + ((("the x norm weight", gain),) if x_norm else ()):
+        if t.shape != (dim,):
+            raise ValueError(f"{name} must be ({dim},)")
+    if not eps > 0.0 or x_norm is not None and not x_eps > 0.0:
+        raise ValueError("eps must be > 0")
+    if torch.is_grad_enabled():
+        _forward_only(x, ln_weight, ln_bias, gain)
+    index = _gpu_index(x, w_up.data, w_gate.data, w_down.data, ln_weight, ln_bias, gain, out, workspace)
+    if ln_weight.dtype is not torch.float32 or not ln_weight.is_contiguous():
+        ln_weight = ln_weight.float().contiguous()
+    if ln_bias.dtype is not torch.float32 or not ln_bias.is_contiguous():
+        ln_bias = ln_bias.float().contiguous()
+    p_gain = 0
+    if gain is not None:
+        if gain.dtype is not dt or not gain.is_contiguous() or gain.data_ptr() & 15:
+            gain = gain.to(dt).clone(memory_format=torch.contiguous_format)
+        p_gain = gain.data_ptr()
+    x = _pieces(x, 2)
+    if out is None:
+        out = x.new_empty((bsz, tokens, dim))
+    elif out.shape != x.shape or out.dtype is not dt or out.stride(2) != 1:
+        raise ValueError("out must match x's shape and dtype with unit feature stride")
+    if bsz == 0 or tokens == 0:
+        return out
+    nbytes = _readout4_workspace(bsz, tokens, dim, ff)
+    if workspace is None:
+        workspace = x.new_empty(nbytes, dtype=torch.uint8)
+    elif workspace.numel() * workspace.element_size() < nbytes or not workspace.is_contiguous():
+        raise ValueError(f"the readout workspace must be {nbytes} contiguous bytes")
+    xs, os_ = _strides(x, 2), out.stride()
+    packed = N.pack_readout4(bsz, tokens, dim, ff, code, float(eps), x.data_ptr(), *xs, p_up, p_gate, p_down, s_up, s_gate,
+                             s_down, ln_weight.data_ptr(), ln_bias.data_ptr(), p_gain, x_eps, out.data_ptr(), os_[0], os_[1],
+                             workspace.data_ptr(), nbytes)
+    _serve_call(N.load_library().uttt_readout4, packed, index, "uttt_readout4")
+    return out
+
+
+def readout4_workspace(bsz: int, tokens: int, dim: int, ff: int, device: torch.device) -> Tensor:
+    """A workspace for ``readout4`` of x (bsz, tokens, dim) and every smaller call."""
+    return torch.empty(max(_readout4_workspace(bsz, tokens, dim, ff), 16), dtype=torch.uint8, device=device)
+
+
+def kv_cache4(*lead: int, window: int, sinks: int, head_dim: int, device: torch.device) -> Tensor:
+    """A ring cache in 4 bits for ``lead`` = ([L,] N, Hkv): uint8 (*lead, blocks, 36 head_dim), a block holding 32 slots, the
+    blocks of the ``sinks`` first."""
+    if head_dim not in (64, 128) or window < 1 or sinks < 0:
+        raise ValueError("head_dim must be 64 or 128, window >= 1 and sinks >= 0")
+    return torch.zeros((*lead, -(-sinks // 32) + -(-window // 32), 36 * head_dim), dtype=torch.uint8, device=device)
+
+
+def _cache4(cache: Tensor, lead: int, window: int, sinks: int) -> Tuple[int, Tuple[int, ...], int]:
+    """Address, the ``lead`` leading strides in bytes and the head_dim of a cache (.., Hkv, blocks, 36 hd)."""
+    shape, strides = cache.shape, cache.stride()
+    if len(shape) != lead + 3 or cache.dtype is not torch.uint8:
+        raise ValueError(f"the cache must be a uint8 {'(L, N' if lead == 2 else '(N'}, Hkv, blocks, bytes) tensor")
+    if not 1 <= window <= 1 << 28 or not 0 <= sinks <= 1 << 28:
+        raise ValueError("window must be in [1, 2^28] and sinks in [0, 2^28]")
+    if shape[-2] != (sinks + 31) // 32 + (window + 31) // 32 or shape[-1] not in (2304, 4608):
+        raise ValueError(f"a cache of window {window} and sinks {sinks} has {(sinks + 31) // 32 + (window + 31) // 32} blocks of "
+                         f"36 head_dim bytes, head_dim 64 or 128, got {tuple(shape[-2:])}")
+    if strides[lead:] != (shape[-2] * shape[-1], shape[-1], 1) and 0 not in shape:
+        if shape[lead] != 1 or strides[lead + 1:] != (shape[-1], 1):
+            raise ValueError("each request's cache must lie together")
+    at = _strides(cache, lead)
+    if cache.data_ptr() & 15 or any(s & 15 for s in at):
+        raise ValueError("each request's cache must be 16-byte aligned")
+    return cache.data_ptr(), at, shape[-1] // 36
+
+
+@functools.lru_cache(maxsize=256)
+def _tree4_workspace(*sizes: int) -> int:
+    return N.load_library().uttt_swa_tree4_workspace(*sizes)
+
+
+def swa_tree4(q: Tensor, k_new: Tensor, v_new: Tensor, cache: Tensor, positions: Tensor, window: int,
+              parents: Optional[Tensor] = None, cos: Optional[Tensor] = None, sin: Optional[Tensor] = None, sinks: int = 0,
+              counts: Optional[Tensor] = None, out: Optional[Tensor] = None,
+              node_outputs: Optional[Tuple[Tensor, Tensor]] = None,
+              workspace: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor]:
+    """``swa_tree`` over a cache in 4 bits (``uttt_swa_tree4``), which it does not write: q (N, T, H, hd), k_new / v_new
+    (N, T, Hkv, hd) (un-rotated when tables are given), T <= 64 nodes, ``cache`` (N, Hkv, blocks, 36 hd) of ``kv_cache4``
+    holding ``positions`` (N,) int64 tokens each.  ``parents``, ``counts`` and what comes back as in ``swa_tree``; a decode step is
+    one node per request, whose keys and values ``kv_commit4`` then takes in.  The new tokens are seen in their own
+    precision.  ``node_outputs``: (N, T, Hkv, hd), each request's part contiguous.  ``workspace``: calls that share one must be
+    ordered."""
+    if q.dim() != 4:
+        raise ValueError("q must be (N, T, H, hd)")
+    n, nodes, heads, hd = shape = q.shape
+    if not 1 <= nodes <= N.MAX_TREE_NODES:
+        raise ValueError(f"a tree has 1 to {N.MAX_TREE_NODES} nodes, got {nodes}")
+    window, sinks = int(window), int(sinks)
+    p_cache, (cache_n,), cache_hd = _cache4(cache, 1, window, sinks)
+    hkv = cache.shape[1]
+    new_shape = (n, nodes, hkv, hd)
+    if cache.shape[0] != n or hd != cache_hd or k_new.shape != new_shape or v_new.shape != new_shape:
+        raise ValueError("new keys / values must be (N, T, Hkv, hd) and the cache (N, Hkv, blocks, 36 hd)")
+    if hkv < 1 or heads < 1 or heads % hkv:
+        raise ValueError("n_heads must be a multiple of n_kv_heads")
+    dt = q.dtype
+    code = _act_code(dt)
+    if k_new.dtype is not dt or v_new.dtype is not dt:
+        raise ValueError("q and new keys / values must share one dtype")
+    p_pos = _per_request(positions, n, torch.int64, "positions")
+    p_counts = 0 if counts is None else _per_request(counts, n, torch.int32, "counts")
+    p_up = p_cos = p_sin = positions_len = 0
+    if parents is not None:
+        if parents.dtype is not torch.int32 or parents.shape != (n, nodes) or not parents.is_contiguous():
+            raise ValueError("parents must be a contiguous int32 (N, nodes) tensor")
+        p_up = parents.data_ptr()
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin must both be given or both omitted")
+    if cos is not None:
+        positions_len = cos.shape[0]
+        p_cos, p_sin = cos.data_ptr(), sin.data_ptr()
+        if (cos.shape != (positions_len, hd) or sin.shape != cos.shape or cos.dtype is not torch.float32
+                or sin.dtype is not torch.float32 or not cos.is_contiguous() or not sin.is_contiguous()
+                or (p_cos | p_sin) & 15):
+            raise ValueError("cos / sin must be contiguous fp32 (positions, head_dim) tables")
+    if torch.is_grad_enabled():
+        _forward_only(q, k_new, v_new)
+    index = _gpu_index(q, k_new, v_new, cache, positions, parents, counts, cos, sin, out, workspace)
+    made = q.new_empty if counts is None else q.new_zeros  # rows behind a request's nodes are not written
+    if out is None:
+        out = made(shape)
+    elif out.shape != shape or out.dtype is not dt or out.stride(3) != 1:
+        raise ValueError("out must match q's shape and dtype with contiguous heads")
+    if node_outputs is not None:
+        k_nodes, v_nodes = node_outputs
+        _gpu_index(q, k_nodes, v_nodes)
+        nodes_n = _strides(k_nodes, 1)[0] if k_nodes.dim() == 4 else 0
+        for t in node_outputs:
+            if t.shape != new_shape or t.dtype is not dt or _pieces(t, 1) is not t or _strides(t, 1)[0] != nodes_n:
+                raise ValueError("node outputs must be (N, nodes, Hkv, hd) tensors of q's dtype, alike, each request's part "
+                                 "contiguous and 16-byte aligned")
+    else:
+        k_nodes, v_nodes = made(new_shape), made(new_shape)
+        nodes_n = nodes * hkv * hd
+    if n == 0:
+        return out, k_nodes, v_nodes
+    mask = 7 if dt is torch.bfloat16 else 3
+    q, *q_at = _heads(q, mask)
+    k_new, *k_at = _heads(k_new, mask)
+    v_new, *v_at = _heads(v_new, mask)
+    nbytes = _tree4_workspace(n, heads, hkv, nodes, hd, window, sinks)
+    p_ws = 0
+    if workspace is not None:
+        if workspace.numel() * workspace.element_size() < nbytes:
+            raise ValueError(f"the tree attention workspace must hold {nbytes} bytes")
+        p_ws, nbytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    elif nbytes > 16:
+        workspace = q.new_empty(nbytes, dtype=torch.uint8)
+        p_ws = workspace.data_ptr()
+    o_at = out.stride()
+    packed = N.pack_swa_tree4(n, heads, hkv, nodes, hd, window, sinks, code, hd ** -0.5, p_pos, p_up, p_counts, p_cos, p_sin,
+                              positions_len, *q_at, *k_at, *v_at, p_cache, cache_n, out.data_ptr(), *o_at[:3],
+                              k_nodes.data_ptr(), v_nodes.data_ptr(), nodes_n, p_ws, nbytes)
+    _serve_call(N.load_library().uttt_swa_tree4, packed, index, "uttt_swa_tree4")
+    return out, k_nodes, v_nodes
+
+
+def kv_commit4(k_nodes: Tensor, v_nodes: Tensor, nodes: Optional[Tensor], counts: Optional[Tensor], cache: Tensor,
+               positions: Tensor, window: int, sinks: int = 0, advance: bool = False) -> None:
+    """``kv_commit`` into caches in 4 bits (``uttt_kv_commit4``): node nodes[n, a], for a < counts[n], becomes the token at
+    positions[n] + a.  k_nodes / v_nodes ([L,] N, T, Hkv, hd), cache ([L,] N, Hkv, blocks, 36 hd), nodes (N, A) int32 (None: node
+    a), counts (N,) int32 (None: all A, or T), positions (N,) int64.  Prompts of any length go in the same way: where a path is
+    longer than the window, a slot's last token stays.  ``advance``: the positions grow by counts afterwards."""
+    if cache.dim() == 4:
+        cache, k_nodes, v_nodes = cache[None], k_nodes[None], v_nodes[None]
+    window, sinks = int(window), int(sinks)
+    p_cache, (cache_l, cache_n), hd = _cache4(cache, 2, window, sinks)
+    layers, n, hkv = cache.shape[:3]
+    shape = k_nodes.shape
+    if len(shape) != 5 or v_nodes.shape != shape or shape[:2] != (layers, n) or shape[3:] != (hkv, hd):
+        raise ValueError("nodes' keys / values must be ([L,] N, T, Hkv, hd), one row per cache")
+    dt = k_nodes.dtype
+    code = _act_code(dt)
+    if v_nodes.dtype is not dt:
+        raise ValueError("nodes' keys and values must share one dtype")
+    path, p_nodes, path_stride = shape[2], 0, 0
+    if nodes is not None:
+        if nodes.dim() != 2 or nodes.shape[0] != n or nodes.dtype is not torch.int32 or (nodes.numel() and nodes.stride(1) != 1):
+            raise ValueError("nodes must be int32 (N, A) with unit column stride")
+        path, p_nodes, path_stride = nodes.shape[1], nodes.data_ptr(), nodes.stride(0)
+    p_counts = 0 if counts is None else _per_request(counts, n, torch.int32, "counts")
+    p_pos = _per_request(positions, n, torch.int64, "positions")
+    if torch.is_grad_enabled():
+        _forward_only(k_nodes, v_nodes)
+    index = _gpu_index(cache, k_nodes, v_nodes, nodes, counts, positions)
+    if layers == 0 or n == 0 or hkv == 0 or path == 0 or shape[2] == 0:
+        return
+    k_nodes, v_nodes = _pieces(k_nodes, 4), _pieces(v_nodes, 4)
+    if _strides(k_nodes, 4) != _strides(v_nodes, 4):
+        k_nodes, v_nodes = (t.clone(memory_format=torch.contiguous_format) for t in (k_nodes, v_nodes))
+    packed = N.pack_kv_commit4(layers, n, hkv, shape[2], path, hd, window, sinks, code, bool(advance), k_nodes.data_ptr(),
+                               v_nodes.data_ptr(), *_strides(k_nodes, 4), p_nodes, path_stride, p_counts, p_cache, cache_l,
+                               cache_n, p_pos)
+    _serve_call(N.load_library().uttt_kv_commit4, packed, index, "uttt_kv_commit4")
+
+
+def kv_values4(cache: Tensor, window: int, sinks: int = 0, dtype: torch.dtype = torch.bfloat16) -> Tuple[Tensor, Tensor]:
+    """What caches in 4 bits hold (``uttt_kv_values4``): keys and values ([L,] N, Hkv, sinks + W, hd) in ``dtype``, in the
+    slots' order of the rings of ``swa_tree``.  Slots without a token hold what their bits stand for."""
+    window, sinks = int(window), int(sinks)
+    lead = 2 if cache.dim() == 5 else 1
+    p_cache, at, hd = _cache4(cache, lead, window, sinks)
+    code = _act_code(dtype)
+    index = _gpu_index(cache)
+    *lead_shape, hkv = cache.shape[:-2]
+    k, v = (torch.empty((*lead_shape, hkv, sinks + window, hd), dtype=dtype, device=cache.device) for _ in range(2))
+    if k.numel() == 0:
+        return k, v
+    layers, n = lead_shape if lead == 2 else (1, *lead_shape)
+    packed = N.pack_kv_values4(layers, n, hkv, hd, window, sinks, code, p_cache, at[0] if lead == 2 else 0, at[-1], k.data_ptr(),
+                               v.data_ptr())
+    _serve_call(N.load_library().uttt_kv_values4, packed, index, "uttt_kv_values4")
+    return k, v
+
+
+def kv_fork4(cache: Tensor, sources: Tensor, positions: Optional[Tensor], window: int, sinks: int = 0) -> None:
+    """``kv_fork`` for caches in 4 bits (``uttt_kv_fork4``), in place: request n takes the cache and the position of request
+    sources[n], as they were before the call.  cache ([L,] N, Hkv, blocks, 36 hd) of at most 128 requests; sources (N,) int32
+    (n itself, or an id out of range: left as it was), positions (N,) int64, or None: whole caches and no position."""
+    if cache.dim() == 4:
+        cache = cache[None]
+    window, sinks = int(window), int(sinks)
+    p_cache, (cache_l, cache_n), hd = _cache4(cache, 2, window, sinks)
+    layers, n, hkv = cache.shape[:3]
+    if n > N.MAX_FORK_REQUESTS:
+        raise ValueError(f"at most {N.MAX_FORK_REQUESTS} requests")
+    p_src = _per_request(sources, n, torch.int32, "sources")
+    p_pos = 0 if positions is None else _per_request(positions, n, torch.int64, "positions")
+    index = _gpu_index(cache, sources, positions)
+    if layers == 0 or n == 0 or hkv == 0:
+        return
+    packed = N.pack_kv_fork4(layers, n, hkv, hd, window, sinks, p_src, p_cache, cache_l, cache_n, p_pos)
+    _serve_call(N.load_library().uttt_kv_fork4, packed, index, "uttt_kv_fork4")
+
+
+@functools.lru_cache(maxsize=256)
+def _beam_workspace(*sizes: int) -> int:
+    return N.load_library().uttt_beam_select_workspace(*sizes)
+
+
+def beam_select(logits: Tensor, scores: Tensor, beams: int, ended: Optional[Tensor] = None, banned: Sequence[int] = (),
+                active_limit: Optional[int] = None, eos: Optional[int] = None, pad: int = 0,
+                out: Optional[Tuple[Tensor, Tensor, Tensor, Tensor]] = None,
+                workspace: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    """Beam search's choice (``uttt_beam_select``): logits (G beams, vocab) bf16 / fp32, a group's beams in neighbouring rows,
+    ``scores`` (rows,) fp32 the beams' sums of log-probabilities so far (-inf: the beam offers nothing, as all but the first
+    do behind a common prompt), ``ended`` (rows,) int32 whether a beam has ended (None: none has; an ended one goes on as it
+    is, with ``pad``).  Per group the ``beams`` <= 32 best of score + log softmax(logits) over the ids below ``active_limit``
+    that are not ``banned`` (softmax over those ids, in 64 bits), the best first, of equal ones the lower row's, then the
+    lower id.  Returns the tokens (rows,) int64, the rows they go on from (rows,) int32 (``kv_fork``'s sources), their scores
+    and whether they have ended (by ``eos``, or before); ``out``, when given, whose scores and ended may be the inputs.  Where a
+    group offers fewer than ``beams``, the rest is ``pad`` at -inf from its own row, ended."""
+    if logits.dim() != 2 or logits.shape[1] > 1 and logits.stride(1) != 1:
+        raise ValueError("logits must be (rows, vocab) with unit column stride")
+    rows, vocab = logits.shape
+    beams = int(beams)
+    if not 1 <= beams <= N.MAX_BEAMS or rows % beams:
+        raise ValueError(f"beams must be 1 to {N.MAX_BEAMS} and divide the rows, got {beams} of {rows}")
+    if not 1 <= vocab <= 1 << 20:
+        raise ValueError("beam search takes vocabularies of 1 to 2^20 ids")
+    if rows > 65535:
+        raise ValueError("at most 65535 rows")
+    ids = [int(b) for b in banned]
+    if len(ids) > 8:
+        raise ValueError("at most 8 excluded ids")
+    if ids and not 0 <= min(ids) <= max(ids) < 1 << 31:
+        raise ValueError("excluded ids must be at least 0 and below 2^31")
+    pad = int(pad)
+    if not 0 <= pad < vocab:
+        raise ValueError("pad must be an id of the vocabulary")
+    if active_limit is not None and int(active_limit) < 0:
+        raise ValueError("active_limit must be >= 0")
+    code = _act_code(logits.dtype)
+    i32, i64, f32 = torch.int32, torch.int64, torch.float32
+    p_s = _row_setting(scores, rows, f32, "scores")
+    p_e = _row_setting(ended, rows, i32, "ended")
+    if torch.is_grad_enabled():
+        _forward_only(logits, scores)
+    if rows > 1 and logits.stride(0) < vocab:
+        logits = logits.contiguous()
+    if out is None:
+        new = logits.new_empty
+        out = new(rows, dtype=i64), new(rows, dtype=i32), new(rows, dtype=f32), new(rows, dtype=i32)
+    index = _gpu_index(logits, scores, ended, workspace, *out)
+    p_out = [_row_setting(t, rows, d, name) for t, d, name in zip(out, (i64, i32, f32, i32), ("tokens", "sources", "scores", "ended"))]
+    if rows == 0:
+        return out
+    nbytes = _beam_workspace(rows, vocab, beams)
+    if workspace is None:
+        workspace = logits.new_empty(nbytes, dtype=torch.uint8)
+    elif workspace.numel() * workspace.element_size() < nbytes or not workspace.is_contiguous():
+        raise ValueError(f"the beam workspace must be {nbytes} contiguous bytes")
+    packed = N.pack_beam_select(rows, vocab, beams, code, len(ids), *ids, *([0] * (8 - len(ids))),
+                                -1 if active_limit is None else int(active_limit), -1 if eos is None else int(eos), pad,
+                                logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, p_s, p_e, *p_out,
+                                workspace.data_ptr(), nbytes)
+    _serve_call(N.load_library().uttt_beam_select, packed, index, "uttt_beam_select")
+    return out
 
 
 # ---------------------------------------------------------------------------
