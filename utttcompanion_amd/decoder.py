@@ -16,8 +16,11 @@ HIP graph.
 
 Beside the step (not in the reference's decoders): ``verify`` runs a tree of drafted tokens per
 request through the model at once, without writing the rings, ``commit`` makes a path of it part
-of the requests, ``speculate_greedy`` does both, and ``fork`` lets requests take over others'
-caches.
+of the requests, ``speculate_greedy`` does both, ``fork`` lets requests take over others'
+caches, and ``beam_search`` keeps the best continuations of a prompt in a group of requests.
+
+With ``weight_bits=4`` the slow weights and the requests' fast weights, with ``cache_bits=4`` the ring
+caches are held in 4 bits (``kernels.pack_weight4``, ``kernels.kv_cache4``); everything above works alike.
 """
 from __future__ import annotations
 
@@ -28,17 +31,24 @@ import torch.nn.functional as F
 
 from . import kernels as K
 from .layer import FastWeightState, linear_residual
-from .model import BOS_ID, PAD_ID, UNK_ID, uTTTModel
+from .model import BOS_ID, EOS_ID, PAD_ID, UNK_ID, uTTTModel
 
 Tensor = torch.Tensor
 
 
 class BatchedDecoder:
-    """N requests, one token each per step, frozen fast weights (decode never writes them)."""
+    """N requests, one token each per step, frozen fast weights (decode never writes them).
 
-    def __init__(self, model: uTTTModel, states: Sequence[FastWeightState], max_positions: int = 8192):
+    ``weight_bits`` 4: the slow weights (the norms before them folded in, embeddings aside) and each request's fast weights in 4 bits,
+    packed when they are first used and here; ``cache_bits`` 4: keys and values in 4 bits (prompts are prefilled in the
+    model's type).  A step's new tokens are seen in their own precision and quantised behind the step."""
+
+    def __init__(self, model: uTTTModel, states: Sequence[FastWeightState], max_positions: int = 8192,
+                 weight_bits: int = 16, cache_bits: int = 16):
         if model.training:
             raise ValueError("call model.eval() before decoding")
+        if weight_bits not in (4, 16) or cache_bits not in (4, 16):
+            raise ValueError("weight_bits and cache_bits must be 4, or 16 for the model's own type")
         if not states:
             raise ValueError("need at least one request state")
         self.model = model
@@ -57,20 +67,37 @@ class BatchedDecoder:
                 raise ValueError("batched decoding needs one shared LayerNorm pair for all requests")
         self.ln_weight = ln_w.detach().float().contiguous()
         self.ln_bias = ln_b.detach().float().contiguous()
-        # per-request read copies in the activation dtype (reference inference_read_weights,
-        # model/uttt_layer.py:648-668): same operands the reference's bf16 matmuls see
+        self.weight_bits, self.cache_bits = weight_bits, cache_bits
+        self.w_up = self.w_gate = self.w_down = None
+        self.fast4: Optional[Tuple[K.Weight4, K.Weight4, K.Weight4]] = None  # up, gate, down in 4 bits
         with torch.no_grad():
-            self.w_up = torch.cat([st.w_up.detach() for st in states]).to(self.dtype).contiguous()
-            self.w_gate = torch.cat([st.w_gate.detach() for st in states]).to(self.dtype).contiguous()
-            self.w_down = torch.cat([st.w_down.detach() for st in states]).to(self.dtype).contiguous()
+            if weight_bits == 4:  # the products run along the last axis
+                self.fast4 = tuple(
+                    K.Weight4(torch.stack([p.data for p in rows]), rows[0].n, rows[0].k)
+                    for rows in ([K.pack_weight4(getattr(st, name)[0].detach().t().to(dev)) for st in states]
+                                 for name in ("w_up", "w_gate", "w_down")))
+            else:
+                # per-request read copies in the activation dtype (reference inference_read_weights,
+                # model/uttt_layer.py:648-668): same operands the reference's bf16 matmuls see
+                self.w_up = torch.cat([st.w_up.detach() for st in states]).to(self.dtype).contiguous()
+                self.w_gate = torch.cat([st.w_gate.detach() for st in states]).to(self.dtype).contiguous()
+                self.w_down = torch.cat([st.w_down.detach() for st in states]).to(self.dtype).contiguous()
         attn = model.layers[0].attn
         self.window, self.hkv, self.hd, self.heads = attn.window_size, attn.n_kv_heads, attn.head_dim, attn.n_heads
         self.sinks = attn.sinks
         # every layer's slots in one tensor: commits and forks take all layers in one launch
         self.slots = self.sinks + self.window
-        self.k_rings, self.v_rings = (torch.zeros((len(model.layers), self.n, self.hkv, self.slots, self.hd),
-                                                  dtype=self.dtype, device=dev) for _ in range(2))
-        self.rings = [(self.k_rings[li], self.v_rings[li]) for li in range(len(model.layers))]
+        self.k_rings = self.v_rings = self.cache4 = None
+        self.rings: List[Tuple[Tensor, Tensor]] = []
+        layers = len(model.layers)
+        if cache_bits == 4:
+            self.cache4 = K.kv_cache4(layers, self.n, self.hkv, window=self.window, sinks=self.sinks, head_dim=self.hd, device=dev)
+            # a step's new keys and values, committed behind its last layer
+            self._new4 = tuple(torch.zeros((layers, self.n, 1, self.hkv, self.hd), dtype=self.dtype, device=dev) for _ in range(2))
+        else:
+            self.k_rings, self.v_rings = (torch.zeros((layers, self.n, self.hkv, self.slots, self.hd),
+                                                      dtype=self.dtype, device=dev) for _ in range(2))
+            self.rings = [(self.k_rings[li], self.v_rings[li]) for li in range(layers)]
         self.cos, self.sin = attn.rope.tables(max_positions, dev)
         self.positions = torch.zeros(self.n, dtype=torch.int64, device=dev)
         self.host_positions = [0] * self.n
@@ -87,6 +114,7 @@ class BatchedDecoder:
         self._states = list(states)
         self._key = self._state_key(states)
         self._folds = {}
+        self._fours = {}  # slow weights in 4 bits
         d_model = model.config.d_model
         self._fused_readout = self.dtype == torch.bfloat16 and d_model <= 2048 and all(
             (blk.uttt.q_norm.eps or 0.0) > 0.0 for blk in model.layers)
@@ -123,18 +151,31 @@ class BatchedDecoder:
     def _load_request(self, i: int, kv_caches, length: int) -> None:
         """Request i's ring slots from a frozen prefill's per-layer caches (the last <= window
         rotated keys / values of ``length`` tokens, behind the sinks)."""
-        if len(kv_caches) != len(self.rings):
-            raise ValueError(f"expected {len(self.rings)} layer caches, got {len(kv_caches)}")
-        for (kr, vr), (k, v) in zip(self.rings, kv_caches):
+        if len(kv_caches) != len(self.model.layers):
+            raise ValueError(f"expected {len(self.model.layers)} layer caches, got {len(kv_caches)}")
+        for li, (k, v) in enumerate(kv_caches):
             cached = k.shape[2]
             if (k.shape != (1, self.hkv, cached, self.hd) or v.shape != k.shape or cached > min(length, self.slots)
                     or cached < min(length, self.slots - 1)):
                 raise ValueError("a cache must be (1, n_kv_heads, min(length, sinks + window) or sinks + window - 1, "
                                  "head_dim)")
+            if self.cache4 is not None:
+                self._quantise(self.cache4[li, i:i + 1], *(t.to(device=self.device, dtype=self.dtype) for t in (k, v)), length)
+                continue
+            kr, vr = self.rings[li]
             slots = self._cached_slots(cached, length)
             kr[i].index_copy_(1, slots, k[0].to(device=self.device, dtype=kr.dtype))
             vr[i].index_copy_(1, slots, v[0].to(device=self.device, dtype=vr.dtype))
         self.host_positions[i] = int(length)
+
+    def _quantise(self, cache: Tensor, k: Tensor, v: Tensor, length: int) -> None:
+        """A request's cached rows (1, Hkv, cached, hd), the sinks in front, into its cache in 4 bits: as tokens at their positions."""
+        cached = k.shape[2]
+        first = min(self.sinks, cached)
+        for start, rows in ((0, slice(0, first)), (length - (cached - first), slice(first, cached))):
+            if rows.stop > rows.start:
+                K.kv_commit4(k[:, :, rows].transpose(1, 2), v[:, :, rows].transpose(1, 2), None, None, cache,
+                             torch.tensor([start], dtype=torch.int64).to(self.device), self.window, self.sinks)
 
     @torch.no_grad()
     def reset(self, kv_caches_per_request: Sequence, lengths: Sequence[int]) -> None:
@@ -143,9 +184,8 @@ class BatchedDecoder:
         if len(kv_caches_per_request) != self.n or len(lengths) != self.n:
             raise ValueError(f"expected caches and lengths for {self.n} requests")
         self._nodes = None
-        for kr, vr in self.rings:
-            kr.zero_()
-            vr.zero_()
+        for t in self._caches():
+            t.zero_()
         for i, (caches, length) in enumerate(zip(kv_caches_per_request, lengths)):
             if length < 1:
                 raise ValueError("a request needs at least one prompt token")
@@ -158,7 +198,13 @@ class BatchedDecoder:
         values up to the window in token order), e.g. to continue a decode eagerly."""
         pos = self.host_positions[i]
         slots = self._cached_slots(min(pos, self.slots), pos)
+        if self.cache4 is not None:
+            k, v = K.kv_values4(self.cache4[:, i:i + 1], self.window, self.sinks, self.dtype)
+            return [(k[li].index_select(2, slots), v[li].index_select(2, slots)) for li in range(k.shape[0])]
         return [(kr[i:i + 1].index_select(2, slots), vr[i:i + 1].index_select(2, slots)) for kr, vr in self.rings]
+
+    def _caches(self) -> List[Tensor]:
+        return [self.cache4] if self.cache4 is not None else [self.k_rings, self.v_rings]
 
     def matches(self, model: uTTTModel, states: Sequence[FastWeightState]) -> bool:
         """Whether this decoder's read copies and LayerNorm pair still stand for ``states`` of
@@ -182,9 +228,24 @@ class BatchedDecoder:
             self._folds[id(weight)] = hit
         return hit[1]
 
+    def _packed4(self, weight: Tensor, norm) -> K.Weight4:
+        """W, or W diag(g) for an RMSNorm ``norm`` applied to its input, in 4 bits, rebuilt when either changes."""
+        key = (weight.data_ptr(), weight._version) + (() if norm is None else (norm.weight.data_ptr(), norm.weight._version))
+        hit = self._fours.get(id(weight))
+        if hit is None or hit[0] != key:
+            w = weight.detach()
+            hit = (key, K.pack_weight4(w if norm is None else w.float() * norm.weight.detach().float()[None, :]), weight)
+            self._fours[id(weight)] = hit
+        return hit[1]
+
     def _linear(self, x: Tensor, weight: Tensor, residual: Optional[Tensor] = None, norm=None) -> Tensor:
-        """norm(x) W^T (+ residual, updated in place): ``uttt_skinny_linear`` for bf16 steps of
-        at most 64 requests (the RMSNorm folded in), the norm and the library GEMM otherwise."""
+        """norm(x) W^T (+ residual, updated in place): ``uttt_linear4`` with weights in 4 bits, ``uttt_skinny_linear`` for bf16
+        steps of at most 64 requests (the RMSNorm folded in), the norm and the library GEMM otherwise."""
+        if self.weight_bits == 4:
+            if norm is not None and not (norm.eps or 0.0) > 0.0:
+                x, norm = norm(x), None
+            return K.linear4(x, self._packed4(weight, norm), out=residual, residual=residual,
+                             x_eps=0.0 if norm is None else norm.eps)
         skinny = (x.dtype == torch.bfloat16 and weight.dtype == torch.bfloat16 and x.shape[0] <= 64
                   and weight.shape[0] % 32 == 0 and x.shape[1] % 64 == 0 and x.stride(1) == 1
                   and weight.is_contiguous() and (norm is None or (norm.eps or 0.0) > 0.0))
@@ -211,16 +272,23 @@ class BatchedDecoder:
             q = qkv[:, :hq].view(n, self.heads, self.hd)
             k = qkv[:, hq:hq + hk].view(n, self.hkv, self.hd)
             v = qkv[:, hq + hk:].view(n, self.hkv, self.hd)
-            kr, vr = self.rings[li]
-            att = K.swa_decode(q, k, v, kr, vr, self.positions, self.cos, self.sin, workspace=self._ws_attn,
-                               sinks=self.sinks)
+            if self.cache4 is not None:
+                att, _, _ = K.swa_tree4(q[:, None], k[:, None], v[:, None], self.cache4[li], self.positions, self.window, None,
+                                        self.cos, self.sin, self.sinks, workspace=self._ws_attn,
+                                        node_outputs=(self._new4[0][li], self._new4[1][li]))
+            else:
+                kr, vr = self.rings[li]
+                att = K.swa_decode(q, k, v, kr, vr, self.positions, self.cos, self.sin, workspace=self._ws_attn,
+                                   sinks=self.sinks)
             h = self._linear(att.reshape(n, -1), attn.wo.weight, residual=h)
             y = self._linear(h, block.uttt.w_q.weight, norm=block.uttt_norm)
             qn = block.uttt.q_norm
             # every layer reads the same per-request copies: odd layers walk them backwards, so
             # each readout starts on the lines the previous one left in the infinity cache
             rev = li % 2 == 1
-            if self._fused_readout:  # q_norm, readout, LayerNorm and residual in one launch
+            if self.fast4 is not None:
+                r = self._readout4(y.view(n, 1, -1), qn, self._ws_read)
+            elif self._fused_readout:  # q_norm, readout, LayerNorm and residual in one launch
                 r = K.swiglu_readout(y.view(n, 1, -1), self.w_up, self.w_gate, self.w_down, self.ln_weight,
                                      self.ln_bias, m.fast_weight_pool.eps, workspace=self._ws_read,
                                      x_norm=(qn.weight, qn.eps), row_counters=self._counters, sweep_reverse=rev)
@@ -231,6 +299,8 @@ class BatchedDecoder:
                                      sweep_reverse=rev)
             h = self._linear(r.view(n, -1), block.uttt.w_o.weight, residual=h)
         logits = self._linear(h, m.lm_head.weight, norm=m.norm)
+        if self.cache4 is not None:
+            K.kv_commit4(*self._new4, None, None, self.cache4, self.positions, self.window, self.sinks)
         self.logits = logits
         # temperature-0 selection: PAD / BOS / UNK and ids past the active vocabulary excluded,
         # written straight into the next step's input (stepping with `next_tokens` copies
@@ -240,6 +310,14 @@ class BatchedDecoder:
                                                out=self.tokens, advance=self.positions)
         else:
             self._sample(logits, advance=self.positions)
+
+    def _readout4(self, y: Tensor, norm, workspace: Optional[Tensor] = None) -> Tensor:
+        """q_norm (inside the call where it has an eps), readout, LayerNorm and residual through the fast weights in 4 bits."""
+        fused = (norm.eps or 0.0) > 0.0
+        if not fused:
+            y = F.rms_norm(y, (y.shape[-1],), norm.weight.to(y.dtype), norm.eps)
+        return K.readout4(y, *self.fast4, self.ln_weight, self.ln_bias, self.model.fast_weight_pool.eps,
+                          x_norm=(norm.weight, norm.eps) if fused else None, workspace=workspace)
 
     def _active_limit(self, logits: Tensor) -> Optional[int]:
         limit = self.model.active_vocab_limit
@@ -254,7 +332,9 @@ class BatchedDecoder:
     def _warm_workspaces(self) -> None:
         from . import _native as N
         lib = N.load_library()
-        if self.sinks:
+        if self.cache4 is not None:
+            nbytes = lib.uttt_swa_tree4_workspace(self.n, self.heads, self.hkv, 1, self.hd, self.window, self.sinks)
+        elif self.sinks:
             code = N.DTYPE_BF16 if self.dtype == torch.bfloat16 else N.DTYPE_F32
             nbytes = lib.uttt_swa_tree_workspace(self.n, self.heads, self.hkv, 1, self.hd, self.slots, code)
         else:
@@ -262,6 +342,9 @@ class BatchedDecoder:
         self._ws_attn = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=self.device)
         d = self.model.config.d_model
         ff = self.model.config.d_ff_fast
+        if self.fast4 is not None:
+            self._ws_read = K.readout4_workspace(self.n, 1, d, ff, self.device)
+            return
         code = N.DTYPE_BF16 if self.dtype == torch.bfloat16 else N.DTYPE_F32
         self._ws_read = torch.zeros(max(N.load_library().uttt_readout_workspace(self.n, 1, d, ff, code), 1),
                                     dtype=torch.uint8, device=self.device)
@@ -271,7 +354,7 @@ class BatchedDecoder:
         """Record one step into a HIP graph (after ``prefill``, or between steps); ``step`` then replays it.  What the
         decoder holds stays as it was: caches, positions, the tokens chosen last and their logits."""
         self._warm_workspaces()
-        held = [t for t in (self.positions, self.tokens, self.logprobs, self.k_rings, self.v_rings) if t is not None]
+        held = [t for t in (self.positions, self.tokens, self.logprobs, *self._caches()) if t is not None]
         saved = [t.clone() for t in held]
         chosen, logits = self.next_tokens, self.logits
         self._step_body()  # warm-up outside the graph (packs, tables, allocator)
@@ -408,16 +491,23 @@ class BatchedDecoder:
             q = qkv[..., :hq].unflatten(-1, (self.heads, self.hd))
             k = qkv[..., hq:hq + hk].unflatten(-1, (self.hkv, self.hd))
             v = qkv[..., hq + hk:].unflatten(-1, (self.hkv, self.hd))
-            att, _, _ = K.swa_tree(q, k, v, *self.rings[li], self.positions, parents, self.cos, self.sin, self.sinks,
-                                   counts, node_outputs=(k_nodes[li], v_nodes[li]))
+            new = dict(counts=counts, node_outputs=(k_nodes[li], v_nodes[li]))
+            if self.cache4 is not None:
+                att, _, _ = K.swa_tree4(q, k, v, self.cache4[li], self.positions, self.window, parents, self.cos, self.sin,
+                                        self.sinks, **new)
+            else:
+                att, _, _ = K.swa_tree(q, k, v, *self.rings[li], self.positions, parents, self.cos, self.sin, self.sinks, **new)
             h = self._linear(att.view(n * nodes, -1), attn.wo.weight, residual=h)
             y = self._linear(h, block.uttt.w_q.weight, norm=block.uttt_norm)
             qn = block.uttt.q_norm
-            uq = F.rms_norm(y, (h.shape[-1],), qn.weight.to(h.dtype), qn.eps).view(n, nodes, -1)
-            if read_ws is None:
-                read_ws = K.readout_workspace(uq, self.w_up)
-            r = K.swiglu_readout(uq, self.w_up, self.w_gate, self.w_down, self.ln_weight, self.ln_bias,
-                                 m.fast_weight_pool.eps, workspace=read_ws, sweep_reverse=li % 2 == 1)
+            if self.fast4 is not None:
+                r = self._readout4(y.view(n, nodes, -1), qn)
+            else:
+                uq = F.rms_norm(y, (h.shape[-1],), qn.weight.to(h.dtype), qn.eps).view(n, nodes, -1)
+                if read_ws is None:
+                    read_ws = K.readout_workspace(uq, self.w_up)
+                r = K.swiglu_readout(uq, self.w_up, self.w_gate, self.w_down, self.ln_weight, self.ln_bias,
+                                     m.fast_weight_pool.eps, workspace=read_ws, sweep_reverse=li % 2 == 1)
             h = self._linear(r.view(n * nodes, -1), block.uttt.w_o.weight, residual=h)
         logits = self._linear(h, m.lm_head.weight, norm=m.norm)
         self._nodes = (k_nodes, v_nodes)
@@ -441,9 +531,11 @@ class BatchedDecoder:
         if used.numel() and not 0 <= int(used.min()) <= int(used.max()) < k_nodes.shape[2]:
             raise ValueError("nodes must be nodes of the verified trees")
         self._nodes = None
-        K.kv_commit(k_nodes, v_nodes, path.to(device=self.device, dtype=torch.int32),
-                    torch.tensor(taken, dtype=torch.int32).to(self.device), self.k_rings, self.v_rings, self.positions,
-                    self.sinks, advance=True)
+        path, count = path.to(device=self.device, dtype=torch.int32), torch.tensor(taken, dtype=torch.int32).to(self.device)
+        if self.cache4 is not None:
+            K.kv_commit4(k_nodes, v_nodes, path, count, self.cache4, self.positions, self.window, self.sinks, advance=True)
+        else:
+            K.kv_commit(k_nodes, v_nodes, path, count, self.k_rings, self.v_rings, self.positions, self.sinks, advance=True)
         self.host_positions = [p + t for p, t in zip(self.host_positions, taken)]
 
     @torch.no_grad()
@@ -501,13 +593,66 @@ class BatchedDecoder:
             raise ValueError(f"sources must be {self.n} requests' indexes")
         self._nodes = None
         index = torch.tensor(src, dtype=torch.int32).to(self.device)
-        K.kv_fork(self.k_rings, self.v_rings, index, self.positions)
+        self._fork_caches(index)
         follow = [t for t in (self.tokens, self.logits, self.logprobs) if t is not None]
         if any(self._states[i] is not self._states[s] for i, s in enumerate(src)):
-            follow += [self.w_up, self.w_gate, self.w_down]
+            follow += [self.w_up, self.w_gate, self.w_down] if self.fast4 is None else [w.data for w in self.fast4]
         index = index.long()
         for t in follow:
             t.copy_(t.index_select(0, index))
         self.host_positions = [self.host_positions[s] for s in src]
         self._states = [self._states[s] for s in src]
         self._key = self._state_key(self._states)
+
+    def _fork_caches(self, sources: Tensor) -> None:
+        """Caches and positions by ``sources`` (N,) int32 on the device."""
+        if self.cache4 is not None:
+            K.kv_fork4(self.cache4, sources, self.positions, self.window, self.sinks)
+        else:
+            K.kv_fork(self.k_rings, self.v_rings, sources, self.positions)
+
+    # ------------------------------------------------------------------ beams
+    @torch.no_grad()
+    def beam_search(self, first_logits: Tensor, beams: int, steps: int, eos: Optional[int] = EOS_ID) -> Tuple[Tensor, Tensor]:
+        """The ``beams`` best continuations of ``steps`` tokens of each prompt that beam search finds: requests [g beams,
+        (g + 1) beams) are group g's, whose first one holds the prompt and the fast weights that all of its beams go on from
+        (the others' are taken over), ``first_logits`` (N, V) as of ``prefill`` with the prompt's in that row.  Every step chooses,
+        on the device, each group's best of score + log-probability (``kernels.beam_select``, PAD, BOS and UNK left out) and
+        reorders the caches by it; a beam that takes ``eos`` keeps its score from there and goes on with PAD.  Returns the tokens
+        (N / beams, beams, steps) int64 and their sums of log-probabilities (N / beams, beams), the best first; where fewer
+        continuations exist, PAD at -inf.  Request i then stands where beam i does, ready for the step with its last token
+        (``self.tokens``).  Refused while the decoder samples."""
+        if self._sampling is not None:
+            raise ValueError("the decoder samples; set_sampling(None) makes its choices greedy again")
+        if not 1 <= beams <= K.N.MAX_BEAMS or self.n % beams:
+            raise ValueError(f"beams must be 1 to {K.N.MAX_BEAMS} and divide the {self.n} requests")
+        if steps < 1 or first_logits.dim() != 2 or first_logits.shape[0] != self.n:
+            raise ValueError(f"steps must be at least 1 and first_logits ({self.n}, vocab)")
+        if max(self.host_positions[::beams]) + steps - 1 > self.cos.shape[0]:
+            raise ValueError("the continuations reach past the end of the RoPE table")
+        n, dev = self.n, self.device
+        if beams > 1:
+            self.fork([i // beams * beams for i in range(n)])
+        self._nodes = None
+        scores = torch.full((n,), float("-inf"), dtype=torch.float32, device=dev)
+        scores[::beams] = 0.0
+        ended = torch.zeros(n, dtype=torch.int32, device=dev)
+        logits, chosen = first_logits, []
+        for i in range(steps):
+            tokens, sources, scores, ended = K.beam_select(logits, scores, beams, ended, (PAD_ID, BOS_ID, UNK_ID),
+                                                           self._active_limit(logits), eos, PAD_ID)
+            chosen.append((tokens, sources))
+            if beams > 1:
+                self._fork_caches(sources)
+            if i + 1 < steps:
+                logits = self.step(tokens)
+        self.tokens.copy_(chosen[-1][0])
+        self.next_tokens = self.tokens
+        self.logits = logits.index_select(0, chosen[-1][1].long())
+        out = torch.empty((n, steps), dtype=torch.int64, device=dev)
+        at = torch.arange(n, device=dev)
+        for i in range(steps - 1, -1, -1):
+            tokens, sources = chosen[i]
+            out[:, i] = tokens[at]
+            at = sources.long()[at]
+        return out.view(-1, beams, steps), scores.view(-1, beams)
