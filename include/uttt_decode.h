@@ -50,8 +50,10 @@ typedef struct {
   const void* w; /* 16-byte aligned */
   const void* residual; int64_t residual_row_stride; /* NULL: none */
   void* out; int64_t out_row_stride;
+  void* workspace; size_t workspace_bytes; /* rewritten by each call; NULL where none is needed */
 } uttt_linear4_args;
 
+size_t uttt_linear4_workspace(int64_t m, int64_t k, int32_t act_dtype);
 int uttt_linear4(const uttt_linear4_args* args, uttt_stream_t stream);
 
 /* ---------------------------------------------------------------------------

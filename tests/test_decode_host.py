@@ -39,7 +39,7 @@ def test_declarations_belong_to_the_abi_version():
     """Other declarations take another UTTT_DECODE_ABI_VERSION: the digest changes together with it."""
     text = re.sub(r"/\*.*?\*/", " ", open(N.DECODE_HEADER_PATH).read(), flags=re.S)
     text = " ".join(re.sub(r"#define UTTT_DECODE_ABI_VERSION \d+", "", text).split())
-    assert (N.DECODE_ABI_VERSION, hashlib.sha256(text.encode()).hexdigest()[:16]) == (1, "012c2b2351689c1c")
+    assert (N.DECODE_ABI_VERSION, hashlib.sha256(text.encode()).hexdigest()[:16]) == (1, "b849dd2f076add7d")
 
 
 def test_library_without_these_entry_points_is_refused(tmp_path, monkeypatch):
@@ -222,7 +222,8 @@ def test_c_refusals(lib):
     a = N.Linear4Args(m=2, n=8, k=40, act_dtype=1, x=16, x_row_stride=40, w=32, out=64, out_row_stride=8)
     for field, value, match in (("act_dtype", 2, "act_dtype"), ("m", 0, "m, n and k"), ("k", 1 << 21, "m, n and k"),
                                 ("x_eps", math.nan, "x_eps"), ("x_eps", -1.0, "x_eps"), ("w", 40, "16-byte"), ("x", None, "non-NULL"),
-                                ("x_row_stride", 39, "row strides"), ("out_row_stride", 7, "row strides")):
+                                ("x_row_stride", 39, "row strides"), ("out_row_stride", 7, "row strides"),
+                                ("act_dtype", 0, "workspace too small")):
         bad = N.Linear4Args.from_buffer_copy(a)
         setattr(bad, field, value)
         refused_c(lib.uttt_linear4, bad, match)

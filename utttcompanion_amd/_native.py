@@ -343,6 +343,7 @@ class Linear4Args(C.Structure):
         ("m", _I64), ("n", _I64), ("k", _I64), ("act_dtype", _I32), ("x_eps", _F),
         ("x", _P), ("x_row_stride", _I64), ("w", _P),
         ("residual", _P), ("residual_row_stride", _I64), ("out", _P), ("out_row_stride", _I64),
+        ("workspace", _P), ("workspace_bytes", C.c_size_t),
     ]
 
 
@@ -445,6 +446,7 @@ SERVE_SIGNATURES = {
 
 DECODE_SIGNATURES = {
     "uttt_decode_abi_version": (C.c_int, []),
+    "uttt_linear4_workspace": (C.c_size_t, [_I64, _I64, _I32]),
     "uttt_linear4": (C.c_int, [_P, _P]),
     "uttt_readout4_workspace": (C.c_size_t, [_I64, _I64, _I64, _I64]),
     "uttt_readout4": (C.c_int, [_P, _P]),

@@ -1735,6 +1735,11 @@ def _weight4(w: Weight4, n: int, k: int, name: str, batch: Optional[int] = None)
     return address, stride
 
 
+@functools.lru_cache(maxsize=256)
+def _linear4_workspace(*sizes: int) -> int:
+    return N.load_library().uttt_linear4_workspace(*sizes)
+
+
 def linear4(x: Tensor, weight: Weight4, out: Optional[Tensor] = None, residual: Optional[Tensor] = None,
             x_eps: float = 0.0) -> Tensor:
     """out = x weight^T (+ residual) with a weight in 4 bits (``uttt_linear4``; ``pack_weight4``): the decode step's
@@ -1769,7 +1774,14 @@ def linear4(x: Tensor, weight: Weight4, out: Optional[Tensor] = None, residual: 
         p_r, r_stride = residual.data_ptr(), residual.stride(0)
     if m == 0:
         return out
-    packed = N.pack_linear4(m, n, k, code, x_eps, x.data_ptr(), x.stride(0), p_w, p_r, r_stride, out.data_ptr(), out.stride(0))
+    p_x, x_stride = x.data_ptr(), x.stride(0)
+    p_ws = nbytes = 0
+    if code == N.DTYPE_F32:
+        nbytes = _linear4_workspace(m, k, code)
+        if nbytes:
+            workspace = x.new_empty(nbytes, dtype=torch.uint8)
+            p_ws = workspace.data_ptr()
+    packed = N.pack_linear4(m, n, k, code, x_eps, p_x, x_stride, p_w, p_r, r_stride, out.data_ptr(), out.stride(0), p_ws, nbytes)
     _serve_call(N.load_library().uttt_linear4, packed, index, "uttt_linear4")
     return out
 
