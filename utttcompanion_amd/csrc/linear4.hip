@@ -374,12 +374,29 @@ struct Prod4Args {
   int64_t os_b, os_m;
 };
 
+// A product's element (m, n): the result, or with SWIGLU (y up, `gate` the gate's) the next product's operands.
+template <typename O, bool SWIGLU>
+__device__ __forceinline__ void finish_row(const Prod4Args& a, int b, int m, int n, float y, float gate) {
+  if (m >= a.m || n >= a.n) return;
+  if constexpr (SWIGLU) {
+    constexpr int HP = sizeof(O) == 2 ? 2 : 3;
+    bf16 p[HP];
+    bf16_parts(silu(gate) * y, p);
+    bf16* out = static_cast<bf16*>(a.out) + b * parts_of_batch(a.m, a.n, HP);
+#pragma unroll
+    for (int q = 0; q < HP; ++q) out[part_place(m, n, q, a.n / 32, HP)] = p[q];
+  } else {
+    if (a.r != nullptr) y += to_f32(static_cast<const O*>(a.r)[(int64_t)m * a.rs_m + n]);
+    (static_cast<O*>(a.out) + b * a.os_b)[(int64_t)m * a.os_m + n] = from_f32<O>(y);
+  }
+}
+
 // Grid (n / (16 NT), m / (16 MT), batch); the W waves divide the columns and meet in LDS.  Operands are loaded 64 columns
 // ahead, pieces of the weights 128.  Rows of one part go through LDS, a wave's own, 8 lanes to 128 bytes of a row: read as
 // operands, where neighbouring lanes are different rows, every lane would be an access of its own (32 rows by 8000 x 2048
 // took 12 us).
 template <typename O, int P, int MT, int NT, int W, bool SWIGLU>
-__global__ void __launch_bounds__(W * 64, W == 8 ? 1 : 2) k_prod4(const Prod4Args a) {
+__global__ void __launch_bounds__(W * 64, W == 4 ? 2 : 1) k_prod4(const Prod4Args a) {
   constexpr int kStage = P == 1 ? W * MT * 2048 : 0, kMeet = W * NT * MT * 1024;
   __shared__ __align__(16) char lds[kStage > kMeet ? kStage : kMeet];
   __shared__ float squares[W][MT * 16];
@@ -542,19 +559,169 @@ __global__ void __launch_bounds__(W * 64, W == 8 ? 1 : 2) k_prod4(const Prod4Arg
       for (int q = 0; q < W; ++q) q2 += squares[q][mm];
       y *= rsqrtf(q2 / (float)a.k + a.x_eps);
     }
-    const int n = (tile0 + s) * 16 + nn, m = m0 + mm;
-    if (m >= a.m || n >= a.n) continue;
-    if constexpr (SWIGLU) {
-      constexpr int HP = sizeof(O) == 2 ? 2 : 3;
-      bf16 p[HP];
-      bf16_parts(silu(gate) * y, p);
-      bf16* out = static_cast<bf16*>(a.out) + b * parts_of_batch(a.m, a.n, HP);
+    finish_row<O, SWIGLU>(a, b, m0 + mm, (tile0 + s) * 16 + nn, y, gate);
+  }
+}
+
+// Many blocks of W: WN waves beside each other take NT blocks of 16 rows each and share x, which passes through LDS in steps
+// that all of them load together; 8 / WN such teams divide the columns.  Of 32 rows by 32000 x 2048 the operands of x are
+// then a fourth of what every wave would fetch for itself.  Grid (n / (16 NT WN), m / (16 MT), batch).
+template <typename O, int MT, int NT, int WN>
+__global__ void __launch_bounds__(512, 2) k_share4(const Prod4Args a) {
+  constexpr int WK = 8 / WN;
+  constexpr int H = WN == 4 ? 2 : 1;            // halves (64 columns) of a step
+  constexpr int kStep = H * 2 * MT * 1024;      // bytes of a step of x
+  constexpr int kEach = kStep / 1024 / WN;      // 1 KB pieces of it that a wave loads: 8 rows of 64 columns
+  static_assert(kStep % (1024 * WN) == 0, "a team loads a step together");
+  constexpr int kStage = WK * 2 * kStep, kMeet = 8 * NT * MT * 1024;
+  __shared__ __align__(16) char lds[kStage > kMeet ? kStage : kMeet];
+  __shared__ float squares[WK][MT * 16];
+  const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wn = w % WN, wk = w / WN;
+  const int lane = threadIdx.x & 63, r = lane & 15, h = lane >> 4;
+  const int tiles = (a.n + 15) >> 4, tile0 = (blockIdx.x * WN + wn) * NT, m0 = blockIdx.y * (16 * MT), b = blockIdx.z;
+  const char* wp[NT];
 #pragma unroll
-      for (int q = 0; q < HP; ++q) out[part_place(m, n, q, a.n / 32, HP)] = p[q];
-    } else {
-      if (a.r != nullptr) y += to_f32(static_cast<const O*>(a.r)[(int64_t)m * a.rs_m + n]);
-      (static_cast<O*>(a.out) + b * a.os_b)[(int64_t)m * a.os_m + n] = from_f32<O>(y);
+  for (int s = 0; s < NT; ++s) wp[s] = a.w[0] + b * a.ws_b[0] + (int64_t)min(tile0 + s, tiles - 1) * a.blocks * kBlockBytes;
+  f32x4 acc[NT][MT], gram[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    gram[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < NT; ++s) acc[s][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  struct Weights {
+    u32x4 code[NT];
+    u32x2 scale[NT];
+  };
+  const int begin = a.blocks * wk / WK, end = a.blocks * (wk + 1) / WK, halves = (a.k + 63) >> 6;
+  const int steps = (a.blocks + WK - 1) / WK * (2 / H);  // of the longest team
+  const bf16* base = a.x + b * a.xs_b;
+  auto weights = [&](int kb) {
+    Weights v;
+    kb = min(kb, max(end - 1, 0));
+#pragma unroll
+    for (int s = 0; s < NT; ++s) {
+      const char* at = wp[s] + (int64_t)kb * kBlockBytes;
+      v.code[s] = *reinterpret_cast<const u32x4*>(at + lane * 16);
+      v.scale[s] = *reinterpret_cast<const u32x2*>(at + 1024 + r * 8);
     }
+    return v;
+  };
+  struct Pieces {
+    bf16x8 x[kEach];
+  };
+  auto load = [&](int half0) {
+    Pieces v;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int piece = i * WN + wn, half = min(half0 + piece / (2 * MT), halves - 1), k0 = half * 64 + 8 * (lane & 7);
+      const bf16* row = base + (int64_t)min(m0 + 8 * (piece % (2 * MT)) + (lane >> 3), a.m - 1) * a.xs_m;
+      v.x[i] = a.aligned && half * 64 + 64 <= a.k ? *reinterpret_cast<const bf16x8*>(row + k0) : load_x8(row, k0, a.k, a.aligned);
+    }
+    return v;
+  };
+  auto store = [&](const Pieces& v, int buf) {
+    char* to = lds + (wk * 2 + buf) * kStep;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int piece = i * WN + wn, t = 8 * (piece % (2 * MT)) + (lane >> 3);
+      *reinterpret_cast<bf16x8*>(to + piece / (2 * MT) * (MT * 2048) + t * 128 + (((lane & 7) ^ row_swz(t)) * 16)) = v.x[i];
+    }
+  };
+  auto multiply = [&](const Weights& q, int buf, int local, int half) {  // `half` of the block of columns, `local` of the step
+    const char* from = lds + (wk * 2 + buf) * kStep + local * (MT * 2048);
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      bf16x8 x[MT];
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        const int row = 16 * t + r;
+        x[t] = *reinterpret_cast<const bf16x8*>(from + row * 128 + (((4 * g + h) ^ row_swz(row)) * 16));
+      }
+      if (a.x_eps > 0.f && wn == 0) {  // a row's sum of squares: the diagonal of x x^T
+#pragma unroll
+        for (int t = 0; t < MT; ++t) gram[t] = mfma16(x[t], x[t], gram[t]);
+      }
+#pragma unroll
+      for (int s = 0; s < NT; ++s) {
+        const bf16x8 c = fp4_values(half ? q.code[s][2 + g] : q.code[s][g]);
+        const float f = bf16_of(half ? q.scale[s][1] : q.scale[s][0], g);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          const f32x4 y = mfma16(x[t], c, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[s][t][i] = fmaf(f, y[i], acc[s][t][i]);
+        }
+      }
+    }
+  };
+  // Step i of a team is in buffer i mod 2.  Behind the barrier that opens it nobody reads the other one any more, which
+  // takes step i + 1; the pieces of the four steps behind it and the next weights are on their way meanwhile.
+  constexpr int kWeights = H == 2 ? 4 : 2;
+  Weights q[kWeights];
+  Pieces pieces[4];
+  // loads come back in order: what the first step needs goes first
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    pieces[u] = load(2 * begin + u * H);
+    if (u < kWeights) q[u] = weights(begin + u);
+  }
+  store(pieces[0], 0);
+  pieces[0] = load(2 * begin + 4 * H);
+  for (int i0 = 0; i0 < steps; i0 += 4) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + u;
+      if (i >= steps) break;
+      __syncthreads();
+      store(pieces[(u + 1) & 3], (u + 1) & 1);
+      pieces[(u + 1) & 3] = load(2 * begin + (i + 5) * H);
+      const int kb = begin + i * H / 2;
+      if constexpr (H == 2) {
+        if (kb < end) {
+          multiply(q[u], u & 1, 0, 0);
+          if (2 * kb + 1 < halves) multiply(q[u], u & 1, 1, 1);
+        }
+        q[u] = weights(kb + 4);
+      } else {
+        if (kb < end && ((u & 1) == 0 || 2 * kb + 1 < halves)) multiply(q[u >> 1], u & 1, 0, u & 1);
+        if (u & 1) q[u >> 1] = weights(kb + 2);
+      }
+    }
+  }
+  if (a.x_eps > 0.f && wn == 0 && r >> 2 == h) {
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      const float lo = r & 1 ? gram[t][1] : gram[t][0], hi = r & 1 ? gram[t][3] : gram[t][2];
+      squares[wk][16 * t + r] = r & 2 ? hi : lo;
+    }
+  }
+  __syncthreads();
+  float* red = reinterpret_cast<float*>(lds);  // [team][wave of it][tile][4 t + i][lane]
+#pragma unroll
+  for (int s = 0; s < NT; ++s)
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) red[((w * NT + s) * (MT * 4) + 4 * t + i) * 64 + lane] = acc[s][t][i];
+  __syncthreads();
+  constexpr int kCols = 16 * NT * WN, kOuts = MT * 16 * kCols / 512 > 0 ? MT * 16 * kCols / 512 : 1;
+#pragma unroll
+  for (int o = 0; o < kOuts; ++o) {
+    const int idx = threadIdx.x + o * 512, col = idx % kCols, mm = idx / kCols;
+    if (mm >= 16 * MT) break;
+    const int nn = col & 15, s = (col >> 4) % NT, of_n = (col >> 4) / NT;
+    const int i = 4 * (mm >> 4) + (mm & 3), l = ((mm & 15) >> 2) * 16 + nn;
+    float y = 0.f;
+#pragma unroll
+    for (int q = 0; q < WK; ++q) y += red[(((q * WN + of_n) * NT + s) * (MT * 4) + i) * 64 + l];
+    if (a.x_eps > 0.f) {
+      float q2 = 0.f;
+#pragma unroll
+      for (int q = 0; q < WK; ++q) q2 += squares[q][mm];
+      y *= rsqrtf(q2 / (float)a.k + a.x_eps);
+    }
+    finish_row<O, false>(a, b, m0 + mm, blockIdx.x * kCols + col, y, 0.f);
   }
 }
 
@@ -567,25 +734,49 @@ void launch_parts(const Parts4Args& x, int batch, hipStream_t st) {
 template <typename O, int P, int NT, int W, bool SWIGLU>
 void launch_rows(const Prod4Args& p, int batch, hipStream_t st) {
   const int tiles = (p.n + 15) / 16, per = SWIGLU ? NT / 2 : NT;
-  const int mt = p.m <= 16 ? 1 : p.m <= 32 || P > 1 || NT > 2 ? 2 : 4;
+  const int mt = p.m <= 16 ? 1 : p.m <= 32 || P > 1 ? 2 : 4;
   const dim3 grid((unsigned)((tiles + per - 1) / per), (unsigned)((p.m + 16 * mt - 1) / (16 * mt)), (unsigned)batch), block(W * 64);
   if (mt == 1)
     hipLaunchKernelGGL((k_prod4<O, P, 1, NT, W, SWIGLU>), grid, block, 0, st, p);
   else if (mt == 2)
     hipLaunchKernelGGL((k_prod4<O, P, 2, NT, W, SWIGLU>), grid, block, 0, st, p);
-  else if constexpr (P == 1 && NT <= 2)
+  else if constexpr (P == 1)
     hipLaunchKernelGGL((k_prod4<O, P, 4, NT, W, SWIGLU>), grid, block, 0, st, p);
 }
 
+template <typename O, int NT, int WN>
+void launch_share(const Prod4Args& p, int batch, hipStream_t st) {
+  const int tiles = (p.n + 15) / 16, per = NT * WN, mt = p.m <= 16 ? 1 : p.m <= 32 ? 2 : 4;
+  const dim3 grid((unsigned)((tiles + per - 1) / per), (unsigned)((p.m + 16 * mt - 1) / (16 * mt)), (unsigned)batch);
+  if (mt == 1)
+    hipLaunchKernelGGL((k_share4<O, 1, NT, WN>), grid, dim3(512), 0, st, p);
+  else if (mt == 2)
+    hipLaunchKernelGGL((k_share4<O, 2, NT, WN>), grid, dim3(512), 0, st, p);
+  else
+    hipLaunchKernelGGL((k_share4<O, 4, NT, WN>), grid, dim3(512), 0, st, p);
+}
+
+// Measured, us, for rows x (n, k): one part, 32 x (32000, 2048): waves for themselves, 4 blocks of W each 17.1, sharing x,
+// teams of 4 with 2 blocks each 14.4; 32 x (16000, 2048): teams of 4 12.7, of 2 with one block each 10.1; 32 x (5504, 2048):
+// eight waves for themselves 7.3, teams of 2 6.8; of 2048 columns alike.  Three parts, which already are in the operands' order: 32
+// x (32000, 2048) sharing 23.8, for themselves 4 blocks each 21.5; 61 x (1999, 5501) sharing 30, eight waves to a block 29, 16 27.
 template <typename O, int P>
 void launch_linear_rows(const Prod4Args& p, int batch, hipStream_t st) {
-  const int64_t tiles = (p.n + 15) / 16;
-  if (tiles * batch >= 1024 && (P > 1 || p.m <= 32))
+  const int64_t tiles = (p.n + 15) / 16 * batch * ((p.m + 31) / 32);
+  if constexpr (P == 1) {
+    if (tiles >= 1536)
+      launch_share<O, 2, 4>(p, batch, st);
+    else if (tiles >= 192)
+      launch_share<O, 1, 2>(p, batch, st);
+    else
+      launch_rows<O, P, 1, 8, false>(p, batch, st);
+  } else if (tiles >= 768) {
     launch_rows<O, P, 4, 4, false>(p, batch, st);
-  else if (tiles * batch >= 512)
-    launch_rows<O, P, 2, 4, false>(p, batch, st);
-  else
+  } else if (p.blocks >= 16) {
+    launch_rows<O, P, 1, 16, false>(p, batch, st);
+  } else {
     launch_rows<O, P, 1, 8, false>(p, batch, st);
+  }
 }
 
 template <typename X, typename T, int P, Row MODE>
