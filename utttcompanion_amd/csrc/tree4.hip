@@ -12,6 +12,7 @@
 // weights are rounded to bf16 for bf16 activations and carried as three parts for fp32; sums are those of the unrounded ones.
 // The new tokens themselves are keys in LDS, in their own precision.
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/uttt_decode.h"
 #include "fp4.h"
@@ -21,9 +22,9 @@ namespace uttt {
 namespace {
 
 constexpr int kSlots = 32;
-constexpr int kWaves = 4;
 constexpr int kMaxNodes4 = 64;
 constexpr int kMaxSplits4 = 64;
+constexpr int kJoin = 4;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kSlack = 8.f;  // weights of up to 2^8 before the maximum moves
 
@@ -130,23 +131,23 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
   }
 }
 
-// KT: new tokens that fit, 32 or 64.
-template <typename T, int HD, int KT>
+// KT: new tokens that fit, 1 (which needs no LDS), 32 or 64; W: waves.
+template <typename T, int HD, int KT, int W>
 struct Smem4 {
   static constexpr int kParts = sizeof(T) == 2 ? 1 : 3;
-  static constexpr int kKeys = kParts * KT * (HD + 8) * 2;    // [part][node][HD + 8]
-  static constexpr int kValues = kParts * HD * (KT + 8) * 2;  // [part][HD][KT + 8]
-  static constexpr int kMeet = kWaves * 16 * (HD + 4) * 4;    // [wave][row][HD + 4]
+  static constexpr int kKeys = KT == 1 ? 0 : kParts * KT * (HD + 8) * 2;    // [part][node][HD + 8]
+  static constexpr int kValues = KT == 1 ? 0 : kParts * HD * (KT + 8) * 2;  // [part][HD][KT + 8]
+  static constexpr int kMeet = W * 16 * (HD + 4) * 4;    // [wave][row][HD + 4]
   static constexpr int kBytes = kKeys + kValues > kMeet ? kKeys + kValues : kMeet;
 };
 
-template <typename T, int HD, int KT>
-__global__ void __launch_bounds__(kWaves * 64) k_swa_tree4(const Tree4Args a) {
+template <typename T, int HD, int KT, int W>
+__global__ void __launch_bounds__(W * 64, W == 4 ? 2 : 1) k_swa_tree4(const Tree4Args a) {
   constexpr int G = HD / 32, D = HD / 16;
   constexpr int QP = sizeof(T) == 2 ? 2 : 3, PP = sizeof(T) == 2 ? 1 : 3, KP = PP;
-  using S = Smem4<T, HD, KT>;
+  using S = Smem4<T, HD, KT, W>;
   __shared__ __align__(16) char smem[S::kBytes];
-  __shared__ float ml[kWaves][16][2];
+  __shared__ float ml[W][16][2];
   __shared__ int odd;
   const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, h = lane >> 4;
   int id = blockIdx.x;
@@ -163,7 +164,7 @@ __global__ void __launch_bounds__(kWaves * 64) k_swa_tree4(const Tree4Args a) {
   T* out = static_cast<T*>(a.out);
   const int n_heads = a.n_kv_heads * a.rep;
   if (tree.bad) {
-    for (int i = threadIdx.x; i < 16 * HD; i += kWaves * 64) {
+    for (int i = threadIdx.x; i < 16 * HD; i += W * 64) {
       const int ri = row0 + i / HD, e = i % HD;
       if (ri >= live) break;
       const int nd = ri / a.rep, hd = kvh * a.rep + ri % a.rep;
@@ -183,27 +184,72 @@ __global__ void __launch_bounds__(kWaves * 64) k_swa_tree4(const Tree4Args a) {
   const int depth = __shfl(tree.depth, node, 64);
   const uint64_t sees = shfl64(tree.sees, node);
 
+  // the cached tokens: blocks of sinks, then of the ring, a wave every fourth of this split's
+  const int sink_held = (int)min(tree.pos, (int64_t)a.sinks);
+  const int ring_held = (int)min(max(tree.pos - a.sinks, (int64_t)0), (int64_t)a.window);
+  // the slot that the next token takes (a 64-bit remainder costs hundreds of instructions)
+  const int64_t past = max(tree.pos - a.sinks, (int64_t)0);
+  const int newest = past >> 32 ? (int)(past % a.window) : (int)((uint32_t)past % (uint32_t)a.window);
+  const int sink_n = (sink_held + kSlots - 1) / kSlots, total = sink_n + (ring_held + kSlots - 1) / kSlots;
+  const int begin = (int)((int64_t)total * split / a.nsplit), end = (int)((int64_t)total * (split + 1) / a.nsplit);
+  const char* cache = a.cache + n * a.c_n + (int64_t)kvh * (a.sink_blocks + a.ring_blocks) * (36 * HD);
+  struct Block {
+    u32x4 kc[HD / 64], vc[HD / 64], ks[G], vs[G];
+  };
+  auto fetch = [&](int b) {
+    Block x;
+    const char* at = cache + (int64_t)(b < sink_n ? b : a.sink_blocks + b - sink_n) * (36 * HD);
+#pragma unroll
+    for (int q = 0; q < HD / 64; ++q) x.kc[q] = *reinterpret_cast<const u32x4*>(at + 1024 * q + 16 * lane);
+#pragma unroll
+    for (int g = 0; g < G; ++g) x.ks[g] = *reinterpret_cast<const u32x4*>(at + 32 * HD + 64 * g + 16 * h);
+#pragma unroll
+    for (int q = 0; q < HD / 64; ++q) x.vc[q] = *reinterpret_cast<const u32x4*>(at + 16 * HD + 1024 * q + 16 * lane);
+#pragma unroll
+    for (int g = 0; g < G; ++g) x.vs[g] = *reinterpret_cast<const u32x4*>(at + 34 * HD + 64 * g + 16 * h);
+    return x;
+  };
+  const int age_limit = min(ring_held, a.window - 1 - depth);  // tokens of the ring that this row sees, from the newest on
+  const int age_clean = min(ring_held, a.window - 1 - tree.deepest);
+  constexpr bool kAhead = sizeof(T) == 2 || HD == 64;  // three parts of 128 elements leave no registers to load ahead
+  Block next{};
+  if (kAhead && begin + w < end) next = fetch(begin + w);
+
+  f32x4 o[D];
+#pragma unroll
+  for (int d = 0; d < D; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+
   // this lane's row of q: elements 32 g + 8 h .., rotated, scaled, in parts
   bf16x8 qf[G][QP];
   {
     const T* qp = static_cast<const T*>(a.q) + n * a.q_n + node * a.q_t + head * a.q_h + 8 * h;
-    float x[G][8];
+    const int64_t at = (tree.pos + depth) * HD + 8 * h;
+    const bool single = KT == 1 && split == 0 && w == 0;  // this wave takes the one new token
+    const int64_t k_at = n * a.k_n + kvh * a.k_h + 8 * h;
+    float x[G][8], k[G][8];
 #pragma unroll
-    for (int g = 0; g < G; ++g) load8(qp + 32 * g, x[g]);
-    if (a.cos_table != nullptr) {
-      const int64_t at = (tree.pos + depth) * HD + 8 * h;
+    for (int g = 0; g < G; ++g) {
+      load8(qp + 32 * g, x[g]);
+      if (single) load8(static_cast<const T*>(a.k) + k_at + 32 * g, k[g]);
+    }
 #pragma unroll
-      for (int g = 0; g < G / 2; ++g) {
-        float c0[8], s0[8], c1[8], s1[8];
-        load8(a.cos_table + at + 32 * g, c0);
-        load8(a.sin_table + at + 32 * g, s0);
-        load8(a.cos_table + at + 32 * (g + G / 2), c1);
-        load8(a.sin_table + at + 32 * (g + G / 2), s1);
+    for (int g = 0; g < G / 2; ++g) {
+      if (a.cos_table == nullptr) break;
+      float c0[8], s0[8], c1[8], s1[8];
+      load8(a.cos_table + at + 32 * g, c0);
+      load8(a.sin_table + at + 32 * g, s0);
+      load8(a.cos_table + at + 32 * (g + G / 2), c1);
+      load8(a.sin_table + at + 32 * (g + G / 2), s1);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float lo = x[g][j], hi = x[g + G / 2][j];
-          x[g][j] = fmaf(lo, c0[j], -(hi * s0[j]));
-          x[g + G / 2][j] = fmaf(hi, c1[j], lo * s1[j]);
+      for (int j = 0; j < 8; ++j) {
+        const float lo = x[g][j], hi = x[g + G / 2][j];
+        x[g][j] = fmaf(lo, c0[j], -(hi * s0[j]));
+        x[g + G / 2][j] = fmaf(hi, c1[j], lo * s1[j]);
+        if (single) {
+          const float k0 = k[g][j], k1 = k[g + G / 2][j];
+          k[g][j] = fmaf(k0, c0[j], -(k1 * s0[j]));
+          k[g + G / 2][j] = fmaf(k1, c1[j], k0 * s1[j]);
         }
       }
     }
@@ -211,21 +257,48 @@ __global__ void __launch_bounds__(kWaves * 64) k_swa_tree4(const Tree4Args a) {
     for (int g = 0; g < G; ++g)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
+        x[g][j] *= a.scale;
         bf16 p[QP];
-        bf16_parts(x[g][j] * a.scale, p);
+        bf16_parts(x[g][j], p);
 #pragma unroll
         for (int i = 0; i < QP; ++i) qf[g][i][j] = p[i];
       }
+    if (single) {  // the one new token is seen by every row: the softmax starts with it
+      float s = 0.f;
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s = fmaf(x[g][j], to_f32(from_f32<T>(k[g][j])), s);
+      s += __shfl_xor(s, 16, 64);
+      s += __shfl_xor(s, 32, 64);
+      m = s;
+      l = h == 0 ? (fabsf(s) < INFINITY ? 1.f : NAN) : 0.f;
+      const T* vp = static_cast<const T*>(a.v) + n * a.v_n + kvh * a.v_h;
+#pragma unroll
+      for (int d = 0; d < D; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[d][i] = to_f32(vp[16 * d + 4 * h + i]);
+      if (a.k_nodes != nullptr && group == 0 && r == 0) {
+        const int64_t to = n * a.nodes_n + (int64_t)kvh * HD + 8 * h;
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          float v[8];
+          load8(vp + 32 * g + 8 * h, v);
+          store8(static_cast<T*>(a.k_nodes) + to + 32 * g, k[g]);
+          store8(static_cast<T*>(a.v_nodes) + to + 32 * g, v);
+        }
+      }
+    }
   }
 
   // the new tokens' keys, rotated and rounded, and values into LDS (and out, for the caches)
   bf16* keys = reinterpret_cast<bf16*>(smem);
   bf16* vals = reinterpret_cast<bf16*>(smem + S::kKeys);
   if (threadIdx.x == 0) odd = 0;
-  if (split == 0) {
+  if (KT > 1 && split == 0) {
     __syncthreads();
     bool strange = false;
-    for (int i = threadIdx.x; i < KT * (HD / 16); i += kWaves * 64) {
+    for (int i = threadIdx.x; i < KT * (HD / 16); i += W * 64) {
       const int nd = i / (HD / 16), e = i % (HD / 16) * 8;  // elements e .. and HD / 2 + e ..
       float k0[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, k1[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       float v0[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, v1[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -282,13 +355,8 @@ __global__ void __launch_bounds__(kWaves * 64) k_swa_tree4(const Tree4Args a) {
     if (strange) odd = 1;
   }
 
-  f32x4 o[D];
-#pragma unroll
-  for (int d = 0; d < D; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;
-
   // the softmax's step: scores (masked: -inf) of 8 keys to weights, the sums so far rescaled where the maximum moves
-  auto weigh = [&](float (&s)[8]) {
+  auto weigh = [&](float (&s)[8], auto clean) {
     float mx = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
     if (__any(mx > m + kSlack)) {
       mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
@@ -303,35 +371,15 @@ __global__ void __launch_bounds__(kWaves * 64) k_swa_tree4(const Tree4Args a) {
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      s[j] = s[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s[j] - m);
+      const float e = __builtin_amdgcn_exp2f(s[j] - m);
+      s[j] = !decltype(clean)::value && s[j] == -INFINITY ? 0.f : e;
       l += s[j];
     }
   };
 
-  // the cached tokens: blocks of sinks, then of the ring, a wave every fourth of this split's
-  const int sink_held = (int)min(tree.pos, (int64_t)a.sinks);
-  const int ring_held = (int)min(max(tree.pos - a.sinks, (int64_t)0), (int64_t)a.window);
-  const int newest = ring_held > 0 ? (int)((tree.pos - a.sinks) % a.window) : 0;  // the slot that the next token takes
-  const int sink_n = (sink_held + kSlots - 1) / kSlots, total = sink_n + (ring_held + kSlots - 1) / kSlots;
-  const int begin = (int)((int64_t)total * split / a.nsplit), end = (int)((int64_t)total * (split + 1) / a.nsplit);
-  const int age_limit = min(ring_held, a.window - 1 - depth);  // tokens of the ring that this row sees, from the newest on
-  const int age_clean = min(ring_held, a.window - 1 - tree.deepest);
-  const char* cache = a.cache + n * a.c_n + (int64_t)kvh * (a.sink_blocks + a.ring_blocks) * (36 * HD);
-  for (int b = begin + w; b < end; b += kWaves) {
-    const bool sink = b < sink_n;
-    const int first = (sink ? b : b - sink_n) * kSlots;  // the block's first slot in its region
-    const char* at = cache + (int64_t)(sink ? b : a.sink_blocks + b - sink_n) * (36 * HD);
-    u32x4 kc[HD / 64], vc[HD / 64], ks[G], vs[G];
-#pragma unroll
-    for (int q = 0; q < HD / 64; ++q) {
-      kc[q] = *reinterpret_cast<const u32x4*>(at + 1024 * q + 16 * lane);
-      vc[q] = *reinterpret_cast<const u32x4*>(at + 16 * HD + 1024 * q + 16 * lane);
-    }
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-      ks[g] = *reinterpret_cast<const u32x4*>(at + 32 * HD + 64 * g + 16 * h);
-      vs[g] = *reinterpret_cast<const u32x4*>(at + 34 * HD + 64 * g + 16 * h);
-    }
+  // One block: every slot seen by every row (CLEAN), or each by itself.
+  auto attend = [&](const Block& x, auto clean, int first, bool sink) {
+    constexpr bool CLEAN = decltype(clean)::value;
     float s[8];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -339,19 +387,15 @@ __global__ void __launch_bounds__(kWaves * 64) k_swa_tree4(const Tree4Args a) {
       for (int i = 0; i < 4; ++i) s[4 * t + i] = 0.f;
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        const bf16x8 k = fp4_values(kc[(t * G + g) >> 2][(t * G + g) & 3]);
+        const bf16x8 k = fp4_values(x.kc[(t * G + g) >> 2][(t * G + g) & 3]);
         f32x4 y{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < QP; ++i) y = mfma16(k, qf[g][i], y);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[4 * t + i] = fmaf(bf16_of(ks[g][2 * t + (i >> 1)], i & 1), y[i], s[4 * t + i]);
+        for (int i = 0; i < 4; ++i) s[4 * t + i] = fmaf(bf16_of(x.ks[g][2 * t + (i >> 1)], i & 1), y[i], s[4 * t + i]);
       }
     }
-    // all 32 slots seen by every row: ages fall from the block's first slot on, unless the newest slot lies inside
-    const int oldest = first < newest ? newest - 1 - first : newest - 1 - first + a.window;
-    const bool clean = sink ? first + kSlots <= sink_held
-                            : first + kSlots <= a.window && !(first < newest && newest < first + kSlots) && oldest < age_clean;
-    if (!clean) {
+    if constexpr (!CLEAN) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int slot = first + 16 * (j >> 2) + 4 * h + (j & 3);
@@ -360,29 +404,42 @@ __global__ void __launch_bounds__(kWaves * 64) k_swa_tree4(const Tree4Args a) {
         s[j] = seen ? s[j] : -INFINITY;
       }
     }
-    weigh(s);
+    weigh(s, clean);
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       bf16x8 p[PP];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        float x = s[j] * bf16_of(vs[g][j >> 1], j & 1);
-        if (!clean) x = s[j] == 0.f ? 0.f : x;  // scales of slots that are not seen may be anything
+        float z = s[j] * bf16_of(x.vs[g][j >> 1], j & 1);
+        if constexpr (!CLEAN) z = s[j] == 0.f ? 0.f : z;  // scales of slots that are not seen may be anything
         bf16 part[PP];
-        bf16_parts(x, part);
+        bf16_parts(z, part);
 #pragma unroll
         for (int i = 0; i < PP; ++i) p[i][j] = part[i];
       }
 #pragma unroll
       for (int d = 2 * g; d < 2 * g + 2; ++d) {
-        const bf16x8 v = fp4_values(vc[d >> 2][d & 3]);
+        const bf16x8 v = fp4_values(x.vc[d >> 2][d & 3]);
 #pragma unroll
         for (int i = 0; i < PP; ++i) o[d] = mfma16(v, p[i], o[d]);
       }
     }
+  };
+  for (int b = begin + w; b < end; b += W) {
+    const Block now = kAhead ? next : fetch(b);
+    if (kAhead && b + W < end) next = fetch(b + W);
+    const bool sink = b < sink_n;
+    const int first = (sink ? b : b - sink_n) * kSlots;  // the block's first slot in its region
+    // ages fall from the block's first slot on, unless the newest slot lies inside
+    const int oldest = first < newest ? newest - 1 - first : newest - 1 - first + a.window;
+    if (sink ? first + kSlots <= sink_held
+             : first + kSlots <= a.window && !(first < newest && newest < first + kSlots) && oldest < age_clean)
+      attend(now, std::true_type{}, first, sink);
+    else
+      attend(now, std::false_type{}, first, sink);
   }
 
-  if (split == 0) {
+  if (KT > 1 && split == 0) {
     __syncthreads();
     const int b = w;  // of the new tokens' blocks
     if (b * kSlots < min(KT, tree.count)) {
@@ -405,7 +462,7 @@ __global__ void __launch_bounds__(kWaves * 64) k_swa_tree4(const Tree4Args a) {
           s[4 * t + i] = (sees >> key) & 1 ? y[i] : -INFINITY;
         }
       }
-      weigh(s);
+      weigh(s, std::false_type{});
       bf16x8 p[PP];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -428,6 +485,7 @@ __global__ void __launch_bounds__(kWaves * 64) k_swa_tree4(const Tree4Args a) {
       if (odd) {  // infinities and NaN among the values, a key at a time, where its weight is not 0
 #pragma unroll
         for (int j = 0; j < 8; ++j)
+#pragma unroll 1
           for (int hh = 0; hh < 4; ++hh) {
             const float x = __shfl(s[j], 16 * hh + r, 64);
             const int key = b * kSlots + 16 * (j >> 2) + 4 * hh + (j & 3);
@@ -457,14 +515,14 @@ __global__ void __launch_bounds__(kWaves * 64) k_swa_tree4(const Tree4Args a) {
     ml[w][r][1] = l;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < 16 * HD; i += kWaves * 64) {
+  for (int i = threadIdx.x; i < 16 * HD; i += W * 64) {
     const int rr = i / HD, e = i % HD, ri = row0 + rr;
     if (ri >= live) break;
     float top = -INFINITY, den = 0.f, num = 0.f;
 #pragma unroll
-    for (int x = 0; x < kWaves; ++x) top = fmaxf(top, ml[x][rr][0]);
+    for (int x = 0; x < W; ++x) top = fmaxf(top, ml[x][rr][0]);
 #pragma unroll
-    for (int x = 0; x < kWaves; ++x) {
+    for (int x = 0; x < W; ++x) {
       const float f = ml[x][rr][0] == -INFINITY ? (ml[x][rr][1] == 0.f ? 0.f : NAN) : __builtin_amdgcn_exp2f(ml[x][rr][0] - top);
       den = fmaf(f, ml[x][rr][1], den);
       num = f == 0.f ? num : fmaf(f, meet[(x * 16 + rr) * (HD + 4) + e], num);
@@ -494,15 +552,32 @@ __global__ void __launch_bounds__(kThreads) k_swa_tree4_join(const Tree4Args a) 
   const int node = (int)(row % a.nodes), head = (int)(row / a.nodes % n_heads), n = (int)(row / a.nodes / n_heads);
   if (a.counts != nullptr && node >= a.counts[n]) return;
   float top = -INFINITY, den = 0.f;
-  for (int s = 0; s < a.nsplit; ++s) top = fmaxf(top, a.part_ml[2 * (s * rows + row)]);
   f32x4 num{0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < a.nsplit; ++s) {
-    const float m = a.part_ml[2 * (s * rows + row)], l = a.part_ml[2 * (s * rows + row) + 1];
-    const float f = m == -INFINITY ? (l == 0.f ? 0.f : NAN) : __builtin_amdgcn_exp2f(m - top);
-    den = fmaf(f, l, den);
-    const f32x4 o = *reinterpret_cast<const f32x4*>(a.part_o + (s * rows + row) * HD + e);
+  for (int s0 = 0; s0 < a.nsplit; s0 += kJoin) {  // the loads of kJoin splits at once
+    float2 ml[kJoin];
+    f32x4 o[kJoin];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) num[i] = f == 0.f ? num[i] : fmaf(f, o[i], num[i]);
+    for (int u = 0; u < kJoin; ++u) {
+      const int64_t part = min(s0 + u, a.nsplit - 1) * rows + row;
+      ml[u] = *reinterpret_cast<const float2*>(a.part_ml + 2 * part);
+      o[u] = *reinterpret_cast<const f32x4*>(a.part_o + part * HD + e);
+    }
+    float next = top;
+#pragma unroll
+    for (int u = 0; u < kJoin; ++u) next = s0 + u < a.nsplit ? fmaxf(next, ml[u].x) : next;
+    const float back = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - next);
+    top = next;
+    den = den == 0.f ? 0.f : den * back;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) num[i] = back == 0.f ? 0.f : num[i] * back;
+#pragma unroll
+    for (int u = 0; u < kJoin; ++u) {
+      if (s0 + u >= a.nsplit) break;
+      const float f = ml[u].x == -INFINITY ? (ml[u].y == 0.f ? 0.f : NAN) : __builtin_amdgcn_exp2f(ml[u].x - top);
+      den = fmaf(f, ml[u].y, den);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) num[i] = f == 0.f ? num[i] : fmaf(f, o[u][i], num[i]);
+    }
   }
   T* out = static_cast<T*>(a.out) + n * a.o_n + node * a.o_t + head * a.o_h + e;
 #pragma unroll
@@ -510,26 +585,37 @@ __global__ void __launch_bounds__(kThreads) k_swa_tree4_join(const Tree4Args a) 
 }
 
 struct Plan4 {
-  int groups, nsplit;
+  int groups, nsplit, waves;
 };
 
 Plan4 plan_tree4(int64_t n_req, int64_t n_heads, int64_t n_kv_heads, int64_t nodes, int64_t blocks) {
   Plan4 p;
   p.groups = (int)((n_heads / n_kv_heads * nodes + 15) / 16);
   const int64_t base = n_req * n_kv_heads * p.groups;
-  p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({512 / base, blocks / 8, (int64_t)kMaxSplits4}));
+  p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({512 / base, blocks / 24, (int64_t)kMaxSplits4}));
+  p.waves = base * p.nsplit <= 256 ? 8 : 4;
   return p;
 }
 
 int64_t blocks_of(int64_t window, int64_t sinks) { return (window + kSlots - 1) / kSlots + (sinks + kSlots - 1) / kSlots; }
 
-template <typename T, int HD>
-void launch_tree4(const Tree4Args& m, hipStream_t st) {
+template <typename T, int HD, int KT>
+void launch_tree4(const Tree4Args& m, int waves, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)m.n_req * m.n_kv_heads * m.nsplit * m.groups));
-  if (m.nodes <= 32)
-    hipLaunchKernelGGL((k_swa_tree4<T, HD, 32>), grid, dim3(kWaves * 64), 0, st, m);
+  if (waves == 4)
+    hipLaunchKernelGGL((k_swa_tree4<T, HD, KT, 4>), grid, dim3(256), 0, st, m);
   else
-    hipLaunchKernelGGL((k_swa_tree4<T, HD, 64>), grid, dim3(kWaves * 64), 0, st, m);
+    hipLaunchKernelGGL((k_swa_tree4<T, HD, KT, 8>), grid, dim3(512), 0, st, m);
+}
+
+template <typename T, int HD>
+void launch_tree4(const Tree4Args& m, int waves, hipStream_t st) {
+  if (m.nodes == 1)
+    launch_tree4<T, HD, 1>(m, waves, st);
+  else if (m.nodes <= 32)
+    launch_tree4<T, HD, 32>(m, waves, st);
+  else
+    launch_tree4<T, HD, 64>(m, waves, st);
   if (m.nsplit > 1) {
     const int64_t n = (int64_t)m.n_req * m.n_kv_heads * m.rows * (HD / 4);
     hipLaunchKernelGGL((k_swa_tree4_join<T, HD>), dim3((unsigned)((n + kThreads - 1) / kThreads)), dim3(kThreads), 0, st, m);
@@ -600,8 +686,8 @@ extern "C" int uttt_swa_tree4(const uttt_swa_tree4_args* a, uttt_stream_t stream
   hipStream_t st = static_cast<hipStream_t>(stream);
   const bool b16 = a->act_dtype == UTTT_DTYPE_BF16;
   if (a->head_dim == 64)
-    b16 ? launch_tree4<bf16, 64>(m, st) : launch_tree4<float, 64>(m, st);
+    b16 ? launch_tree4<bf16, 64>(m, p.waves, st) : launch_tree4<float, 64>(m, p.waves, st);
   else
-    b16 ? launch_tree4<bf16, 128>(m, st) : launch_tree4<float, 128>(m, st);
+    b16 ? launch_tree4<bf16, 128>(m, p.waves, st) : launch_tree4<float, 128>(m, p.waves, st);
   return launch_status("uttt_swa_tree4");
 }
