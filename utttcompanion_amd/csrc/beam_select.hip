@@ -4,11 +4,10 @@
 // precision, so that the order of candidates of different beams is the definition's; the exponentials are fp32 ones (their
 // errors average out far below what separates two beams), their sums 64-bit ones.
 //
-// Within a row the order is that of (logit, id), so the first launch, a workgroup per stretch of a row with the stretch in
-// registers, finds each stretch's maximum, sum and `beams` best by (logit, id) alone.  No sort: the beams-th largest of a
-// wave's 64 lane maxima, found bit by bit with ballots, is a bound that at least `beams` elements reach; the few that
-// reach the largest bound of the waves are listed in LDS and ranked against each other.  The second launch, a workgroup per
-// group, does the same with the stretches' best and their values.
+// Within a row the order is that of (logit, id), so the first launch, a workgroup per part of a row, finds each part's maximum,
+// sum and `beams` best by (logit, id) alone.  No sort: the beams-th largest of a wave's 64 lane maxima, found bit by bit
+// with ballots, is a bound that at least `beams` elements reach; the few that reach it are listed in LDS and, at the end,
+// ranked against each other.  The second launch, a workgroup per group, does the same with the parts' best and their values.
 #include <algorithm>
 
 #include "../../include/uttt_decode.h"
@@ -21,11 +20,13 @@ namespace {
 constexpr int kMaxBeams = 32;
 constexpr int kPer = 16;                     // elements of a thread
 constexpr int kStretch = kThreads * kPer;    // of a workgroup
-constexpr int kListed = 1024;                // elements at the bound that LDS holds; more (equal logits) are chosen one by one
+constexpr int kListed = 512;                 // elements at the bound that a list holds; more (equal logits) are chosen one by one
 constexpr int kMergeThreads = 1024;
+constexpr int kFill = 1024;                  // workgroups that parts of rows are cut into, where there are fewer rows
+constexpr float kLog2e = 1.44269504088896340736f;
 
 struct BeamArgs {
-  int rows, beams, splits, n_banned;
+  int rows, beams, parts, n_banned;
   int64_t vocab, limit;
   int banned[8];
   const void* logits;
@@ -37,9 +38,9 @@ struct BeamArgs {
   int32_t* sources;
   float* out_scores;
   int32_t* ended_out;
-  double* sums;      // (rows, splits)
-  uint64_t* best;    // (rows, splits, beams): ordered logit above, ~id below; 0: none
-  float* tops;       // (rows, splits)
+  double* sums;      // (rows, parts)
+  uint64_t* best;    // (rows, parts, beams): ordered logit above, ~id below; 0: none
+  float* tops;       // (rows, parts)
 };
 
 // Floats in the order of unsigned integers (NaN apart), and back.
@@ -58,11 +59,12 @@ __device__ __forceinline__ double unordered(uint64_t k) {
   return __longlong_as_double((long long)(k >> 63 ? k & ~(1ull << 63) : ~k));
 }
 
-// The largest key that at least `want` lanes reach.
+// The largest key of BITS upper bits that at least `want` lanes reach.
+template <int BITS>
 __device__ __forceinline__ uint32_t reached_by(uint32_t key, int want) {
   uint32_t t = 0;
 #pragma unroll
-  for (int bit = 31; bit >= 0; --bit) {
+  for (int bit = 31; bit >= 32 - BITS; --bit) {
     const uint32_t next = t | 1u << bit;
     if (__popcll(__ballot(key >= next)) >= want) t = next;
   }
@@ -79,101 +81,157 @@ __device__ __forceinline__ uint64_t wave_max64(uint64_t x) {
   return x;
 }
 
-// Grid (stretches, rows).
+// Grid (parts of a row, rows).  A part's stretches pass through registers, the next one on its way: each thread keeps the
+// maximum and the sum of what it has seen, each wave the bound that its lanes' maxima give (it only rises, so what is not listed
+// when it passes by is never among the best) and the list of what reached it.  The waves meet at the end.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) k_beam_part(const BeamArgs a) {
-  constexpr int kVec = Lanes16<T>::kVec;
-  __shared__ uint64_t list[kListed];
-  __shared__ uint64_t wide[kThreads / 64];
-  __shared__ float tops[kThreads / 64];
-  __shared__ double sums[kThreads / 64];
-  __shared__ uint32_t bounds[kThreads / 64];
-  __shared__ int listed;
-  const int row = blockIdx.y, split = blockIdx.x, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  constexpr int kVec = Lanes16<T>::kVec, kWaves = kThreads / 64;
+  __shared__ uint64_t lists[kWaves][kListed];
+  __shared__ uint64_t best_of[kListed];
+  __shared__ uint64_t wide[kWaves];
+  __shared__ float tops[kWaves];
+  __shared__ double sums[kWaves];
+  __shared__ uint32_t bounds[kWaves];
+  __shared__ int counts[kWaves];
+  __shared__ int chosen;
+  const int row = blockIdx.y, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (a.ended_in != nullptr && a.ended_in[row] != 0) return;  // its one continuation needs no logit
   const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
-  const int64_t base = (int64_t)split * kStretch;
   const bool aligned = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-  float v[kPer];
+  const int limit = (int)a.limit, vocab = (int)a.vocab;
+  const int all = (limit + kStretch - 1) / kStretch;
+  const int begin = (int)((int64_t)all * blockIdx.x / a.parts), end = (int)((int64_t)all * (blockIdx.x + 1) / a.parts);
   // element j of a thread is id base + at(j); 16-byte pieces where the row allows them, single ones otherwise
   auto at = [&](int j) {
     return aligned ? ((j / kVec) * kThreads + (int)threadIdx.x) * kVec + j % kVec : j * kThreads + (int)threadIdx.x;
   };
-  if (aligned && base + kStretch <= a.vocab) {
-    uint4 piece[kPer / kVec];
+  struct Values {
+    float v[kPer];
+  };
+  auto load = [&](int i) {
+    Values r;
+    const int base = i * kStretch;
+    if (aligned && base + kStretch <= vocab) {
+      uint4 piece[kPer / kVec];
 #pragma unroll
-    for (int c = 0; c < kPer / kVec; ++c) piece[c] = *reinterpret_cast<const uint4*>(x + base + at(c * kVec));
+      for (int c = 0; c < kPer / kVec; ++c) piece[c] = *reinterpret_cast<const uint4*>(x + base + at(c * kVec));
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) v[j] = Lanes16<T>::get(piece[j / kVec], j % kVec);
-  } else {
+      for (int j = 0; j < kPer; ++j) r.v[j] = Lanes16<T>::get(piece[j / kVec], j % kVec);
+    } else {
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) v[j] = base + at(j) < a.vocab ? to_f32(x[base + at(j)]) : -INFINITY;
-  }
-  if (threadIdx.x == 0) listed = 0;
+      for (int j = 0; j < kPer; ++j) r.v[j] = base + at(j) < vocab ? to_f32(x[base + at(j)]) : -INFINITY;
+    }
+    return r;
+  };
+  // ids that are out of use as -inf; -0 as 0: the order is the values'
+  auto prepare = [&](Values& r, int i) {
+    const int base = i * kStretch;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) r.v[j] += 0.f;
+    if (base + kStretch > limit) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) r.v[j] = base + at(j) >= limit ? -INFINITY : r.v[j];
+    }
+    for (int q = 0; q < a.n_banned; ++q) {
+      const int id = a.banned[q] - base;
+      if (id < 0 || id >= kStretch) continue;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) r.v[j] = at(j) == id ? -INFINITY : r.v[j];
+    }
+  };
   float top = -INFINITY;
+  double sum = 0.0;
+  uint32_t bound = 0;
+  int count = 0;  // of this wave's list
+  Values next;
+  if (begin < end) next = load(begin);
+  for (int i = begin; i < end; ++i) {
+    Values now = next;
+    if (i + 1 < end) next = load(i + 1);
+    prepare(now, i);
+    float high = top;
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    const int64_t id = base + at(j);
-    bool out = id >= a.limit;
-    for (int i = 0; i < a.n_banned; ++i) out |= id == a.banned[i];
-    v[j] = out ? -INFINITY : v[j] + 0.f;  // -0 is 0: the order is the values'
-    top = fmaxf(top, v[j]);
+    for (int j = 0; j < kPer; ++j) high = fmaxf(high, now.v[j]);
+    bound = max(bound, reached_by<16>(ordered(high), a.beams));
+    const float least = fmaxf(unordered(max(bound, ordered(-INFINITY))), -3.402823466e38f);
+    float part = 0.f;
+    const float from = high == -INFINITY ? 0.f : high;  // differences first: a rounded product would move the whole sum
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      part += __builtin_amdgcn_exp2f((now.v[j] - from) * kLog2e);
+      const uint64_t here = __ballot(now.v[j] >= least);
+      if (here != 0) {
+        const int to = count + __popcll(here & ((1ull << lane) - 1));
+        if (now.v[j] >= least && to < kListed)
+          lists[w][to] = (uint64_t)ordered(now.v[j]) << 32 | (uint32_t)~(uint32_t)(i * kStretch + at(j));
+        count += __popcll(here);
+      }
+    }
+    sum = (top == high ? sum : sum * (double)__builtin_amdgcn_exp2f((top - from) * kLog2e)) + (double)part;
+    top = high;
   }
-  const uint32_t mine = reached_by(ordered(top), a.beams);
   const float wave_top = wave_max(top);
   if (lane == 0) {
-    bounds[w] = mine;
+    bounds[w] = bound;
     tops[w] = wave_top;
+    counts[w] = count;
   }
+  if (threadIdx.x == 0) chosen = 0;
   __syncthreads();
-  const uint32_t bound = max(max(bounds[0], bounds[1]), max(bounds[2], bounds[3]));
-  const float all = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-  double sum = 0.0;
-  const uint32_t none = ordered(-INFINITY);
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    sum += (double)(v[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((v[j] - all) * 1.44269504088896340736f));
-    const uint32_t k = ordered(v[j]);
-    if (k >= bound && k > none) {
-      const int i = atomicAdd(&listed, 1);
-      if (i < kListed) list[i] = (uint64_t)k << 32 | (uint32_t)~(uint32_t)(base + at(j));
-    }
-  }
+  const uint32_t reach = max(max(bounds[0], bounds[1]), max(bounds[2], bounds[3]));
+  const float over = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  const int64_t place = (int64_t)row * a.parts + blockIdx.x;
+  uint64_t* best = a.best + place * a.beams;
+  // a thread without a finite maximum has seen nothing, or NaN
+  sum = top == -INFINITY ? (sum == sum ? 0.0 : sum) : sum * (double)__builtin_amdgcn_exp2f((top - over) * kLog2e);
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
   if (lane == 0) sums[w] = sum;
-  __syncthreads();
-  const int64_t part = (int64_t)row * a.splits + split;
-  if (threadIdx.x == 0) {
-    a.sums[part] = sums[0] + sums[1] + sums[2] + sums[3];
-    a.tops[part] = all;
+  const bool fits = max(max(counts[0], counts[1]), max(counts[2], counts[3])) <= kListed;
+  if (fits) {
+    for (int i = lane; i < count; i += 64) {
+      const uint64_t k = lists[w][i];
+      if ((uint32_t)(k >> 32) >= reach) {
+        const int to = atomicAdd(&chosen, 1);
+        if (to < kListed) best_of[to] = k;
+      }
+    }
   }
-  uint64_t* best = a.best + part * a.beams;
-  const int n = listed;
-  if (n <= kListed) {
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    a.sums[place] = sums[0] + sums[1] + sums[2] + sums[3];
+    a.tops[place] = over;
+  }
+  const int n = chosen;
+  if (fits && n <= kListed) {
     for (int i = threadIdx.x; i < n; i += kThreads) {
-      const uint64_t k = list[i];
+      const uint64_t k = best_of[i];
       int rank = 0;
-      for (int j = 0; j < n; ++j) rank += list[j] > k;
+      for (int j = 0; j < n; ++j) rank += best_of[j] > k;
       if (rank < a.beams) best[rank] = k;
     }
     for (int i = n + threadIdx.x; i < a.beams; i += kThreads) best[i] = 0;
     return;
   }
   uint64_t last = ~0ull;
-  for (int i = 0; i < a.beams; ++i) {  // the best below the last one
+  for (int q = 0; q < a.beams; ++q) {  // too many equal logits for the lists: the best below the last one, each by another pass
     uint64_t found = 0;
+    for (int i = begin; i < end; ++i) {
+      Values now = load(i);
+      prepare(now, i);
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const uint64_t k = (uint64_t)ordered(v[j]) << 32 | (uint32_t)~(uint32_t)(base + at(j));
-      if (v[j] > -INFINITY && k < last && k > found) found = k;
+      for (int j = 0; j < kPer; ++j) {
+        const uint64_t k = (uint64_t)ordered(now.v[j]) << 32 | (uint32_t)~(uint32_t)(i * kStretch + at(j));
+        if (now.v[j] > -INFINITY && k < last && k > found) found = k;
+      }
     }
     found = wave_max64(found);
     if (lane == 0) wide[w] = found;
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < kThreads / 64; ++j) found = found > wide[j] ? found : wide[j];
-    if (threadIdx.x == 0) best[i] = found;
+    for (int j = 0; j < kWaves; ++j) found = found > wide[j] ? found : wide[j];
+    if (threadIdx.x == 0) best[q] = found;
     last = found;
     __syncthreads();
   }
@@ -204,11 +262,11 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const BeamArgs a) 
     float top = -INFINITY;
     double sum = 0.0;
     if (!over) {
-      for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, a.tops[(int64_t)row * a.splits + s]);
+      for (int s = lane; s < a.parts; s += 64) top = fmaxf(top, a.tops[(int64_t)row * a.parts + s]);
       top = wave_max(top);
-      for (int s = lane; s < a.splits; s += 64) {
-        const float t = a.tops[(int64_t)row * a.splits + s];
-        const double part = a.sums[(int64_t)row * a.splits + s];
+      for (int s = lane; s < a.parts; s += 64) {
+        const float t = a.tops[(int64_t)row * a.parts + s];
+        const double part = a.sums[(int64_t)row * a.parts + s];
         // NaN sums stay NaN: a row with NaN offers nothing
         sum += t == -INFINITY ? part : part * exp((double)t - (double)top);
       }
@@ -223,7 +281,7 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const BeamArgs a) 
     }
   }
   __syncthreads();
-  const int per = a.splits * a.beams, total = a.beams * per;
+  const int per = a.parts * a.beams, total = a.beams * per;
   // candidate i: its key and place; 0: none
   auto look = [&](int i, uint32_t& place) -> uint64_t {
     const int b = i / per, j = i - b * per;
@@ -240,7 +298,7 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const BeamArgs a) 
   };
   uint32_t high = 0, place;
   for (int i = threadIdx.x; i < total; i += kMergeThreads) high = max(high, (uint32_t)(look(i, place) >> 32));
-  const uint32_t mine = reached_by(high, a.beams);
+  const uint32_t mine = reached_by<32>(high, a.beams);
   if (lane == 0) bounds[w] = mine;
   __syncthreads();
   uint32_t bound = 0;
@@ -323,7 +381,10 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const BeamArgs a) 
   }
 }
 
-int64_t stretches(int64_t vocab) { return (vocab + kStretch - 1) / kStretch; }
+// Parts of a row: as many as fill the card, a stretch at least each.
+int64_t row_parts(int64_t rows, int64_t vocab) {
+  return std::max<int64_t>(1, std::min<int64_t>((vocab + kStretch - 1) / kStretch, kFill / rows));
+}
 
 }  // namespace
 }  // namespace uttt
@@ -332,7 +393,7 @@ using namespace uttt;
 
 extern "C" size_t uttt_beam_select_workspace(int64_t rows, int64_t vocab, int64_t beams) {
   if (rows < 1 || vocab < 1 || beams < 1) return 0;
-  return (size_t)rows * (size_t)stretches(vocab) * (8 * (size_t)beams + 8 + 4);
+  return (size_t)rows * (size_t)row_parts(rows, vocab) * (8 * (size_t)beams + 8 + 4);
 }
 
 extern "C" int uttt_beam_select(const uttt_beam_select_args* a, uttt_stream_t stream) {
@@ -353,17 +414,17 @@ extern "C" int uttt_beam_select(const uttt_beam_select_args* a, uttt_stream_t st
   m.rows = (int)a->rows; m.beams = (int)a->beams; m.n_banned = a->n_banned;
   m.vocab = a->vocab;
   m.limit = a->active_limit < 0 ? a->vocab : std::min(a->active_limit, a->vocab);
-  m.splits = (int)std::max<int64_t>(1, stretches(m.limit));
+  m.parts = (int)row_parts(a->rows, m.limit);
   for (int i = 0; i < 8; ++i) m.banned[i] = a->banned[i];
   m.logits = a->logits; m.row_stride = a->row_stride;
   m.scores = a->scores; m.ended_in = a->ended_in;
   m.eos = a->eos; m.pad = a->pad;
   m.tokens = a->tokens; m.sources = a->sources; m.out_scores = a->out_scores; m.ended_out = a->ended_out;
   m.best = static_cast<uint64_t*>(a->workspace);
-  m.sums = reinterpret_cast<double*>(m.best + (int64_t)m.rows * m.splits * m.beams);
-  m.tops = reinterpret_cast<float*>(m.sums + (int64_t)m.rows * m.splits);
+  m.sums = reinterpret_cast<double*>(m.best + (int64_t)m.rows * m.parts * m.beams);
+  m.tops = reinterpret_cast<float*>(m.sums + (int64_t)m.rows * m.parts);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)m.splits, (unsigned)m.rows);
+  const dim3 grid((unsigned)m.parts, (unsigned)m.rows);
   if (a->dtype == UTTT_DTYPE_BF16)
     hipLaunchKernelGGL(k_beam_part<bf16>, grid, dim3(kThreads), 0, st, m);
   else
