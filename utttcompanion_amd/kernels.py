@@ -1715,21 +1715,23 @@ def pack_weight4(weight: Tensor) -> Weight4:
     return Weight4(data, n, k)
 
 
-def _weight4(w: Weight4, n: int, k: int, name: str, batch: Optional[int] = None) -> Tuple[int, int]:
-    """The address and the batch's stride in bytes (0: one matrix) of a packed weight that has to be (n, k)."""
-    data = w.data
-    shape = data.shape
-    if w.n != n or w.k != k or shape[-3:] != ((n + 15) // 16, (k + 127) // 128, 1152) or data.dtype is not torch.uint8:
-        raise ValueError(f"{name} must be a packed weight of ({n}, {k}), got ({w.n}, {w.k}) with {tuple(shape)} {data.dtype}")
+def _weight4(w: Weight4, n: int, k: int, name: str, batch: int = 0) -> Tuple[int, int]:
+    """The address and the batch's stride in bytes (0: one matrix) of a packed weight that has to be (n, k); ``batch`` 0: of a
+    product that takes one matrix."""
+    data, wn, wk = w
+    shape, strides = data.shape, data.stride()
+    blocks = (k + 127) // 128
+    if (wn != n or wk != k or len(shape) < 3 or shape[-1] != 1152 or shape[-2] != blocks or shape[-3] != (n + 15) // 16
+            or data.dtype is not torch.uint8):
+        raise ValueError(f"{name} must be a packed weight of ({n}, {k}), got ({wn}, {wk}) with {tuple(shape)} {data.dtype}")
     address = data.data_ptr()
-    inner = data.stride()[-3:]
-    if inner != (shape[-2] * 1152, 1152, 1) or address & 15:
+    if strides[-1] != 1 or strides[-2] != 1152 or strides[-3] != blocks * 1152 or address & 15:
         raise ValueError(f"{name} must lie together, 16-byte aligned")
     if len(shape) == 3:
         return address, 0
-    if len(shape) != 4 or batch is None or shape[0] not in (1, batch):
-        raise ValueError(f"{name} must hold one matrix" + ("" if batch is None else f" or {batch}"))
-    stride = data.stride(0) if shape[0] > 1 else 0
+    if len(shape) != 4 or not batch or shape[0] != 1 and shape[0] != batch:
+        raise ValueError(f"{name} must hold one matrix" + (f" or {batch}" if batch else ""))
+    stride = strides[0] if shape[0] > 1 else 0
     if stride & 15:
         raise ValueError(f"{name} must lie together, 16-byte aligned")
     return address, stride
@@ -1810,9 +1812,8 @@ def readout4(x: Tensor, w_up: Weight4, w_gate: Weight4, w_down: Weight4, ln_weig
     p_gate, s_gate = _weight4(w_gate, ff, dim, "w_gate", bsz)
     p_down, s_down = _weight4(w_down, dim, ff, "w_down", bsz)
     gain, x_eps = (None, 0.0) if x_norm is None else (x_norm[0], float(x_norm[1]))
-    for name, t in (("ln_weight", ln_weight), ("ln_bias", ln_bias)) + ((("the x norm weight", gain),) if x_norm else ()):
-        if t.shape != (dim,):
-            raise ValueError(f"{name} must be ({dim},)")
+    if ln_weight.shape != (dim,) or ln_bias.shape != (dim,) or gain is not None and gain.shape != (dim,):
+        raise ValueError(f"ln_weight, ln_bias and the x norm weight must be ({dim},)")
     if not eps > 0.0 or x_norm is not None and not x_eps > 0.0:
         raise ValueError("eps must be > 0")
     if torch.is_grad_enabled():
@@ -1827,7 +1828,10 @@ def readout4(x: Tensor, w_up: Weight4, w_gate: Weight4, w_down: Weight4, ln_weig
         if gain.dtype is not dt or not gain.is_contiguous() or gain.data_ptr() & 15:
             gain = gain.to(dt).clone(memory_format=torch.contiguous_format)
         p_gain = gain.data_ptr()
-    x = _pieces(x, 2)
+    xs = x.stride()
+    if xs[2] != 1 or (xs[0] | xs[1]) & (7 if dt is torch.bfloat16 else 3) or x.data_ptr() & 15:
+        x = _pieces(x, 2)
+        xs = _strides(x, 2)
     if out is None:
         out = x.new_empty((bsz, tokens, dim))
     elif out.shape != x.shape or out.dtype is not dt or out.stride(2) != 1:
@@ -1839,8 +1843,8 @@ def readout4(x: Tensor, w_up: Weight4, w_gate: Weight4, w_down: Weight4, ln_weig
         workspace = x.new_empty(nbytes, dtype=torch.uint8)
     elif workspace.numel() * workspace.element_size() < nbytes or not workspace.is_contiguous():
         raise ValueError(f"the readout workspace must be {nbytes} contiguous bytes")
-    xs, os_ = _strides(x, 2), out.stride()
-    packed = N.pack_readout4(bsz, tokens, dim, ff, code, float(eps), x.data_ptr(), *xs, p_up, p_gate, p_down, s_up, s_gate,
+    os_ = out.stride()
+    packed = N.pack_readout4(bsz, tokens, dim, ff, code, float(eps), x.data_ptr(), xs[0], xs[1], p_up, p_gate, p_down, s_up, s_gate,
                              s_down, ln_weight.data_ptr(), ln_bias.data_ptr(), p_gain, x_eps, out.data_ptr(), os_[0], os_[1],
                              workspace.data_ptr(), nbytes)
     _serve_call(N.load_library().uttt_readout4, packed, index, "uttt_readout4")
@@ -1867,16 +1871,19 @@ def _cache4(cache: Tensor, lead: int, window: int, sinks: int) -> Tuple[int, Tup
         raise ValueError(f"the cache must be a uint8 {'(L, N' if lead == 2 else '(N'}, Hkv, blocks, bytes) tensor")
     if not 1 <= window <= 1 << 28 or not 0 <= sinks <= 1 << 28:
         raise ValueError("window must be in [1, 2^28] and sinks in [0, 2^28]")
-    if shape[-2] != (sinks + 31) // 32 + (window + 31) // 32 or shape[-1] not in (2304, 4608):
+    blocks, size = shape[-2], shape[-1]
+    if blocks != (sinks + 31) // 32 + (window + 31) // 32 or size != 2304 and size != 4608:
         raise ValueError(f"a cache of window {window} and sinks {sinks} has {(sinks + 31) // 32 + (window + 31) // 32} blocks of "
                          f"36 head_dim bytes, head_dim 64 or 128, got {tuple(shape[-2:])}")
-    if strides[lead:] != (shape[-2] * shape[-1], shape[-1], 1) and 0 not in shape:
-        if shape[lead] != 1 or strides[lead + 1:] != (shape[-1], 1):
+    if strides[-1] != 1 or strides[-2] != size or strides[lead] != blocks * size and shape[lead] != 1:
+        if 0 not in shape:
             raise ValueError("each request's cache must lie together")
-    at = _strides(cache, lead)
-    if cache.data_ptr() & 15 or any(s & 15 for s in at):
-        raise ValueError("each request's cache must be 16-byte aligned")
-    return cache.data_ptr(), at, shape[-1] // 36
+    address, at = cache.data_ptr(), strides[:lead]
+    if (address | at[0] | at[-1]) & 15:
+        at = _strides(cache, lead)  # a dimension of one element has no stride that matters
+        if address & 15 or any(s & 15 for s in at):
+            raise ValueError("each request's cache must be 16-byte aligned")
+    return address, at, size // 36
 
 
 @functools.lru_cache(maxsize=256)
@@ -2000,11 +2007,16 @@ def kv_commit4(k_nodes: Tensor, v_nodes: Tensor, nodes: Optional[Tensor], counts
     index = _gpu_index(cache, k_nodes, v_nodes, nodes, counts, positions)
     if layers == 0 or n == 0 or hkv == 0 or path == 0 or shape[2] == 0:
         return
-    k_nodes, v_nodes = _pieces(k_nodes, 4), _pieces(v_nodes, 4)
-    if _strides(k_nodes, 4) != _strides(v_nodes, 4):
-        k_nodes, v_nodes = (t.clone(memory_format=torch.contiguous_format) for t in (k_nodes, v_nodes))
-    packed = N.pack_kv_commit4(layers, n, hkv, shape[2], path, hd, window, sinks, code, bool(advance), k_nodes.data_ptr(),
-                               v_nodes.data_ptr(), *_strides(k_nodes, 4), p_nodes, path_stride, p_counts, p_cache, cache_l,
+    at = k_nodes.stride()
+    p_k, p_v = k_nodes.data_ptr(), v_nodes.data_ptr()
+    if (v_nodes.stride() != at or at[4] != 1 or (at[0] | at[1] | at[2] | at[3]) & (7 if dt is torch.bfloat16 else 3)
+            or (p_k | p_v) & 15):
+        k_nodes, v_nodes = _pieces(k_nodes, 4), _pieces(v_nodes, 4)
+        if _strides(k_nodes, 4) != _strides(v_nodes, 4):
+            k_nodes, v_nodes = (t.clone(memory_format=torch.contiguous_format) for t in (k_nodes, v_nodes))
+        at = _strides(k_nodes, 4)
+        p_k, p_v = k_nodes.data_ptr(), v_nodes.data_ptr()
+    packed = N.pack_kv_commit4(layers, n, hkv, shape[2], path, hd, window, sinks, code, bool(advance), p_k, p_v, *at[:4], p_nodes, path_stride, p_counts, p_cache, cache_l,
                                cache_n, p_pos)
     _serve_call(N.load_library().uttt_kv_commit4, packed, index, "uttt_kv_commit4")
 
@@ -2017,11 +2029,12 @@ def kv_values4(cache: Tensor, window: int, sinks: int = 0, dtype: torch.dtype = 
     p_cache, at, hd = _cache4(cache, lead, window, sinks)
     code = _act_code(dtype)
     index = _gpu_index(cache)
-    *lead_shape, hkv = cache.shape[:-2]
-    k, v = (torch.empty((*lead_shape, hkv, sinks + window, hd), dtype=dtype, device=cache.device) for _ in range(2))
+    shape = (*cache.shape[:-2], sinks + window, hd)
+    k, v = cache.new_empty(shape, dtype=dtype), cache.new_empty(shape, dtype=dtype)
     if k.numel() == 0:
         return k, v
-    layers, n = lead_shape if lead == 2 else (1, *lead_shape)
+    hkv = shape[-3]
+    layers, n = shape[:2] if lead == 2 else (1, shape[0])
     packed = N.pack_kv_values4(layers, n, hkv, hd, window, sinks, code, p_cache, at[0] if lead == 2 else 0, at[-1], k.data_ptr(),
                                v.data_ptr())
     _serve_call(N.load_library().uttt_kv_values4, packed, index, "uttt_kv_values4")
