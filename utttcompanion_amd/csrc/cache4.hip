@@ -13,8 +13,7 @@ namespace {
 constexpr int kSlots = 32;
 
 struct Commit4Args {
-  int heads, n_nodes, path, sink_blocks, ring_blocks;
-  int64_t window, sinks;
+  int heads, n_nodes, path, sink_blocks, ring_blocks, window, sinks;
   const void *k, *v;
   int64_t s_l, s_n, s_t, s_h;  // elements
   const int32_t* nodes;
@@ -25,24 +24,28 @@ struct Commit4Args {
   const int64_t* positions;
 };
 
-// Eight neighbours in fp32.
+// Eight neighbours as they lie in memory, and in fp32.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
-  if constexpr (sizeof(T) == 2) {
-    const bf16x8 t = *reinterpret_cast<const bf16x8*>(p);
+struct Eight {
+  u32x4 raw[sizeof(T) / 2];
+};
+
+template <typename T>
+__device__ __forceinline__ Eight<T> load8(const T* p) {
+  Eight<T> e;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = to_f32(t[j]);
-  } else {
-    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[j] = a[j];
-      v[4 + j] = b[j];
-    }
-  }
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) e.raw[i] = reinterpret_cast<const u32x4*>(p)[i];
+  return e;
 }
 
-// Codes (a word) and scale of a group that the four lanes 16 h + r of an r hold, eight values each.
+template <typename T>
+__device__ __forceinline__ void widen8(const Eight<T>& e, float (&v)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    v[j] = sizeof(T) == 2 ? bf16_of(e.raw[0][(j >> 1) & 3], j & 1) : __uint_as_float(e.raw[(int)sizeof(T) / 2 - 1 ? j >> 2 : 0][j & 3]);
+}
+
+// Codes (a word) and scale of a group that four neighbouring lanes hold, eight values each.
 __device__ __forceinline__ uint32_t quantise8(const float (&v)[8], bf16& scale) {
   float largest = 0.f;
   bool fine = true;
@@ -52,92 +55,107 @@ __device__ __forceinline__ uint32_t quantise8(const float (&v)[8], bf16& scale) 
     fine &= fabsf(v[j]) < INFINITY;
   }
   largest = fine ? largest : INFINITY;
-  largest = fmaxf(largest, __shfl_xor(largest, 16, 64));
-  largest = fmaxf(largest, __shfl_xor(largest, 32, 64));
+  largest = fmaxf(largest, __shfl_xor(largest, 1, 64));
+  largest = fmaxf(largest, __shfl_xor(largest, 2, 64));
   scale = fp4_scale(largest, largest < INFINITY);
-  const float s = to_f32(scale);
-  uint32_t w = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) w |= fp4_code(v[j], s) << (4 * j);
-  return w;
+  return fp4_codes(v, to_f32(scale));
 }
 
 // Where a slot's scale stands among its group's.
 __device__ __forceinline__ int scale_place(int slot) { return ((slot & 15) >> 2) * 8 + (slot >> 4) * 4 + (slot & 3); }
 
 // One block of slots per workgroup: the first wave takes the keys, the second the values.  A wave finds which token each of
-// its 32 slots takes, quantises row by row (a lane has 8 elements of a slot, four lanes a group) and stores what changes; the
-// values' words go over eight slots, so codes pass through LDS and slots that no token takes keep their nibbles.
-// Grid (blocks that a path can touch, requests x heads, layers).
+// its 32 slots takes, reads their rows (neighbouring lanes a row's neighbouring pieces), quantises, and turns the codes through LDS
+// to the cache's words; slots that no token takes keep their bits.  Grid (blocks that a path can touch, requests x heads,
+// layers).
 template <typename T, int HD>
 __global__ void __launch_bounds__(128) k_kv_commit4(const Commit4Args a) {
-  __shared__ uint32_t codes[kSlots][HD / 8 + 1];
+  constexpr int kRow = HD / 8, kPasses = kSlots * kRow / 64;  // pieces of a row, and a lane's of the block
+  __shared__ uint32_t codes[2][kSlots][kRow + 1];
   const int n = blockIdx.y / a.heads, head = blockIdx.y % a.heads, l = blockIdx.z;
   const int64_t pos = a.positions[n];
   const int count = a.counts ? min(max(a.counts[n], 0), a.path) : a.path;
   if (pos < 0 || count == 0) return;
   // the steps of the path that take sinks, then the ring's
-  const int first = (int)min((int64_t)count, max(a.sinks - pos, (int64_t)0)), ring = count - first;
-  const int64_t r0 = ring > 0 ? (pos + first - a.sinks) % a.window : 0;
-  const int sink0 = (int)(first > 0 ? pos / kSlots : 0);
-  const int sink_n = first > 0 ? (int)((pos + first - 1) / kSlots) - sink0 + 1 : 0;
-  const int ring0 = (int)(r0 / kSlots);
+  const int first = (int)min((int64_t)count, max((int64_t)a.sinks - pos, (int64_t)0)), ring = count - first;
+  const int64_t past = max(pos + first - a.sinks, (int64_t)0);
+  // a 64-bit remainder costs hundreds of instructions
+  const int r0 = past >> 32 ? (int)(past % a.window) : (int)((uint32_t)past % (uint32_t)a.window);
+  const int sink_from = (int)min(pos, (int64_t)a.sinks), sink0 = sink_from / kSlots;
+  const int sink_n = first > 0 ? (sink_from + first - 1) / kSlots - sink0 + 1 : 0;
+  const int ring0 = r0 / kSlots;
   int ring_n = 0;
   if (ring >= a.window) {
     ring_n = a.ring_blocks;
   } else if (ring > 0) {
-    const int64_t end = r0 + ring;
-    ring_n = end <= a.window ? (int)((end - 1) / kSlots) - ring0 + 1
-                             : min(a.ring_blocks, a.ring_blocks - ring0 + (int)((end - a.window - 1) / kSlots) + 1);
+    const int end = r0 + ring;
+    ring_n = end <= a.window ? (end - 1) / kSlots - ring0 + 1
+                             : min(a.ring_blocks, a.ring_blocks - ring0 + (end - a.window - 1) / kSlots + 1);
   }
   const int c = blockIdx.x;
   if (c >= sink_n + ring_n) return;
   const bool sink = c < sink_n;
-  const int block = sink ? sink0 + c : (ring0 + (c - sink_n)) % a.ring_blocks;  // of its region
-  const int lane = threadIdx.x & 63, r = lane & 15, h = lane >> 4;
-  const bool values = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) != 0;
+  int block = sink ? sink0 + c : ring0 + (c - sink_n);  // of its region
+  if (!sink && block >= a.ring_blocks) block -= a.ring_blocks;
+  const int lane = threadIdx.x & 63, r = lane & 15, h = lane >> 4, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const bool values = w != 0;
   // the node that slot `lane & 31` of the block takes, -1: none
   int mine = -1;
   {
-    const int64_t slot = (int64_t)block * kSlots + (lane & 31);
-    int64_t step = -1;
+    const int slot = block * kSlots + (lane & 31);
+    int step = -1;
     if (sink) {
-      if (slot >= pos && slot < pos + first) step = slot - pos;
+      if (slot >= sink_from && slot < sink_from + first) step = slot - sink_from;
     } else if (slot < a.window) {
-      const int64_t d = slot >= r0 ? slot - r0 : slot - r0 + a.window;
-      if (d < ring) step = first + d + (ring - 1 - d) / a.window * a.window;  // the last of the slot's steps
+      int d = slot >= r0 ? slot - r0 : slot - r0 + a.window;
+      if (d < ring) {
+        if (ring > a.window) d += (ring - 1 - d) / a.window * a.window;  // the last of the slot's steps
+        step = first + d;
+      }
     }
     if (step >= 0) {
-      mine = a.nodes ? a.nodes[n * a.path_stride + step] : (int)step;
+      mine = a.nodes ? a.nodes[n * a.path_stride + step] : step;
       if (mine >= a.n_nodes) mine = -1;
     }
   }
   char* at = a.cache + l * a.c_l + n * a.c_n +
              ((int64_t)head * (a.sink_blocks + a.ring_blocks) + (sink ? 0 : a.sink_blocks) + block) * (36 * HD);
-  const T* src = static_cast<const T*>(values ? a.v : a.k) + l * a.s_l + n * a.s_n + head * a.s_h;
+  const T* src = static_cast<const T*>(values ? a.v : a.k) + l * a.s_l + n * a.s_n + head * a.s_h + 8 * (lane % kRow);
   char* scales = at + 32 * HD + (values ? 2 * HD : 0);
+  Eight<T> row[kPasses];
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const int slot = 16 * t + r, node = __shfl(mine, slot, 64);
-    uint32_t words[HD / 32];
+  for (int i = 0; i < kPasses; ++i) {
+    const int node = __shfl(mine, (i * 64 + lane) / kRow, 64);
+    row[i] = Eight<T>{};
+    if (node >= 0) row[i] = load8(src + node * a.s_t);
+  }
 #pragma unroll
-    for (int g = 0; g < HD / 32; ++g) {
-      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (node >= 0) load8(src + node * a.s_t + 32 * g + 8 * h, v);
-      bf16 s;
-      words[g] = quantise8(v, s);
-      if (h == 0 && node >= 0) *reinterpret_cast<bf16*>(scales + g * 64 + scale_place(slot) * 2) = s;
-      if (values) codes[slot][4 * g + h] = words[g];
-    }
-    if (!values && node >= 0) {
+  for (int i = 0; i < kPasses; ++i) {
+    const int slot = (i * 64 + lane) / kRow, piece = lane % kRow;
+    const bool taken = __shfl(mine, slot, 64) >= 0;
+    if (!__any(taken)) continue;
+    float v[8];
+    widen8(row[i], v);
+    bf16 s;
+    codes[w][slot][piece] = quantise8(v, s);
+    if (taken && (piece & 3) == 0) *reinterpret_cast<bf16*>(scales + (piece >> 2) * 64 + scale_place(slot) * 2) = s;
+  }
+  __syncthreads();
+  if (!values) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int slot = 16 * t + r;
+      if (__shfl(mine, slot, 64) < 0) continue;
+      uint32_t words[HD / 32];
+#pragma unroll
+      for (int g = 0; g < HD / 32; ++g) words[g] = codes[0][slot][4 * g + h];
       if constexpr (HD == 64)
         *reinterpret_cast<u32x2*>(at + 16 * lane + 8 * t) = u32x2{words[0], words[1]};
       else
         *reinterpret_cast<u32x4*>(at + 1024 * t + 16 * lane) = u32x4{words[0], words[1], words[2], words[3]};
     }
+    return;
   }
-  __syncthreads();
-  if (!values) return;
   uint32_t taken = 0;  // the nibbles of this lane's words that are new
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
@@ -153,11 +171,11 @@ __global__ void __launch_bounds__(128) k_kv_commit4(const Commit4Args a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int e = 16 * (4 * q + i) + r;
-      uint32_t w = 0;
+      uint32_t word = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        w |= (codes[16 * (j >> 2) + 4 * h + (j & 3)][e >> 3] >> (4 * (e & 7)) & 15u) << (4 * j);
-      out[i] = (out[i] & ~taken) | (w & taken);
+        word |= (codes[1][16 * (j >> 2) + 4 * h + (j & 3)][e >> 3] >> (4 * (e & 7)) & 15u) << (4 * j);
+      out[i] = (out[i] & ~taken) | (word & taken);
     }
     *to = out;
   }
@@ -346,7 +364,7 @@ extern "C" int uttt_kv_commit4(const uttt_kv_commit4_args* a, uttt_stream_t stre
   Commit4Args m{};
   m.heads = (int)a->n_kv_heads; m.n_nodes = (int)a->n_nodes; m.path = (int)a->path;
   m.sink_blocks = (int)s.sink_blocks(); m.ring_blocks = (int)s.ring_blocks();
-  m.window = a->window; m.sinks = a->sinks;
+  m.window = (int)a->window; m.sinks = (int)a->sinks;
   m.k = a->k_nodes; m.v = a->v_nodes;
   m.s_l = a->nodes_stride_l; m.s_n = a->nodes_stride_n; m.s_t = a->nodes_stride_t; m.s_h = a->nodes_stride_h;
   m.nodes = a->nodes; m.path_stride = a->path_stride; m.counts = a->counts;
