@@ -23,11 +23,14 @@ constexpr int kMaxWaves4 = 8;
 constexpr int kCounterPitch = 64;  // a row's counter has a cache line of its own
 constexpr int kRowLds = 49152;  // bytes of a row's parts that k_gemv4 takes
 
-// Eight neighbours of a row from column k0 on, zeros from k on.
-__device__ __forceinline__ bf16x8 load_x8(const bf16* row, int k0, int k, bool aligned) {
+// Eight neighbours of a row from column k0 on, zeros from k on.  Rows lie anywhere: 16-byte loads need no alignment here.
+typedef bf16x8 bf16x8_any __attribute__((aligned(2)));
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+
+__device__ __forceinline__ bf16x8 load_x8(const bf16* row, int k0, int k) {
   bf16x8 v;
-  if (aligned && k0 + 8 <= k) {
-    v = *reinterpret_cast<const bf16x8*>(row + k0);
+  if (k0 + 8 <= k) {
+    v = *reinterpret_cast<const bf16x8_any*>(row + k0);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = k0 + j < k ? row[k0 + j] : static_cast<bf16>(0.f);
@@ -36,13 +39,13 @@ __device__ __forceinline__ bf16x8 load_x8(const bf16* row, int k0, int k, bool a
 }
 
 template <typename X>
-__device__ __forceinline__ void load_x8(const X* row, int k0, int k, bool aligned, float (&v)[8]) {
+__device__ __forceinline__ void load_x8(const X* row, int k0, int k, float (&v)[8]) {
   if constexpr (sizeof(X) == 2) {
-    const bf16x8 t = load_x8(row, k0, k, aligned);
+    const bf16x8 t = load_x8(row, k0, k);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = to_f32(t[j]);
-  } else if (aligned && k0 + 8 <= k) {
-    const f32x4 a = *reinterpret_cast<const f32x4*>(row + k0), b = *reinterpret_cast<const f32x4*>(row + k0 + 4);
+  } else if (k0 + 8 <= k) {
+    const f32x4 a = *reinterpret_cast<const f32x4_any*>(row + k0), b = *reinterpret_cast<const f32x4_any*>(row + k0 + 4);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       v[j] = a[j];
@@ -149,7 +152,6 @@ enum class Row { kLinear, kSwiglu, kDown };
 
 struct Gemv4Args {
   int n, k, blocks, tiles, split;  // split: waves that divide a tile's columns
-  int aligned;
   float x_eps;
   const void* x;  // (k,) per batch; kDown: bf16 parts (P, k)
   int64_t xs_b;
@@ -201,17 +203,17 @@ __global__ void __launch_bounds__(kMaxWaves4 * 64) k_gemv4(const Gemv4Args a) {
     bf16x8 p[P];
     if constexpr (MODE == Row::kDown) {
 #pragma unroll
-      for (int i = 0; i < P; ++i) p[i] = load_x8(static_cast<const bf16*>(a.x) + b * a.xs_b + (int64_t)i * a.k, k0, a.k, true);
+      for (int i = 0; i < P; ++i) p[i] = load_x8(static_cast<const bf16*>(a.x) + b * a.xs_b + (int64_t)i * a.k, k0, a.k);
     } else {
       float v[8];
-      load_x8(static_cast<const X*>(a.x) + b * a.xs_b, k0, a.k, a.aligned, v);
+      load_x8(static_cast<const X*>(a.x) + b * a.xs_b, k0, a.k, v);
       if (a.x_eps > 0.f) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) squares = fmaf(v[j], v[j], squares);
       }
       if (a.gain != nullptr) {
         float g[8];
-        load_x8(static_cast<const X*>(a.gain), k0, a.k, true, g);
+        load_x8(static_cast<const X*>(a.gain), k0, a.k, g);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] *= g[j];
       }
@@ -312,7 +314,7 @@ __device__ __forceinline__ int64_t part_place(int m, int k, int part, int groups
 }
 
 struct Parts4Args {
-  int m, k, aligned;
+  int m, k;
   float x_eps;
   const void* x;
   int64_t xs_b, xs_m;
@@ -334,7 +336,7 @@ __global__ void __launch_bounds__(kThreads) k_parts4(const Parts4Args a) {
     float squares = 0.f;
     for (int k0 = threadIdx.x * 8; k0 < a.k; k0 += kThreads * 8) {
       float v[8];
-      load_x8(row, k0, a.k, a.aligned, v);
+      load_x8(row, k0, a.k, v);
 #pragma unroll
       for (int j = 0; j < 8; ++j) squares = fmaf(v[j], v[j], squares);
     }
@@ -343,10 +345,10 @@ __global__ void __launch_bounds__(kThreads) k_parts4(const Parts4Args a) {
   const int k0 = blockIdx.y * kPartsColumns + threadIdx.x * 8;
   if (k0 >= wide) return;
   float v[8];
-  load_x8(row, k0, a.k, a.aligned, v);
+  load_x8(row, k0, a.k, v);
   if (a.gain != nullptr) {
     float g[8];
-    load_x8(static_cast<const X*>(a.gain), k0, a.k, true, g);
+    load_x8(static_cast<const X*>(a.gain), k0, a.k, g);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] *= g[j];
   }
@@ -362,9 +364,9 @@ __global__ void __launch_bounds__(kThreads) k_parts4(const Parts4Args a) {
 }
 
 struct Prod4Args {
-  int m, n, k, blocks, aligned;  // aligned: rows of one part in 16-byte pieces
-  float x_eps;                   // > 0 (one part): rows of x are RMS-normalised
-  const bf16* x;                 // one part: rows; more: operands (parts_of_batch)
+  int m, n, k, blocks;
+  float x_eps;    // > 0 (one part): rows of x are RMS-normalised
+  const bf16* x;  // one part: rows; more: operands (parts_of_batch)
   int64_t xs_b, xs_m;
   const char* w[2];
   int64_t ws_b[2];
@@ -441,11 +443,11 @@ __global__ void __launch_bounds__(W * 64, W == 4 ? 2 : 1) k_prod4(const Prod4Arg
     Ahead v;
     if constexpr (P == 1) {
       const int k0 = half * 64 + 8 * (lane & 7);
-      const bool plain = a.aligned && half * 64 + 64 <= a.k;
+      const bool plain = half * 64 + 64 <= a.k;
 #pragma unroll
       for (int i = 0; i < 2 * MT; ++i) {
         const bf16* row = base + (int64_t)min(m0 + 8 * i + (lane >> 3), a.m - 1) * a.xs_m;
-        v.x[i] = plain ? *reinterpret_cast<const bf16x8*>(row + k0) : load_x8(row, k0, a.k, a.aligned);
+        v.x[i] = plain ? *reinterpret_cast<const bf16x8_any*>(row + k0) : load_x8(row, k0, a.k);
       }
     } else {
 #pragma unroll
@@ -616,7 +618,7 @@ __global__ void __launch_bounds__(512, 2) k_share4(const Prod4Args a) {
     for (int i = 0; i < kEach; ++i) {
       const int piece = i * WN + wn, half = min(half0 + piece / (2 * MT), halves - 1), k0 = half * 64 + 8 * (lane & 7);
       const bf16* row = base + (int64_t)min(m0 + 8 * (piece % (2 * MT)) + (lane >> 3), a.m - 1) * a.xs_m;
-      v.x[i] = a.aligned && half * 64 + 64 <= a.k ? *reinterpret_cast<const bf16x8*>(row + k0) : load_x8(row, k0, a.k, a.aligned);
+      v.x[i] = half * 64 + 64 <= a.k ? *reinterpret_cast<const bf16x8_any*>(row + k0) : load_x8(row, k0, a.k);
     }
     return v;
   };
@@ -830,7 +832,7 @@ void launch_readout4(const uttt_readout4_args* a, hipStream_t st) {
              *down = static_cast<const char*>(a->w_down);
   if (at.single) {
     Gemv4Args g{};
-    g.n = F; g.k = D; g.blocks = (D + 127) / 128; g.aligned = 1;
+    g.n = F; g.k = D; g.blocks = (D + 127) / 128;
     g.x = a->x; g.xs_b = a->x_stride_b; g.gain = a->x_norm_weight;
     g.x_eps = a->x_norm_weight ? a->x_norm_eps : 0.f;
     g.w[0] = up; g.ws_b[0] = a->w_up_stride; g.w[1] = gate; g.ws_b[1] = a->w_gate_stride;
@@ -856,7 +858,6 @@ void launch_readout4(const uttt_readout4_args* a, hipStream_t st) {
   p.m = M; p.n = F; p.k = D; p.blocks = (D + 127) / 128;
   p.w[0] = up; p.ws_b[0] = a->w_up_stride; p.w[1] = gate; p.ws_b[1] = a->w_gate_stride;
   p.out = hidden;
-  p.aligned = 1;
   bool whole = false;  // bf16 as it is
   if constexpr (sizeof(T) == 2) {
     whole = a->x_norm_weight == nullptr;
@@ -867,7 +868,7 @@ void launch_readout4(const uttt_readout4_args* a, hipStream_t st) {
   }
   if (!whole) {
     Parts4Args x{};
-    x.m = M; x.k = D; x.aligned = 1;
+    x.m = M; x.k = D;
     x.x_eps = a->x_norm_weight ? a->x_norm_eps : 0.f;
     x.x = a->x; x.xs_b = a->x_stride_b; x.xs_m = a->x_stride_t;
     x.gain = a->x_norm_weight;
@@ -916,7 +917,6 @@ extern "C" int uttt_linear4(const uttt_linear4_args* a, uttt_stream_t stream) {
   if (a->m == 1 && row_lds(a->k, b16 ? 1 : 3) <= kRowLds) {
     Gemv4Args g{};
     g.n = (int)a->n; g.k = (int)a->k; g.blocks = (int)((a->k + 127) / 128);
-    g.aligned = aligned16(a->x);
     g.x_eps = a->x_eps;
     g.x = a->x;
     g.w[0] = static_cast<const char*>(a->w);
@@ -935,11 +935,9 @@ extern "C" int uttt_linear4(const uttt_linear4_args* a, uttt_stream_t stream) {
   p.w[0] = static_cast<const char*>(a->w);
   p.r = a->residual; p.rs_m = a->residual_row_stride;
   p.out = a->out; p.os_m = a->out_row_stride;
-  p.aligned = whole_pieces(a->x, a->m == 1 ? 0 : a->x_row_stride, 0, 8);
   if (!b16) {
     Parts4Args x{};
     x.m = p.m; x.k = p.k;
-    x.aligned = whole_pieces(a->x, a->m == 1 ? 0 : a->x_row_stride, 0, 4);
     x.x_eps = a->x_eps;
     x.x = a->x; x.xs_m = a->x_row_stride;
     x.out = static_cast<bf16*>(a->workspace);
