@@ -78,6 +78,29 @@ def test_linear(m, n, k, dt, norm, res):
     within(got, want, linear_bound(xd, w, k, dt, norm, want, r.double() if res else None))
 
 
+@pytest.mark.parametrize("m,n,k", [(5, 100, 11000), (16, 64, 2048), (61, 199, 5501), (2, 1, 1921)])
+def test_linear_whose_columns_are_divided(m, n, k):
+    """Workgroups that share rows and columns of the result: eager, and replayed from a graph between other calls."""
+    g = gen(m + n + k)
+    x, r = normal(g, m, k), normal(g, m, n)
+    p = K.pack_weight4(normal(g, n, k).to(DEV))
+    w, xd = R.weight_values(p.data, n, k), x.double()
+    want = (xd * (xd.pow(2).mean(1, keepdim=True) + 1e-6).rsqrt()) @ w.T + r.double()
+    xg, rg = x.to(DEV), r.to(DEV)
+    eager = K.linear4(xg, p, residual=rg, x_eps=1e-6)
+    within(eager, want, linear_bound(xd, w, k, torch.float32, 1e-6, want, r.double()))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = K.linear4(xg, p, residual=rg, x_eps=1e-6)
+        twice = K.linear4(xg, p, residual=held, x_eps=1e-6)
+    then = K.linear4(xg, p, residual=eager, x_eps=1e-6)
+    for _ in range(3):
+        held.zero_(), twice.zero_()
+        graph.replay()
+        assert torch.equal(K.linear4(xg, p, residual=rg, x_eps=1e-6), eager)
+        assert torch.equal(held, eager) and torch.equal(twice, then)
+
+
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
 def test_linear_takes_any_rows(dt):
     """Views at odd offsets with wide rows, expanded rows, results into views, and onto the residual itself."""

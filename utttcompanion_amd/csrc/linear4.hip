@@ -320,6 +320,8 @@ struct Parts4Args {
   int64_t xs_b, xs_m;
   const void* gain;
   bf16* out;
+  unsigned* counters;  // of the product that follows, cleared here
+  int n_counters;
 };
 
 constexpr int kPartsColumns = kThreads * 8;
@@ -331,6 +333,8 @@ __global__ void __launch_bounds__(kThreads) k_parts4(const Parts4Args a) {
   __shared__ float scratch[kMaxWaves4];
   const int m = blockIdx.x, b = blockIdx.z, wide = (a.k + 63) / 64 * 64;
   const X* row = static_cast<const X*>(a.x) + b * a.xs_b + m * a.xs_m;
+  if (m == 0 && blockIdx.y == 0 && b == 0)
+    for (int i = threadIdx.x; i < a.n_counters; i += kThreads) a.counters[i * kCounterPitch] = 0;
   float norm = 1.f;
   if (a.x_eps > 0.f) {
     float squares = 0.f;
@@ -374,7 +378,17 @@ struct Prod4Args {
   int64_t rs_m;
   void* out;  // SWIGLU: the next product's operands
   int64_t os_b, os_m;
+  int nsplit;          // > 1: workgroups that divide the columns of the same rows and tiles
+  float* part;         // their sums, (group, split, 16 MT rows, 16 NT columns)
+  unsigned* counters;  // of a group's splits that have stored theirs
 };
+
+constexpr int kMaxSplits = 8;
+constexpr int kSplitGroups = 256;        // at least two splits each
+constexpr int kSplitFloats = 32 * 64;    // of a workgroup
+
+// Products whose columns may be divided over workgroups.
+constexpr bool splits(int parts, int nt, int w, bool swiglu) { return parts == 3 && nt == 4 && w == 4 && !swiglu; }
 
 // A product's element (m, n): the result, or with SWIGLU (y up, `gate` the gate's) the next product's operands.
 template <typename O, bool SWIGLU>
@@ -405,7 +419,9 @@ __global__ void __launch_bounds__(W * 64, W == 4 ? 2 : 1) k_prod4(const Prod4Arg
   const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, r = lane & 15, h = lane >> 4;
   constexpr int TILES = SWIGLU ? NT / 2 : NT;  // tiles of n
-  const int tiles = (a.n + 15) >> 4, tile0 = blockIdx.x * TILES, m0 = blockIdx.y * (16 * MT), b = blockIdx.z;
+  constexpr bool kSplits = splits(P, NT, W, SWIGLU);
+  const int nsplit = kSplits ? a.nsplit : 1, split = kSplits ? blockIdx.x % nsplit : 0;
+  const int tiles = (a.n + 15) >> 4, tile0 = blockIdx.x / nsplit * TILES, m0 = blockIdx.y * (16 * MT), b = blockIdx.z;
   const char* wp[NT];
 #pragma unroll
   for (int s = 0; s < NT; ++s) {
@@ -513,7 +529,8 @@ __global__ void __launch_bounds__(W * 64, W == 4 ? 2 : 1) k_prod4(const Prod4Arg
       }
     }
   };
-  const int begin = a.blocks * w / W, end = a.blocks * (w + 1) / W, halves = (a.k + 63) >> 6;
+  const int part = split * W + w, parts = nsplit * W;
+  const int begin = a.blocks * part / parts, end = a.blocks * (part + 1) / parts, halves = (a.k + 63) >> 6;
   if (begin < end) {
     Weights next = weights(begin);
     Ahead first = ahead(2 * begin);
@@ -544,6 +561,8 @@ __global__ void __launch_bounds__(W * 64, W == 4 ? 2 : 1) k_prod4(const Prod4Arg
       for (int i = 0; i < 4; ++i) red[((w * NT + s) * (MT * 4) + 4 * t + i) * 64 + lane] = acc[s][t][i];
   __syncthreads();
   constexpr int kOuts = MT * TILES * 4 / W > 0 ? MT * TILES * 4 / W : 1;  // of a thread: 16 TILES neighbours of 16 MT rows
+  const int group = blockIdx.y * (gridDim.x / nsplit) + blockIdx.x / nsplit;
+  float* sums = kSplits && nsplit > 1 ? a.part + (int64_t)group * nsplit * kSplitFloats : nullptr;
 #pragma unroll
   for (int o = 0; o < kOuts; ++o) {
     const int idx = threadIdx.x + o * W * 64, nn = idx & 15, s = (idx >> 4) % TILES, mm = idx / (16 * TILES);
@@ -561,7 +580,38 @@ __global__ void __launch_bounds__(W * 64, W == 4 ? 2 : 1) k_prod4(const Prod4Arg
       for (int q = 0; q < W; ++q) q2 += squares[q][mm];
       y *= rsqrtf(q2 / (float)a.k + a.x_eps);
     }
-    finish_row<O, SWIGLU>(a, b, m0 + mm, (tile0 + s) * 16 + nn, y, gate);
+    if (kSplits && sums != nullptr)
+      __hip_atomic_store(sums + split * kSplitFloats + idx, y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    else
+      finish_row<O, SWIGLU>(a, b, m0 + mm, (tile0 + s) * 16 + nn, y, gate);
+  }
+  if constexpr (kSplits) {
+    if (sums == nullptr) return;
+    // The group's last workgroup adds up, in the splits' order: stores past the caches, every thread waits for its own, then the
+    // group's count goes up; the last one reads past the caches.  The launch before cleared the counts.
+    __shared__ bool last;
+    wait_vmcnt<0>();
+    __syncthreads();
+    if (threadIdx.x == 0)
+      last = (int)__hip_atomic_fetch_add(a.counters + group * kCounterPitch, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+             nsplit - 1;
+    __syncthreads();
+    if (!last) return;
+    float v[kMaxSplits][kOuts];
+#pragma unroll
+    for (int q = 0; q < kMaxSplits; ++q)
+#pragma unroll
+      for (int o = 0; o < kOuts; ++o)
+        v[q][o] = __hip_atomic_load(sums + min(q, nsplit - 1) * kSplitFloats + threadIdx.x + o * W * 64, __ATOMIC_RELAXED,
+                                    __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+    for (int o = 0; o < kOuts; ++o) {
+      const int idx = threadIdx.x + o * W * 64, nn = idx & 15, s = (idx >> 4) % TILES, mm = idx / (16 * TILES);
+      float y = v[0][o];
+#pragma unroll
+      for (int q = 1; q < kMaxSplits; ++q) y += q < nsplit ? v[q][o] : 0.f;
+      finish_row<O, SWIGLU>(a, b, m0 + mm, (tile0 + s) * 16 + nn, y, 0.f);
+    }
   }
 }
 
@@ -737,7 +787,8 @@ template <typename O, int P, int NT, int W, bool SWIGLU>
 void launch_rows(const Prod4Args& p, int batch, hipStream_t st) {
   const int tiles = (p.n + 15) / 16, per = SWIGLU ? NT / 2 : NT;
   const int mt = p.m <= 16 ? 1 : p.m <= 32 || P > 1 ? 2 : 4;
-  const dim3 grid((unsigned)((tiles + per - 1) / per), (unsigned)((p.m + 16 * mt - 1) / (16 * mt)), (unsigned)batch), block(W * 64);
+  const int nsplit = splits(P, NT, W, SWIGLU) ? p.nsplit : 1;
+  const dim3 grid((unsigned)((tiles + per - 1) / per * nsplit), (unsigned)((p.m + 16 * mt - 1) / (16 * mt)), (unsigned)batch), block(W * 64);
   if (mt == 1)
     hipLaunchKernelGGL((k_prod4<O, P, 1, NT, W, SWIGLU>), grid, block, 0, st, p);
   else if (mt == 2)
@@ -762,6 +813,9 @@ void launch_share(const Prod4Args& p, int batch, hipStream_t st) {
 // teams of 4 with 2 blocks each 14.4; 32 x (16000, 2048): teams of 4 12.7, of 2 with one block each 10.1; 32 x (5504, 2048):
 // eight waves for themselves 7.3, teams of 2 6.8; of 2048 columns alike.  Three parts, which already are in the operands' order: 32
 // x (32000, 2048) sharing 23.8, for themselves 4 blocks each 21.5; 61 x (1999, 5501) sharing 30, eight waves to a block 29, 16 27.
+// What bounds that last one is x, read once per workgroup: 4 blocks of W each and the columns divided over 8 workgroups
+// instead 18.8 (with the rows' parts 24.0 before), 32 x (2048, 5504) 14.3 for 19.8, 5 x (100, 11000) 10.3 for 19.1; of few
+// columns it is the second exchange that costs (7 x (300, 1000) 7.9 for 6.5): from 16 blocks of columns on, 4 a workgroup.
 template <typename O, int P>
 void launch_linear_rows(const Prod4Args& p, int batch, hipStream_t st) {
   const int64_t tiles = (p.n + 15) / 16 * batch * ((p.m + 31) / 32);
@@ -772,7 +826,7 @@ void launch_linear_rows(const Prod4Args& p, int batch, hipStream_t st) {
       launch_share<O, 1, 2>(p, batch, st);
     else
       launch_rows<O, P, 1, 8, false>(p, batch, st);
-  } else if (tiles >= 768) {
+  } else if (tiles >= 768 || p.nsplit > 1) {
     launch_rows<O, P, 4, 4, false>(p, batch, st);
   } else if (p.blocks >= 16) {
     launch_rows<O, P, 1, 16, false>(p, batch, st);
@@ -784,9 +838,10 @@ void launch_linear_rows(const Prod4Args& p, int batch, hipStream_t st) {
 template <typename X, typename T, int P, Row MODE>
 void launch_gemv(Gemv4Args g, int batch, hipStream_t st) {
   g.tiles = (g.n + 15) / 16;
-  // waves enough to fill the card's 4096 places, as far as a tile has columns to divide
+  // waves enough to fill half of the card's 4096 places, as far as a tile has columns to divide (4096, 2048 and 1024 waves are
+  // within 10% of each other)
   g.split = 1;
-  while (g.split < kMaxWaves4 && 2 * g.split <= g.blocks && (int64_t)g.tiles * batch * g.split < 4096) g.split *= 2;
+  while (g.split < kMaxWaves4 && 2 * g.split <= g.blocks && (int64_t)g.tiles * batch * g.split < 2048) g.split *= 2;
   const int waves = std::max(4, g.split), per = waves / g.split;
   const size_t lds = (size_t)P * ((size_t)g.blocks * 256 + 64);
   hipLaunchKernelGGL((k_gemv4<X, T, P, MODE>), dim3((unsigned)((g.tiles + per - 1) / per), (unsigned)batch), dim3(waves * 64), lds, st, g);
@@ -810,6 +865,16 @@ struct Readout4Layout {
     counters = z + align_up((size_t)B * T * D * 4);
     parts = counters + align_up((size_t)B * kCounterPitch * 4);
     total = parts + (single ? 0 : align_up((size_t)B * parts_of_batch(T, D, 3) * 2));
+  }
+};
+
+// Where a product's buffers lie in its workspace: x's parts, the sums of splits and their counters.
+struct Linear4Layout {
+  size_t sums, counters, total;
+  Linear4Layout(int64_t m, int64_t k) {
+    sums = align_up((size_t)parts_of_batch(m, k, 3) * 2);
+    counters = sums + (size_t)2 * kSplitGroups * kSplitFloats * 4;
+    total = counters + (size_t)kSplitGroups * kCounterPitch * 4;
   }
 };
 
@@ -855,6 +920,7 @@ void launch_readout4(const uttt_readout4_args* a, hipStream_t st) {
     return;
   }
   Prod4Args p{};
+  p.nsplit = 1;
   p.m = M; p.n = F; p.k = D; p.blocks = (D + 127) / 128;
   p.w[0] = up; p.ws_b[0] = a->w_up_stride; p.w[1] = gate; p.ws_b[1] = a->w_gate_stride;
   p.out = hidden;
@@ -878,6 +944,7 @@ void launch_readout4(const uttt_readout4_args* a, hipStream_t st) {
     launch_rows<T, HP, 2, 4, true>(p, B, st);
   }
   Prod4Args q{};
+  q.nsplit = 1;
   q.m = M; q.n = D; q.k = F; q.blocks = (F + 127) / 128;
   q.x = hidden; q.xs_b = parts_of_batch(M, F, HP);
   q.w[0] = down; q.ws_b[0] = a->w_down_stride;
@@ -895,7 +962,7 @@ extern "C" int uttt_decode_abi_version(void) { return UTTT_DECODE_ABI_VERSION; }
 
 extern "C" size_t uttt_linear4_workspace(int64_t m, int64_t k, int32_t act_dtype) {
   if (m < 1 || k < 1 || act_dtype == UTTT_DTYPE_BF16 || (m == 1 && row_lds(k, 3) <= kRowLds)) return 0;
-  return (size_t)parts_of_batch(m, k, 3) * 2;
+  return Linear4Layout(m, k).total;
 }
 
 extern "C" int uttt_linear4(const uttt_linear4_args* a, uttt_stream_t stream) {
@@ -929,6 +996,7 @@ extern "C" int uttt_linear4(const uttt_linear4_args* a, uttt_stream_t stream) {
     return launch_status("uttt_linear4");
   }
   Prod4Args p{};
+  p.nsplit = 1;
   p.m = (int)a->m; p.n = (int)a->n; p.k = (int)a->k; p.blocks = (int)((a->k + 127) / 128);
   p.x_eps = a->x_eps;
   p.x = static_cast<const bf16*>(a->x); p.xs_m = a->x_row_stride;
@@ -942,6 +1010,13 @@ extern "C" int uttt_linear4(const uttt_linear4_args* a, uttt_stream_t stream) {
     x.x = a->x; x.xs_m = a->x_row_stride;
     x.out = static_cast<bf16*>(a->workspace);
     p.x = x.out;
+    const Linear4Layout at(a->m, a->k);
+    const int64_t groups = (a->n + 63) / 64 * ((a->m + 31) / 32);
+    if (p.blocks >= 16)
+      p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)kMaxSplits, 2 * kSplitGroups / groups, p.blocks / 4}));
+    p.part = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + at.sums);
+    p.counters = x.counters = reinterpret_cast<unsigned*>(static_cast<char*>(a->workspace) + at.counters);
+    x.n_counters = p.nsplit > 1 ? (int)groups : 0;
     launch_parts<float, 3>(x, 1, st);
   }
   if (b16)

@@ -156,9 +156,17 @@ __global__ void __launch_bounds__(W * 64, W == 4 ? 2 : 1) k_swa_tree4(const Tree
   const int split = id % a.nsplit;
   id /= a.nsplit;
   const int kvh = id % a.n_kv_heads, n = id / a.n_kv_heads;
+  const int row0 = group * 16;
+  // a lane's row of q: elements 32 g + 8 h .. (of one node per request on its way before anything else is known)
+  float x[G][8];
+  auto load_q = [&](int node, int head) {
+    const T* qp = static_cast<const T*>(a.q) + n * a.q_n + node * a.q_t + head * a.q_h + 8 * h;
+#pragma unroll
+    for (int g = 0; g < G; ++g) load8(qp + 32 * g, x[g]);
+  };
+  if (KT == 1) load_q(0, kvh * a.rep + min(row0 + r, a.rep - 1));
   const Tree tree = read_tree(a, n);
   const int live = tree.count * a.rep;  // rows of nodes that exist, a node's heads together
-  const int row0 = group * 16;
   if (row0 >= live) return;
   const int row = min(row0 + r, live - 1), node = row / a.rep, head = kvh * a.rep + row % a.rep;
   T* out = static_cast<T*>(a.out);
@@ -220,19 +228,17 @@ __global__ void __launch_bounds__(W * 64, W == 4 ? 2 : 1) k_swa_tree4(const Tree
   for (int d = 0; d < D; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
 
-  // this lane's row of q: elements 32 g + 8 h .., rotated, scaled, in parts
+  // the row rotated, scaled, in parts
   bf16x8 qf[G][QP];
   {
-    const T* qp = static_cast<const T*>(a.q) + n * a.q_n + node * a.q_t + head * a.q_h + 8 * h;
+    if (KT > 1) load_q(node, head);
     const int64_t at = (tree.pos + depth) * HD + 8 * h;
     const bool single = KT == 1 && split == 0 && w == 0;  // this wave takes the one new token
     const int64_t k_at = n * a.k_n + kvh * a.k_h + 8 * h;
-    float x[G][8], k[G][8];
+    float k[G][8];
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      load8(qp + 32 * g, x[g]);
+    for (int g = 0; g < G; ++g)
       if (single) load8(static_cast<const T*>(a.k) + k_at + 32 * g, k[g]);
-    }
 #pragma unroll
     for (int g = 0; g < G / 2; ++g) {
       if (a.cos_table == nullptr) break;
@@ -588,11 +594,16 @@ struct Plan4 {
   int groups, nsplit, waves;
 };
 
+// Workgroups to 256, of at least 20 blocks, of eight waves where they fit that number.  Measured, us: one token of 32
+// requests over 4096 slots of 128 for 16 heads on 4: to 256 workgroups 25.2, to 512 27.0, to 1024 34.4; 8 such 17.5, 17.6,
+// 17.0; one 15.2, 15.4, 14.6; 32 over 1024 slots of 64, 12 and 20 blocks at least: 11.3, 9.8.  Waves, four and eight to a
+// workgroup: 256 workgroups (32 over 4096) 28.0 and 25.2, (64 over 1024 of 128) 17.5 and 16.0, 4 (one over 512) 7.8 and
+// 7.4; 384 (96 over 1024) 22.8 and 27.6, 1024 (trees of 64 nodes) 118 and 141.
 Plan4 plan_tree4(int64_t n_req, int64_t n_heads, int64_t n_kv_heads, int64_t nodes, int64_t blocks) {
   Plan4 p;
   p.groups = (int)((n_heads / n_kv_heads * nodes + 15) / 16);
   const int64_t base = n_req * n_kv_heads * p.groups;
-  p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({512 / base, blocks / 24, (int64_t)kMaxSplits4}));
+  p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({256 / base, blocks / 20, (int64_t)kMaxSplits4}));
   p.waves = base * p.nsplit <= 256 ? 8 : 4;
   return p;
 }
