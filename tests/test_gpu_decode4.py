@@ -101,6 +101,22 @@ def test_linear_whose_columns_are_divided(m, n, k):
         assert torch.equal(held, eager) and torch.equal(twice, then)
 
 
+@pytest.mark.parametrize("n", [40, 3100, 24600])
+@pytest.mark.parametrize("k", [1, 7, 8, 9, 20, 63, 65, 190, 532, 1029])
+def test_linear_whose_last_columns_are_few(n, k):
+    """Rows in bf16 whose last pieces are short, at few, many and very many outputs, between numbers that are not finite."""
+    g = gen(n + k)
+    m = 18
+    wide = torch.full((m, k + 16), math.nan, dtype=torch.bfloat16)
+    wide[:, 8:8 + k] = normal(g, m, k, dtype=torch.bfloat16)
+    wide[3:5, 8 + k:] = math.inf
+    x = wide.to(DEV)[:, 8:8 + k]
+    p = K.pack_weight4(normal(g, n, k).to(DEV))
+    w, xd = R.weight_values(p.data, n, k), x.double().cpu()
+    want = xd @ w.T
+    within(K.linear4(x, p), want, linear_bound(xd, w, k, torch.bfloat16, 0.0, want, None))
+
+
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
 def test_linear_takes_any_rows(dt):
     """Views at odd offsets with wide rows, expanded rows, results into views, and onto the residual itself."""

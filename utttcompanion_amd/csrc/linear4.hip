@@ -27,10 +27,22 @@ constexpr int kRowLds = 49152;  // bytes of a row's parts that k_gemv4 takes
 typedef bf16x8 bf16x8_any __attribute__((aligned(2)));
 typedef f32x4 f32x4_any __attribute__((aligned(4)));
 
+// A row's eight neighbours that end with the row, to those from column k0 on.
+__device__ __forceinline__ bf16x8 tail_x8(bf16x8 v, int k0, int k) {
+  typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
+  const u64x2 q = __builtin_bit_cast(u64x2, v);
+  const int over = min(max(k0 + 8 - k, 0), 8), bits = 16 * (over & 3);
+  const uint64_t low = over >= 4 ? q.y : q.x, high = over >= 4 ? 0 : q.y;
+  const u64x2 y{low >> bits | (high << 1) << (63 - bits), high >> bits};
+  return __builtin_bit_cast(bf16x8, over == 8 ? u64x2{0, 0} : y);
+}
+
 __device__ __forceinline__ bf16x8 load_x8(const bf16* row, int k0, int k) {
   bf16x8 v;
   if (k0 + 8 <= k) {
     v = *reinterpret_cast<const bf16x8_any*>(row + k0);
+  } else if (k >= 8) {
+    v = tail_x8(*reinterpret_cast<const bf16x8_any*>(row + k - 8), k0, k);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = k0 + j < k ? row[k0 + j] : static_cast<bf16>(0.f);
@@ -617,7 +629,7 @@ __global__ void __launch_bounds__(W * 64, W == 4 ? 2 : 1) k_prod4(const Prod4Arg
 
 // Many blocks of W: WN waves beside each other take NT blocks of 16 rows each and share x, which passes through LDS in steps
 // that all of them load together; 8 / WN such teams divide the columns.  Of 32 rows by 32000 x 2048 the operands of x are
-// then a fourth of what every wave would fetch for itself.  Grid (n / (16 NT WN), m / (16 MT), batch).
+// then a fourth of what every wave would fetch for itself.  Rows of 8 columns or more.  Grid (n / (16 NT WN), m / (16 MT), batch).
 template <typename O, int MT, int NT, int WN>
 __global__ void __launch_bounds__(512, 2) k_share4(const Prod4Args a) {
   constexpr int WK = 8 / WN;
@@ -668,15 +680,17 @@ __global__ void __launch_bounds__(512, 2) k_share4(const Prod4Args a) {
     for (int i = 0; i < kEach; ++i) {
       const int piece = i * WN + wn, half = min(half0 + piece / (2 * MT), halves - 1), k0 = half * 64 + 8 * (lane & 7);
       const bf16* row = base + (int64_t)min(m0 + 8 * (piece % (2 * MT)) + (lane >> 3), a.m - 1) * a.xs_m;
-      v.x[i] = half * 64 + 64 <= a.k ? *reinterpret_cast<const bf16x8_any*>(row + k0) : load_x8(row, k0, a.k);
+      v.x[i] = *reinterpret_cast<const bf16x8_any*>(row + min(k0, a.k - 8));
     }
     return v;
   };
-  auto store = [&](const Pieces& v, int buf) {
+  auto store = [&](Pieces v, int buf, int half0) {
     char* to = lds + (wk * 2 + buf) * kStep;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       const int piece = i * WN + wn, t = 8 * (piece % (2 * MT)) + (lane >> 3);
+      const int half = min(half0 + piece / (2 * MT), halves - 1);
+      if (half * 64 + 64 > a.k) v.x[i] = tail_x8(v.x[i], half * 64 + 8 * (lane & 7), a.k);
       *reinterpret_cast<bf16x8*>(to + piece / (2 * MT) * (MT * 2048) + t * 128 + (((lane & 7) ^ row_swz(t)) * 16)) = v.x[i];
     }
   };
@@ -718,7 +732,7 @@ __global__ void __launch_bounds__(512, 2) k_share4(const Prod4Args a) {
     pieces[u] = load(2 * begin + u * H);
     if (u < kWeights) q[u] = weights(begin + u);
   }
-  store(pieces[0], 0);
+  store(pieces[0], 0, 2 * begin);
   pieces[0] = load(2 * begin + 4 * H);
   for (int i0 = 0; i0 < steps; i0 += 4) {
 #pragma unroll
@@ -726,7 +740,7 @@ __global__ void __launch_bounds__(512, 2) k_share4(const Prod4Args a) {
       const int i = i0 + u;
       if (i >= steps) break;
       __syncthreads();
-      store(pieces[(u + 1) & 3], (u + 1) & 1);
+      store(pieces[(u + 1) & 3], (u + 1) & 1, 2 * begin + (i + 1) * H);
       pieces[(u + 1) & 3] = load(2 * begin + (i + 5) * H);
       const int kb = begin + i * H / 2;
       if constexpr (H == 2) {
@@ -820,9 +834,9 @@ template <typename O, int P>
 void launch_linear_rows(const Prod4Args& p, int batch, hipStream_t st) {
   const int64_t tiles = (p.n + 15) / 16 * batch * ((p.m + 31) / 32);
   if constexpr (P == 1) {
-    if (tiles >= 1536)
+    if (tiles >= 1536 && p.k >= 8)
       launch_share<O, 2, 4>(p, batch, st);
-    else if (tiles >= 192)
+    else if (tiles >= 192 && p.k >= 8)
       launch_share<O, 1, 2>(p, batch, st);
     else
       launch_rows<O, P, 1, 8, false>(p, batch, st);
