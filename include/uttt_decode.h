@@ -40,7 +40,7 @@ int uttt_decode_abi_version(void);
  * 1. out = x W^T (+ residual) with W in 4 bits, for the rows of a decode step: the slow projections and the LM head
  *    (engine/inference.py:222-279).  x_eps > 0: the rows of x are RMS-normalised first (the norm's weight belongs into W's
  *    columns before they are quantised).  Products are formed from x's own values (fp32 ones whole), sums in fp32;
- *    the result is rounded once.  out may be the residual.  x of any alignment and row stride >= k.
+ *    the result is rounded once.  out may be the residual, and lies apart from x.  x of any alignment and row stride >= k.
  * ------------------------------------------------------------------------- */
 typedef struct {
   int64_t m, n, k; /* m <= 2^20, n <= 2^24, k <= 2^20 */
@@ -99,7 +99,7 @@ typedef struct {
   const void* v_new; int64_t v_stride_n, v_stride_t, v_stride_h;
   const void* cache; int64_t cache_stride_n; /* bytes; (Hkv, blocks, 36 head_dim) inside; 0: one cache for all */
   void* out; int64_t o_stride_n, o_stride_t, o_stride_h;
-  void* k_nodes; void* v_nodes; int64_t nodes_stride_n; /* (nodes, Hkv, hd) inside; both or neither */
+  void* k_nodes; void* v_nodes; int64_t nodes_stride_n; /* (nodes, Hkv, hd) inside; both or neither; not k_new / v_new */
   void* workspace; size_t workspace_bytes; /* rewritten by every call: calls sharing it must be ordered */
 } uttt_swa_tree4_args;
 

@@ -430,6 +430,34 @@ def test_requests_out_of_range_are_nan(t):
     assert all((m[:4] == 3).all() and (m[4] != 3).any() for m in marks)
 
 
+@pytest.mark.parametrize("t", [1, 3])
+def test_the_largest_positions(t):
+    """Positions next to 2^63: past the tables where there are any; without them one like any other behind a full window."""
+    g = gen(t)
+    window, sinks, hd = 50, 2, 64
+    c = cache_of(g, 1, 2, 1, window, sinks, hd)[0].to(DEV)
+    q, k_new, v_new = (normal(g, 2, t, h, hd).to(DEV) for h in (2, 1, 1))
+    far = torch.tensor([2 ** 63 - 1, 2 ** 63 - 2])
+    cos, sin = (x.to(DEV) for x in tables(100, hd))
+    assert torch.isnan(K.swa_tree4(q, k_new, v_new, c, far.to(DEV), window, None, cos, sin, sinks)[0]).all()
+    alike = sinks + window * 4 + (far - sinks) % window  # the same slots, the same window
+    got, want = (K.swa_tree4(q, k_new, v_new, c, p.to(DEV), window, sinks=sinks)[0] for p in (far, alike))
+    assert torch.equal(got, want) and not torch.isnan(got).any()
+
+
+def test_outputs_apart_from_inputs():
+    g = gen(9)
+    x = normal(g, 3, 64).to(DEV)
+    p = K.pack_weight4(normal(g, 64, 64).to(DEV))
+    with pytest.raises(ValueError, match="apart from x"):
+        K.linear4(x, p, out=x)
+    c = cache_of(g, 1, 1, 1, 32, 0, 64)[0].to(DEV)
+    q, k, v = (normal(g, 1, 20, 1, 64).to(DEV) for _ in range(3))
+    for nodes in ((k, v), (torch.empty_like(k), k), (v, torch.empty_like(k))):
+        with pytest.raises(ValueError, match="apart from the new"):
+            K.swa_tree4(q, k, v, c, torch.tensor([5], device=DEV), 32, node_outputs=nodes)
+
+
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
 def test_what_a_query_does_not_see_may_be_anything(dt):
     """Scales that are NaN or infinite in slots without a visible token, infinities and NaN in nodes on other branches, rows

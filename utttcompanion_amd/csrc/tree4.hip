@@ -91,11 +91,11 @@ __device__ __forceinline__ Tree read_tree(const Tree4Args& a, int n) {
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) deepest = max(deepest, __shfl_xor(deepest, off, 64));
   t.deepest = deepest;
-  if (a.cos_table != nullptr && t.count > 0) t.bad |= t.pos + deepest >= a.table_len;
+  if (a.cos_table != nullptr && t.count > 0) t.bad |= t.pos >= a.table_len - deepest;
   if (deepest >= a.window) {  // ancestors may be out of the window
     for (int j = 0; j < t.count; ++j) {
       const int dj = __shfl(t.depth, j, 64);
-      if (t.depth - dj >= a.window && t.pos + dj >= a.sinks) path &= ~(1ull << j);
+      if (t.depth - dj >= a.window && t.pos >= a.sinks - dj) path &= ~(1ull << j);
     }
   }
   t.sees = path;

@@ -1746,7 +1746,7 @@ def linear4(x: Tensor, weight: Weight4, out: Optional[Tensor] = None, residual: 
             x_eps: float = 0.0) -> Tensor:
     """out = x weight^T (+ residual) with a weight in 4 bits (``uttt_linear4``; ``pack_weight4``): the decode step's
     projections and LM head (reference engine/inference.py:263-276).  x (m, k) bf16 or fp32, any m, k and row stride;
-    ``residual`` (m, n) may be ``out`` itself.  ``x_eps`` > 0 RMS-normalises x's rows first (pack the weight with
+    ``residual`` (m, n) may be ``out`` itself; else both lie apart from it.  ``x_eps`` > 0 RMS-normalises x's rows first (pack the weight with
     the norm weight multiplied into its columns).  Products are of x's whole values, sums fp32, rounded once."""
     if x.dim() != 2 or x.shape[1] != weight.k:
         raise ValueError(f"x must be (m, {weight.k}), got {tuple(x.shape)}")
@@ -1767,6 +1767,8 @@ def linear4(x: Tensor, weight: Weight4, out: Optional[Tensor] = None, residual: 
         out = x.new_empty((m, n))
     elif out.shape != (m, n) or out.dtype is not dt or n > 1 and out.stride(1) != 1 or m > 1 and out.stride(0) < n:
         raise ValueError(f"out must be ({m}, {n}) of x's dtype with unit column stride and rows apart")
+    elif out.data_ptr() == x.data_ptr():
+        raise ValueError("out must lie apart from x")
     p_r = r_stride = 0
     if residual is not None:
         if residual.shape != (m, n) or residual.dtype is not dt or n > 1 and residual.stride(1) != 1:
@@ -1900,8 +1902,8 @@ def swa_tree4(q: Tensor, k_new: Tensor, v_new: Tensor, cache: Tensor, positions:
     (N, T, Hkv, hd) (un-rotated when tables are given), T <= 64 nodes, ``cache`` (N, Hkv, blocks, 36 hd) of ``kv_cache4``
     holding ``positions`` (N,) int64 tokens each.  ``parents``, ``counts`` and what comes back as in ``swa_tree``; a decode step is
     one node per request, whose keys and values ``kv_commit4`` then takes in.  The new tokens are seen in their own
-    precision.  ``node_outputs``: (N, T, Hkv, hd), each request's part contiguous.  ``workspace``: calls that share one must be
-    ordered."""
+    precision.  ``node_outputs``: (N, T, Hkv, hd), each request's part contiguous, apart from ``k_new`` and ``v_new``.
+    ``workspace``: calls that share one must be ordered."""
     if q.dim() != 4:
         raise ValueError("q must be (N, T, H, hd)")
     n, nodes, heads, hd = shape = q.shape
@@ -1951,6 +1953,8 @@ def swa_tree4(q: Tensor, k_new: Tensor, v_new: Tensor, cache: Tensor, positions:
             if t.shape != new_shape or t.dtype is not dt or _pieces(t, 1) is not t or _strides(t, 1)[0] != nodes_n:
                 raise ValueError("node outputs must be (N, nodes, Hkv, hd) tensors of q's dtype, alike, each request's part "
                                  "contiguous and 16-byte aligned")
+        if {k_nodes.data_ptr(), v_nodes.data_ptr()} & {k_new.data_ptr(), v_new.data_ptr()} and n:
+            raise ValueError("node outputs must lie apart from the new keys and values")
     else:
         k_nodes, v_nodes = made(new_shape), made(new_shape)
         nodes_n = nodes * hkv * hd
