@@ -266,3 +266,14 @@ def test_strides_streams_capture_and_repeatability():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip((out, *nodes), want)), i
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_the_largest_positions_are_past_the_tables(dtype):
+    from utttcompanion_amd import kernels as K
+    n, t, heads, hkv, hd, window, sinks = 2, 4, 4, 2, 64, 48, 4
+    qkv, rings, _, _, (cos, sin) = make(n, t, heads, hkv, hd, window, sinks, [30] * n, dtype, 6)
+    q, k, v = qkv.to(DEV).split([heads, hkv, hkv], dim=2)
+    pos = torch.tensor([2 ** 63 - 1, 2 ** 63 - 2], device=DEV)
+    out, _, _ = K.swa_tree(q, k, v, *(r.to(DEV) for r in rings), pos, None, cos.to(DEV), sin.to(DEV), sinks=sinks)
+    assert bool(out.isnan().all())

@@ -96,11 +96,11 @@ __device__ __forceinline__ Tree read_tree(const TreeArgs& a, int n, int count, i
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) d = max(d, __shfl_xor(d, off, 64));
   t.deepest = uniform(d);
-  t.bad = __any(bad) || pos < 0 || (a.cos_table != nullptr && pos + t.deepest >= a.table_len);
+  t.bad = __any(bad) || pos < 0 || (a.cos_table != nullptr && pos >= a.table_len - t.deepest);
   if (t.deepest >= a.window && !t.bad) {  // ancestors out of the window
     for (int j = 0; j < count; ++j) {
       const int dj = __shfl(t.depth, j, 64);
-      if (t.depth - dj >= a.window && pos + dj >= a.sinks) t.sees &= ~(1ull << j);
+      if (t.depth - dj >= a.window && pos >= a.sinks - dj) t.sees &= ~(1ull << j);
     }
   }
   return t;
