@@ -62,6 +62,20 @@ def test_equal_logits(vocab, dt):
     check(few, torch.zeros(4, device=DEV), 2, banned=(7, 16, 25))
 
 
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("groups,beams,vocab", [(1, 32, 131072), (2, 32, 131072), (1, 20, 50000)])
+def test_beams_of_unlike_scores(groups, beams, vocab, dt):
+    """Many candidates of a few beams among the best: scores far apart, beams whose logits are alike, coarse logits."""
+    g = torch.Generator().manual_seed(groups + beams + vocab)
+    rows = groups * beams
+    x = torch.randn(rows, vocab, generator=g)
+    alike = x[:1].repeat(rows, 1)
+    for logits in (x, alike, (4 * x).round() / 4):
+        for spread in (0.01, 1.0, 8.0):
+            scores = spread * torch.randn(rows, generator=g)
+            check(logits.to(dt).to(DEV), scores.to(DEV), beams)
+
+
 def test_rows_that_offer_nothing():
     g = torch.Generator().manual_seed(3)
     x = torch.randn(8, 600, generator=g).to(DEV)

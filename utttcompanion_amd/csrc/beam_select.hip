@@ -7,7 +7,9 @@
 // Within a row the order is that of (logit, id), so the first launch, a workgroup per part of a row, finds each part's maximum,
 // sum and `beams` best by (logit, id) alone.  No sort: the beams-th largest of a wave's 64 lane maxima, found bit by bit
 // with ballots, is a bound that at least `beams` elements reach; the few that reach it are listed in LDS and, at the end,
-// ranked against each other.  The second launch, a workgroup per group, does the same with the parts' best and their values.
+// ranked against each other.  16 x 16 rows of 131072 fp32 ids take 24 to 26 us, what reading them takes (5.2 TB/s).
+// The second launch, a workgroup per group, does the same with the parts' best and their values: 5 to 8 us of latency, some
+// 30 more for many beams whose scores lie far apart (one group of 32 of 131072 ids 54 to 71 for both launches).
 #include <algorithm>
 
 #include "../../include/uttt_decode.h"
@@ -20,9 +22,11 @@ namespace {
 constexpr int kMaxBeams = 32;
 constexpr int kPer = 16;                     // elements of a thread
 constexpr int kStretch = kThreads * kPer;    // of a workgroup
-constexpr int kListed = 512;                 // elements at the bound that a list holds; more (equal logits) are chosen one by one
+constexpr int kListed = 512;                 // elements at the bound that a list holds; more are chosen one by one
 constexpr int kMergeThreads = 1024;
-constexpr int kFill = 1024;                  // workgroups that parts of rows are cut into, where there are fewer rows
+// Workgroups that parts of rows are cut into, where there are fewer rows.  Both launches, us, with 512, 1024 and 2048: 16 x 16
+// beams of 131072 ids 37.8, 38.6, 41.9; one group of 16 of them 23.7, 22.8, 28.8; 64 x 4 of 50000 21.9, 19.6, 22.4.
+constexpr int kFill = 1024;
 constexpr float kLog2e = 1.44269504088896340736f;
 
 struct BeamArgs {
@@ -248,7 +252,7 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const BeamArgs a) 
   __shared__ double add[kMaxBeams];  // score_b - log sum_b
   __shared__ float tops[kMaxBeams];
   __shared__ int kind[kMaxBeams];  // 0: offers none, 1: its ids, 2: ended
-  __shared__ uint32_t bounds[kWaves];
+  __shared__ uint32_t bounds[kWaves], shares[kWaves], highs[kWaves];
   __shared__ uint64_t wide_v[kWaves];
   __shared__ uint32_t wide_p[kWaves];
   __shared__ int listed;
@@ -296,26 +300,73 @@ __global__ void __launch_bounds__(kMergeThreads) k_beam_merge(const BeamArgs a) 
     place = (uint32_t)(b * a.vocab) + (uint32_t)~(uint32_t)k;
     return ordered(((double)unordered((uint32_t)(k >> 32)) - (double)tops[b]) + add[b]);
   };
-  uint32_t high = 0, place;
+  uint32_t high = 0, place, bound = 0;
   for (int i = threadIdx.x; i < total; i += kMergeThreads) high = max(high, (uint32_t)(look(i, place) >> 32));
   const uint32_t mine = reached_by<32>(high, a.beams);
   if (lane == 0) bounds[w] = mine;
   __syncthreads();
-  uint32_t bound = 0;
 #pragma unroll
   for (int j = 0; j < kWaves; ++j) bound = max(bound, bounds[j]);
-  for (int i = threadIdx.x; i < total; i += kMergeThreads) {
-    const uint64_t v = look(i, place);
-    if (v != 0 && (uint32_t)(v >> 32) >= bound) {
-      const int to = atomicAdd(&listed, 1);
-      if (to < kListed) {
-        values[to] = v;
-        places[to] = place;
+  int n;
+  // Where more reach it than the list holds (beams of very different scores, equal logits), what a share of the `beams` reaches
+  // in every wave is another bound; then bounds are halved towards a higher one that `beams` still reach.  One group of 32 beams
+  // of 131072 bf16 ids: 54 to 71 us, choosing its 32 one by one 660.
+  for (uint32_t over = ~0u, tries = 0;; ++tries) {
+    for (int i = threadIdx.x; i < total; i += kMergeThreads) {
+      const uint64_t v = look(i, place);
+      if (v != 0 && (uint32_t)(v >> 32) >= bound) {
+        const int to = atomicAdd(&listed, 1);
+        if (to < kListed) {
+          values[to] = v;
+          places[to] = place;
+        }
       }
     }
+    __syncthreads();
+    n = listed;
+    if (n <= kListed) break;
+    uint32_t next = bound;
+    if (tries == 0) {
+      const uint32_t share = reached_by<32>(high, (a.beams + kWaves - 1) / kWaves);
+      uint32_t highest = high;
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) highest = max(highest, (uint32_t)__shfl_xor((int)highest, off, 64));
+      if (lane == 0) {
+        shares[w] = share;
+        highs[w] = highest;
+      }
+      __syncthreads();
+      uint32_t common = ~0u;
+      over = 0;
+#pragma unroll
+      for (int j = 0; j < kWaves; ++j) {
+        common = min(common, shares[j]);
+        over = max(over, highs[j] + 1);
+      }
+      next = max(bound, common);
+    }
+    while (next == bound && over - next > 1) {
+      const uint32_t mid = next + (over - next) / 2;
+      int reached = 0;
+      for (int i = threadIdx.x; i < total; i += kMergeThreads) reached += (uint32_t)(look(i, place) >> 32) >= mid;
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) reached += __shfl_xor(reached, off, 64);
+      if (lane == 0) bounds[w] = reached;
+      __syncthreads();
+      reached = 0;
+#pragma unroll
+      for (int j = 0; j < kWaves; ++j) reached += bounds[j];
+      __syncthreads();
+      if (reached < a.beams)
+        over = mid;
+      else
+        next = mid;
+    }
+    if (next == bound) break;  // equal ones
+    bound = next;
+    if (threadIdx.x == 0) listed = 0;
+    __syncthreads();
   }
-  __syncthreads();
-  const int n = listed;
   auto emit = [&](int rank, uint64_t v, uint32_t p) {
     const int b = (int)(p / a.vocab);
     const int64_t token = p - b * a.vocab;
