@@ -158,12 +158,12 @@ int uttt_kv_fork4(const uttt_kv_fork4_args* args, uttt_stream_t stream);
 
 /* ---------------------------------------------------------------------------
  * 7. Beam search's choice: per group of `beams` rows, over beams b and the ids v that are below active_limit, not banned
- *    and above -inf, the `beams` best of  score_b + x_bv - log sum_v exp(x_bv)  (sum over those ids; in 64 bits), of equal
- *    ones the lower beam's, then the lower id.  A beam with ended_in != 0 offers one continuation instead, `pad` at its own
- *    score; one whose score or whose largest logit is not finite offers none.  Results, the best first: the token, the row it
- *    goes on from (uttt_kv_fork's sources), its score, and whether the beam has ended (its row had, or the token is
- *    eos; eos < 0: no id ends one).  Where a group offers fewer than `beams`, the rest are `pad` at -inf
- *    from their own rows, ended.
+ *    and above -inf, the `beams` best of  score_b + x_bv - log sum_v exp(x_bv)  (sum over those ids, of fp32 exponentials
+ *    in 64 bits; the scores in 64 bits), of equal ones the lower beam's, then the lower id.  A beam with ended_in != 0
+ *    offers one continuation instead, `pad` at its own score; one whose score or whose largest logit is not finite, or with
+ *    NaN among those ids, offers none.  Results, the best first: the token, the row it goes on from (uttt_kv_fork's
+ *    sources), its score, and whether the beam has ended (its row had, or the token is eos; eos < 0: no id ends one).
+ *    Where a group offers fewer than `beams`, the rest are `pad` at -inf from their own rows, ended.
  * ------------------------------------------------------------------------- */
 typedef struct {
   int64_t rows, vocab, beams; /* rows a multiple of beams; beams <= 32; vocab <= 2^20 */

@@ -41,7 +41,8 @@ class BatchedDecoder:
 
     ``weight_bits`` 4: the slow weights (the norms before them folded in, embeddings aside) and each request's fast weights in 4 bits,
     packed when they are first used and here; ``cache_bits`` 4: keys and values in 4 bits (prompts are prefilled in the
-    model's type).  A step's new tokens are seen in their own precision and quantised behind the step."""
+    model's type).  A step's or a tree's new tokens are seen in their own precision and quantised behind it, so that
+    speculated tokens may differ from stepped ones where logits are close."""
 
     def __init__(self, model: uTTTModel, states: Sequence[FastWeightState], max_positions: int = 8192,
                  weight_bits: int = 16, cache_bits: int = 16):
