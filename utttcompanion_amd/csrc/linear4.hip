@@ -148,7 +148,7 @@ __device__ __forceinline__ void readout_norm(const Norm4Args& a, const float* z,
   }
 }
 
-// Grid (T, B).
+// Grid (T, B).  Latency: 3 us for 32 rows of 768.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) k_readout4_norm(const Norm4Args a) {
   __shared__ float scratch[kMaxWaves4];
@@ -177,7 +177,10 @@ struct Gemv4Args {
   Norm4Args norm;
 };
 
-// A tile of 16 rows of W per `split` waves, 4 waves at least to a workgroup.  Grid (tiles, batch).
+// A tile of 16 rows of W per `split` waves, 4 waves at least to a workgroup: x's parts are read from LDS as rows of the operand,
+// so that one product serves them all, and the codes go from memory into the product.  Bound by reading W where there
+// is much of it: a row by 32000 x 2048 7.8 us (4.7 TB/s), readouts of 32 x (2048, 5504) 115 us (5.3 TB/s, partly from the infinity
+// cache); by latency where not: 3.4 us by 1280 x 768, a readout of 768 x 2048 5 + 6.  Grid (tiles, batch).
 template <typename X, typename T, int P, Row MODE>
 __global__ void __launch_bounds__(kMaxWaves4 * 64) k_gemv4(const Gemv4Args a) {
   constexpr int S = MODE == Row::kSwiglu ? 2 : 1;
@@ -339,7 +342,7 @@ struct Parts4Args {
 constexpr int kPartsColumns = kThreads * 8;
 
 // Rows as bf16 parts, RMS-normalised and multiplied by the norm's weight where there is one.  Grid (m, columns, B); every
-// workgroup of a row forms its sum of squares.
+// workgroup of a row forms its sum of squares.  Latency: 61 rows of 5501 fp32 values 3 to 5 us.
 template <typename X, int P>
 __global__ void __launch_bounds__(kThreads) k_parts4(const Parts4Args a) {
   __shared__ float scratch[kMaxWaves4];
@@ -422,7 +425,7 @@ __device__ __forceinline__ void finish_row(const Prod4Args& a, int b, int m, int
 // Grid (n / (16 NT), m / (16 MT), batch); the W waves divide the columns and meet in LDS.  Operands are loaded 64 columns
 // ahead, pieces of the weights 128.  Rows of one part go through LDS, a wave's own, 8 lanes to 128 bytes of a row: read as
 // operands, where neighbouring lanes are different rows, every lane would be an access of its own (32 rows by 8000 x 2048
-// took 12 us).
+// took 12 us for 7).  Latency at a few hundred tiles: 32 rows by 768 x 768 3.7 us, by 2048 x 2048 5.
 template <typename O, int P, int MT, int NT, int W, bool SWIGLU>
 __global__ void __launch_bounds__(W * 64, W == 4 ? 2 : 1) k_prod4(const Prod4Args a) {
   constexpr int kStage = P == 1 ? W * MT * 2048 : 0, kMeet = W * NT * MT * 1024;
@@ -627,9 +630,11 @@ __global__ void __launch_bounds__(W * 64, W == 4 ? 2 : 1) k_prod4(const Prod4Arg
   }
 }
 
-// Many blocks of W: WN waves beside each other take NT blocks of 16 rows each and share x, which passes through LDS in steps
-// that all of them load together; 8 / WN such teams divide the columns.  Of 32 rows by 32000 x 2048 the operands of x are
-// then a fourth of what every wave would fetch for itself.  Rows of 8 columns or more.  Grid (n / (16 NT WN), m / (16 MT), batch).
+// Many blocks of W: WN waves beside each other take NT blocks of 16 rows each and share x, which passes through LDS in
+// steps that all of them load together; 8 / WN such teams divide the columns.  Of 32 rows by 32000 x 2048 the operands of x
+// are then a fourth of what every wave would fetch for itself; 12.6 us (13.9 with the norm, whose sums are products too),
+// bound by conversions, scales and products (1520 vector instructions a wave), 64 rows 21.4.  Rows of 8 columns or more.
+// Grid (n / (16 NT WN), m / (16 MT), batch).
 template <typename O, int MT, int NT, int WN>
 __global__ void __launch_bounds__(512, 2) k_share4(const Prod4Args a) {
   constexpr int WK = 8 / WN;
@@ -802,7 +807,8 @@ void launch_rows(const Prod4Args& p, int batch, hipStream_t st) {
   const int tiles = (p.n + 15) / 16, per = SWIGLU ? NT / 2 : NT;
   const int mt = p.m <= 16 ? 1 : p.m <= 32 || P > 1 ? 2 : 4;
   const int nsplit = splits(P, NT, W, SWIGLU) ? p.nsplit : 1;
-  const dim3 grid((unsigned)((tiles + per - 1) / per * nsplit), (unsigned)((p.m + 16 * mt - 1) / (16 * mt)), (unsigned)batch), block(W * 64);
+  const dim3 grid((unsigned)((tiles + per - 1) / per * nsplit), (unsigned)((p.m + 16 * mt - 1) / (16 * mt)), (unsigned)batch);
+  const dim3 block(W * 64);
   if (mt == 1)
     hipLaunchKernelGGL((k_prod4<O, P, 1, NT, W, SWIGLU>), grid, block, 0, st, p);
   else if (mt == 2)
@@ -858,7 +864,8 @@ void launch_gemv(Gemv4Args g, int batch, hipStream_t st) {
   while (g.split < kMaxWaves4 && 2 * g.split <= g.blocks && (int64_t)g.tiles * batch * g.split < 2048) g.split *= 2;
   const int waves = std::max(4, g.split), per = waves / g.split;
   const size_t lds = (size_t)P * ((size_t)g.blocks * 256 + 64);
-  hipLaunchKernelGGL((k_gemv4<X, T, P, MODE>), dim3((unsigned)((g.tiles + per - 1) / per), (unsigned)batch), dim3(waves * 64), lds, st, g);
+  const dim3 grid((unsigned)((g.tiles + per - 1) / per), (unsigned)batch);
+  hipLaunchKernelGGL((k_gemv4<X, T, P, MODE>), grid, dim3(waves * 64), lds, st, g);
 }
 
 int64_t padded(int64_t k) { return (k + 127) / 128 * 128; }
@@ -892,6 +899,9 @@ struct Linear4Layout {
   }
 };
 
+// One token a row: two launches, each row's last workgroup of the second normalising it.  More: products of rows in parts, with
+// SwiGLU four waves to a workgroup (32 rows of 4 tokens, 768 x 2048: 43 us, with eight 50; 16 of 8 29 and 32; one of 16, 2048 x
+// 5504: 27 either way).
 template <typename T>
 void launch_readout4(const uttt_readout4_args* a, hipStream_t st) {
   constexpr int HP = sizeof(T) == 2 ? 2 : 3;  // parts of the hidden values

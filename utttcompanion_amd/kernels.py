@@ -1746,8 +1746,8 @@ def linear4(x: Tensor, weight: Weight4, out: Optional[Tensor] = None, residual: 
             x_eps: float = 0.0) -> Tensor:
     """out = x weight^T (+ residual) with a weight in 4 bits (``uttt_linear4``; ``pack_weight4``): the decode step's
     projections and LM head (reference engine/inference.py:263-276).  x (m, k) bf16 or fp32, any m, k and row stride;
-    ``residual`` (m, n) may be ``out`` itself; else both lie apart from it.  ``x_eps`` > 0 RMS-normalises x's rows first (pack the weight with
-    the norm weight multiplied into its columns).  Products are of x's whole values, sums fp32, rounded once."""
+    ``residual`` (m, n) may be ``out`` itself; else both lie apart from it.  ``x_eps`` > 0 RMS-normalises x's rows first (pack
+    the weight with the norm weight multiplied into its columns).  Products are of x's whole values, sums fp32, rounded once."""
     if x.dim() != 2 or x.shape[1] != weight.k:
         raise ValueError(f"x must be (m, {weight.k}), got {tuple(x.shape)}")
     m, k = x.shape
@@ -2020,8 +2020,8 @@ def kv_commit4(k_nodes: Tensor, v_nodes: Tensor, nodes: Optional[Tensor], counts
             k_nodes, v_nodes = (t.clone(memory_format=torch.contiguous_format) for t in (k_nodes, v_nodes))
         at = _strides(k_nodes, 4)
         p_k, p_v = k_nodes.data_ptr(), v_nodes.data_ptr()
-    packed = N.pack_kv_commit4(layers, n, hkv, shape[2], path, hd, window, sinks, code, bool(advance), p_k, p_v, *at[:4], p_nodes, path_stride, p_counts, p_cache, cache_l,
-                               cache_n, p_pos)
+    packed = N.pack_kv_commit4(layers, n, hkv, shape[2], path, hd, window, sinks, code, bool(advance), p_k, p_v, *at[:4], p_nodes,
+                               path_stride, p_counts, p_cache, cache_l, cache_n, p_pos)
     _serve_call(N.load_library().uttt_kv_commit4, packed, index, "uttt_kv_commit4")
 
 
