@@ -146,6 +146,35 @@ def test_all_in_four_bits(dtype):
     assert tokens.shape == (4, 6) and (logprobs <= 0).all()
 
 
+@pytest.mark.parametrize("captured", [False, True])
+def test_weights_in_four_bits_follow_the_model(captured):
+    """Weights and norms changed in place between steps, eager and captured, and verified trees between captured steps."""
+    model, states, prompts = make(3, torch.float32)
+    a = decoder(model, states, weight_bits=4)
+    first = a.prefill(prompts)
+    caches = [a.export_kv_caches(i) for i in range(4)]
+    if captured:
+        a.capture()
+    a.step(first.argmax(-1))
+    with torch.no_grad():
+        block = model.layers[1]
+        for w in (block.attn.wk.weight, block.attn.wo.weight, block.uttt.w_q.weight, block.uttt.w_o.weight, model.lm_head.weight):
+            w.mul_(1.0 + 0.5 * torch.rand(w.shape, generator=torch.Generator().manual_seed(len(w))).to(DEV))
+        block.attn_norm.weight.mul_(1.25)
+        model.norm.weight.mul_(0.75)
+    b = decoder(model, states, weight_bits=4)
+    for dec in (a, b):
+        dec.reset(caches, [len(p) for p in prompts])
+    tokens = first.argmax(-1)
+    for i in range(3):
+        if i == 1:
+            tree = tokens[:, None].repeat(1, 2)
+            assert torch.equal(a.verify(tree), b.verify(tree))
+        x, y = a.step(tokens).clone(), b.step(tokens).clone()
+        assert torch.equal(x, y)
+        tokens = y.argmax(-1)
+
+
 def eager_beams(model, state, prompt, beams, steps, eos):
     """Beam search by whole forwards of every hypothesis."""
     limit = model.active_vocab_limit
@@ -227,3 +256,13 @@ def test_refusals():
     dec.set_sampling(0.7)
     with pytest.raises(ValueError, match="samples"):
         dec.beam_search(first, 2, 4)
+
+
+def test_weights_whose_changes_are_not_counted_are_refused():
+    import copy
+    model, states, _ = make()
+    with torch.inference_mode():
+        other = copy.deepcopy(model)
+    assert any(p.is_inference() for p in other.parameters())
+    with pytest.raises(ValueError, match="inference tensors"):
+        decoder(other, states, weight_bits=4)

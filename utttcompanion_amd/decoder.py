@@ -40,7 +40,7 @@ class BatchedDecoder:
     """N requests, one token each per step, frozen fast weights (decode never writes them).
 
     ``weight_bits`` 4: the slow weights (the norms before them folded in, embeddings aside) and each request's fast weights in 4 bits,
-    packed when they are first used and here; ``cache_bits`` 4: keys and values in 4 bits (prompts are prefilled in the
+    packed when they are first used (again when the model's have changed) and here; ``cache_bits`` 4: keys and values in 4 bits (prompts are prefilled in the
     model's type).  A step's or a tree's new tokens are seen in their own precision and quantised behind it, so that
     speculated tokens may differ from stepped ones where logits are close."""
 
@@ -50,6 +50,8 @@ class BatchedDecoder:
             raise ValueError("call model.eval() before decoding")
         if weight_bits not in (4, 16) or cache_bits not in (4, 16):
             raise ValueError("weight_bits and cache_bits must be 4, or 16 for the model's own type")
+        if weight_bits == 4 and any(p.is_inference() for p in model.parameters()):
+            raise ValueError("weights in 4 bits follow the model's, whose changes inference tensors do not count")
         if not states:
             raise ValueError("need at least one request state")
         self.model = model
@@ -229,24 +231,47 @@ class BatchedDecoder:
             self._folds[id(weight)] = hit
         return hit[1]
 
-    def _packed4(self, weight: Tensor, norm) -> K.Weight4:
-        """W, or W diag(g) for an RMSNorm ``norm`` applied to its input, in 4 bits, rebuilt when either changes."""
-        key = (weight.data_ptr(), weight._version) + (() if norm is None else (norm.weight.data_ptr(), norm.weight._version))
-        hit = self._fours.get(id(weight))
+    def _packed4(self, name: Tuple, weight: Tensor, norm) -> K.Weight4:
+        """W, or W diag(g) for an RMSNorm ``norm`` applied to its input, in 4 bits, packed again (in place: a captured step reads
+        it) when either changes."""
+        key = (id(weight), weight.data_ptr(), weight._version)
+        if norm is not None:
+            key += (id(norm.weight), norm.weight.data_ptr(), norm.weight._version)
+        hit = self._fours.get(name)
         if hit is None or hit[0] != key:
             w = weight.detach()
-            hit = (key, K.pack_weight4(w if norm is None else w.float() * norm.weight.detach().float()[None, :]), weight)
-            self._fours[id(weight)] = hit
+            packed = K.pack_weight4(w if norm is None else w.float() * norm.weight.detach().float()[None, :])
+            if hit is not None:
+                hit[1].data.copy_(packed.data)
+                packed = hit[1]
+            hit = self._fours[name] = (key, packed, weight, norm and norm.weight)  # what the key names stays alive
         return hit[1]
 
-    def _linear(self, x: Tensor, weight: Tensor, residual: Optional[Tensor] = None, norm=None) -> Tensor:
-        """norm(x) W^T (+ residual, updated in place): ``uttt_linear4`` with weights in 4 bits, ``uttt_skinny_linear`` for bf16
-        steps of at most 64 requests (the RMSNorm folded in), the norm and the library GEMM otherwise."""
+    def _refresh4(self) -> None:
+        """The packed slow weights of a captured step as the model's are now."""
+        m = self.model
+        for li, block in enumerate(m.layers):
+            self._packed4(("qkv", li), block.attn.packed_qkv().to(self.dtype), self._folds_in(block.attn_norm))
+            self._packed4(("wo", li), block.attn.wo.weight, None)
+            self._packed4(("q", li), block.uttt.w_q.weight, self._folds_in(block.uttt_norm))
+            self._packed4(("o", li), block.uttt.w_o.weight, None)
+        self._packed4(("head",), m.lm_head.weight, self._folds_in(m.norm))
+
+    @staticmethod
+    def _folds_in(norm):
+        """An RMSNorm that ``uttt_linear4`` applies, None for one that has no eps of its own."""
+        return norm if norm is not None and (norm.eps or 0.0) > 0.0 else None
+
+    def _linear(self, x: Tensor, weight: Tensor, name: Tuple, residual: Optional[Tensor] = None, norm=None) -> Tensor:
+        """norm(x) W^T (+ residual, updated in place): ``uttt_linear4`` with weights in 4 bits (``name`` W's among them),
+        ``uttt_skinny_linear`` for bf16 steps of at most 64 requests (the RMSNorm folded in), the norm and the library GEMM
+        otherwise."""
         if self.weight_bits == 4:
-            if norm is not None and not (norm.eps or 0.0) > 0.0:
-                x, norm = norm(x), None
-            return K.linear4(x, self._packed4(weight, norm), out=residual, residual=residual,
-                             x_eps=0.0 if norm is None else norm.eps)
+            folds = self._folds_in(norm)
+            if norm is not folds:
+                x = norm(x)
+            return K.linear4(x, self._packed4(name, weight, folds), out=residual, residual=residual,
+                             x_eps=0.0 if folds is None else folds.eps)
         skinny = (x.dtype == torch.bfloat16 and weight.dtype == torch.bfloat16 and x.shape[0] <= 64
                   and weight.shape[0] % 32 == 0 and x.shape[1] % 64 == 0 and x.stride(1) == 1
                   and weight.is_contiguous() and (norm is None or (norm.eps or 0.0) > 0.0))
@@ -267,7 +292,7 @@ class BatchedDecoder:
         h = F.embedding(self.tokens, m.tok_embeddings.weight)  # (N, D)
         for li, block in enumerate(m.layers):
             attn = block.attn
-            qkv = self._linear(h, attn.packed_qkv().to(h.dtype), norm=block.attn_norm)  # (N, (H + 2 Hkv) hd)
+            qkv = self._linear(h, attn.packed_qkv().to(h.dtype), ("qkv", li), norm=block.attn_norm)  # (N, (H + 2 Hkv) hd)
             hq = self.heads * self.hd
             hk = self.hkv * self.hd
             q = qkv[:, :hq].view(n, self.heads, self.hd)
@@ -281,8 +306,8 @@ class BatchedDecoder:
                 kr, vr = self.rings[li]
                 att = K.swa_decode(q, k, v, kr, vr, self.positions, self.cos, self.sin, workspace=self._ws_attn,
                                    sinks=self.sinks)
-            h = self._linear(att.reshape(n, -1), attn.wo.weight, residual=h)
-            y = self._linear(h, block.uttt.w_q.weight, norm=block.uttt_norm)
+            h = self._linear(att.reshape(n, -1), attn.wo.weight, ("wo", li), residual=h)
+            y = self._linear(h, block.uttt.w_q.weight, ("q", li), norm=block.uttt_norm)
             qn = block.uttt.q_norm
             # every layer reads the same per-request copies: odd layers walk them backwards, so
             # each readout starts on the lines the previous one left in the infinity cache
@@ -298,8 +323,8 @@ class BatchedDecoder:
                 r = K.swiglu_readout(uq.view(n, 1, -1), self.w_up, self.w_gate, self.w_down, self.ln_weight,
                                      self.ln_bias, m.fast_weight_pool.eps, workspace=self._ws_read,
                                      sweep_reverse=rev)
-            h = self._linear(r.view(n, -1), block.uttt.w_o.weight, residual=h)
-        logits = self._linear(h, m.lm_head.weight, norm=m.norm)
+            h = self._linear(r.view(n, -1), block.uttt.w_o.weight, ("o", li), residual=h)
+        logits = self._linear(h, m.lm_head.weight, ("head",), norm=m.norm)
         if self.cache4 is not None:
             K.kv_commit4(*self._new4, None, None, self.cache4, self.positions, self.window, self.sinks)
         self.logits = logits
@@ -384,6 +409,8 @@ class BatchedDecoder:
         if self._sampling is not None:  # ahead of the step, so that a replay draws new ones
             self._sampling["uniforms"].uniform_(generator=self._sampling["generator"])
         if self._graph is not None:
+            if self.weight_bits == 4:
+                self._refresh4()
             self._graph.replay()
             self.next_tokens, self.logits = self.tokens, self._graph_logits
         else:
@@ -488,7 +515,7 @@ class BatchedDecoder:
         read_ws = None
         for li, block in enumerate(m.layers):
             attn = block.attn
-            qkv = self._linear(h, attn.packed_qkv().to(h.dtype), norm=block.attn_norm).view(n, nodes, -1)
+            qkv = self._linear(h, attn.packed_qkv().to(h.dtype), ("qkv", li), norm=block.attn_norm).view(n, nodes, -1)
             q = qkv[..., :hq].unflatten(-1, (self.heads, self.hd))
             k = qkv[..., hq:hq + hk].unflatten(-1, (self.hkv, self.hd))
             v = qkv[..., hq + hk:].unflatten(-1, (self.hkv, self.hd))
@@ -498,8 +525,8 @@ class BatchedDecoder:
                                         self.sinks, **new)
             else:
                 att, _, _ = K.swa_tree(q, k, v, *self.rings[li], self.positions, parents, self.cos, self.sin, self.sinks, **new)
-            h = self._linear(att.view(n * nodes, -1), attn.wo.weight, residual=h)
-            y = self._linear(h, block.uttt.w_q.weight, norm=block.uttt_norm)
+            h = self._linear(att.view(n * nodes, -1), attn.wo.weight, ("wo", li), residual=h)
+            y = self._linear(h, block.uttt.w_q.weight, ("q", li), norm=block.uttt_norm)
             qn = block.uttt.q_norm
             if self.fast4 is not None:
                 r = self._readout4(y.view(n, nodes, -1), qn)
@@ -509,8 +536,8 @@ class BatchedDecoder:
                     read_ws = K.readout_workspace(uq, self.w_up)
                 r = K.swiglu_readout(uq, self.w_up, self.w_gate, self.w_down, self.ln_weight, self.ln_bias,
                                      m.fast_weight_pool.eps, workspace=read_ws, sweep_reverse=li % 2 == 1)
-            h = self._linear(r.view(n * nodes, -1), block.uttt.w_o.weight, residual=h)
-        logits = self._linear(h, m.lm_head.weight, norm=m.norm)
+            h = self._linear(r.view(n * nodes, -1), block.uttt.w_o.weight, ("o", li), residual=h)
+        logits = self._linear(h, m.lm_head.weight, ("head",), norm=m.norm)
         self._nodes = (k_nodes, v_nodes)
         return logits.view(n, nodes, -1)
 
