@@ -231,46 +231,56 @@ class BatchedDecoder:
             self._folds[id(weight)] = hit
         return hit[1]
 
-    def _packed4(self, name: Tuple, weight: Tensor, norm) -> K.Weight4:
-        """W, or W diag(g) for an RMSNorm ``norm`` applied to its input, in 4 bits, packed again (in place: a captured step reads
-        it) when either changes."""
-        key = (id(weight), weight.data_ptr(), weight._version)
-        if norm is not None:
-            key += (id(norm.weight), norm.weight.data_ptr(), norm.weight._version)
+    def _packed4(self, name: Tuple, weights: Tuple[Tensor, ...], norm) -> K.Weight4:
+        """W (``weights``, one below the other), or W diag(g) for an RMSNorm ``norm`` applied to its input, in 4 bits, packed again
+        (in place: a captured step reads it) when any of them changes."""
+        sources = weights if norm is None else (*weights, norm.weight)
+        key = [(id(t), t.data_ptr(), t._version) for t in sources]
         hit = self._fours.get(name)
         if hit is None or hit[0] != key:
-            w = weight.detach()
-            packed = K.pack_weight4(w if norm is None else w.float() * norm.weight.detach().float()[None, :])
-            if hit is not None:
-                hit[1].data.copy_(packed.data)
-                packed = hit[1]
-            hit = self._fours[name] = (key, packed, weight, norm and norm.weight)  # what the key names stays alive
+            with torch.inference_mode(False), torch.no_grad():  # the next pack is copied into this one, in whatever mode
+                w = weights[0].detach() if len(weights) == 1 else torch.cat([t.detach() for t in weights]).to(self.dtype)
+                packed = K.pack_weight4(w if norm is None else w.float() * norm.weight.detach().float()[None, :])
+                if hit is not None:
+                    hit[1].data.copy_(packed.data)
+                    packed = hit[1]
+            hit = self._fours[name] = (key, packed, sources)  # what the key names stays alive
         return hit[1]
 
     def _refresh4(self) -> None:
         """The packed slow weights of a captured step as the model's are now."""
         m = self.model
         for li, block in enumerate(m.layers):
-            self._packed4(("qkv", li), block.attn.packed_qkv().to(self.dtype), self._folds_in(block.attn_norm))
-            self._packed4(("wo", li), block.attn.wo.weight, None)
-            self._packed4(("q", li), block.uttt.w_q.weight, self._folds_in(block.uttt_norm))
-            self._packed4(("o", li), block.uttt.w_o.weight, None)
-        self._packed4(("head",), m.lm_head.weight, self._folds_in(m.norm))
+            attn, uttt = block.attn, block.uttt
+            self._packed4(("qkv", li), self._qkv(attn), self._folds_in(block.attn_norm))
+            self._packed4(("wo", li), (attn.wo.weight,), None)
+            self._packed4(("q", li), (uttt.w_q.weight,), self._folds_in(block.uttt_norm))
+            self._packed4(("o", li), (uttt.w_o.weight,), None)
+        self._packed4(("head",), (m.lm_head.weight,), self._folds_in(m.norm))
+
+    def _qkv(self, attn) -> Union[Tensor, Tuple[Tensor, ...]]:
+        """The QKV weight in the activations' type: packed, or with weights in 4 bits its parts, whose changes it
+        follows."""
+        if self.weight_bits == 4:
+            return attn.wq.weight, attn.wk.weight, attn.wv.weight
+        return attn.packed_qkv().to(self.dtype)
 
     @staticmethod
     def _folds_in(norm):
         """An RMSNorm that ``uttt_linear4`` applies, None for one that has no eps of its own."""
         return norm if norm is not None and (norm.eps or 0.0) > 0.0 else None
 
-    def _linear(self, x: Tensor, weight: Tensor, name: Tuple, residual: Optional[Tensor] = None, norm=None) -> Tensor:
-        """norm(x) W^T (+ residual, updated in place): ``uttt_linear4`` with weights in 4 bits (``name`` W's among them),
-        ``uttt_skinny_linear`` for bf16 steps of at most 64 requests (the RMSNorm folded in), the norm and the library GEMM
+    def _linear(self, x: Tensor, weight: Union[Tensor, Tuple[Tensor, ...]], name: Tuple, residual: Optional[Tensor] = None,
+                norm=None) -> Tensor:
+        """norm(x) W^T (+ residual, updated in place): ``uttt_linear4`` with weights in 4 bits (``name`` W's among them, ``weight``
+        its parts where there are several), ``uttt_skinny_linear`` for bf16 steps of at most 64 requests (the RMSNorm folded in), the norm and the library GEMM
         otherwise."""
         if self.weight_bits == 4:
             folds = self._folds_in(norm)
             if norm is not folds:
                 x = norm(x)
-            return K.linear4(x, self._packed4(name, weight, folds), out=residual, residual=residual,
+            weights = weight if isinstance(weight, tuple) else (weight,)
+            return K.linear4(x, self._packed4(name, weights, folds), out=residual, residual=residual,
                              x_eps=0.0 if folds is None else folds.eps)
         skinny = (x.dtype == torch.bfloat16 and weight.dtype == torch.bfloat16 and x.shape[0] <= 64
                   and weight.shape[0] % 32 == 0 and x.shape[1] % 64 == 0 and x.stride(1) == 1
@@ -292,7 +302,7 @@ class BatchedDecoder:
         h = F.embedding(self.tokens, m.tok_embeddings.weight)  # (N, D)
         for li, block in enumerate(m.layers):
             attn = block.attn
-            qkv = self._linear(h, attn.packed_qkv().to(h.dtype), ("qkv", li), norm=block.attn_norm)  # (N, (H + 2 Hkv) hd)
+            qkv = self._linear(h, self._qkv(attn), ("qkv", li), norm=block.attn_norm)  # (N, (H + 2 Hkv) hd)
             hq = self.heads * self.hd
             hk = self.hkv * self.hd
             q = qkv[:, :hq].view(n, self.heads, self.hd)
@@ -515,7 +525,7 @@ class BatchedDecoder:
         read_ws = None
         for li, block in enumerate(m.layers):
             attn = block.attn
-            qkv = self._linear(h, attn.packed_qkv().to(h.dtype), ("qkv", li), norm=block.attn_norm).view(n, nodes, -1)
+            qkv = self._linear(h, self._qkv(attn), ("qkv", li), norm=block.attn_norm).view(n, nodes, -1)
             q = qkv[..., :hq].unflatten(-1, (self.heads, self.hd))
             k = qkv[..., hq:hq + hk].unflatten(-1, (self.hkv, self.hd))
             v = qkv[..., hq + hk:].unflatten(-1, (self.hkv, self.hd))

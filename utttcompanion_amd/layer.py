@@ -444,8 +444,10 @@ class SlidingWindowAttention(nn.Module):
             self._packed_qkv_key = None
             return
         if self._packed_qkv is None or key != self._packed_qkv_key:
-            self._packed_qkv = torch.cat([t.detach() for t in (self.wq.weight, self.wk.weight, self.wv.weight)],
-                                         dim=0)
+            # an ordinary tensor also where it is first built in inference mode: its version is read
+            with torch.inference_mode(False), torch.no_grad():
+                self._packed_qkv = torch.cat([t.detach() for t in (self.wq.weight, self.wk.weight, self.wv.weight)],
+                                             dim=0)
             self._packed_qkv_key = key
 
     def train(self, mode: bool = True):
