@@ -83,7 +83,8 @@ int uttt_readout4(const uttt_readout4_args* args, uttt_stream_t stream);
  *    (uttt_serve.h), the cache as above and never written.  Scores and sums are formed in fp32 from the values that
  *    the codes stand for.  One node per request is a decode step, whose token uttt_kv_commit4 then takes in.
  *    A request with a negative position, a position past the tables, or a node whose parent is neither -1 nor an
- *    earlier node gets NaN outputs and no key or value is written.  Values that a query does not see may be anything.
+ *    earlier node gets NaN outputs and no key or value is written.  Values that a query does not see may be anything;
+ *    a key whose score is -inf has no weight.
  * ------------------------------------------------------------------------- */
 typedef struct {
   int64_t n_req, n_heads, n_kv_heads, nodes, head_dim; /* head_dim 64 or 128; nodes in 1..64 */

@@ -1,0 +1,53 @@
+"""Attention over caches in 4 bits where numbers are not finite: a key of score -inf has no weight, one of +inf or NaN makes the rows
+that see it NaN."""
+import math
+
+import pytest
+import torch
+
+import decode_reference as R
+from test_gpu_decode4 import DEV, STEP, U, cache_of, gen, normal, within
+from utttcompanion_amd import kernels as K
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("t", [1, 6, 40])
+def test_infinite_new_keys(t, hd, dt):
+    """Single infinite elements of a few nodes' keys, seen by heads whose q has either sign, or 0, there."""
+    g = gen(t + hd)
+    window, sinks, heads, hkv = 50, 3, 4, 2
+    positions = torch.tensor([0, 30, 200])
+    n = len(positions)
+    c = cache_of(g, 1, n, hkv, window, sinks, hd)[0]
+    q, k, v = (normal(g, n, t, h, hd) for h in (heads, hkv, hkv))
+    q[1, 0, 1, 5] = 0.0
+    q, k, v = (x.to(dt) for x in (q, k, v))
+    parents = None
+    if t > 1:
+        parents = torch.tensor([[i // 2 - 1 if i % 2 else i - 1 for i in range(t)]] * n, dtype=torch.int32)
+        parents[:, 0] = -1
+    strange = [(0, 0), (1, 0), (2, min(3, t - 1))] + ([(0, 4), (1, 33), (2, 35)] if t > 33 else [])
+    for i, (row, node) in enumerate(strange):
+        k[row, node, 0, (5, 61)[i % 2]] = -math.inf if i % 3 == 2 else math.inf
+    out = K.swa_tree4(q.to(DEV), k.to(DEV), v.to(DEV), c.to(DEV), positions.to(DEV), window,
+                      None if parents is None else parents.to(DEV), sinks=sinks)[0].cpu()
+    keys, vals = R.cache_values(c, hd)
+    calm = torch.where(torch.isfinite(k), k, torch.zeros_like(k))
+    carried, weight = (2.0 ** -16, 2.0 ** -8) if dt is torch.bfloat16 else (2.0 ** -23, 2.0 ** -23)
+    none = some = 0
+    for i in range(n):
+        up = [-1] if parents is None else parents[i].tolist()
+        args = v[i].double(), keys[i], vals[i], int(positions[i]), window, sinks, up, t
+        want, size, seen = R.tree(q[i].double(), k[i].double(), *args)
+        score = R.tree(q[i].double(), calm[i].double(), *args)[2]  # of the keys that have a weight, and more
+        ds = score * (carried + (34 + hd / 32 + 8) * U) + 4 * U * 40
+        chain = (34 + (window + sinks + t) / 32 + 80) * U
+        rel = (2 * ds * (1 + ds)).unsqueeze(-1) + weight + 2 * chain + 8 * U
+        bad = torch.isnan(want).any(-1)
+        assert torch.isnan(out[i][bad]).all()
+        within(out[i][~bad], want[~bad], (rel * size + STEP[dt] * want.abs() * (1 + 2 ** -7))[~bad])
+        none, some = none + int(bad.sum()), some + int((~bad & ~torch.isfinite(seen)).sum())
+    assert none and some

@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(W * 64, W == 4 ? 2 : 1) k_swa_tree4(const Tree
       s += __shfl_xor(s, 16, 64);
       s += __shfl_xor(s, 32, 64);
       m = s;
-      l = h == 0 ? (fabsf(s) < INFINITY ? 1.f : NAN) : 0.f;
+      l = h == 0 ? (fabsf(s) < INFINITY ? 1.f : s == -INFINITY ? 0.f : NAN) : 0.f;  // at -inf its value goes with the first rescale
       const T* vp = static_cast<const T*>(a.v) + n * a.v_n + kvh * a.v_h;
 #pragma unroll
       for (int d = 0; d < D; ++d)
