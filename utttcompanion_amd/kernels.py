@@ -1560,8 +1560,8 @@ def _tree_call(q: Tensor, k_new: Tensor, v_new: Tensor, k_ring: Tensor, v_ring: 
     nbytes = _tree_workspace(n, heads, hkv, nodes, hd, slots, code)
     p_ws = 0
     if workspace is not None:
-        if workspace.numel() * workspace.element_size() < nbytes:
-            raise ValueError(f"the tree attention workspace must hold {nbytes} bytes")
+        if workspace.numel() * workspace.element_size() < nbytes or not workspace.is_contiguous():
+            raise ValueError(f"the tree attention workspace must be {nbytes} contiguous bytes")
         p_ws, nbytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     elif nbytes > 16:
         workspace = q.new_empty(nbytes, dtype=torch.uint8)
@@ -1967,8 +1967,8 @@ def swa_tree4(q: Tensor, k_new: Tensor, v_new: Tensor, cache: Tensor, positions:
     nbytes = _tree4_workspace(n, heads, hkv, nodes, hd, window, sinks)
     p_ws = 0
     if workspace is not None:
-        if workspace.numel() * workspace.element_size() < nbytes:
-            raise ValueError(f"the tree attention workspace must hold {nbytes} bytes")
+        if workspace.numel() * workspace.element_size() < nbytes or not workspace.is_contiguous():
+            raise ValueError(f"the tree attention workspace must be {nbytes} contiguous bytes")
         p_ws, nbytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     elif nbytes > 16:
         workspace = q.new_empty(nbytes, dtype=torch.uint8)
