@@ -51,3 +51,28 @@ def test_infinite_new_keys(t, hd, dt):
         within(out[i][~bad], want[~bad], (rel * size + STEP[dt] * want.abs() * (1 + 2 ** -7))[~bad])
         none, some = none + int(bad.sum()), some + int((~bad & ~torch.isfinite(seen)).sum())
     assert none and some
+
+
+@pytest.mark.parametrize("layers_inside", [False, True])
+def test_caches_between_others(layers_inside):
+    """Every other request of an odd number, every other layer: taken in and forked in place, what lies between left alone."""
+    g = gen(6)
+    window, sinks, hd, hkv, t = 40, 2, 64, 2, 9
+    whole = cache_of(g, 5, 5, hkv, window, sinks, hd).to(DEV)
+    if layers_inside:
+        whole = whole.transpose(0, 1)
+    k, v = (normal(g, 3, 3, t, hkv, hd).to(DEV) for _ in range(2))
+    positions = torch.tensor([0, 5, 77], device=DEV)
+    for pick in ((slice(None, None, 2), slice(None, None, 2)), (slice(0, 3), slice(None, None, 2)), (slice(None, None, 2), slice(2, 5))):
+        got, at = whole.clone(memory_format=torch.preserve_format), positions.clone()
+        view = got[pick]
+        alone, alone_at = view.clone(memory_format=torch.contiguous_format), positions.clone()
+        for c, p in ((view, at), (alone, alone_at)):
+            K.kv_commit4(k, v, None, None, c, p, window, sinks, advance=True)
+            K.kv_fork4(c, torch.tensor([2, 0, 1], dtype=torch.int32, device=DEV), p, window, sinks)
+        assert torch.equal(view, alone) and torch.equal(at, alone_at)
+        want = whole.clone()
+        want[pick] = alone
+        assert torch.equal(got, want)
+        for a, b in zip(K.kv_values4(view, window, sinks), K.kv_values4(alone, window, sinks)):
+            assert torch.equal(a.view(torch.int16), b.view(torch.int16))

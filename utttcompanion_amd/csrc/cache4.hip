@@ -327,9 +327,12 @@ int check_cache(const CacheShape& s, bool written) {
                "the cache must be non-NULL and 16-byte aligned with strides of whole 16-byte pieces");
   if (!written) return UTTT_OK;
   const int64_t slab = s.slab();
+  // the nearer of the two dimensions lies inside the other, whose strides reach past its last cache
+  const bool inside = s.c_l >= s.c_n;  // requests inside layers
+  const int64_t near = inside ? s.c_n : s.c_l, far = inside ? s.c_l : s.c_n, n_near = inside ? s.n_req : s.layers;
   const bool apart = s.n_req == 1 || s.layers == 1
                          ? (s.n_req == 1 || s.c_n >= slab) && (s.layers == 1 || s.c_l >= slab)
-                         : s.c_l >= s.c_n ? s.c_n >= slab && s.c_l / s.n_req >= s.c_n : s.c_l >= slab && s.c_n / s.layers >= s.c_l;
+                         : near >= slab && (far - slab) / near >= n_near - 1;
   UTTT_REQUIRE(apart, "the requests' caches must not overlap");
   return UTTT_OK;
 }
