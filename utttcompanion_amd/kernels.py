@@ -1767,7 +1767,7 @@ def linear4(x: Tensor, weight: Weight4, out: Optional[Tensor] = None, residual: 
         out = x.new_empty((m, n))
     elif out.shape != (m, n) or out.dtype is not dt or n > 1 and out.stride(1) != 1 or m > 1 and out.stride(0) < n:
         raise ValueError(f"out must be ({m}, {n}) of x's dtype with unit column stride and rows apart")
-    elif out.data_ptr() == x.data_ptr():
+    elif m and out.data_ptr() == x.data_ptr():
         raise ValueError("out must lie apart from x")
     p_r = r_stride = 0
     if residual is not None:
