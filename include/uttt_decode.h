@@ -159,10 +159,11 @@ int uttt_kv_fork4(const uttt_kv_fork4_args* args, uttt_stream_t stream);
 
 /* ---------------------------------------------------------------------------
  * 7. Beam search's choice: per group of `beams` rows, over beams b and the ids v that are below active_limit, not banned
- *    and above -inf, the `beams` best of  score_b + x_bv - log sum_v exp(x_bv)  (sum over those ids, of fp32 exponentials
- *    in 64 bits; the scores in 64 bits), of equal ones the lower beam's, then the lower id.  A beam with ended_in != 0
- *    offers one continuation instead, `pad` at its own score; one whose score or whose largest logit is not finite, or with
- *    NaN among those ids, offers none.  Results, the best first: the token, the row it goes on from (uttt_kv_fork's
+ *    and above -inf, the `beams` best of  score_b + x_bv - log sum_v exp(x_bv)  (sum over those ids), of equal ones the
+ *    lower beam's, then the lower id.  Scores are compared in 64 bits; a sum of exponentials is an fp32 one, off by some 2^-23
+ *    (at most 2^-15) of itself, so that values of two beams that are closer than that may change places.  A beam with
+ *    ended_in != 0 offers one continuation instead, `pad` at its own score; one whose score or whose largest logit is not
+ *    finite, or with NaN among those ids, offers none.  Results, the best first: the token, the row it goes on from (uttt_kv_fork's
  *    sources), its score, and whether the beam has ended (its row had, or the token is eos; eos < 0: no id ends one).
  *    Where a group offers fewer than `beams`, the rest are `pad` at -inf from their own rows, ended.
  * ------------------------------------------------------------------------- */

@@ -1,8 +1,11 @@
 // Beam search's choice, written for gfx950 (MI355X): the `beams` best continuations of every group of beams.
 //
-// value(b, v) = score_b + (x_bv - max_b) - log sum_v exp(x_bv - max_b), formed in 64 bits from logits in their own
-// precision, so that the order of candidates of different beams is the definition's; the exponentials are fp32 ones (their
-// errors average out far below what separates two beams), their sums 64-bit ones.
+// value(b, v) = score_b + (x_bv - max_b) - log sum_v exp(x_bv - max_b), formed in 64 bits from logits in their own precision and
+// the row's sum.  Within a row the order is exact.  Between rows it is the definition's where two values differ by more than the
+// sums' errors: exponentials are fp32 ones of fp32 differences, added up by sixteens in fp32 and from there on in 64
+// bits.  A term is off by 2^-24 (2.25 d + 2) of itself, d its distance from the top (difference, product with log2 e,
+// exponential; log(vocab) at most on average), sixteen of them by 2^-20, and a thread's sum by up to 2^-23 more each time its top
+// moves: 2^-15 at most, where logits rise all through a row of 2^20, and 2^-23 where they are as random as a model's.
 //
 // Within a row the order is that of (logit, id), so the first launch, a workgroup per part of a row, finds each part's maximum,
 // sum and `beams` best by (logit, id) alone.  No sort: the beams-th largest of a wave's 64 lane maxima, found bit by bit
