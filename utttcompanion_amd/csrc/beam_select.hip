@@ -10,7 +10,9 @@
 // Within a row the order is that of (logit, id), so the first launch, a workgroup per part of a row, finds each part's maximum,
 // sum and `beams` best by (logit, id) alone.  No sort: the beams-th largest of a wave's 64 lane maxima, found bit by bit
 // with ballots, is a bound that at least `beams` elements reach; the few that reach it are listed in LDS and, at the end,
-// ranked against each other.  16 x 16 rows of 131072 fp32 ids take 24 to 26 us, what reading them takes (5.2 TB/s).
+// ranked against each other.  16 x 16 rows of 131072 fp32 ids take 24 to 26 us, what reading them takes (5.2 TB/s).  Rows off 16
+// bytes, and a row's last stretch, are read element by element: both launches 60 us at 16 x 16 x 131073 bf16 ids, 31 at 131072 (fp32
+// 38 and 35; 16 x 4 of 50001 13.7 and 12.4).
 // The second launch, a workgroup per group, does the same with the parts' best and their values: 5 to 8 us of latency, some
 // 30 more for many beams whose scores lie far apart (one group of 32 of 131072 ids 54 to 71 for both launches).
 #include <algorithm>

@@ -632,8 +632,10 @@ __global__ void __launch_bounds__(W * 64, W == 4 ? 2 : 1) k_prod4(const Prod4Arg
 
 // Many blocks of W: WN waves beside each other take NT blocks of 16 rows each and share x, which passes through LDS in
 // steps that all of them load together; 8 / WN such teams divide the columns.  Of 32 rows by 32000 x 2048 the operands of x
-// are then a fourth of what every wave would fetch for itself; 12.6 us (13.9 with the norm, whose sums are products too),
-// bound by conversions, scales and products (1520 vector instructions a wave), 64 rows 21.4.  Rows of 8 columns or more.
+// are then a fourth of what every wave would fetch for itself; 12.1 us (13.5 with the norm, whose sums are products too), 64 rows
+// 17.8 (20.6).  No single rate bounds it: the bytes are 8.2 us, the vector instructions (3000 a SIMD) 5, the products under 2; 250
+// workgroups of eight waves are one a unit, so that nothing else runs while a step's barrier and its loads are waited for.
+// Rows of 8 columns or more.
 // Grid (n / (16 NT WN), m / (16 MT), batch).
 template <typename O, int MT, int NT, int WN>
 __global__ void __launch_bounds__(512, 2) k_share4(const Prod4Args a) {
@@ -830,12 +832,16 @@ void launch_share(const Prod4Args& p, int batch, hipStream_t st) {
 }
 
 // Measured, us, for rows x (n, k): one part, 32 x (32000, 2048): waves for themselves, 4 blocks of W each 17.1, sharing x,
-// teams of 4 with 2 blocks each 14.4; 32 x (16000, 2048): teams of 4 12.7, of 2 with one block each 10.1; 32 x (5504, 2048):
-// eight waves for themselves 7.3, teams of 2 6.8; of 2048 columns alike.  Three parts, which already are in the operands' order: 32
-// x (32000, 2048) sharing 23.8, for themselves 4 blocks each 21.5; 61 x (1999, 5501) sharing 30, eight waves to a block 29, 16 27.
-// What bounds that last one is x, read once per workgroup: 4 blocks of W each and the columns divided over 8 workgroups
-// instead 18.8 (with the rows' parts 24.0 before), 32 x (2048, 5504) 14.3 for 19.8, 5 x (100, 11000) 10.3 for 19.1; of few
-// columns it is the second exchange that costs (7 x (300, 1000) 7.9 for 6.5): from 16 blocks of columns on, 4 a workgroup.
+// teams of 4 with 2 blocks each 12.1, of 4 with one block 12.6, of 2 with one 16.8 (8 rows 9.5, 9.1, 10.4; 64 rows 17.8, 23.1, 32.3);
+// 32 x (16000, 2048): teams of 4 with 2 blocks 12.7, of 2 with one 10.1 (64 rows 16.4, 16.8, of 4 with one block 12.1);
+// 32 x (5504, 2048): eight waves for themselves 7.3, teams of 2 6.8; of 2048 columns alike.  More rows convert W again for
+// every 64 of them: 128 x (32000, 2048) 41, 256 77, 1024 298, where the library's product of 16-bit weights takes 26, 33 and 102 (64
+// rows 23 and 23); 1024 x (1280, 768) 12.4 and 8.7.
+// Three parts, which already are in the operands' order: 32 x (32000, 2048) sharing 23.8, for themselves 4 blocks each 21.5; 61 x
+// (1999, 5501) sharing 30, eight waves to a block 29, 16 27.  What bounds that last one is x, read once per workgroup: 4 blocks of W
+// each and the columns divided over 8 workgroups instead 18.8 (with the rows' parts 24.0 before), 32 x (2048, 5504) 14.3 for 19.8, 5 x
+// (100, 11000) 10.3 for 19.1; of few columns it is the second exchange that costs (7 x (300, 1000) 7.9 for 6.5): from 16 blocks of
+// columns on, 4 a workgroup.
 template <typename O, int P>
 void launch_linear_rows(const Prod4Args& p, int batch, hipStream_t st) {
   const int64_t tiles = (p.n + 15) / 16 * batch * ((p.m + 31) / 32);
@@ -900,8 +906,9 @@ struct Linear4Layout {
 };
 
 // One token a row: two launches, each row's last workgroup of the second normalising it.  More: products of rows in parts, with
-// SwiGLU four waves to a workgroup (32 rows of 4 tokens, 768 x 2048: 43 us, with eight 50; 16 of 8 29 and 32; one of 16, 2048 x
-// 5504: 27 either way).
+// SwiGLU four waves to a workgroup (32 rows of 4 tokens, 768 x 2048: 40 us, with eight 50; 16 of 8 28.5 and 32; one of 16, 2048 x
+// 5504: 24 to 27 either way).  What bounds those is a launch or two more than one token has, the parts' and the norm's, and x's operands
+// from memory for every two blocks of W (32 rows of one token 25, of 16 43, of 64 103, where W is read and converted twice).
 template <typename T>
 void launch_readout4(const uttt_readout4_args* a, hipStream_t st) {
   constexpr int HP = sizeof(T) == 2 ? 2 : 3;  // parts of the hidden values

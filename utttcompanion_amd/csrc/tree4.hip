@@ -9,13 +9,15 @@
 //   O^T = V^T (P s)^T  the values' scales go onto the weights, a group of 32 elements at a time; a lane's 8 weights
 //                      are the operand as they are, since the cache keeps its words of 8 slots in that order
 // Rows of q are rotated in fp32, scaled, and carried as bf16 parts: two (16 bits) for bf16 activations, three (all 24) for fp32;
-// weights are rounded to bf16 for bf16 activations and carried as three parts for fp32; sums are those of the unrounded ones.
+// weights are rounded to bf16 for bf16 activations (as attention over 16-bit rings has them: an error of 2.2e-3 against 64 bits
+// where the result's own rounding is 1.65e-3; a second part would double the values' products) and carried as three parts for fp32;
+// sums are those of the unrounded ones.
 // The new tokens themselves are keys in LDS, in their own precision; a single one stays in registers.
 //
-// 32 requests over 4096 slots, 16 heads on 4 of 128: 21 us and 4 of the join, 2.9 TB/s.  What bounds it is vector work, half of the
-// SIMD cycles: per block 64 conversions of codes, as many scales unpacked and applied to scores, then to weights; a tile has 16
-// columns of which 4 heads to a kv head fill 4.  One request over 512 slots: 7.4 us of latency.  Trees of more than 16
-// rows walk the cache once per 16 (16 trees of 64 nodes 118 us).
+// 32 requests over 4096 slots, 16 heads on 4 of 128: 21 us and 4 of the join, 2.9 TB/s (fp32 activations 32 us).  What bounds it
+// is vector work, half of the SIMD cycles: per block 64 conversions of codes, as many scales unpacked and applied to scores, then to
+// weights; a tile has 16 columns of which 4 heads to a kv head fill 4.  One request over 512 slots: 7.4 us of latency.  Trees of
+// more than 16 rows walk the cache once per 16 (16 trees of 64 nodes 118 us).
 #include <algorithm>
 #include <type_traits>
 
