@@ -12,6 +12,14 @@ from utttcompanion_amd import kernels as K
 pytestmark = pytest.mark.gpu
 
 
+def attention_bound(score, size, want, hd, keys, dt):
+    """What test_gpu_decode4 allows an output, from the largest sum of magnitudes behind a score and the sum behind the output."""
+    carried, weight = (2.0 ** -16, 2.0 ** -8) if dt is torch.bfloat16 else (2.0 ** -23, 2.0 ** -23)
+    ds = score * (carried + (34 + hd / 32 + 8) * U) + 4 * U * 40
+    rel = (2 * ds * (1 + ds)).unsqueeze(-1) + weight + 2 * (34 + keys / 32 + 80) * U + 8 * U
+    return rel * size + STEP[dt] * want.abs() * (1 + 2 ** -7)
+
+
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("t", [1, 6, 40])
@@ -36,21 +44,52 @@ def test_infinite_new_keys(t, hd, dt):
                       None if parents is None else parents.to(DEV), sinks=sinks)[0].cpu()
     keys, vals = R.cache_values(c, hd)
     calm = torch.where(torch.isfinite(k), k, torch.zeros_like(k))
-    carried, weight = (2.0 ** -16, 2.0 ** -8) if dt is torch.bfloat16 else (2.0 ** -23, 2.0 ** -23)
     none = some = 0
     for i in range(n):
         up = [-1] if parents is None else parents[i].tolist()
         args = v[i].double(), keys[i], vals[i], int(positions[i]), window, sinks, up, t
         want, size, seen = R.tree(q[i].double(), k[i].double(), *args)
         score = R.tree(q[i].double(), calm[i].double(), *args)[2]  # of the keys that have a weight, and more
-        ds = score * (carried + (34 + hd / 32 + 8) * U) + 4 * U * 40
-        chain = (34 + (window + sinks + t) / 32 + 80) * U
-        rel = (2 * ds * (1 + ds)).unsqueeze(-1) + weight + 2 * chain + 8 * U
         bad = torch.isnan(want).any(-1)
         assert torch.isnan(out[i][bad]).all()
-        within(out[i][~bad], want[~bad], (rel * size + STEP[dt] * want.abs() * (1 + 2 ** -7))[~bad])
+        within(out[i][~bad], want[~bad], attention_bound(score, size, want, hd, window + sinks + t, dt)[~bad])
         none, some = none + int(bad.sum()), some + int((~bad & ~torch.isfinite(seen)).sum())
     assert none and some
+
+
+def whole_in_two_parts(g, n, hd):
+    """n fp32 numbers, of either sign, that times the scale of head_dim ``hd`` are two bf16 parts and nothing more: what is left of
+    the product behind the first has its own leading 8 bits alone.  Products are kept whole between the parts, or rounded."""
+    scale = torch.tensor(hd ** -0.5, dtype=torch.float32) * torch.tensor(1.44269504088896340736, dtype=torch.float32)
+    x = 0.5 + torch.rand(1 << 23, generator=g)
+    rounded = x * scale
+    first = (rounded.view(torch.int32) & -65536).view(torch.float32)
+    rest = (x.double() * scale.double() - first.double()).float()
+    fused, apart = x[rest.view(torch.int32) & 65535 == 0], x[(rounded - first).view(torch.int32) & 65535 == 0]
+    half = n // 2
+    assert len(fused) >= half and len(apart) >= n - half
+    x = torch.cat([fused[:half], apart[:n - half]])[torch.randperm(n, generator=g)]
+    return x * torch.where(torch.rand(n, generator=g) < 0.5, -1.0, 1.0)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("t", [2, 36])
+def test_infinite_new_keys_where_a_part_of_q_is_zero(t, hd):
+    """fp32 rows whose third part is 0 at the infinite element of node 0's key, which every node sees; full windows behind it."""
+    g = gen(t + hd)
+    window, heads, hkv = 50, 4, 2
+    c = cache_of(g, 1, 1, hkv, window, 0, hd)[0]
+    q, k, v = (normal(g, 1, t, h, hd) for h in (heads, hkv, hkv))
+    q[..., 9] = whole_in_two_parts(g, t * heads, hd).view(1, t, heads)
+    k[0, 0, :, 9] = math.inf
+    out = K.swa_tree4(q.to(DEV), k.to(DEV), v.to(DEV), c.to(DEV), torch.tensor([80], device=DEV), window)[0].cpu()
+    negative = q[0, ..., 9] < 0  # scores of -inf
+    assert torch.isfinite(out[0][negative]).all() and torch.isnan(out[0][~negative]).all() and negative.any() and not negative.all()
+    keys, vals = R.cache_values(c, hd)
+    args = v[0].double(), keys[0], vals[0], 80, window, 0, list(range(-1, t - 1)), t
+    want, size, _ = R.tree(q[0].double(), k[0].double(), *args)
+    score = R.tree(q[0].double(), torch.where(torch.isfinite(k[0]), k[0], torch.zeros_like(k[0])).double(), *args)[2]
+    within(out[0][negative], want[negative], attention_bound(score, size, want, hd, window + t, torch.float32)[negative])
 
 
 @pytest.mark.parametrize("layers_inside", [False, True])

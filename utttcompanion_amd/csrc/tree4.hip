@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(W * 64, W == 4 ? 2 : 1) k_swa_tree4(const Tree
   using S = Smem4<T, HD, KT, W>;
   __shared__ __align__(16) char smem[S::kBytes];
   __shared__ float ml[W][16][2];
-  __shared__ int odd;
+  __shared__ int odd, odd_keys;  // new values, new keys that are not finite
   const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, h = lane >> 4;
   int id = blockIdx.x;
   const int group = id % a.groups;
@@ -308,10 +308,10 @@ __global__ void __launch_bounds__(W * 64, W == 4 ? 2 : 1) k_swa_tree4(const Tree
   // the new tokens' keys, rotated and rounded, and values into LDS (and out, for the caches)
   bf16* keys = reinterpret_cast<bf16*>(smem);
   bf16* vals = reinterpret_cast<bf16*>(smem + S::kKeys);
-  if (threadIdx.x == 0) odd = 0;
+  if (threadIdx.x == 0) odd = odd_keys = 0;
   if (KT > 1 && split == 0) {
     __syncthreads();
-    bool strange = false;
+    bool strange = false, strange_keys = false;
     for (int i = threadIdx.x; i < KT * (HD / 16); i += W * 64) {
       const int nd = i / (HD / 16), e = i % (HD / 16) * 8;  // elements e .. and HD / 2 + e ..
       float k0[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, k1[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -350,9 +350,11 @@ __global__ void __launch_bounds__(W * 64, W == 4 ? 2 : 1) k_swa_tree4(const Tree
       for (int j = 0; j < 8; ++j) {
         bf16 p[KP];
         bf16_parts(k0[j], p);
+        strange_keys |= !(fabsf(to_f32(p[0])) < INFINITY);
 #pragma unroll
         for (int i = 0; i < KP; ++i) keys[(i * KT + nd) * (HD + 8) + e + j] = p[i];
         bf16_parts(k1[j], p);
+        strange_keys |= !(fabsf(to_f32(p[0])) < INFINITY);
 #pragma unroll
         for (int i = 0; i < KP; ++i) keys[(i * KT + nd) * (HD + 8) + HD / 2 + e + j] = p[i];
         // what is not finite is left out of the products and added to the rows that see it
@@ -367,6 +369,7 @@ __global__ void __launch_bounds__(W * 64, W == 4 ? 2 : 1) k_swa_tree4(const Tree
       }
     }
     if (strange) odd = 1;
+    if (strange_keys) odd_keys = 1;
   }
 
   // the softmax's step: scores (masked: -inf) of 8 keys to weights, the sums so far rescaled where the maximum moves
@@ -470,6 +473,14 @@ __global__ void __launch_bounds__(W * 64, W == 4 ? 2 : 1) k_swa_tree4(const Tree
             for (int x = 0; x < QP; ++x)
               if (KP == 1 || i + x < QP) y = mfma16(k, qf[g][x], y);  // products below 2^-24 of the whole are left out
           }
+        if (odd_keys) {  // an infinite key times a part of q that is 0 is NaN: the first part, 0 only where q is, has the score
+          f32x4 z{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int g = 0; g < G; ++g)
+            z = mfma16(*reinterpret_cast<const bf16x8*>(keys + (b * kSlots + 16 * t + r) * (HD + 8) + 32 * g + 8 * h), qf[g][0], z);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[i] = fabsf(z[i]) < INFINITY ? y[i] : z[i];
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int key = b * kSlots + 16 * t + 4 * h + i;
