@@ -273,8 +273,8 @@ class BatchedDecoder:
     def _linear(self, x: Tensor, weight: Union[Tensor, Tuple[Tensor, ...]], name: Tuple, residual: Optional[Tensor] = None,
                 norm=None) -> Tensor:
         """norm(x) W^T (+ residual, updated in place): ``uttt_linear4`` with weights in 4 bits (``name`` W's among them, ``weight``
-        its parts where there are several), ``uttt_skinny_linear`` for bf16 steps of at most 64 requests (the RMSNorm folded in), the norm and the library GEMM
-        otherwise."""
+        its parts where there are several), ``uttt_skinny_linear`` for bf16 steps of at most 64 requests (the RMSNorm folded
+        in), the norm and the library GEMM otherwise."""
         if self.weight_bits == 4:
             folds = self._folds_in(norm)
             if norm is not folds:

@@ -2080,9 +2080,10 @@ def beam_select(logits: Tensor, scores: Tensor, beams: int, ended: Optional[Tens
     is, with ``pad``).  Per group the ``beams`` <= 32 best of score + log softmax(logits) over the ids below ``active_limit``
     that are not ``banned`` (softmax over those ids), the best first, of equal ones the lower row's, then the lower id.  Scores
     are compared in 64 bits; a softmax's sum is off by some 2^-23 (at most 2^-15) of itself, so values of two rows that are
-    closer than that may change places.  Returns the tokens (rows,) int64, the rows they go on from (rows,) int32 (``kv_fork``'s sources), their scores
-    and whether they have ended (by ``eos``, or before); ``out``, when given, whose scores and ended may be the inputs.  Where a
-    group offers fewer than ``beams``, the rest is ``pad`` at -inf from its own row, ended."""
+    closer than that may change places.  Returns the tokens (rows,) int64, the rows they go on from (rows,) int32
+    (``kv_fork``'s sources), their scores and whether they have ended (by ``eos``, or before); ``out``, when given, whose
+    scores and ended may be the inputs.  Where a group offers fewer than ``beams``, the rest is ``pad`` at -inf from its own
+    row, ended."""
     if logits.dim() != 2 or logits.shape[1] > 1 and logits.stride(1) != 1:
         raise ValueError("logits must be (rows, vocab) with unit column stride")
     rows, vocab = logits.shape
